@@ -375,6 +375,90 @@ int mi_linear(const void* x, int64_t x_stride, const void* weight, const void* b
 int mi_linear_silu(const void* x, int64_t x_stride, const void* weight, void* out, int64_t out_stride,
                    int32_t rows, int32_t n, int32_t k, mi_stream_t stream);
 
+/* mi_post_norm_add_rms_norm: the norms after a block and before the next, for
+ * layers that normalise a block's output before it joins the residual stream
+ * (no counterpart in the reference, whose layers add it as it is):
+ *   s = x + scale * gate * (y * rsqrt(mean(y^2) + eps) * post_weight)
+ *   x_out = bf16(s),  h_out = bf16(s * rsqrt(mean(s^2) + eps) * weight)
+ * in fp32, h from s before its rounding.  gate (bf16) may be null (1), hold a
+ * value per column (gate_per_column != 0; row stride 0: the same for all rows)
+ * or one value per row (gate_per_column 0: gate[row * gate_row_stride]).
+ * hidden: multiple of 8, <= 16384; rows, weights and a gate per column 16-byte
+ * aligned.  x_out may be x and h_out may be y; no other overlap. */
+int mi_post_norm_add_rms_norm(const void* x, int64_t x_stride, const void* y, int64_t y_stride,
+                              const void* post_weight, const void* weight, const void* gate,
+                              int64_t gate_row_stride, int32_t gate_per_column, void* x_out,
+                              int64_t x_out_stride, void* h_out, int64_t h_stride, int64_t rows,
+                              int32_t hidden, float eps, float scale, mi_stream_t stream);
+
+/* ------------------------------------------------------------------------ *
+ * MXFP4: 4-bit floating point (e2m1) in blocks of 32 along a row, each with a
+ * power of two (e8m0), after the OCP Microscaling Formats v1.0; and linear
+ * layers whose weight, or both operands, are held in it.  No counterpart in
+ * the reference.
+ *
+ * A matrix [rows][cols] (cols a multiple of 32, at most 2^20) lives in two
+ * device buffers of mi_mxfp4_codes_size / mi_mxfp4_scales_size bytes, in tiles
+ * of 16 rows x 128 columns in matrix-instruction operand order (rows and
+ * columns past the matrix are zeros); both 16-byte aligned.
+ * mi_mxfp4_pack / mi_mxfp4_unpack exchange that with row-major
+ * codes [rows][cols / 2] (the even column in the lower half of a byte, 16-byte
+ * aligned) and scale bytes [rows][cols / 32].
+ *
+ * Quantisation of a block: e = max(floor(log2 max|x|) - 2, -127); each code is
+ * the e2m1 value nearest to x / 2^e (ties to even, 6 at most in magnitude),
+ * the scale byte e + 127.  A block with an infinity or a NaN becomes NaN as a
+ * whole (scale byte 255).
+ * ------------------------------------------------------------------------ */
+size_t mi_mxfp4_codes_size(int64_t rows, int64_t cols);
+size_t mi_mxfp4_scales_size(int64_t rows, int64_t cols);
+
+int mi_mxfp4_quantize(const void* x, int64_t x_stride, void* codes, void* scales, int64_t rows,
+                      int64_t cols, mi_stream_t stream);
+int mi_mxfp4_dequantize(const void* codes, const void* scales, void* out, int64_t out_stride,
+                        int64_t rows, int64_t cols, mi_stream_t stream);
+int mi_mxfp4_pack(const void* row_codes, const void* row_scales, void* codes, void* scales,
+                  int64_t rows, int64_t cols, mi_stream_t stream);
+int mi_mxfp4_unpack(const void* codes, const void* scales, void* row_codes, void* row_scales,
+                    int64_t rows, int64_t cols, mi_stream_t stream);
+
+/* out = x W^T (+ bias) with W [n][k] in MXFP4, fp32 accumulation, one rounding
+ * to bf16.  x_scales null: x is [rows][k] bf16 with row stride x_stride (16-byte
+ * aligned rows); else x, x_scales are an MXFP4 matrix [rows][k] and x_stride is
+ * not read.  silu != 0: W is [2 n][k], n gate rows and then n up rows, and
+ * out = silu(x Wg^T) * (x Wu^T) (MLP, model.py:301-311); no bias then.
+ * rows 0..2^22, n 1..2^24 (any), k a multiple of 32 up to 2^20, x_stride at most
+ * 2^22; bias [n] or null.  No workspace; the result does not depend on timing. */
+int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_scales, const void* codes,
+                    const void* scales, const void* bias, void* out, int64_t out_stride,
+                    int64_t rows, int64_t n, int64_t k, int32_t silu, mi_stream_t stream);
+
+/* ------------------------------------------------------------------------ *
+ * One draw per row from given uniform numbers, with top-k, top-p and min-p.
+ * Beside mi_sample (scheduler.py:310-343), for callers that bring their own
+ * random numbers or filter by more than top-p.
+ *
+ * logits: [batch][vocab] bf16 (row stride in elements, any alignment).  With
+ * w_i = exp((l_i - max l) / temperature), tokens ordered by descending logit
+ * and, among equals, ascending index: kept are the first top_k (<= 0: all); of
+ * them those with w_i >= min_p (<= 0: all; at most 1); of those the shortest
+ * prefix whose mass reaches top_p of theirs (>= 1: all); always the first.
+ * out_tokens[row]: the lowest index whose cumulative kept weight, in index
+ * order, exceeds uniforms[row] (in [0, 1)) times the kept total; in 64 bits.
+ * Rows with temperature <= 0 (or NaN), and rows with no logit above -infinity,
+ * give argmax (lowest index among equals; a greedy row ranks NaN highest, a
+ * drawn one never takes it).  +infinity: only such logits have weight.
+ * top_k / top_p / min_p: device arrays [batch] or null (off).
+ * At most 65,535 rows of 2^20 tokens.  workspace: mi_draw_workspace_size bytes,
+ * 16-byte aligned, need not be initialised; one call at a time.
+ * ------------------------------------------------------------------------ */
+size_t mi_draw_workspace_size(int32_t batch_size, int32_t vocab_size);
+
+int mi_draw(const void* logits, int64_t logits_row_stride, int32_t batch_size, int32_t vocab_size,
+            const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+            const float* uniforms, int64_t* out_tokens, void* workspace, size_t workspace_bytes,
+            mi_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

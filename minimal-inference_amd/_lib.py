@@ -86,6 +86,26 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mi_silu_mul": (_c_i32, [_vp, _c_i64, _vp, _c_i64, _c_i64, _c_i32, _vp]),
     "mi_linear": (_c_i32, [_vp, _c_i64, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32, _vp]),
     "mi_linear_silu": (_c_i32, [_vp, _c_i64, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32, _vp]),
+    "mi_post_norm_add_rms_norm": (
+        _c_i32,
+        [_vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _c_i64, _c_i32, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_i32, _c_f32,
+         _c_f32, _vp],
+    ),
+    "mi_mxfp4_codes_size": (_c_sz, [_c_i64, _c_i64]),
+    "mi_mxfp4_scales_size": (_c_sz, [_c_i64, _c_i64]),
+    "mi_mxfp4_quantize": (_c_i32, [_vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _vp]),
+    "mi_mxfp4_dequantize": (_c_i32, [_vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp]),
+    "mi_mxfp4_pack": (_c_i32, [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _vp]),
+    "mi_mxfp4_unpack": (_c_i32, [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _vp]),
+    "mi_linear_mxfp4": (
+        _c_i32,
+        [_vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _vp],
+    ),
+    "mi_draw_workspace_size": (_c_sz, [_c_i32, _c_i32]),
+    "mi_draw": (
+        _c_i32,
+        [_vp, _c_i64, _c_i32, _c_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_sz, _vp],
+    ),
     "mi_page_table_state_size": (_c_sz, [_c_i32, _c_i32, _c_i32]),
     "mi_page_table_init": (ctypes.c_int, [_vp, _c_i32, _c_i32, _c_i32, _vp]),
     "mi_page_table_step": (

@@ -1,0 +1,187 @@
+// Projections of few rows with an MXFP4 weight (decode steps): out = x W^T (+ bias)
+// or silu(x Wg^T) * (x Wu^T), fp32 accumulation and one rounding; x bf16 or MXFP4.
+//
+// Bound: HBM, the one read of W, 0.53 bytes per weight.  A workgroup of 4 waves owns
+// 16 R rows of W over all of k and the waves split k: wave w takes the slabs of 128 k
+// w, w + 4, ...  A tile of W is an operand as it is loaded, so it goes from memory to
+// the matrix instructions through registers alone, D slabs ahead.  With bf16 rows
+// its codes become bf16 by one instruction per pair, exactly, and x passes through a
+// wave-private LDS slot into operand order; with MXFP4 rows x's tiles are operands
+// too and one scaled instruction does a slab.  The waves meet once, at the end, where
+// their accumulators are added in wave order: the result does not depend on timing.
+#include "mi_mx4_linear.h"
+
+namespace mi::mx4 {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kXSlot = 16 * kSlab * 2;  // a block of 16 bf16 rows of a slab
+
+template <int R, int MB, int D, bool MX, bool GLU>
+__global__ __launch_bounds__(64 * kWaves) void few_kernel(LinearParams p) {
+  constexpr int HALVES = GLU ? 2 : 1, COLS = 16 * R / HALVES;
+  static_assert(R % HALVES == 0, "gate and up tiles in pairs");
+  constexpr int SLOT = MX ? 0 : MB * kXSlot, RED = R * MB * 1024;
+  __shared__ __attribute__((aligned(16))) char smem[kWaves * (SLOT > RED ? SLOT : RED)];
+  lds_t* const lds = (lds_t*)smem;
+  const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
+  const int g = lane >> 4, n = lane & 15;
+  const int col0 = int(blockIdx.x) * COLS;
+  const int steps = (p.slabs - w + kWaves - 1) / kWaves;  // this wave's slabs: w, w + 4, ...
+
+  const char *wbase[HALVES], *sbase[HALVES];
+  int wsize[HALVES], ssize[HALVES];
+  LaneRow at[R];
+#pragma unroll
+  for (int h = 0; h < HALVES; ++h) {
+    const int row = h * p.n + col0, tile = row / kTileRows, tiles = min(R / HALVES + 1, p.w_tiles - tile);
+    wbase[h] = p.w + int64_t(tile) * p.slabs * kTileBytes;
+    sbase[h] = p.ws + int64_t(tile) * p.quads * kQuadBytes;
+    wsize[h] = tiles * p.slabs * kTileBytes;
+    ssize[h] = tiles * p.quads * kQuadBytes;
+#pragma unroll
+    for (int r = h; r < R; r += HALVES) at[r] = lane_row(p, row, row + r / HALVES * 16 + n, g);
+  }
+  // bf16: load i of block b takes 4 rows, lane l chunk l % 16 of row l / 16
+  const int lr = lane >> 4, lc = lane & 15;
+  const int rows = int(p.rows), stride = int(p.x_stride * 2);
+  const int xsize = MX ? (rows + 15) / 16 * p.slabs * kTileBytes : (rows - 1) * stride + p.k * 2;
+  const int xssize = (rows + 15) / 16 * p.quads * kQuadBytes;
+
+  u32x4_t wr[D][R], xr[D][MX ? MB : 4 * MB];
+  uint32_t wscale[D][R], xscale[D][MB];
+  auto load = [&](int d, int step) {
+    const int slab = step * kWaves + w;
+    const bool ok = step < steps;
+    __amdgpu_buffer_rsrc_t rw[HALVES], rs[HALVES];
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) {
+      rw[h] = buffer(wbase[h] + slab * kTileBytes, ok ? wsize[h] - slab * kTileBytes : 0);
+      rs[h] = buffer(sbase[h] + step * kQuadBytes, ok ? ssize[h] - step * kQuadBytes : 0);
+    }
+    // W is read once: non-temporal
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      wr[d][r] = __builtin_amdgcn_raw_buffer_load_b128(rw[r % HALVES], at[r].codes, 0, kCacheNT);
+      wscale[d][r] = __builtin_amdgcn_raw_buffer_load_b32(rs[r % HALVES], at[r].scales, 0, 0);
+    }
+    if constexpr (MX) {
+      const __amdgpu_buffer_rsrc_t rx = buffer(p.x + slab * kTileBytes, ok ? xsize - slab * kTileBytes : 0);
+      const __amdgpu_buffer_rsrc_t rxs = buffer(p.xs + step * kQuadBytes, ok ? xssize - step * kQuadBytes : 0);
+#pragma unroll
+      for (int b = 0; b < MB; ++b) {
+        xr[d][b] = __builtin_amdgcn_raw_buffer_load_b128(rx, b * p.slabs * kTileBytes + lane * 16, 0, 0);
+        xscale[d][b] = __builtin_amdgcn_raw_buffer_load_b32(rxs, b * p.quads * kQuadBytes + lane * 4, 0, 0);
+      }
+    } else {
+      const int off = slab * kSlab * 2;
+      const __amdgpu_buffer_rsrc_t rx = buffer(p.x + off, ok ? xsize - off : 0);
+      // past a row's end lies the next row: out of range instead
+      const bool in = off + lc * 16 < p.k * 2;
+#pragma unroll
+      for (int i = 0; i < 4 * MB; ++i)
+        xr[d][i] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? (4 * i + lr) * stride + lc * 16 : 0x7ffffff0, 0, 0);
+    }
+  };
+
+  f32x4_t acc[R][MB];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int b = 0; b < MB; ++b) acc[r][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  lds_t* const slot = lds + w * SLOT;
+  // row 4 i + lr, whose place in a row depends on the row modulo 8
+  const int so[2] = {lr * 256 + chunk_slot(lr, lc) * 16, lr * 256 + chunk_slot(4 + lr, lc) * 16};
+  int ro[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) ro[s] = n * 256 + chunk_slot(n, 4 * g + s) * 16;
+
+#pragma unroll
+  for (int d = 0; d < D; ++d) {
+    load(d, d);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // (no branch inside a round of D steps: the steps past the last one add zeros)
+  for (int s0 = 0; s0 < steps; s0 += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if constexpr (MX) {
+        u32x4_t a[R], x[MB];
+        uint32_t as[R], xs[MB];
+#pragma unroll
+        for (int r = 0; r < R; ++r) a[r] = wr[d][r], as[r] = wscale[d][r] >> (8 * w);
+#pragma unroll
+        for (int b = 0; b < MB; ++b) x[b] = xr[d][b], xs[b] = xscale[d][b] >> (8 * w);
+        load(d, s0 + d + D);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int b = 0; b < MB; ++b) acc[r][b] = mfma_fp4<0, 0>(a[r], as[r], x[b], xs[b], acc[r][b]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4 * MB; ++i) lds_store16(slot + i * 1024 + so[i & 1], xr[d][i]);
+        u32x4_t a[R];
+        float as[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) a[r] = wr[d][r], as[r] = scale_f32(wscale[d][r] >> (8 * w) & 255u);
+        load(d, s0 + d + D);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          bf16x8_t x[MB];
+#pragma unroll
+          for (int b = 0; b < MB; ++b)
+            x[b] = __builtin_bit_cast(bf16x8_t, lds_load16(slot + b * kXSlot + ro[s]));
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const bf16x8_t v = to_bf16(a[r][s], as[r]);
+#pragma unroll
+            for (int b = 0; b < MB; ++b) acc[r][b] = mfma_16x16x32_bf16(v, x[b], acc[r][b]);
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // Lane (g, n) holds columns 4 g .. 4 g + 3 of the output of row 16 b + n.
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+      lds_store16(lds + (w * R * MB + r * MB + b) * 1024 + lane * 16, __builtin_bit_cast(u32x4_t, acc[r][b]));
+  __syncthreads();
+  auto total = [&](int q) {
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int o = 0; o < kWaves; ++o)
+      sum += __builtin_bit_cast(f32x4_t, lds_load16(lds + (o * R * MB + q) * 1024 + lane * 16));
+    return sum;
+  };
+  for (int q = w; q < R / HALVES * MB; q += kWaves) {
+    const int r = q / MB, b = q - r * MB;  // r: the tile (or pair of tiles)
+    const f32x4_t sum = total(HALVES * r * MB + b);
+    f32x4_t up = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (GLU) up = total((HALVES * r + 1) * MB + b);
+    const int m = b * 16 + n, col = col0 + r * 16 + 4 * g;
+    if (m < rows && col < p.n) store4<GLU>(p, m, col, sum, up);
+  }
+}
+
+template <bool MX, bool GLU>
+void launch(const LinearParams& p, hipStream_t stream) {
+  constexpr int R = GLU ? 2 : 1;
+  const int cols = 16 * R / (GLU ? 2 : 1);
+  const dim3 grid((p.n + cols - 1) / cols);
+  if (p.rows <= 16) hipLaunchKernelGGL((few_kernel<R, 1, 2, MX, GLU>), grid, dim3(64 * kWaves), 0, stream, p);
+  else hipLaunchKernelGGL((few_kernel<R, 2, 2, MX, GLU>), grid, dim3(64 * kWaves), 0, stream, p);
+}
+
+}  // namespace
+
+void launch_few(const LinearParams& p, bool glu, hipStream_t stream) {
+  if (p.xs) glu ? launch<true, true>(p, stream) : launch<true, false>(p, stream);
+  else glu ? launch<false, true>(p, stream) : launch<false, false>(p, stream);
+}
+
+}  // namespace mi::mx4

@@ -1,0 +1,69 @@
+// What the launches of MXFP4 projections share: arguments, the rows of W that a
+// lane reads, and the end of a product.
+#pragma once
+
+#include "mi_mx4.h"
+
+namespace mi::mx4 {
+
+struct LinearParams {
+  const char* x;     // bf16 rows, or tiles of codes
+  int64_t x_stride;  // of bf16 rows
+  const char* xs;    // scales of x's tiles; null: x is bf16
+  const char* w;
+  const char* ws;
+  const uint16_t* bias;  // null: none
+  uint16_t* out;
+  int64_t o_stride;
+  int64_t rows;
+  int n, k;  // n: columns of out; with the gated product W holds n gate rows, then n up rows
+  int slabs, quads;
+  int w_tiles;  // row tiles of W
+  bool vec;     // out and bias take 8-byte accesses
+};
+
+// Row h n + first + i of W (i the lane's row of 16): its 16 codes' place from the
+// tile of row h n + first on.  n need not be a multiple of 16, so a lane's up row may
+// lie in another tile than its neighbour's.
+struct LaneRow {
+  int codes, scales;
+};
+__device__ __forceinline__ LaneRow lane_row(const LinearParams& p, int base_row, int row, int g) {
+  const int tile = row / kTileRows - base_row / kTileRows, at = row % kTileRows + 16 * g;
+  return {tile * p.slabs * kTileBytes + at * 16, tile * p.quads * kQuadBytes + at * 4};
+}
+
+// Columns col .. col + 3 of out's row m from a lane's sums (and, gated, those of the
+// up rows): bias or silu(gate) * up in fp32, one rounding.
+template <bool GLU>
+__device__ __forceinline__ void store4(const LinearParams& p, int64_t m, int col, f32x4_t sum, f32x4_t up) {
+  uint16_t* const out = p.out + m * p.o_stride + col;
+  if constexpr (GLU) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = silu(sum[i]) * up[i];
+  }
+  if (p.vec) {
+    if (!GLU && p.bias) {
+      const u32x2_t b = *reinterpret_cast<const u32x2_t*>(p.bias + col);
+      sum[0] += bf16_lo(b.x);
+      sum[1] += bf16_hi(b.x);
+      sum[2] += bf16_lo(b.y);
+      sum[3] += bf16_hi(b.y);
+    }
+    *reinterpret_cast<u32x2_t*>(out) = u32x2_t{cvt_pk_bf16(sum[0], sum[1]), cvt_pk_bf16(sum[2], sum[3])};
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (col + i < p.n) out[i] = cvt_bf16(!GLU && p.bias ? sum[i] + bf16_to_f32(p.bias[col + i]) : sum[i]);
+}
+
+// Slot of 16-byte chunk c in a staged row of 256 bytes: the 8 rows that an operand
+// read touches together at one chunk fall on distinct banks.
+__device__ __forceinline__ int chunk_slot(int r, int c) { return c ^ ((r & 7) << 1); }
+
+void launch_few(const LinearParams& p, bool glu, hipStream_t stream);   // up to kFewRows rows
+void launch_many(const LinearParams& p, bool glu, hipStream_t stream);
+constexpr int kFewRows = 32;
+
+}  // namespace mi::mx4

@@ -8,7 +8,9 @@ model.py:301-311).  Both run one HIP kernel (``mi_add_rms_norm`` /
 ``mi_silu_mul``); there is no torch fallback.  ``linear(x, weight, bias)`` is
 ``F.linear`` with a decode step's few rows on ``mi_linear``, and
 ``linear_silu(x, gate_up)`` is ``silu_mul(linear(x, gate_up))`` with those rows
-in one launch (``mi_linear_silu``).
+in one launch (``mi_linear_silu``).  ``post_norm_add_rms_norm`` is the step between
+blocks of layers that normalise a block's output too: norm, gate, residual scale,
+sum and the next norm in one kernel (``mi_post_norm_add_rms_norm``).
 """
 
 from __future__ import annotations
@@ -21,7 +23,7 @@ from torch.autograd import forward_ad
 from torch.overrides import has_torch_function
 
 from . import _lib
-from ._util import require_dtype, require_gpu, stream_of
+from ._util import call_on, require_dtype, require_gpu, stream_of
 
 
 def _rows(name: str, t: torch.Tensor, width: int | None = None) -> None:
@@ -61,6 +63,62 @@ def add_rms_norm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tens
               xo.stride(0) if xo is not None else 0, h_out.data_ptr() if norm else None,
               h_out.stride(0) if norm else 0, rows, hidden, float(eps), stream_of(x))
     return h_out if norm else None
+
+
+def post_norm_add_rms_norm(x: torch.Tensor, y: torch.Tensor, post_weight: torch.Tensor, weight: torch.Tensor,
+                           eps: float, *, gate: torch.Tensor | None = None, scale: float = 1.0,
+                           x_out: torch.Tensor | None = None, h_out: torch.Tensor | None = None) -> torch.Tensor:
+    """A block's output y into the residual stream, and the next block's input:
+
+        s = x + scale * gate * rms_norm(y, post_weight)
+        x_out = bf16(s)            (in place in ``x`` when ``x_out`` is not given)
+        return bf16(rms_norm(s, weight))
+
+    in fp32, the second norm from s before its rounding.  ``gate``: [hidden], [rows, 1]
+    or [rows, hidden].  x_out may be x, and h_out y; other overlaps are undefined.
+    """
+    _rows("x", x)
+    rows, hidden = x.shape
+    _rows("y", y, hidden)
+    for name, w in (("post_weight", post_weight), ("weight", weight)):
+        require_gpu(name, w)
+        require_dtype(name, w, torch.bfloat16)
+        if w.shape != (hidden,) or not w.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous [{hidden}] tensor")
+    if x_out is None:
+        x_out = x
+    else:
+        _rows("x_out", x_out, hidden)
+    if h_out is None:
+        h_out = torch.empty(rows, hidden, dtype=x.dtype, device=x.device)
+    else:
+        _rows("h_out", h_out, hidden)
+    if y.shape[0] != rows or x_out.shape[0] != rows or h_out.shape[0] != rows:
+        raise ValueError("x, y, x_out and h_out must have as many rows")
+    g_ptr, g_stride, g_column = None, 0, 0
+    if gate is not None:
+        require_gpu("gate", gate)
+        require_dtype("gate", gate, torch.bfloat16)
+        g_ptr = gate.data_ptr()
+        if gate.shape == (hidden,) and gate.is_contiguous():
+            g_column = 1
+        elif gate.shape == (rows, 1):
+            g_stride = gate.stride(0)
+        elif gate.shape == (rows, hidden) and gate.stride(1) == 1:
+            g_stride, g_column = gate.stride(0), 1
+        else:
+            raise ValueError(f"gate must be [{hidden}], [{rows}, 1] or [{rows}, {hidden}] with a contiguous last axis; "
+                             f"got {tuple(gate.shape)}")
+    tensors = (x, y, post_weight, weight, x_out, h_out) if gate is None else (x, y, post_weight, weight, x_out, h_out, gate)
+    for t in tensors:
+        if t.get_device() != x.get_device():
+            raise ValueError(f"tensors on {t.device} and {x.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("an input requires a gradient: there is no backward pass")
+    call_on(x, "mi_post_norm_add_rms_norm", x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0),
+            post_weight.data_ptr(), weight.data_ptr(), g_ptr, g_stride, g_column, x_out.data_ptr(), x_out.stride(0),
+            h_out.data_ptr(), h_out.stride(0), rows, hidden, eps, scale)
+    return h_out
 
 
 def silu_mul(gate_up: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
