@@ -172,7 +172,7 @@ def prepare(case, seed):
         if case["kind"] == "linear":
             from minimal_inference_amd.mxfp4 import MXFP4
 
-            state["weight"] = MXFP4.from_codes(x["codes"], x["scales"])
+            state["weight"] = MXFP4.from_codes(x["codes"].to(torch.uint8), x["scales"])
         if case["kind"] == "sample":
             from minimal_inference_amd.sampling import Sampler
 
