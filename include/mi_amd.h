@@ -428,10 +428,17 @@ int mi_mxfp4_unpack(const void* codes, const void* scales, void* row_codes, void
  * not read.  silu != 0: W is [2 n][k], n gate rows and then n up rows, and
  * out = silu(x Wg^T) * (x Wu^T) (MLP, model.py:301-311); no bias then.
  * rows 0..2^22, n 1..2^24 (any), k a multiple of 32 up to 2^20, x_stride at most
- * 2^22; bias [n] or null.  No workspace; the result does not depend on timing. */
+ * 2^22; bias [n] or null.  The result does not depend on timing.
+ * workspace (16-byte aligned; may be null) holds partial sums of workgroups that
+ * share k: mi_linear_mxfp4_workspace_size bytes are what the fastest form takes
+ * (often 0); with fewer, one that takes no more is run, with the same results
+ * within fp32 rounding.  It need not be initialised; one call at a time. */
+size_t mi_linear_mxfp4_workspace_size(int64_t rows, int64_t n, int64_t k, int32_t silu,
+                                      int32_t x_mxfp4);
 int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_scales, const void* codes,
                     const void* scales, const void* bias, void* out, int64_t out_stride,
-                    int64_t rows, int64_t n, int64_t k, int32_t silu, mi_stream_t stream);
+                    int64_t rows, int64_t n, int64_t k, int32_t silu, void* workspace,
+                    size_t workspace_bytes, mi_stream_t stream);
 
 /* ------------------------------------------------------------------------ *
  * One draw per row from given uniform numbers, with top-k, top-p and min-p.

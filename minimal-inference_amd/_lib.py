@@ -97,9 +97,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mi_mxfp4_dequantize": (_c_i32, [_vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp]),
     "mi_mxfp4_pack": (_c_i32, [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _vp]),
     "mi_mxfp4_unpack": (_c_i32, [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _vp]),
+    "mi_linear_mxfp4_workspace_size": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_i32, _c_i32]),
     "mi_linear_mxfp4": (
         _c_i32,
-        [_vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _vp],
+        [_vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _vp, _c_sz, _vp],
     ),
     "mi_draw_workspace_size": (_c_sz, [_c_i32, _c_i32]),
     "mi_draw": (

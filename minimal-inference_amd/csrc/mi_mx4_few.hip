@@ -168,20 +168,57 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(LinearParams p) {
   }
 }
 
-template <bool MX, bool GLU>
+template <int R, int MB, int D, bool MX, bool GLU>
+void run(const LinearParams& p, hipStream_t stream) {
+  constexpr int COLS = 16 * R / (GLU ? 2 : 1);
+  hipLaunchKernelGGL((few_kernel<R, MB, D, MX, GLU>), dim3((p.n + COLS - 1) / COLS), dim3(64 * kWaves), 0, stream, p);
+}
+
+// The form of a launch, from the tiles of W and the 16-row blocks of x (us, weights
+// rotated through 600 MB):
+//                              rows   R 1 D 4   R 2 D 2   R 4 D 2   R 8 D 1   R 8 D 2
+//   N  4096 K  4096               8     5.2       6.3       7.2       10.6      10.5
+//   N  4096 K  4096              32     7.9       8.1      10.0       14.1      15.3
+//   N  4096 K 14336               8    12.3      16.8      19.5       32.7      27.9
+//   N 10240 K  8192               8    16.2      13.1      12.8       19.7      17.9
+//   N 10240 K  8192              32    28.7      22.2      17.7       25.4      27.5
+//   gated 2 x 4864, K 896         1               4.8       4.4        5.8       6.2
+//   gated 2 x 14336, K 4096       1              15.6      13.4       14.7      14.1
+//   gated 2 x 14336, K 4096      16              18.1      14.5       14.4      14.0
+//   gated 2 x 14336, K 4096      32              24.6      18.2       15.8      17.7
+//   MXFP4 x: N 4096 K 4096        8     4.0       5.0       6.3        9.9       8.8
+//   MXFP4 x: N 10240 K 8192      48    18.7      15.8      13.7       18.2      19.4
+// Every workgroup reads x, so tiles as many as still leave a workgroup for most CUs:
+// one up to 256 tiles (loads in flight bound it then: D 4), four beyond; eight where
+// there are over 1,024 tiles and x is two blocks, whose bf16 rows are then the larger
+// part of what is read.
+template <int MB, bool MX, bool GLU>
+void pick(const LinearParams& p, hipStream_t stream) {
+  if constexpr (!MX && MB == 2) {
+    if (p.w_tiles > 1024) return run<8, MB, 1, MX, GLU>(p, stream);
+  }
+  if (p.w_tiles > 256) return run<4, MB, 2, MX, GLU>(p, stream);
+  run<GLU ? 2 : 1, MB, (MB > 1 && !MX ? 2 : 4), MX, GLU>(p, stream);
+}
+
+template <bool GLU>
 void launch(const LinearParams& p, hipStream_t stream) {
-  constexpr int R = GLU ? 2 : 1;
-  const int cols = 16 * R / (GLU ? 2 : 1);
-  const dim3 grid((p.n + cols - 1) / cols);
-  if (p.rows <= 16) hipLaunchKernelGGL((few_kernel<R, 1, 2, MX, GLU>), grid, dim3(64 * kWaves), 0, stream, p);
-  else hipLaunchKernelGGL((few_kernel<R, 2, 2, MX, GLU>), grid, dim3(64 * kWaves), 0, stream, p);
+  const int blocks = int((p.rows + 15) / 16);
+  if (p.xs) {
+    if (blocks == 1) pick<1, true, GLU>(p, stream);
+    else if (blocks == 2) pick<2, true, GLU>(p, stream);
+    else if (blocks == 3) pick<3, true, GLU>(p, stream);
+    else pick<4, true, GLU>(p, stream);
+  } else {
+    if (blocks == 1) pick<1, false, GLU>(p, stream);
+    else pick<2, false, GLU>(p, stream);
+  }
 }
 
 }  // namespace
 
 void launch_few(const LinearParams& p, bool glu, hipStream_t stream) {
-  if (p.xs) glu ? launch<true, true>(p, stream) : launch<true, false>(p, stream);
-  else glu ? launch<false, true>(p, stream) : launch<false, false>(p, stream);
+  glu ? launch<true>(p, stream) : launch<false>(p, stream);
 }
 
 }  // namespace mi::mx4

@@ -19,6 +19,8 @@ struct LinearParams {
   int n, k;  // n: columns of out; with the gated product W holds n gate rows, then n up rows
   int slabs, quads;
   int w_tiles;  // row tiles of W
+  f32x4_t* parts;   // sums of workgroups that share k
+  int split_slabs;  // slabs that one of them takes
   bool vec;     // out and bias take 8-byte accesses
 };
 
@@ -62,8 +64,15 @@ __device__ __forceinline__ void store4(const LinearParams& p, int64_t m, int col
 // read touches together at one chunk fall on distinct banks.
 __device__ __forceinline__ int chunk_slot(int r, int c) { return c ^ ((r & 7) << 1); }
 
-void launch_few(const LinearParams& p, bool glu, hipStream_t stream);   // up to kFewRows rows
-void launch_many(const LinearParams& p, bool glu, hipStream_t stream);
-constexpr int kFewRows = 32;
+constexpr int64_t kMaxRows = 1 << 22, kMaxN = 1 << 24, kMaxStride = 1 << 22;
+
+// Whether the few-row kernel is the faster one.  (Two blocks of bf16 rows along a long k
+// are read by every one of its workgroups: 32 x 14,336 x 4,096 19.1 us, the blocks of
+// 128 rows of W with k in parts 14.5; 32 x 4,096 x 4,096 7.6, 10.0.)
+inline bool few(bool mx, int64_t rows, int64_t w_rows, int64_t k) {
+  return mx ? rows <= 64 : rows <= 16 || (rows <= 32 && (w_rows > 4096 || k < 8192));
+}
+void launch_few(const LinearParams& p, bool glu, hipStream_t stream);
+void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t stream);
 
 }  // namespace mi::mx4

@@ -17,8 +17,14 @@ __device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t rs, lds_t* dst,
 #endif
 }
 
-// MB blocks of 16 rows of x and NT tiles of W per wave.
-template <int WM, int WN, int MB, int NT, bool MX, bool GLU>
+// MB blocks of 16 rows of x and NT tiles of W per wave.  Slabs are staged STAGES deep:
+// before slab s is multiplied the loads of the STAGES - 2 slabs behind it may be in
+// flight, and after the barrier its predecessor's buffer is filled again.  Loads past
+// the last slab are out of range, so that every wait counts the same loads.
+//
+// SPLIT: the workgroup takes p.split_slabs slabs and leaves its sums, in fp32, for
+// combine_kernel.
+template <int WM, int WN, int MB, int NT, int STAGES, bool MX, bool GLU, bool SPLIT>
 __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
   constexpr int WAVES = WM * WN, HALVES = GLU ? 2 : 1;
   constexpr int XBLK = MX ? kTileBytes : 16 * kSlab * 2;  // 16 rows of x of a slab
@@ -26,14 +32,22 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
   constexpr int XBYTES = WM * MB * XBLK, STAGE = XBYTES + TILES * kTileBytes;
   constexpr int XLOADS = XBYTES / 1024 / WAVES, WLOADS = TILES / WAVES;
   static_assert(XBYTES / 1024 % WAVES == 0 && TILES % WAVES == 0 && NT % HALVES == 0, "even shares");
-  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+  static_assert(STAGES * STAGE <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(16))) char smem[STAGES * STAGE];
   lds_t* const lds = (lds_t*)smem;
   const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
   const int wm = w / WN, wn = w % WN;
   const int g = lane >> 4, n = lane & 15;
-  const int col0 = int(blockIdx.x) * COLS;
-  const int64_t m0 = int64_t(blockIdx.y) * BM;
+  // Workgroups go to the eight XCDs in turn.  Each XCD gets a run of tiles, down the
+  // rows of x first, so that the tiles of W in its L2 serve them all.
+  const int mt = int((p.rows + BM - 1) / BM), nt = (p.n + COLS - 1) / COLS, all = mt * nt;
+  const int id = int(blockIdx.x), xcd = id & 7, in = id >> 3, each = all / 8, more = all % 8;
+  const int tile_id = xcd * each + min(xcd, more) + in;
+  const int col0 = tile_id / mt * COLS;
+  const int64_t m0 = int64_t(tile_id % mt) * BM;
   const int rows = int(min(int64_t(BM), p.rows - m0));
+  const int slab0 = SPLIT ? int(blockIdx.y) * p.split_slabs : 0;
+  const int slab_end = SPLIT ? min(slab0 + p.split_slabs, p.slabs) : p.slabs;
 
   const char *wbase[HALVES], *sbase[HALVES];
   int wsize[HALVES], ssize[HALVES];
@@ -69,45 +83,49 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
     const int stride = int(p.x_stride * 2);
     xbase = p.x + m0 * p.x_stride * 2;
     xsize = (rows - 1) * stride + p.k * 2;
-    // load i: 4 rows, lane l slot l % 16 of row l / 16.  A row's permutation depends
-    // on the row modulo 8: one chunk for even i, one for odd (two chunks to test)
+    // load i: 4 rows, lane l slot l % 16 of row l / 16
 #pragma unroll
     for (int i = 0; i < XLOADS; ++i) {
       const int row = (w * XLOADS + i) * 4 + (lane >> 4);
       xv[i] = row * stride + chunk_slot(row, lane & 15) * 16;
     }
   }
+  // a lane's k of its even and odd loads: a row's permutation depends on it modulo 8
+  const int xk[2] = {chunk_slot(w * XLOADS * 4 + (lane >> 4), lane & 15) * 16,
+                     chunk_slot(w * XLOADS * 4 + 4 + (lane >> 4), lane & 15) * 16};
   auto load = [&](int slab, int buf) {
     lds_t* const stage = lds + buf * STAGE;
+    const bool ok = slab < slab_end;
     const int off = MX ? slab * kTileBytes : slab * kSlab * 2;
-    const __amdgpu_buffer_rsrc_t rx = buffer(xbase + off, xsize - off);
+    const __amdgpu_buffer_rsrc_t rx = buffer(xbase + off, ok ? xsize - off : 0);
 #pragma unroll
     for (int i = 0; i < XLOADS; ++i) {
       int v = xv[i];
-      if constexpr (!MX) {
-        const int row = (w * XLOADS + i) * 4 + (lane >> 4);
-        if (off + chunk_slot(row, lane & 15) * 16 >= p.k * 2) v = 0x7ffffff0;  // past the row's end lies the next row
-      }
+      if constexpr (!MX) v = off + xk[i & 1] < p.k * 2 ? v : 0x7ffffff0;  // past the row's end lies the next row
       lds_dma16(rx, stage + (w * XLOADS + i) * 1024, v);
     }
+    __amdgpu_buffer_rsrc_t rw[HALVES];
 #pragma unroll
-    for (int i = 0; i < WLOADS; ++i) {
-      const int h = (w * WLOADS + i) % HALVES;
-      lds_dma16(buffer(wbase[h] + slab * kTileBytes, wsize[h] - slab * kTileBytes),
-                stage + XBYTES + (w * WLOADS + i) * kTileBytes, wv[i]);
-    }
+    for (int h = 0; h < HALVES; ++h)
+      rw[h] = buffer(wbase[h] + slab * kTileBytes, ok ? wsize[h] - slab * kTileBytes : 0);
+#pragma unroll
+    for (int i = 0; i < WLOADS; ++i)
+      lds_dma16(rw[(w * WLOADS + i) % HALVES], stage + XBYTES + (w * WLOADS + i) * kTileBytes, wv[i]);
   };
-  uint32_t wscale[NT], xscale[MB], wnext[NT], xnext[MB];
+  uint32_t wnext[NT], xnext[MX ? MB : 1];
   auto load_scales = [&](int quad) {
+    const bool ok = quad < p.quads;
     const int off = quad * kQuadBytes;
+    __amdgpu_buffer_rsrc_t rs[HALVES];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-      wnext[t] = __builtin_amdgcn_raw_buffer_load_b32(buffer(sbase[t % HALVES] + off, ssize[t % HALVES] - off), wsv[t], 0, 0);
+    for (int h = 0; h < HALVES; ++h) rs[h] = buffer(sbase[h] + off, ok ? ssize[h] - off : 0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) wnext[t] = __builtin_amdgcn_raw_buffer_load_b32(rs[t % HALVES], wsv[t], 0, 0);
     if constexpr (MX) {
+      const __amdgpu_buffer_rsrc_t rx = buffer(xsbase + off, ok ? xssize - off : 0);
 #pragma unroll
       for (int b = 0; b < MB; ++b)
-        xnext[b] = __builtin_amdgcn_raw_buffer_load_b32(buffer(xsbase + off, xssize - off),
-                                                        (wm * MB + b) * p.quads * kQuadBytes + lane * 4, 0, 0);
+        xnext[b] = __builtin_amdgcn_raw_buffer_load_b32(rx, (wm * MB + b) * p.quads * kQuadBytes + lane * 4, 0, 0);
     }
   };
 
@@ -120,50 +138,62 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
 #pragma unroll
   for (int s = 0; s < 4; ++s) ro[s] = n * 256 + chunk_slot(n, 4 * g + s) * 16;
 
-  load(0, 0);
-  load_scales(0);
-  for (int slab = 0; slab < p.slabs; ++slab) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    __syncthreads();
-    if ((slab & 3) == 0) {
+  constexpr int kInFlight = (STAGES - 2) * (XLOADS + WLOADS);
+  static_assert(kInFlight < 64, "vmcnt");
+  load_scales(slab0 >> 2);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) wscale[t] = wnext[t];
+  for (int i = 0; i < STAGES - 1; ++i) load(slab0 + i, i);
+  int buf = 0, before = STAGES - 1;
+  for (int quad = slab0 >> 2; 4 * quad < slab_end; ++quad) {
+    uint32_t wscale[NT], xscale[MX ? MB : 1];
 #pragma unroll
-      for (int b = 0; b < MB; ++b) xscale[b] = xnext[b];
-    }
-    if (slab + 1 < p.slabs) {
-      load(slab + 1, (slab + 1) & 1);
-      if ((slab & 3) == 3) load_scales((slab + 1) >> 2);
-    }
-    const lds_t* const xl = lds + (slab & 1) * STAGE + wm * MB * XBLK;
-    const lds_t* const wl = lds + (slab & 1) * STAGE + XBYTES + wn * NT * kTileBytes + lane * 16;
-    const int shift = 8 * (slab & 3);
-    u32x4_t a[NT];
+    for (int t = 0; t < NT; ++t) wscale[t] = wnext[t];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) a[t] = lds_load16(wl + t * kTileBytes);
-    if constexpr (MX) {
-      u32x4_t x[MB];
+    for (int b = 0; b < (MX ? MB : 1); ++b) xscale[b] = xnext[b];
+    auto step = [&]<int S>() {
+      const int slab = 4 * quad + S;
+      if ((SPLIT && slab < slab0) || slab >= slab_end) return;
+      // vmcnt: this slab is in LDS; lgkmcnt: this wave has read the one before
+      __builtin_amdgcn_s_waitcnt(0x0070 | (kInFlight & 15) | (kInFlight >> 4 << 14));
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      if (S == 0 || (SPLIT && slab == slab0)) load_scales(quad + 1);
+      load(slab + STAGES - 1, before);
+      const lds_t* const xl = lds + buf * STAGE + wm * MB * XBLK;
+      const lds_t* const wl = lds + buf * STAGE + XBYTES + wn * NT * kTileBytes + lane * 16;
+      before = buf;
+      buf = buf + 1 == STAGES ? 0 : buf + 1;
+      u32x4_t a[NT];
 #pragma unroll
-      for (int b = 0; b < MB; ++b) x[b] = lds_load16(xl + b * XBLK + lane * 16);
+      for (int t = 0; t < NT; ++t) a[t] = lds_load16(wl + t * kTileBytes);
+      if constexpr (MX) {
+        u32x4_t x[MB];
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+        for (int b = 0; b < MB; ++b) x[b] = lds_load16(xl + b * XBLK + lane * 16);
 #pragma unroll
-        for (int b = 0; b < MB; ++b)
-          acc[t][b] = mfma_fp4<0, 0>(a[t], wscale[t] >> shift, x[b], xscale[b] >> shift, acc[t][b]);
-    } else {
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        bf16x8_t x[MB];
+          for (int b = 0; b < MB; ++b) acc[t][b] = mfma_fp4<S, S>(a[t], wscale[t], x[b], xscale[b], acc[t][b]);
+      } else {
 #pragma unroll
-        for (int b = 0; b < MB; ++b) x[b] = __builtin_bit_cast(bf16x8_t, lds_load16(xl + b * XBLK + ro[s]));
+        for (int s = 0; s < 4; ++s) {
+          bf16x8_t x[MB];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const bf16x8_t v = to_bf16(a[t][s], scale_f32(wscale[t] >> shift & 255u));
+          for (int b = 0; b < MB; ++b) x[b] = __builtin_bit_cast(bf16x8_t, lds_load16(xl + b * XBLK + ro[s]));
 #pragma unroll
-          for (int b = 0; b < MB; ++b) acc[t][b] = mfma_16x16x32_bf16(v, x[b], acc[t][b]);
+          for (int t = 0; t < NT; ++t) {
+            const bf16x8_t v = to_bf16(a[t][s], scale_f32(wscale[t] >> (8 * S) & 255u));
+#pragma unroll
+            for (int b = 0; b < MB; ++b) acc[t][b] = mfma_16x16x32_bf16(v, x[b], acc[t][b]);
+          }
         }
       }
-    }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    step.template operator()<0>();
+    step.template operator()<1>();
+    step.template operator()<2>();
+    step.template operator()<3>();
   }
 
   // Lane (g, n) holds columns 4 g .. 4 g + 3 of a tile for row n of a block.
@@ -174,33 +204,174 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
 #pragma unroll
     for (int b = 0; b < MB; ++b) {
       const int m = (wm * MB + b) * 16 + n;
-      if (m < rows) store4<GLU>(p, m0 + m, col, acc[t][b], acc[t + HALVES - 1][b]);
+      if (m >= rows) continue;
+      if constexpr (SPLIT) {
+        // [part][half][row][columns, in fours]
+        const int64_t fours = (p.n + 3) / 4;
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+          p.parts[((int64_t(blockIdx.y) * HALVES + h) * p.rows + m0 + m) * fours + col / 4] = acc[t + h][b];
+      } else {
+        store4<GLU>(p, m0 + m, col, acc[t][b], acc[t + HALVES - 1][b]);
+      }
     }
   }
 }
 
+// The sum of the parts in their order, and the end of the product.
+template <bool GLU>
+__global__ __launch_bounds__(256) void combine_kernel(LinearParams p, int parts) {
+  constexpr int HALVES = GLU ? 2 : 1;
+  const int fours = (p.n + 3) / 4;
+  const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x, one = p.rows * fours;
+  if (at >= one) return;
+  f32x4_t sum = p.parts[at], up = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (GLU) up = p.parts[one + at];
+#pragma unroll 4
+  for (int i = 1; i < parts; ++i) {
+    sum += p.parts[i * HALVES * one + at];
+    if constexpr (GLU) up += p.parts[(i * HALVES + 1) * one + at];
+  }
+  store4<GLU>(p, at / fours, int(at % fours) * 4, sum, up);
+}
+
+// ---------------------------------------------------------------- which form
+// Forms of the kernel: rows of x and of W per workgroup, and the time of a slab with
+// one workgroup on every CU (us, measured; the larger the block, the fewer the bytes
+// that each product needs and the fewer the workgroups).  A launch takes its start, a
+// slab's time for every slab of every round of workgroups, and, where workgroups share
+// k, the combining launch with the parts' way to memory and back.  Model and measured
+// (us): 77 x 18,944 x 3,584, 80-row blocks, 9 parts 21.9 / 22.5, whole 95.3 / 95.5;
+// 128 x 8,192 x 10,240, 128 x 128, 3 parts 32.2 / 32.2, whole 59.2 / 57.9;
+// 512 x 14,336 x 4,096, 128 x 128, 2 parts 64.3 / 62.9, whole 100.9 / 95.9.
+struct Form {
+  int rows, tiles;  // 16-row tiles of W
+  float slab_us;
+  bool split;
+};
+constexpr Form kBf16Forms[] = {{32, 8, 0.45f, true}, {64, 8, 0.56f, true}, {80, 8, 0.63f, true}, {128, 8, 0.87f, true},
+                               {128, 16, 1.65f, false}};
+constexpr Form kMxForms[] = {{128, 8, 0.34f, true}, {256, 16, 1.0f, false}};
+constexpr float kStartUs = 3.5f, kCombineUs = 2.5f, kCombineBytesPerUs = 4.4e6f;
+constexpr int kMaxParts = 32;
+
+struct Choice {
+  float us;
+  int form, parts, split_slabs;
+  size_t bytes;  // of the parts
+};
+
+// The fastest by that count within `room` bytes for parts.
+Choice choose(bool mx, bool glu, int64_t rows, int64_t n, int slabs, size_t room) {
+  Choice best = {1e30f, 0, 1, slabs, 0};
+  const int cus = mi::num_cus(), forms = mx ? 2 : 5;
+  for (int f = 0; f < forms; ++f) {
+    const Form& form = mx ? kMxForms[f] : kBf16Forms[f];
+    const int64_t cols = form.tiles * kTileRows / (glu ? 2 : 1);
+    const int64_t tiles = (rows + form.rows - 1) / form.rows * ((n + cols - 1) / cols);
+    for (int want = 1; want <= (form.split ? kMaxParts : 1); ++want) {
+      const int each = (slabs + want - 1) / want, parts = (slabs + each - 1) / each;
+      if (parts != want || (want > 1 && (each < 2 || tiles * (want - 1) >= 2 * cus))) continue;
+      const size_t bytes = want > 1 ? size_t(want) * (glu ? 2 : 1) * rows * ((n + 3) / 4) * 16 : 0;
+      if (bytes > room) continue;
+      float us = kStartUs + float((tiles * want + cus - 1) / cus) * each * form.slab_us;
+      if (want > 1) us += kCombineUs + 2 * float(bytes) / kCombineBytesPerUs;
+      if (us < best.us) best = {us, f, want, each, bytes};
+    }
+  }
+  return best;
+}
+
+// The few-row kernel's time, from W's bytes.
+float few_us(const LinearParams& p) { return 4.f + float(p.w_tiles) * p.slabs * 1.0625e3f / 4e6f; }
+
+template <int WM, int WN, int MB, int NT, int STAGES, bool MX, bool GLU, bool SPLIT>
+void run(const LinearParams& p, int parts, hipStream_t stream) {
+  constexpr int BM = WM * MB * 16, COLS = WN * NT * 16 / (GLU ? 2 : 1);
+  const dim3 grid(uint32_t((p.rows + BM - 1) / BM * ((p.n + COLS - 1) / COLS)), parts);
+  hipLaunchKernelGGL((many_kernel<WM, WN, MB, NT, STAGES, MX, GLU, SPLIT>), grid, dim3(64 * WM * WN), 0, stream, p);
+}
+
+template <bool MX, bool GLU, bool SPLIT>
+void run_form(const LinearParams& p, int form, int parts, hipStream_t stream) {
+  if constexpr (MX) {
+    if (SPLIT || form == 0) run<2, 2, 4, 4, 4, true, GLU, SPLIT>(p, parts, stream);
+    else run<2, 4, 8, 4, 3, true, GLU, false>(p, 1, stream);
+  } else {
+    if (form == 0) run<1, 4, 2, 2, 4, false, GLU, SPLIT>(p, parts, stream);
+    else if (form == 1) run<2, 4, 2, 2, 4, false, GLU, SPLIT>(p, parts, stream);
+    else if (form == 2) run<1, 4, 5, 2, 4, false, GLU, SPLIT>(p, parts, stream);
+    else if (SPLIT || form == 3) run<2, 4, 4, 2, 3, false, GLU, SPLIT>(p, parts, stream);
+    else run<2, 4, 4, 4, 3, false, GLU, false>(p, 1, stream);
+  }
+}
+
 template <bool MX, bool GLU>
-void launch(const LinearParams& p, hipStream_t stream) {
-  const int cols = 128 / (GLU ? 2 : 1);
-  const dim3 grid((p.n + cols - 1) / cols, uint32_t((p.rows + 127) / 128));
-  hipLaunchKernelGGL((many_kernel<2, 2, 4, 4, MX, GLU>), grid, dim3(256), 0, stream, p);
+void launch(const LinearParams& p, const Choice& c, hipStream_t stream) {
+  LinearParams q = p;
+  q.split_slabs = c.split_slabs;
+  if (c.parts == 1) {
+    run_form<MX, GLU, false>(q, c.form, 1, stream);
+    return;
+  }
+  run_form<MX, GLU, true>(q, c.form, c.parts, stream);
+  const int64_t fours = p.rows * ((p.n + 3) / 4);
+  hipLaunchKernelGGL((combine_kernel<GLU>), dim3(uint32_t((fours + 255) / 256)), dim3(256), 0, stream, q, c.parts);
+}
+
+// The rows behind the last whole block of 128, where they are few enough for the
+// few-row kernel.
+int64_t rest_of(bool mx, int64_t rows) {
+  const int64_t rest = rows % (mx ? 256 : 128);
+  return rest <= (mx ? 64 : 16) && rest < rows ? rest : 0;
 }
 
 }  // namespace
 
-void launch_many(const LinearParams& p, bool glu, hipStream_t stream) {
-  if (p.xs) glu ? launch<true, true>(p, stream) : launch<true, false>(p, stream);
-  else glu ? launch<false, true>(p, stream) : launch<false, false>(p, stream);
+size_t many_workspace(bool mx, bool glu, int64_t rows, int64_t n, int slabs) {
+  return choose(mx, glu, rows, n, slabs, size_t(1) << 28).bytes;
+}
+
+void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t stream) {
+  const bool mx = p.xs != nullptr;
+  LinearParams q = p;
+  Choice c = choose(mx, glu, p.rows, p.n, p.slabs, room);
+  // (4,105 x 4,096 x 6,144: 792 blocks are four rounds; 768 and nine rows of the few-row
+  // kernel three and 7 us)
+  if (const int64_t rest = rest_of(mx, p.rows)) {
+    const Choice whole = choose(mx, glu, p.rows - rest, p.n, p.slabs, room);
+    if (whole.us + few_us(p) < c.us) {
+      c = whole;
+      q.rows = p.rows - rest;
+    }
+  }
+  if (mx) glu ? launch<true, true>(q, c, stream) : launch<true, false>(q, c, stream);
+  else glu ? launch<false, true>(q, c, stream) : launch<false, false>(q, c, stream);
+  if (q.rows == p.rows) return;
+  LinearParams rest = p;
+  rest.rows = p.rows - q.rows;
+  rest.x += mx ? q.rows / kTileRows * p.slabs * kTileBytes : q.rows * p.x_stride * 2;
+  if (mx) rest.xs += q.rows / kTileRows * p.quads * kQuadBytes;
+  rest.out += q.rows * p.o_stride;
+  launch_few(rest, glu, stream);
 }
 
 }  // namespace mi::mx4
 
+extern "C" size_t mi_linear_mxfp4_workspace_size(int64_t rows, int64_t n, int64_t k, int32_t silu, int32_t x_mxfp4) {
+  using namespace mi::mx4;
+  if (rows <= 0 || rows > kMaxRows || n <= 0 || n > kMaxN || k <= 0 || k % kBlock || k > kMaxK ||
+      few(x_mxfp4 != 0, rows, silu ? 2 * n : n, k))
+    return 0;
+  return many_workspace(x_mxfp4 != 0, silu != 0, rows, n, int(slabs(k)));
+}
+
 extern "C" int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_scales, const void* codes,
                                const void* scales, const void* bias, void* out, int64_t out_stride, int64_t rows,
-                               int64_t n, int64_t k, int32_t silu, mi_stream_t stream) {
+                               int64_t n, int64_t k, int32_t silu, void* workspace, size_t workspace_bytes,
+                               mi_stream_t stream) {
   using namespace mi::mx4;
   mi::clear_error();
-  constexpr int64_t kMaxRows = 1 << 22, kMaxN = 1 << 24, kMaxStride = 1 << 22;
   if (rows < 0 || rows > kMaxRows || n <= 0 || n > kMaxN || k <= 0 || k % kBlock || k > kMaxK)
     return mi::fail(MI_ERR_INVALID, "linear_mxfp4: rows %lld (0..2^22), n %lld (1..2^24), k %lld (multiple of %d, at most %d)",
                     (long long)rows, (long long)n, (long long)k, kBlock, kMaxK);
@@ -208,10 +379,11 @@ extern "C" int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_sc
   if (rows == 0) return MI_OK;
   if (!x || !codes || !scales || !out) return mi::fail(MI_ERR_INVALID, "linear_mxfp4: null pointer argument");
   const uintptr_t aligned = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(codes) |
-                            reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(x_scales);
+                            reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(x_scales) |
+                            reinterpret_cast<uintptr_t>(workspace);
   if ((aligned & 15) || ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) & 1) ||
       (!x_scales && x_stride % 8))
-    return mi::fail(MI_ERR_INVALID, "linear_mxfp4: x rows, codes and scales must be 16-byte aligned");
+    return mi::fail(MI_ERR_INVALID, "linear_mxfp4: x rows, codes, scales and workspace must be 16-byte aligned");
   if (out_stride < n || (!x_scales && (x_stride < k || x_stride > kMaxStride)))
     return mi::fail(MI_ERR_INVALID, "linear_mxfp4: row strides %lld (at most 2^22) / %lld for k %lld, n %lld",
                     (long long)x_stride, (long long)out_stride, (long long)k, (long long)n);
@@ -233,7 +405,8 @@ extern "C" int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_sc
   p.vec = n % 4 == 0 && out_stride % 4 == 0 &&
           ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) & 7) == 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (rows <= kFewRows) launch_few(p, silu != 0, s);
-  else launch_many(p, silu != 0, s);
+  p.parts = static_cast<mi::f32x4_t*>(workspace);
+  if (few(x_scales != nullptr, rows, silu ? 2 * n : n, k)) launch_few(p, silu != 0, s);
+  else launch_many(p, silu != 0, workspace ? workspace_bytes : 0, s);
   return mi::check_launch("linear_mxfp4");
 }

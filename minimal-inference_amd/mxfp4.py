@@ -15,12 +15,16 @@ pass: inputs that ask for gradients are refused.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
+from . import _lib
 from ._util import call_on, require_dtype, require_gpu
 
 BLOCK = 32
 _TILE_ROWS, _SLAB, _TILE_BYTES, _QUAD_BYTES = 16, 128, 1024, 256
+_FEW_ROWS = 16  # no call of up to so many rows takes a workspace
 
 
 def _rows_of(name: str, t: torch.Tensor) -> tuple[int, int]:
@@ -144,10 +148,18 @@ def _linear(x, weight: MXFP4, bias, out, silu: bool) -> torch.Tensor:
             raise ValueError(f"bias must be a contiguous [{n}] tensor on {like.device}")
     out = _out(out, rows, n, like)
     if rows and n:
+        room = _workspace_size(rows, n, k, silu, scales is not None) if rows > _FEW_ROWS else 0
+        # (a tensor of this call's own: calls on several streams and in graphs share nothing)
+        workspace = torch.empty(room, dtype=torch.uint8, device=like.device) if room else None
         call_on(like, "mi_linear_mxfp4", data, stride, scales, weight.codes.data_ptr(), weight.scales.data_ptr(),
                 bias.data_ptr() if bias is not None else None, out.data_ptr(), out.stride(0), rows, n, k,
-                1 if silu else 0)
+                1 if silu else 0, workspace.data_ptr() if room else None, room)
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_size(rows: int, n: int, k: int, silu: bool, x_mxfp4: bool) -> int:
+    return int(_lib.load().mi_linear_mxfp4_workspace_size(rows, n, k, silu, x_mxfp4))
 
 
 def linear_mxfp4(x: torch.Tensor | MXFP4, weight: MXFP4, bias: torch.Tensor | None = None,

@@ -32,11 +32,12 @@ def test_sizes():
     {"rows": -1}, {"rows": (1 << 22) + 1}, {"n": 0}, {"n": (1 << 24) + 1}, {"k": 48}, {"k": 0}, {"k": (1 << 20) + 32},
     {"x": None}, {"codes": None}, {"scales": None}, {"out": None}, {"x": FAKE + 8}, {"codes": FAKE + 8},
     {"scales": FAKE + 8}, {"out": FAKE + 1}, {"bias": FAKE + 1}, {"x_stride": 56}, {"x_stride": 68},
-    {"x_stride": (1 << 22) + 8}, {"out_stride": 31}, {"silu": 1, "bias": FAKE}, {"x_scales": FAKE + 4}])
+    {"x_stride": (1 << 22) + 8}, {"out_stride": 31}, {"silu": 1, "bias": FAKE}, {"x_scales": FAKE + 4},
+    {"ws": FAKE + 8, "ws_bytes": 1 << 20}])
 def test_linear_mxfp4_refuses(change):
     mod, lib = _lib()
     a = dict(x=FAKE, x_stride=64, x_scales=None, codes=FAKE, scales=FAKE, bias=None, out=FAKE, out_stride=32, rows=4,
-             n=32, k=64, silu=0) | change
+             n=32, k=64, silu=0, ws=None, ws_bytes=0) | change
     assert lib.mi_linear_mxfp4(*a.values(), None) == mod.MI_ERR_INVALID
     assert mod.last_error().startswith("linear_mxfp4")
 
