@@ -21,7 +21,13 @@
 // other values outside the counted range takes the draw kernel's second path, which
 // finds the same boundary by bisection over the 2^16 values, a pass over the row each.
 //
-// Bound: 48 rows x 152,064: the count launch's LDS atomics and the draw launch's chain.
+// Bound: latency.  48 rows x 152,064 (us): count 8.6, of which the LDS atomics take 3.5 (16
+// cycles a wave's, at any spread of values) and the arithmetic of a token's bin as much
+// beside them; draw 21, a chain on one CU per row: 3 until the row's counts are there,
+// 2 for the powers and sums, 1.4 for the boundary, 1 for the chunks' masses, 5 for 32,768
+// tokens' weights out of LDS, 1.5 to the token.  One row of 32,768: 3.9 and 10.
+// (In the first form every thread had a contiguous run of bins, sums went through LDS
+// shuffles and all waves searched alike: 13 + 45, one row 11 + 23.)
 #include <math.h>
 
 #include "mi_common.h"
@@ -29,41 +35,41 @@
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kChunk = 32768;                  // tokens of a workgroup of the count launch
-constexpr int kPerThread = kChunk / kThreads;  // contiguous tokens of a thread
-constexpr int kMaxVocab = 1 << 20, kMaxChunks = kMaxVocab / kChunk, kMaxRows = 65535;
+constexpr int kMaxVocab = 1 << 20, kMaxRows = 65535;
+constexpr int kMaxChunks = 32;
 constexpr int kLoField = 127 - 30, kHiField = 127 + 8;  // exponent fields [2^-30, 2^8)
 constexpr int kSide = (kHiField - kLoField) * 128;      // values of one sign
 constexpr int kZeroBin = kSide;
-constexpr int kPerBinThread = 10;
-constexpr int kBins = kThreads * kPerBinThread;  // bins in descending order of value; the last few unused
-static_assert(2 * kSide + 1 <= kBins, "bins");
-constexpr int kOut = -1;
+constexpr int kPairs = 5;  // pairs of bins per thread of the draw kernel
+constexpr int kBins = kThreads * kPairs * 2;  // in descending order of value; the last few unused
+constexpr int kGroups = kBins / 128;          // a wave's share of one pair per thread
+constexpr int kSpareBin = kBins - 64;
+static_assert(2 * kSide + 1 <= kSpareBin && kSpareBin % 2 == 0, "bins");
 // what a chunk holds outside the bins
 constexpr uint32_t kTinyOrHigh = 1, kLow = 2;
-constexpr uint32_t kMinusInf = 0x007F;  // its key
+// Order-preserving keys: 0x8000 + the magnitude's bits with the sign; NaN 0 (never
+// drawn) or, in greedy rows, 0xffff (above +inf).
+constexpr uint32_t kMinusInf = 0x8000 - 0x7f80;
 
-// Order-preserving key of a bf16 value, -0 as +0; a NaN gets `nan`.
 __device__ __forceinline__ uint32_t key_of(uint32_t b, uint32_t nan) {
-  if ((b & 0x7fffu) > 0x7f80u) return nan;
-  if (b == 0x8000u) b = 0;
-  return (b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u);
+  const uint32_t mag = b & 0x7fffu;
+  return mag > 0x7f80u ? nan : (b & 0x8000u) ? 0x8000u - mag : 0x8000u + mag;
 }
 __device__ __forceinline__ double value_of_key(uint32_t k) {
-  const uint32_t b = (k & 0x8000u) ? (k & 0x7fffu) : (~k & 0xffffu);
+  const uint32_t b = k >= 0x8000u ? k - 0x8000u : 0x8000u | (0x8000u - k);
   return double(__uint_as_float(b << 16));
 }
+// A value's bin; as an unsigned number over all of them for values outside.
 __device__ __forceinline__ int bin_of(uint32_t b) {
-  const uint32_t mag = b & 0x7fffu;
-  if (mag == 0) return kZeroBin;
-  const int off = int(mag) - kLoField * 128;
-  if (off < 0 || off >= kSide) return kOut;
-  return (b & 0x8000u) ? kZeroBin + 1 + off : kZeroBin - 1 - off;
+  const int mag = int(b & 0x7fffu);
+  const int off = mag ? mag - (kLoField * 128 - 1) : 0;  // 1 .. kSide
+  if (unsigned(off) > unsigned(kSide) || (off == 0 && mag)) return -1;
+  return (b & 0x8000u) ? kZeroBin + off : kZeroBin - off;
 }
-__device__ __forceinline__ uint32_t bits_of_bin(int bin) {
-  if (bin == kZeroBin) return 0;
-  return bin < kZeroBin ? uint32_t(kZeroBin - 1 - bin + kLoField * 128)
-                        : 0x8000u | uint32_t(bin - kZeroBin - 1 + kLoField * 128);
+__device__ __forceinline__ uint32_t key_of_bin(int bin) {
+  if (bin == kZeroBin) return 0x8000u;
+  const int mag = (bin < kZeroBin ? kZeroBin - bin : bin - kZeroBin) + kLoField * 128 - 1;
+  return uint32_t(bin < kZeroBin ? 0x8000 + mag : 0x8000 - mag);
 }
 
 struct DrawParams {
@@ -81,105 +87,248 @@ struct DrawParams {
   uint32_t* outside;           // [row][chunk]
 };
 
-// Eight tokens from `at` on; past the end: NaN bits, which weigh nothing.
-__device__ __forceinline__ void load8(const uint16_t* row, int at, int vocab, uint32_t (&b)[8]) {
+constexpr uint32_t kPad = 0x7fff7fffu;
+// Eight tokens from `at` on, packed; past the end: NaN bits, which weigh nothing.
+__device__ __forceinline__ uint4 load8(const uint16_t* row, int at, int vocab) {
+  uint4 v;
   if (at + 8 <= vocab) {
-    uint4 v;
     __builtin_memcpy(&v, row + at, 16);
-    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) b[2 * j] = x[j] & 0xffffu, b[2 * j + 1] = x[j] >> 16;
-    return;
+    return v;
   }
+  uint32_t x[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) b[j] = at + j < vocab ? row[at + j] : 0x7fffu;
+  for (int j = 0; j < 4; ++j)
+    x[j] = (at + 2 * j < vocab ? row[at + 2 * j] : 0x7fffu) | (at + 2 * j + 1 < vocab ? row[at + 2 * j + 1] : 0x7fffu) << 16;
+  return make_uint4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ uint32_t token(const uint4& v, int j) {
+  const uint32_t x = j < 2 ? v.x : j < 4 ? v.y : j < 6 ? v.z : v.w;
+  return j & 1 ? x >> 16 : x & 0xffffu;
 }
 
-__device__ __forceinline__ unsigned long long wave_max_u64(unsigned long long v) {
-  for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned long long)__shfl_xor((long long)v, o));
+// ---------------------------------------------------------------- wave sums
+// Every step adds the same two values in both of the lanes that exchange them, so all
+// lanes end with the same bits.
+constexpr int kRowShr = 0x110, kRowBcast15 = 0x142, kRowBcast31 = 0x143;
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ int lanes(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double lanes(double v) {
+  const long long b = __double_as_longlong(v);
+  return __longlong_as_double((long long)(uint32_t(lanes<CTRL, ROWS>(int(b)))) |
+                              (long long)(lanes<CTRL, ROWS>(int(b >> 32))) << 32);
+}
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  const long long b = __double_as_longlong(v);
+  return __longlong_as_double((long long)(uint32_t(lane_value(int(b), lane))) |
+                              (long long)(lane_value(int(b >> 32), lane)) << 32);
+}
+template <typename T>
+__device__ __forceinline__ T last_lane(T v) { return lane_value(v, 63); }
+// Inclusive prefix sum over the lanes; the last lane's is the wave's sum.
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+  v += lanes<kRowShr + 1>(v);
+  v += lanes<kRowShr + 2>(v);
+  v += lanes<kRowShr + 4>(v);
+  v += lanes<kRowShr + 8>(v);
+  v += lanes<kRowBcast15, 0xa>(v);
+  v += lanes<kRowBcast31, 0xc>(v);
   return v;
 }
-__device__ __forceinline__ double wave_sum_f64(double v) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+template <typename T>
+__device__ __forceinline__ T wave_sum(T v) { return last_lane(wave_scan(v)); }
+
+// Four sums at once: lane l gets that of value l % 4.
+constexpr int kRowRor = 0x120;
+__device__ __forceinline__ double wave_sum4(double a, double b, double c, double d) {
+  const bool one = threadIdx.x & 1, two = threadIdx.x & 2;
+  const double ab = (one ? b : a) + lanes<mi::kDppQuadSwap1>(one ? a : b);
+  const double cd = (one ? d : c) + lanes<mi::kDppQuadSwap1>(one ? c : d);
+  double v = (two ? cd : ab) + lanes<mi::kDppQuadSwap2>(two ? ab : cd);
+  v += lanes<kRowRor + 4>(v);
+  v += lanes<kRowRor + 8>(v);
+  v += __shfl_xor(v, 16);
+  v += __shfl_xor(v, 32);
   return v;
 }
 
-__global__ __launch_bounds__(kThreads) void count_kernel(DrawParams p) {
-  __shared__ uint32_t hist[kBins];
-  __shared__ unsigned long long best[kWaves];
-  __shared__ uint32_t outside;
-  const int tid = threadIdx.x, chunk = blockIdx.x;
-  const int64_t row = blockIdx.y;
-  const bool greedy = !(p.temperature[row] > 0.f);
-  const uint16_t* logits = p.logits + row * p.stride;
-  const int base = chunk * kChunk;
-  if (!greedy)
-    for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
-  if (tid == 0) outside = 0;
-  __syncthreads();
-  unsigned long long top = 0;
-  uint32_t seen = 0;
-#pragma unroll
-  for (int i = 0; i < kPerThread / 8; ++i) {
-    const int at = base + (i * kThreads + tid) * 8;
-    if (at >= p.vocab) break;
-    uint32_t b[8];
-    load8(logits, at, p.vocab, b);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (at + j >= p.vocab) break;
-      // greedy: a NaN ranks highest, as in argmax; a draw never takes one
-      const unsigned long long k = key_of(b[j], greedy ? 0x10000u : 0u);
-      top = max(top, k << 32 | (0xffffffffu - uint32_t(at + j)));
-      if (greedy || k == 0) continue;
-      const int bin = bin_of(b[j]);
-      if (bin >= 0) atomicAdd(&hist[bin], 1u);
-      else if (k != kMinusInf) seen |= (b[j] & 0x8000u) && (b[j] & 0x7fffu) >= kHiField * 128u ? kLow : kTinyOrHigh;
-    }
-  }
-  top = wave_max_u64(top);
-  if ((tid & 63) == 0) best[tid >> 6] = top;
-  if (seen) atomicOr(&outside, seen);
-  __syncthreads();
-  const int64_t slot = row * p.chunks + chunk;
-  if (tid == 0) {
-    for (int w = 1; w < kWaves; ++w) top = max(top, best[w]);
-    p.winner[slot] = top;
-    p.outside[slot] = outside;
-  }
-  if (greedy) return;
-  uint32_t* counts = p.counts + slot * (kBins / 2);
-  for (int i = tid; i < kBins / 2; i += kThreads) counts[i] = hist[2 * i] | hist[2 * i + 1] << 16;
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  for (int o = 32; o > 0; o >>= 1) v = max(v, uint32_t(__shfl_xor(int(v), o)));
+  return v;
 }
-
-// Block-wide sums in a fixed order.  `red` holds one value per wave; every thread
-// gets the result.
+// Sum over the workgroup in wave order; every thread gets it.
 template <typename T>
 __device__ __forceinline__ T block_sum(T v, T* red) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  v = wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   T sum = red[0];
+#pragma unroll
   for (int w = 1; w < kWaves; ++w) sum += red[w];
   return sum;
 }
-// Exclusive prefix sum over the threads.
-template <typename T>
-__device__ __forceinline__ T block_prefix(T v, T* red) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T inc = v;
-  for (int o = 1; o < 64; o <<= 1) {
-    const T up = __shfl_up(inc, o);
-    if (lane >= o) inc += up;
+
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
+typedef __attribute__((ext_vector_type(2))) short s16x2_t;
+// The keys (without the NaN rule) of a pair of tokens.
+__device__ __forceinline__ u16x2_t key_pair(uint32_t x) {
+  const s16x2_t sign = __builtin_bit_cast(s16x2_t, x) >> 15;
+  const s16x2_t mag = __builtin_bit_cast(s16x2_t, x & 0x7fff7fffu);
+  return __builtin_bit_cast(u16x2_t, (mag ^ sign) - sign) + (unsigned short)0x8000;
+}
+
+// G groups of eight tokens per thread, 8,192 G tokens per workgroup.
+template <int G>
+__global__ __launch_bounds__(kThreads) void count_kernel(DrawParams p) {
+  constexpr int kChunk = kThreads * 8 * G;
+  __shared__ uint32_t hist[kBins];
+  __shared__ uint32_t best[kWaves];
+  __shared__ uint32_t outside;
+  __shared__ int first;
+  const int tid = threadIdx.x, chunk = blockIdx.x;
+  const int64_t row = blockIdx.y;
+  const uint16_t* logits = p.logits + row * p.stride;
+  const int base = chunk * kChunk;
+  uint32_t v[4 * G];
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    const int at = base + (i * kThreads + tid) * 8;
+    const uint4 x = at < p.vocab ? load8(logits, at, p.vocab) : make_uint4(kPad, kPad, kPad, kPad);
+    v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+  }
+  const bool greedy = !(p.temperature[row] > 0.f);
+#pragma unroll
+  for (int i = 0; i < kBins / kThreads; ++i) hist[i * kThreads + tid] = 0;
+  if (tid == 0) outside = 0, first = 0;
+  __syncthreads();
+  // the largest key (NaN 0, or highest where the row is greedy), and the counts
+  auto place = [&](int i, int h) { return ((i >> 2) * kThreads + tid) * 8 + (i & 3) * 2 + h; };
+  // Without a branch per token (with one it took twice as long): a value outside the
+  // bins counts in an unused one of its lane's own, since all of a wave's on one, as
+  // masked tokens are, would queue.
+  const uint32_t spare = uint32_t(kSpareBin + (tid & 63));
+  u16x2_t mags = {0, 0}, keys = {0, 0};
+  bool other = false;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    if (base + (g * kThreads + tid) * 8 >= p.vocab) break;
+#pragma unroll
+    for (int i = 4 * g; i < 4 * g + 4; ++i) {
+      mags = __builtin_elementwise_max(mags, __builtin_bit_cast(u16x2_t, v[i] & 0x7fff7fffu));
+      keys = __builtin_elementwise_max(keys, key_pair(v[i]));
+    }
+    if (greedy) continue;
+#pragma unroll
+    for (int i = 4 * g; i < 4 * g + 4; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t mag = h ? v[i] >> 16 & 0x7fffu : v[i] & 0x7fffu;
+        const bool negative = h ? int(v[i]) < 0 : (v[i] & 0x8000u) != 0;
+        const uint32_t above = kZeroBin + (kLoField * 128 - 1) - mag, below = kZeroBin - (kLoField * 128 - 1) + mag;
+        const bool in = mag - kLoField * 128 < unsigned(kSide);
+        uint32_t bin = negative ? below : above;
+        bin = in ? bin : spare;
+        bin = mag ? bin : uint32_t(kZeroBin);
+        other |= bin == spare;
+        atomicAdd(&hist[bin], 1u);
+      }
+  }
+  uint32_t top = max(uint32_t(keys.x), uint32_t(keys.y));
+  const bool nan_here = max(uint32_t(mags.x), uint32_t(mags.y)) > 0x7f80u;
+  const uint32_t nan = greedy ? 0xffffu : 0u;
+  auto key_at = [&](int i, int h) -> uint32_t {
+    const int local = place(i, h);
+    return base + local < p.vocab ? key_of(h ? v[i] >> 16 : v[i] & 0xffffu, nan) : 0u;
+  };
+  if (nan_here) {
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < 4 * G; ++i) top = max(top, max(key_at(i, 0), key_at(i, 1)));
+  }
+  const uint32_t mine = top;
+  top = wave_max(top);
+  if ((tid & 63) == 0) best[tid >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) top = max(top, best[w]);
+  const int64_t slot = row * p.chunks + chunk;
+  if (mine == top) {
+    int at = 0;  // 0x10000 - the first place
+    if (nan_here) {
+#pragma unroll
+      for (int i = 4 * G - 1; i >= 0; --i)
+#pragma unroll
+        for (int h = 1; h >= 0; --h)
+          if (key_at(i, h) == top && base + place(i, h) < p.vocab) at = 0x10000 - place(i, h);
+    } else {
+#pragma unroll
+      for (int i = 4 * G - 1; i >= 0; --i) {
+        const u16x2_t k = key_pair(v[i]);
+        if (k.y == top) at = 0x10000 - place(i, 1);
+        if (k.x == top) at = 0x10000 - place(i, 0);
+      }
+    }
+    if (at) atomicMax(&first, at);
+  }
+  if (other) {
+    uint32_t seen = 0;
+#pragma unroll
+    for (int i = 0; i < 4 * G; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t b = h ? v[i] >> 16 : v[i] & 0xffffu, key = key_of(b, 0);
+        if (key > kMinusInf && bin_of(b) < 0)
+          seen |= key < 0x8000u && (b & 0x7fffu) >= kHiField * 128u ? kLow : kTinyOrHigh;
+      }
+    if (seen) atomicOr(&outside, seen);
   }
   __syncthreads();
-  if (lane == 63) red[wave] = inc;
-  __syncthreads();
-  T before = 0;
-  for (int w = 0; w < wave; ++w) before += red[w];
-  T left = __shfl_up(inc, 1);
-  return before + (lane ? left : T(0));
+  if (tid == 0) {
+    p.winner[slot] = (unsigned long long)top << 32 | (0xffffffffu - uint32_t(base + 0x10000 - first));
+    p.outside[slot] = outside;
+  }
+  if (greedy) return;
+  uint32_t* counts = p.counts + slot * (kBins / 2);
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    const int d = i * kThreads + tid;
+    uint2 c = *reinterpret_cast<const uint2*>(&hist[2 * d]);
+    if (2 * d >= kSpareBin) c = make_uint2(0u, 0u);
+    counts[d] = c.x | c.y << 16;
+  }
+}
+
+// 2^y for y <= 0 (y below -1,100 counts as that: 0) to some 2^-52 relative: the whole
+// part by the exponent, 2^f for |f| <= 1/2 by the exponential series in f ln 2, whose
+// first term left out is 2e-16 at most.
+struct Series {
+  double c[13];
+  constexpr Series() : c() {
+    double term = 1.0;
+    for (int k = 0; k < 13; ++k) {
+      c[k] = term;
+      term *= 0.693147180559945309417232121458 / (k + 1);
+    }
+  }
+};
+__device__ constexpr Series kSeries;
+__device__ __forceinline__ double exp2_f64(double y) {
+  y = fmax(y, -1100.0);
+  const double n = rint(y), f = y - n;
+  double v = kSeries.c[12];
+#pragma unroll
+  for (int k = 11; k >= 0; --k) v = fma(v, f, kSeries.c[k]);
+  return ldexp(v, int(n));
+}
+
+// A whole number below 2^32 in 64 bits (the conversion takes four times an addition).
+__device__ __forceinline__ double whole(uint32_t n) {
+  return __longlong_as_double(0x4330000000000000ll | n) - 0x1p52;
 }
 
 // How many of `most` tokens of weight w, the first of them behind the mass `before`,
@@ -190,290 +339,471 @@ __device__ __forceinline__ int reach(double before, double w, double target, int
   return m < double(most) ? max(int(m), 1) : most;  // (w = 0 gives infinity: all)
 }
 
+struct Place {
+  int bin, kept;  // the last bin, and how many of its tokens
+  int count_before;  // tokens, and
+  double before;     // mass, of the bins ahead of it
+};
+
+struct Shared {
+  Place last;
+  double total;
+  double weight[kBins];
+  uint32_t count[kBins];  // of tokens that min_p keeps
+  double group_mass[kGroups];
+  int group_count[kGroups];
+  double mass[kMaxChunks][kWaves];
+  double chunk_mass[kMaxChunks];
+  int chunk_ties[kMaxChunks];
+  double redd[kWaves];
+  int redi[kWaves];
+};
+
+// The first bin at which `reached` holds of the (count, mass) of all bins up to and
+// with it -- else the last of the `bins_end` bins that holds a token -- by groups and
+// then by pairs, in every wave alike.
+template <typename F>
+__device__ __forceinline__ Place find_bin(const Shared& s, int bins_end, F reached) {
+  const int lane = threadIdx.x & 63;
+  int group = 0, count_before = 0, count_ahead = 0;  // ahead: of the group
+  double mass_before = 0.0, mass_ahead = 0.0;
+#pragma unroll
+  for (int part = 0; part < (kGroups + 63) / 64; ++part) {
+    const int g = part * 64 + lane;
+    const bool in = g < kGroups && 128 * g < bins_end;
+    const int c = in ? s.group_count[g] : 0;
+    const int ci = count_before + wave_scan(c);
+    const double mi = mass_before + wave_scan(in ? s.group_mass[g] : 0.0);
+    const unsigned long long hit = __ballot(c && reached(ci, mi)), any = __ballot(c != 0);
+    if (any) {
+      const int at = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
+      group = part * 64 + at;
+      count_ahead = at ? __builtin_amdgcn_readlane(ci, at - 1) : count_before;
+      mass_ahead = at ? lane_value(mi, at - 1) : mass_before;
+    }
+    if (hit) break;
+    count_before = last_lane(ci);
+    mass_before = last_lane(mi);
+  }
+  const int bin = 128 * group + 2 * lane;
+  const int c0 = bin < bins_end ? int(s.count[bin]) : 0, c1 = bin + 1 < bins_end ? int(s.count[bin + 1]) : 0;
+  const double m0 = c0 * s.weight[bin], m1 = c1 * s.weight[bin + 1];
+  const int ci = count_ahead + wave_scan(c0 + c1);
+  const double mi = mass_ahead + wave_scan(m0 + m1);
+  const bool hit0 = c0 && reached(ci - c1, mi - m1), hit1 = c1 && reached(ci, mi);
+  const unsigned long long hit = __ballot(hit0 || hit1), any = __ballot(c0 || c1);
+  const int at = hit ? __builtin_ctzll(hit) : any ? 63 - __builtin_clzll(any) : 0;
+  const bool second = hit ? !hit0 : c1 != 0;
+  Place r;
+  r.bin = __builtin_amdgcn_readlane(bin + (second ? 1 : 0), at);
+  r.kept = __builtin_amdgcn_readlane(second ? c1 : c0, at);
+  r.count_before = __builtin_amdgcn_readlane(second ? ci - c1 : ci - c1 - c0, at);
+  r.before = lane_value(second ? mi - m1 : mi - m1 - m0, at);
+  return r;
+}
+
+// A row's maximum and parameters.
+struct Row {
+  const uint16_t* logits;
+  int vocab, top_k;
+  uint32_t kmax;
+  double lmax, per_t, top_p, min_p, u;  // per_t: log2 e / temperature
+  __device__ __forceinline__ double weigh(uint32_t key) const {
+    if (key == kmax) return 1.0;
+    if (key <= kMinusInf || lmax == INFINITY) return 0.0;
+    return exp2_f64((value_of_key(key) - lmax) * per_t);
+  }
+};
+
+// (count, mass) of the row's tokens with key >= k, in a fixed order.
+__device__ __noinline__ void tokens_from(const Row& r, Shared& s, uint32_t k, int* n, double* m) {
+  int c = 0;
+  double sum = 0.0;
+#pragma unroll 1
+  for (int at = threadIdx.x; at < r.vocab; at += kThreads) {
+    const uint32_t key = key_of(r.logits[at], 0);
+    if (key >= k) ++c, sum += r.weigh(key);
+  }
+  *n = block_sum(c, s.redi);
+  *m = block_sum(sum, s.redd);
+}
+
+// The draw of a row with values outside the bins: the boundary by bisection over the
+// keys, then the token by a pass over the row, kThreads tokens at a time.
+__device__ __noinline__ int draw_outside(const Row& r, Shared& s) {
+  // the least key above minus infinity that min_p keeps
+  uint32_t lo = kMinusInf, hi = r.kmax;  // lo fails, hi holds
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (r.weigh(mid) >= r.min_p) hi = mid;
+    else lo = mid;
+  }
+  uint32_t least = hi;
+  int n;
+  double m;
+  tokens_from(r, s, least, &n, &m);
+  int most = 0x7fffffff;  // tokens with key `least` that are kept
+  if (n > r.top_k) {      // the largest key from which on there are top_k
+    lo = least, hi = r.kmax + 1;  // lo has them, hi has not
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      tokens_from(r, s, mid, &n, &m);
+      if (n >= r.top_k) lo = mid;
+      else hi = mid;
+    }
+    least = lo;
+    tokens_from(r, s, least + 1, &n, &m);
+    most = r.top_k - n;
+    m += most * r.weigh(least);
+  }
+  if (r.top_p < 1.0) {
+    const double target = r.top_p * m;
+    lo = least, hi = r.kmax + 1;  // lo reaches the target, hi does not
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      tokens_from(r, s, mid, &n, &m);
+      if (m >= target) lo = mid;
+      else hi = mid;
+    }
+    int above;
+    double before;
+    tokens_from(r, s, lo + 1, &above, &before);
+    tokens_from(r, s, lo, &n, &m);
+    most = min(lo == least ? most : 0x7fffffff, n - above);
+    most = max(reach(before, r.weigh(lo), target, most), lo == r.kmax ? 1 : 0);
+    least = lo;
+  }
+  int above;
+  double total;
+  tokens_from(r, s, least + 1, &above, &total);
+  tokens_from(r, s, least, &n, &m);
+  int room = min(most, n - above);
+  total += room * r.weigh(least);
+  const double target = r.u * total;
+  // the first token that takes the sum over the target, or the last with a weight
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  double sum = 0.0;
+  int drawn = 0;
+#pragma unroll 1
+  for (int base = 0; base < r.vocab; base += kThreads) {
+    const int at = base + tid;
+    const uint32_t key = at < r.vocab ? key_of(r.logits[at], 0) : 0u;
+    const int rank = wave_scan(int(key == least));
+    __syncthreads();
+    if (lane == 63) s.redi[wave] = rank;
+    __syncthreads();
+    int ahead = 0, ties = 0;
+#pragma unroll 1
+    for (int w = 0; w < kWaves; ++w) {
+      ahead += w < wave ? s.redi[w] : 0;
+      ties += s.redi[w];
+    }
+    const double w0 = key > least || (key == least && ahead + rank <= room) ? r.weigh(key) : 0.0;
+    const double run = wave_scan(w0);
+    const unsigned long long any = __ballot(w0 > 0.0);
+    if (lane == 63) s.redd[wave] = run;
+    __syncthreads();
+    double before = sum;
+#pragma unroll 1
+    for (int w = 0; w < wave; ++w) before += s.redd[w];
+    const unsigned long long over = __ballot(w0 > 0.0 && before + run > target);
+    if (lane == 0) s.redi[wave] = over ? __builtin_ctzll(over) : any ? 64 + 63 - __builtin_clzll(any) : -1;
+    __syncthreads();
+    bool found = false;
+#pragma unroll 1
+    for (int w = 0; w < kWaves && !found; ++w) {
+      const int in = s.redi[w];
+      if (in >= 0) drawn = base + 64 * w + (in & 63);
+      found = in >= 0 && in < 64;
+      sum += s.redd[w];
+    }
+    if (found) break;
+    room -= min(ties, room);
+  }
+  return drawn;
+}
+
+template <int G>
 __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
-  __shared__ double weight[kBins];
-  __shared__ double mass[kMaxChunks][kWaves];
-  __shared__ double redd[kWaves];
-  __shared__ int redi[kWaves];
-  __shared__ unsigned long long last;  // last kept bin << 32 | how many of its tokens
-  __shared__ int drawn, final_kept;
+  constexpr int kChunk = kThreads * 8 * G;
+  __shared__ __attribute__((aligned(16))) Shared s;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x;
-  const uint16_t* logits = p.logits + row * p.stride;
-  const float tf = p.temperature[row];
-  const bool greedy = !(tf > 0.f);
+  const uint32_t* row_counts = p.counts + row * p.chunks * (kBins / 2) + tid;
 
+  // (all of the row's parameters and counts are asked for before any is used)
+  const float tf = p.temperature[row], uf = p.u[row];
+  const int kf = p.top_k ? p.top_k[row] : 0;
+  const float pf = p.top_p ? p.top_p[row] : 1.f, mf = p.min_p ? p.min_p[row] : 0.f;
   unsigned long long top = 0;
   uint32_t outside = 0;
-  for (int c = 0; c < p.chunks; ++c) {
-    top = max(top, p.winner[row * p.chunks + c]);
-    outside |= p.outside[row * p.chunks + c];
+  if (lane < p.chunks) {
+    top = p.winner[row * p.chunks + lane];
+    outside = p.outside[row * p.chunks + lane];
   }
-  const uint32_t kmax = uint32_t(top >> 32);
-  if (greedy || kmax <= kMinusInf) {  // nothing has a weight: the row's argmax
+  constexpr int kTogether = 5;  // chunks whose counts are loaded at once
+  uint32_t counts[kTogether][kPairs];
+  auto load_counts = [&](int c0) {
+#pragma unroll
+    for (int q = 0; q < kTogether; ++q)
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j)
+        counts[q][j] = c0 + q < p.chunks ? row_counts[(c0 + q) * (kBins / 2) + j * kThreads] : 0u;
+  };
+  load_counts(0);
+  for (int o = 1; o < p.chunks; o <<= 1) {
+    top = max(top, (unsigned long long)__shfl_xor((long long)top, o));
+    outside |= uint32_t(__shfl_xor(int(outside), o));
+  }
+  top = (unsigned long long)__builtin_amdgcn_readfirstlane(int(top >> 32)) << 32 |
+        uint32_t(__builtin_amdgcn_readfirstlane(int(top)));
+  outside = uint32_t(__builtin_amdgcn_readfirstlane(int(outside)));
+  const bool greedy = !(tf > 0.f);
+  Row r;
+  r.kmax = uint32_t(top >> 32);
+  if (greedy || r.kmax <= kMinusInf) {  // nothing has a weight: the row's argmax
     if (tid == 0) p.out[row] = int64_t(0xffffffffu - uint32_t(top));
     return;
   }
-  const double t = double(tf), lmax = value_of_key(kmax);
-  auto weigh = [&](uint32_t key) -> double {
-    if (key == kmax) return 1.0;
-    if (key <= kMinusInf || lmax == INFINITY) return 0.0;
-    return exp((value_of_key(key) - lmax) / t);
-  };
-  const int top_k = p.top_k && p.top_k[row] > 0 ? p.top_k[row] : 0x7fffffff;
-  const double top_p = p.top_p && p.top_p[row] < 1.f ? double(p.top_p[row]) : 2.0;
-  const double min_p = p.min_p && p.min_p[row] > 0.f ? fmin(double(p.min_p[row]), 1.0) : 0.0;
-  const double u = double(p.u[row]);
-  const bool low_matters = (outside & kLow) && (-256.0 - lmax) / t > -45.0;
-  const bool fast = !(outside & kTinyOrHigh) && !low_matters;
-  if (tid == 0) last = 0, drawn = 0x7fffffff, final_kept = -1;
-  __syncthreads();
+  r.logits = p.logits + row * p.stride;
+  r.vocab = p.vocab;
+  r.per_t = 1.4426950408889634073599 / double(tf);
+  r.lmax = value_of_key(r.kmax);
+  r.top_k = kf > 0 ? kf : 0x7fffffff;
+  r.top_p = pf < 1.f ? double(pf) : 2.0;
+  r.min_p = mf > 0.f ? fmin(double(mf), 1.0) : 0.0;
+  r.u = fmax(double(uf), 0.0);
+  const bool low_matters = (outside & kLow) && (-256.0 - r.lmax) * r.per_t > -64.0;
+  if ((outside & kTinyOrHigh) || low_matters) {
+    const Row copy = r;  // (r itself stays in registers)
+    const int drawn = draw_outside(copy, s);
+    if (tid == 0) p.out[row] = drawn;
+    return;
+  }
 
-  uint32_t key_last;  // kept: keys above it and the first `ties` tokens with it
-  int ties;
-  double total;
-  if (fast) {
-    // this thread's bins, in descending order of value
-    int cnt[kPerBinThread] = {};
-    for (int c = 0; c < p.chunks; ++c) {
-      const uint32_t* counts = p.counts + (row * p.chunks + c) * (kBins / 2) + tid * (kPerBinThread / 2);
+  // pair d = 1,024 j + tid: this thread's bins 2 d and 2 d + 1, group 16 j + wave
+  {
+    uint2 cnt[kPairs] = {};
+    for (int c0 = 0; c0 < p.chunks; c0 += kTogether) {
+      if (c0) load_counts(c0);
 #pragma unroll
-      for (int j = 0; j < kPerBinThread / 2; ++j) {
-        cnt[2 * j] += counts[j] & 0xffffu;
-        cnt[2 * j + 1] += counts[j] >> 16;
-      }
-    }
-    double w[kPerBinThread];
-    int own = 0;
+      for (int q = 0; q < kTogether; ++q)
 #pragma unroll
-    for (int j = 0; j < kPerBinThread; ++j) {
-      const int bin = tid * kPerBinThread + j;
-      w[j] = cnt[j] ? weigh(key_of(bits_of_bin(bin), 0)) : 0.0;
-      if (w[j] < min_p) cnt[j] = 0;
-      weight[bin] = w[j];
-      own += cnt[j];
-    }
-    int before = block_prefix(own, redi);
-    double held = 0.0;
-#pragma unroll
-    for (int j = 0; j < kPerBinThread; ++j) {
-      const int all = cnt[j];
-      cnt[j] = min(all, max(top_k - before, 0));
-      before += all;
-      held += cnt[j] * w[j];
-    }
-    double mass_before = block_prefix(held, redd);
-    const double target = top_p * block_sum(held, redd);
-    held = 0.0;
-    unsigned long long mine = 0;
-#pragma unroll
-    for (int j = 0; j < kPerBinThread; ++j) {
-      const int bin = tid * kPerBinThread + j;
-      if (cnt[j]) {
-        // (the most likely token is kept whatever top_p is)
-        const int kept = top_p > 1.0 ? cnt[j] : max(reach(mass_before, w[j], target, cnt[j]),
-                                                    key_of(bits_of_bin(bin), 0) == kmax ? 1 : 0);
-        mass_before += cnt[j] * w[j];
-        held += kept * w[j];
-        if (kept) mine = (unsigned long long)bin << 32 | uint32_t(kept);
-      }
-    }
-    mine = wave_max_u64(mine);
-    if (lane == 0 && mine) atomicMax(&last, mine);
-    total = block_sum(held, redd);  // (its barriers publish `last` too)
-    const int last_bin = int(last >> 32);
-    ties = int(uint32_t(last));
-    key_last = key_of(bits_of_bin(last_bin), 0);
-    // each chunk's mass above the last kept value
-    for (int c = 0; c < p.chunks; ++c) {
-      const uint32_t* counts = p.counts + (row * p.chunks + c) * (kBins / 2) + tid * (kPerBinThread / 2);
-      double s = 0.0;
-      if (tid * kPerBinThread < last_bin) {
-#pragma unroll
-        for (int j = 0; j < kPerBinThread; ++j) {
-          const uint32_t n = counts[j / 2] >> (16 * (j & 1)) & 0xffffu;
-          if (tid * kPerBinThread + j < last_bin) s += n * w[j];
+        for (int j = 0; j < kPairs; ++j) {
+          cnt[j].x += counts[q][j] & 0xffffu;
+          cnt[j].y += counts[q][j] >> 16;
         }
-      }
-      s = wave_sum_f64(s);
-      if (lane == 0) mass[c][wave] = s;
     }
-  } else {
-    // (count, mass) of the tokens with key >= k, in a fixed order
-    auto tokens_from = [&](uint32_t k, int* n, double* m) {
-      int c = 0;
-      double s = 0.0;
-      for (int at = tid * 8; at < p.vocab; at += kThreads * 8) {
-        uint32_t b[8];
-        load8(logits, at, p.vocab, b);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t key = key_of(b[j], 0);
-          if (key >= k) ++c, s += weigh(key);
-        }
-      }
-      *n = block_sum(c, redi);
-      *m = block_sum(s, redd);
-    };
-    // the least key above minus infinity that min_p keeps
-    uint32_t lo = kMinusInf, hi = kmax;  // lo fails, hi holds
-    while (hi - lo > 1) {
-      const uint32_t mid = (lo + hi) / 2;
-      if (weigh(mid) >= min_p) hi = mid;
-      else lo = mid;
-    }
-    uint32_t least = hi;
-    int n;
-    double m;
-    tokens_from(least, &n, &m);
-    int most = 0x7fffffff;  // tokens with key `least` that are kept
-    if (n > top_k) {        // the largest key from which on there are top_k
-      lo = least, hi = kmax + 1;  // lo has them, hi has not
-      while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        tokens_from(mid, &n, &m);
-        if (n >= top_k) lo = mid;
-        else hi = mid;
-      }
-      least = lo;
-      tokens_from(least + 1, &n, &m);
-      most = top_k - n;
-      m += most * weigh(least);
-    }
-    const double target = top_p * m;
-    if (top_p < 1.0) {
-      lo = least, hi = kmax + 1;  // lo reaches the target, hi does not
-      while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        tokens_from(mid, &n, &m);
-        if (m >= target && mid > least) lo = mid;
-        else hi = mid;
-      }
-      int above;
-      double before;
-      tokens_from(lo + 1, &above, &before);
-      tokens_from(lo, &n, &m);
-      most = min(lo == least ? most : 0x7fffffff, n - above);
-      most = max(reach(before, weigh(lo), target, most), lo == kmax ? 1 : 0);
-      least = lo;
-    }
-    tokens_from(least + 1, &n, &total);
-    key_last = least;
-    int at_least;
-    tokens_from(least, &at_least, &m);
-    ties = min(most, at_least - n);
-    total += ties * weigh(least);
-    for (int c = 0; c < p.chunks; ++c) {
-      double s = 0.0;
+    for (int j = 0; j < kPairs; ++j) *reinterpret_cast<uint2*>(&s.count[2 * (j * kThreads + tid)]) = cnt[j];
+  }
 #pragma unroll 1
-      for (int i = 0; i < kPerThread / 8; ++i) {
-        const int at = c * kChunk + (i * kThreads + tid) * 8;
-        if (at >= p.vocab) break;
-        uint32_t b[8];
-        load8(logits, at, p.vocab, b);
+  for (int j = 0; j < kPairs; ++j) {
+    const int bin = 2 * (j * kThreads + tid);
+    uint2 c = *reinterpret_cast<const uint2*>(&s.count[bin]);
+    double w0 = 0.0, w1 = 0.0, m = 0.0;
+    int n = 0;
+    if (__ballot(c.x + c.y != 0)) {
+      // (a bin above the maximum is empty and its power may be infinite)
+      w0 = c.x ? r.weigh(key_of_bin(bin)) : 0.0;
+      w1 = c.y ? r.weigh(key_of_bin(bin + 1)) : 0.0;
+      if (w0 < r.min_p) c.x = 0;
+      if (w1 < r.min_p) c.y = 0;
+      *reinterpret_cast<uint2*>(&s.count[bin]) = c;
+      n = wave_sum(int(c.x + c.y));
+      m = wave_sum(whole(c.x) * w0 + whole(c.y) * w1);
+    }
+    *reinterpret_cast<double2*>(&s.weight[bin]) = make_double2(w0, w1);
+    if (lane == 0) s.group_count[j * kWaves + wave] = n, s.group_mass[j * kWaves + wave] = m;
+  }
+  __syncthreads();
+  if (wave == 0) {  // (in every wave alike it took three times as long)
+    Place at = find_bin(s, kBins, [&](int n, double) { return n >= r.top_k; });
+    at.kept = min(at.kept, r.top_k - at.count_before);
+    double all = at.before + at.kept * s.weight[at.bin];
+    if (r.top_p < 1.0) {
+      const double target = r.top_p * all;
+      const Place cut = find_bin(s, at.bin + 1, [&](int, double m) { return m >= target; });
+      // (the most likely token is kept whatever top_p is)
+      const int most = cut.bin == at.bin ? at.kept : cut.kept;
+      at.kept = max(reach(cut.before, s.weight[cut.bin], target, most), key_of_bin(cut.bin) == r.kmax ? 1 : 0);
+      at.bin = cut.bin;
+      all = cut.before + at.kept * s.weight[at.bin];
+    }
+    if (lane == 0) s.last = at, s.total = all;
+  }
+  __syncthreads();
+  // kept: the bins before last_bin and the first `ties` tokens of it
+  const int last_bin = s.last.bin, ties = s.last.kept;
+  const double target = r.u * s.total, w_last = s.weight[last_bin];
+  // each chunk's mass above the last kept value, and its tokens with it
+  for (int c0 = 0; c0 < p.chunks; c0 += kTogether) {
+    if (c0 || p.chunks > kTogether) load_counts(c0);
+    double m[kTogether] = {};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t key = key_of(b[j], 0);
-          if (key > key_last) s += weigh(key);
-        }
+    for (int j = 0; j < kPairs; ++j) {
+      const int bin = 2 * (j * kThreads + tid), group = j * kWaves + wave;
+      if (128 * group > last_bin || s.group_count[group] == 0) continue;
+      double2 w = *reinterpret_cast<const double2*>(&s.weight[bin]);
+      if (bin >= last_bin) w.x = 0.0;
+      if (bin + 1 >= last_bin) w.y = 0.0;
+#pragma unroll
+      for (int q = 0; q < kTogether; ++q) {
+        m[q] += whole(counts[q][j] & 0xffffu) * w.x + whole(counts[q][j] >> 16) * w.y;
+        if (j * kThreads + tid == last_bin / 2 && c0 + q < p.chunks)
+          s.chunk_ties[c0 + q] = int(counts[q][j] >> (16 * (last_bin & 1)) & 0xffffu);
       }
-      s = wave_sum_f64(s);
-      if (lane == 0) mass[c][wave] = s;
+    }
+    const double four = wave_sum4(m[0], m[1], m[2], m[3]);
+    if (lane < 4 && c0 + lane < p.chunks) s.mass[c0 + lane][wave] = four;
+    if (c0 + 4 < p.chunks) {
+      m[4] = wave_sum(m[4]);
+      if (lane == 0) s.mass[c0 + 4][wave] = m[4];
     }
   }
   __syncthreads();
-
-  // the chunk of the draw
-  const double w_last = weigh(key_last);
-  const double target = u * total;
-  auto tokens_at_last = [&](int c) -> int {  // tokens with the last kept key in a chunk
-    if (fast) {
-      const int bin = int(last >> 32);
-      return int(p.counts[(row * p.chunks + c) * (kBins / 2) + bin / 2] >> (16 * (bin & 1)) & 0xffffu);
-    }
-    int n = 0;
-    for (int i = 0; i < kPerThread / 8; ++i) {
-      const int at = c * kChunk + (i * kThreads + tid) * 8;
-      if (at >= p.vocab) break;
-      uint32_t b[8];
-      load8(logits, at, p.vocab, b);
+  if (tid < p.chunks) {
+    double m = 0.0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) n += key_of(b[j], 0) == key_last;
-    }
-    return block_sum(n, redi);
-  };
-  int chunk = 0, ties_left = ties;
-  double cum = 0.0;
-  int last_chunk = 0, last_ties = ties;
-  double last_cum = 0.0;
-  for (int c = 0; c < p.chunks; ++c) {
-    double s = 0.0;
-    for (int w = 0; w < kWaves; ++w) s += mass[c][w];
-    const int here = min(tokens_at_last(c), ties_left);
-    s += here * w_last;
-    chunk = c;
-    if (s > 0.0) last_chunk = c, last_ties = ties_left, last_cum = cum;
-    if (cum + s > target) break;
-    cum += s;
-    ties_left -= here;
+    for (int w = 0; w < kWaves; ++w) m += s.mass[tid][w];
+    s.chunk_mass[tid] = m;
   }
-  if (chunk != last_chunk) chunk = last_chunk, ties_left = last_ties, cum = last_cum;  // u so near 1 that no sum exceeds it
+  __syncthreads();
+  // The chunk of the draw: the first whose mass takes the sum over the target, or, with u
+  // so near 1 that none does, the last that has any.
+  int chunk = 0, room = ties, left = ties;
+  double cum = 0.0, sum = 0.0;
+  for (int c = 0; c < p.chunks; ++c) {
+    const int here = min(s.chunk_ties[c], left);
+    const double m = s.chunk_mass[c] + here * w_last;
+    if (m > 0.0) chunk = c, room = left, cum = sum;
+    if (sum + m > target) break;
+    sum += m;
+    left -= here;
+  }
 
-  const int first = chunk * kChunk + tid * kPerThread;
-  uint32_t keep = 0, tie = 0;  // of this thread's 32 tokens
-  uint32_t packed[kPerThread / 2];
+  // Its tokens once more: wave w has 512 G of them in a row, group i of a lane the
+  // eight from 512 i + 8 lane on.
+  const int first = chunk * kChunk + wave * 512 * G + lane * 8;
+  uint4 v[G];
 #pragma unroll
-  for (int i = 0; i < kPerThread / 8; ++i) {
-    uint32_t b[8] = {0x7fffu, 0x7fffu, 0x7fffu, 0x7fffu, 0x7fffu, 0x7fffu, 0x7fffu, 0x7fffu};
-    if (first + i * 8 < p.vocab) load8(logits, first + i * 8, p.vocab, b);
+  for (int i = 0; i < G; ++i) {
+    v[i] = make_uint4(kPad, kPad, kPad, kPad);
+    if (first + i * 512 < p.vocab) v[i] = load8(r.logits, first + i * 512, p.vocab);
+  }
+  const bool some = s.chunk_ties[chunk] > room;  // not all of its tokens with the last value are kept
+  uint32_t dropped[G] = {};                      // of a group's eight, a bit each
+  if (some) {
+    int n = 0, inc[G];
+    uint32_t same[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      same[i] = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) same[i] |= uint32_t(bin_of(token(v[i], j)) == last_bin) << j;
+      inc[i] = wave_scan(int(__popc(same[i])));
+      const int all = last_lane(inc[i]);
+      inc[i] += n;
+      n += all;
+    }
+    __syncthreads();
+    if (lane == 0) s.redi[wave] = n;
+    __syncthreads();
+    int ahead = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) ahead += w < wave ? s.redi[w] : 0;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      int rank = ahead + inc[i] - int(__popc(same[i]));
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (same[i] >> j & 1) dropped[i] |= uint32_t(rank++ >= room) << j;
+    }
+  }
+  // a token's kept weight
+  auto held = [&](int i, int j) -> double {
+    const unsigned bin = unsigned(bin_of(token(v[i], j)));
+    const double m = s.weight[min(bin, unsigned(kBins - 1))];  // (the last bin is an unused one)
+    return bin > unsigned(last_bin) || (dropped[i] >> j & 1) ? 0.0 : m;
+  };
+  double group[G], mine = 0.0;
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    group[i] = 0.0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) group[i] += held(i, j);
+    mine += group[i];
+  }
+  mine = wave_sum(mine);
+  __syncthreads();
+  if (lane == 0) s.redd[wave] = mine;
+  __syncthreads();
+  // The wave, its group, the lane, the token, each found as the chunk was.
+  int the_wave = 0;
+  sum = cum;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const double m = s.redd[w];
+    if (m > 0.0 && !(cum > target)) the_wave = w, sum = cum;
+    cum += m;
+  }
+  if (wave != the_wave) return;
+  int gi = 0;
+  double ahead = sum, inc = 0.0;
+  bool done = false;
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    const double run = wave_scan(group[i]);
+    const double m = last_lane(run);
+    if (!done && m > 0.0) gi = i, ahead = sum, inc = run;
+    if (!done && sum + m > target) done = true;
+    sum += m;
+  }
+  double g = group[0];
+#pragma unroll
+  for (int i = 1; i < G; ++i)
+    if (gi == i) g = group[i];
+  const unsigned long long over = __ballot(g > 0.0 && ahead + inc > target), any = __ballot(g > 0.0);
+  const int the_lane = over ? __builtin_ctzll(over) : any ? 63 - __builtin_clzll(any) : 0;
+  if (lane != the_lane) return;
+  double at = ahead + (inc - g);
+  int drawn = first + gi * 512;
+  bool stop = false;
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    if (gi != i) continue;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t key = key_of(b[j], 0);
-      if (key > key_last) keep |= 1u << (i * 8 + j);
-      if (key == key_last) tie |= 1u << (i * 8 + j);
-      if (j & 1) packed[(i * 8 + j) / 2] |= b[j] << 16;
-      else packed[(i * 8 + j) / 2] = b[j];
+      const double m = held(i, j);
+      if (!stop && m > 0.0) drawn = first + i * 512 + j;
+      at += m;
+      if (m > 0.0 && at > target) stop = true;
     }
   }
-  int room = ties_left - block_prefix(int(__popc(tie)), redi);  // ties that this thread keeps
-  double s = 0.0;
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    if (tie >> i & 1) {
-      if (room > 0) keep |= 1u << i;
-      --room;
-    }
-    const uint32_t b = packed[i / 2] >> (16 * (i & 1)) & 0xffffu;
-    if (keep >> i & 1) s += fast ? weight[bin_of(b)] : weigh(key_of(b, 0));
-  }
-  double at = cum + block_prefix(s, redd);
-  if (keep) {
-    atomicMax(&final_kept, first + 31 - int(__clz(keep)));
-    if (at + s > target) {
-#pragma unroll
-      for (int i = 0; i < kPerThread; ++i) {
-        const uint32_t b = packed[i / 2] >> (16 * (i & 1)) & 0xffffu;
-        if (!(keep >> i & 1)) continue;
-        at += fast ? weight[bin_of(b)] : weigh(key_of(b, 0));
-        if (at > target) {
-          atomicMin(&drawn, first + i);
-          break;
-        }
-      }
-    }
-  }
-  __syncthreads();
-  if (tid == 0) p.out[row] = drawn != 0x7fffffff ? drawn : final_kept;
+  p.out[row] = drawn;
 }
 
-size_t counts_bytes(int64_t batch, int64_t chunks) { return size_t(batch) * chunks * (kBins / 2) * 4; }
+// Tokens of a workgroup: few enough that a small batch takes more CUs (and a thread
+// looks up fewer weights at the end), as long as the counts of a row's chunks, 20 KB
+// each, stay few.
+int groups_for(int64_t batch, int64_t vocab) {
+  if (vocab <= 8 * 8192 && batch * ((vocab + 8191) / 8192) <= 256) return 1;
+  if (vocab <= 32 * 16384 && batch * ((vocab + 16383) / 16384) <= 256) return 2;
+  return 4;
+}
+int64_t chunks_of(int64_t vocab, int groups) { return (vocab + 8192 * groups - 1) / (8192 * groups); }
+// The most (row, chunk) places that up to `batch` rows take.
+int64_t places(int64_t batch, int64_t vocab) {
+  const int64_t fine = batch * chunks_of(vocab, 1), coarse = batch * chunks_of(vocab, 4);
+  return coarse > 256 ? coarse : fine < 256 ? fine : 256;
+}
+constexpr size_t kPlaceBytes = kBins / 2 * 4 + 8 + 4;
 
 }  // namespace
 
 extern "C" size_t mi_draw_workspace_size(int32_t batch_size, int32_t vocab_size) {
   if (batch_size <= 0 || batch_size > kMaxRows || vocab_size <= 0 || vocab_size > kMaxVocab) return 0;
-  const int64_t chunks = (vocab_size + kChunk - 1) / kChunk;
-  return counts_bytes(batch_size, chunks) + size_t(batch_size) * chunks * 12;
+  return size_t(places(batch_size, vocab_size)) * kPlaceBytes;
 }
 
 extern "C" int mi_draw(const void* logits, int64_t logits_row_stride, int32_t batch_size, int32_t vocab_size,
@@ -497,19 +827,29 @@ extern "C" int mi_draw(const void* logits, int64_t logits_row_stride, int32_t ba
   p.logits = static_cast<const uint16_t*>(logits);
   p.stride = logits_row_stride;
   p.vocab = vocab_size;
-  p.chunks = (vocab_size + kChunk - 1) / kChunk;
+  const int groups = groups_for(batch_size, vocab_size);
+  p.chunks = int(chunks_of(vocab_size, groups));
   p.temperature = temperature;
   p.top_k = top_k;
   p.top_p = top_p;
   p.min_p = min_p;
   p.u = uniforms;
   p.out = out_tokens;
+  const size_t used = size_t(batch_size) * p.chunks;
   p.counts = static_cast<uint32_t*>(workspace);
-  char* at = static_cast<char*>(workspace) + counts_bytes(batch_size, p.chunks);
-  p.winner = reinterpret_cast<unsigned long long*>(at);
-  p.outside = reinterpret_cast<uint32_t*>(at + size_t(batch_size) * p.chunks * 8);
+  p.winner = reinterpret_cast<unsigned long long*>(p.counts + used * (kBins / 2));
+  p.outside = reinterpret_cast<uint32_t*>(p.winner + used);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(count_kernel, dim3(p.chunks, batch_size), dim3(kThreads), 0, s, p);
-  hipLaunchKernelGGL(draw_kernel, dim3(batch_size), dim3(kThreads), 0, s, p);
+  const dim3 chunks(p.chunks, batch_size), rows(batch_size), threads(kThreads);
+  if (groups == 1) {
+    hipLaunchKernelGGL(count_kernel<1>, chunks, threads, 0, s, p);
+    hipLaunchKernelGGL(draw_kernel<1>, rows, threads, 0, s, p);
+  } else if (groups == 2) {
+    hipLaunchKernelGGL(count_kernel<2>, chunks, threads, 0, s, p);
+    hipLaunchKernelGGL(draw_kernel<2>, rows, threads, 0, s, p);
+  } else {
+    hipLaunchKernelGGL(count_kernel<4>, chunks, threads, 0, s, p);
+    hipLaunchKernelGGL(draw_kernel<4>, rows, threads, 0, s, p);
+  }
   return mi::check_launch("draw_kernel");
 }
