@@ -65,6 +65,13 @@ def add_rms_norm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tens
     return h_out if norm else None
 
 
+def _refuse(name: str, t: torch.Tensor, shape, device) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: there is no backward pass")
+    raise ValueError(f"{name} must be {tuple(shape)} bfloat16 on {device} with a contiguous last axis; got "
+                     f"{tuple(t.shape)} {t.dtype} on {t.device}")
+
+
 def post_norm_add_rms_norm(x: torch.Tensor, y: torch.Tensor, post_weight: torch.Tensor, weight: torch.Tensor,
                            eps: float, *, gate: torch.Tensor | None = None, scale: float = 1.0,
                            x_out: torch.Tensor | None = None, h_out: torch.Tensor | None = None) -> torch.Tensor:
@@ -78,27 +85,24 @@ def post_norm_add_rms_norm(x: torch.Tensor, y: torch.Tensor, post_weight: torch.
     or [rows, hidden].  x_out may be x, and h_out y; other overlaps are undefined.
     """
     _rows("x", x)
-    rows, hidden = x.shape
-    _rows("y", y, hidden)
-    for name, w in (("post_weight", post_weight), ("weight", weight)):
-        require_gpu(name, w)
-        require_dtype(name, w, torch.bfloat16)
-        if w.shape != (hidden,) or not w.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous [{hidden}] tensor")
+    shape = rows, hidden = x.shape
     if x_out is None:
         x_out = x
-    else:
-        _rows("x_out", x_out, hidden)
     if h_out is None:
         h_out = torch.empty(rows, hidden, dtype=x.dtype, device=x.device)
-    else:
-        _rows("h_out", h_out, hidden)
-    if y.shape[0] != rows or x_out.shape[0] != rows or h_out.shape[0] != rows:
-        raise ValueError("x, y, x_out and h_out must have as many rows")
+    device, grad = x.get_device(), torch.is_grad_enabled()
+    for name, t in (("x", x), ("y", y), ("x_out", x_out), ("h_out", h_out)):
+        if (t.shape != shape or t.dtype != torch.bfloat16 or t.get_device() != device or t.stride(1) != 1
+                or (grad and t.requires_grad)):
+            _refuse(name, t, shape, x.device)
+    for name, t in (("post_weight", post_weight), ("weight", weight)):
+        if (t.shape != (hidden,) or t.dtype != torch.bfloat16 or t.get_device() != device or t.stride(0) != 1
+                or (grad and t.requires_grad)):
+            _refuse(name, t, (hidden,), x.device)
     g_ptr, g_stride, g_column = None, 0, 0
     if gate is not None:
-        require_gpu("gate", gate)
-        require_dtype("gate", gate, torch.bfloat16)
+        if gate.dtype != torch.bfloat16 or gate.get_device() != device or (grad and gate.requires_grad):
+            _refuse("gate", gate, gate.shape, x.device)
         g_ptr = gate.data_ptr()
         if gate.shape == (hidden,) and gate.is_contiguous():
             g_column = 1
@@ -109,12 +113,6 @@ def post_norm_add_rms_norm(x: torch.Tensor, y: torch.Tensor, post_weight: torch.
         else:
             raise ValueError(f"gate must be [{hidden}], [{rows}, 1] or [{rows}, {hidden}] with a contiguous last axis; "
                              f"got {tuple(gate.shape)}")
-    tensors = (x, y, post_weight, weight, x_out, h_out) if gate is None else (x, y, post_weight, weight, x_out, h_out, gate)
-    for t in tensors:
-        if t.get_device() != x.get_device():
-            raise ValueError(f"tensors on {t.device} and {x.device}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError("an input requires a gradient: there is no backward pass")
     call_on(x, "mi_post_norm_add_rms_norm", x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0),
             post_weight.data_ptr(), weight.data_ptr(), g_ptr, g_stride, g_column, x_out.data_ptr(), x_out.stride(0),
             h_out.data_ptr(), h_out.stride(0), rows, hidden, eps, scale)

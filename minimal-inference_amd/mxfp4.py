@@ -48,28 +48,29 @@ def _out(out: torch.Tensor | None, rows: int, cols: int, like: torch.Tensor) -> 
 class MXFP4:
     """A matrix of microscaled 4-bit floats on a GPU, in operand order."""
 
-    __slots__ = ("rows", "cols", "codes", "scales")
+    __slots__ = ("rows", "cols", "device", "buffer", "codes_ptr", "scales_ptr")
 
     def __init__(self, rows: int, cols: int, device):
         """Room for [rows, cols]; its contents are undefined until they are written."""
-        if rows < 0 or cols <= 0 or cols % BLOCK or cols > 1 << 20:
-            raise ValueError(f"an MXFP4 matrix has columns in blocks of {BLOCK}, at most 2^20; got [{rows}, {cols}]")
+        if rows < 0 or rows > 1 << 31 or cols <= 0 or cols % BLOCK or cols > 1 << 20:
+            raise ValueError(f"an MXFP4 matrix has up to 2^31 rows, columns in blocks of {BLOCK}, at most 2^20; got "
+                             f"[{rows}, {cols}]")
         self.rows, self.cols = rows, cols
         tiles = -(-rows // _TILE_ROWS)
-        self.codes = torch.empty(tiles * -(-cols // _SLAB) * _TILE_BYTES, dtype=torch.uint8, device=device)
-        self.scales = torch.empty(tiles * -(-cols // (4 * _SLAB)) * _QUAD_BYTES, dtype=torch.uint8, device=device)
+        # one allocation (two cost 1.1 us more per call): the codes, then the scales
+        codes = tiles * -(-cols // _SLAB) * _TILE_BYTES
+        self.buffer = torch.empty(codes + tiles * -(-cols // (4 * _SLAB)) * _QUAD_BYTES, dtype=torch.uint8, device=device)
+        self.device = self.buffer.device
+        self.codes_ptr = self.buffer.data_ptr()
+        self.scales_ptr = self.codes_ptr + codes
 
     @property
     def shape(self) -> tuple[int, int]:
         return self.rows, self.cols
 
     @property
-    def device(self) -> torch.device:
-        return self.codes.device
-
-    @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return self.buffer.numel()
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "MXFP4":
@@ -77,7 +78,7 @@ class MXFP4:
         half) and scale bytes [rows, cols / 32], both uint8."""
         _check_codes(codes, scales)
         m = cls(codes.shape[0], 2 * codes.shape[1], codes.device)
-        call_on(codes, "mi_mxfp4_pack", codes.data_ptr(), scales.data_ptr(), m.codes.data_ptr(), m.scales.data_ptr(),
+        call_on(codes, "mi_mxfp4_pack", codes.data_ptr(), scales.data_ptr(), m.codes_ptr, m.scales_ptr,
                 m.rows, m.cols)
         return m
 
@@ -85,14 +86,14 @@ class MXFP4:
         """Row-major codes and scale bytes, as ``from_codes`` takes them."""
         codes = torch.empty(self.rows, self.cols // 2, dtype=torch.uint8, device=self.device)
         scales = torch.empty(self.rows, self.cols // BLOCK, dtype=torch.uint8, device=self.device)
-        call_on(codes, "mi_mxfp4_unpack", self.codes.data_ptr(), self.scales.data_ptr(), codes.data_ptr(),
+        call_on(codes, "mi_mxfp4_unpack", self.codes_ptr, self.scales_ptr, codes.data_ptr(),
                 scales.data_ptr(), self.rows, self.cols)
         return codes, scales
 
     def dequantize(self, out: torch.Tensor | None = None) -> torch.Tensor:
         """The values as bf16 [rows, cols], exactly."""
-        out = _out(out, self.rows, self.cols, self.codes)
-        call_on(out, "mi_mxfp4_dequantize", self.codes.data_ptr(), self.scales.data_ptr(), out.data_ptr(),
+        out = _out(out, self.rows, self.cols, self.buffer)
+        call_on(out, "mi_mxfp4_dequantize", self.codes_ptr, self.scales_ptr, out.data_ptr(),
                 out.stride(0), self.rows, self.cols)
         return out
 
@@ -119,7 +120,7 @@ def quantize_mxfp4(x: torch.Tensor, out: MXFP4 | None = None) -> MXFP4:
         out = MXFP4(rows, cols, x.device)
     elif out.shape != (rows, cols) or out.device != x.device:
         raise ValueError(f"out must be [{rows}, {cols}] on {x.device}; got {out.shape} on {out.device}")
-    call_on(x, "mi_mxfp4_quantize", x.data_ptr(), x.stride(0), out.codes.data_ptr(), out.scales.data_ptr(), rows, cols)
+    call_on(x, "mi_mxfp4_quantize", x.data_ptr(), x.stride(0), out.codes_ptr, out.scales_ptr, rows, cols)
     return out
 
 
@@ -133,7 +134,7 @@ def _linear(x, weight: MXFP4, bias, out, silu: bool) -> torch.Tensor:
         n //= 2
     if isinstance(x, MXFP4):
         rows, k = x.rows, x.cols
-        data, scales, stride, like = x.codes.data_ptr(), x.scales.data_ptr(), 0, x.codes
+        data, scales, stride, like = x.codes_ptr, x.scales_ptr, 0, x.buffer
     else:
         rows, k = _rows_of("x", x)
         data, scales, stride, like = x.data_ptr(), None, x.stride(0), x
@@ -151,7 +152,7 @@ def _linear(x, weight: MXFP4, bias, out, silu: bool) -> torch.Tensor:
         room = _workspace_size(rows, n, k, silu, scales is not None) if rows > _FEW_ROWS else 0
         # (a tensor of this call's own: calls on several streams and in graphs share nothing)
         workspace = torch.empty(room, dtype=torch.uint8, device=like.device) if room else None
-        call_on(like, "mi_linear_mxfp4", data, stride, scales, weight.codes.data_ptr(), weight.scales.data_ptr(),
+        call_on(like, "mi_linear_mxfp4", data, stride, scales, weight.codes_ptr, weight.scales_ptr,
                 bias.data_ptr() if bias is not None else None, out.data_ptr(), out.stride(0), rows, n, k,
                 1 if silu else 0, workspace.data_ptr() if room else None, room)
     return out
