@@ -17,14 +17,20 @@ __device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t rs, lds_t* dst,
 #endif
 }
 
+constexpr int kGroupM = 4;
+
 // MB blocks of 16 rows of x and NT tiles of W per wave.  Slabs are staged STAGES deep:
 // before slab s is multiplied the loads of the STAGES - 2 slabs behind it may be in
 // flight, and after the barrier its predecessor's buffer is filled again.  Loads past
 // the last slab are out of range, so that every wait counts the same loads.
 //
+// PER slabs stand between two barriers: two for the largest blocks of MXFP4 rows, so that
+// the second's operands are read while the first is multiplied (8,192 x 8,192 x 10,240
+// 342 -> 329 us; all operands a slab ahead in registers spilled).
+//
 // SPLIT: the workgroup takes p.split_slabs slabs and leaves its sums, in fp32, for
 // combine_kernel.
-template <int WM, int WN, int MB, int NT, int STAGES, bool MX, bool GLU, bool SPLIT>
+template <int WM, int WN, int MB, int NT, int STAGES, bool MX, bool GLU, bool SPLIT, int PER = 1>
 __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
   constexpr int WAVES = WM * WN, HALVES = GLU ? 2 : 1;
   constexpr int XBLK = MX ? kTileBytes : 16 * kSlab * 2;  // 16 rows of x of a slab
@@ -32,19 +38,23 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
   constexpr int XBYTES = WM * MB * XBLK, STAGE = XBYTES + TILES * kTileBytes;
   constexpr int XLOADS = XBYTES / 1024 / WAVES, WLOADS = TILES / WAVES;
   static_assert(XBYTES / 1024 % WAVES == 0 && TILES % WAVES == 0 && NT % HALVES == 0, "even shares");
-  static_assert(STAGES * STAGE <= 160 * 1024, "LDS");
-  __shared__ __attribute__((aligned(16))) char smem[STAGES * STAGE];
+  static_assert(STAGES * PER * STAGE <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(16))) char smem[STAGES * PER * STAGE];
   lds_t* const lds = (lds_t*)smem;
   const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
   const int wm = w / WN, wn = w % WN;
   const int g = lane >> 4, n = lane & 15;
-  // Workgroups go to the eight XCDs in turn.  Each XCD gets a run of tiles, down the
-  // rows of x first, so that the tiles of W in its L2 serve them all.
+  // Workgroups go to the eight XCDs in turn.  Each XCD gets a run of tiles, in groups of
+  // kGroupM down the rows of x, so that those it holds at a time share tiles of x and of
+  // W in its L2.  (us, 8,192 x 8,192 x 10,240 in 4 bits: groups of 64 376, 16 354, 8 344,
+  // 4 345; 4,096 x 4,096 x 6,144 bf16 169, 164, 161, 157.)
   const int mt = int((p.rows + BM - 1) / BM), nt = (p.n + COLS - 1) / COLS, all = mt * nt;
-  const int id = int(blockIdx.x), xcd = id & 7, in = id >> 3, each = all / 8, more = all % 8;
-  const int tile_id = xcd * each + min(xcd, more) + in;
-  const int col0 = tile_id / mt * COLS;
-  const int64_t m0 = int64_t(tile_id % mt) * BM;
+  const int id = int(blockIdx.x), xcd = id & 7, each = all / 8, more = all % 8;
+  const int tile_id = xcd * each + min(xcd, more) + (id >> 3);
+  const int group = tile_id / (kGroupM * nt), in = tile_id - group * kGroupM * nt;
+  const int high = min(kGroupM, mt - group * kGroupM);
+  const int col0 = in / high * COLS;
+  const int64_t m0 = int64_t(group * kGroupM + in % high) * BM;
   const int rows = int(min(int64_t(BM), p.rows - m0));
   const int slab0 = SPLIT ? int(blockIdx.y) * p.split_slabs : 0;
   const int slab_end = SPLIT ? min(slab0 + p.split_slabs, p.slabs) : p.slabs;
@@ -138,11 +148,12 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
 #pragma unroll
   for (int s = 0; s < 4; ++s) ro[s] = n * 256 + chunk_slot(n, 4 * g + s) * 16;
 
-  constexpr int kInFlight = (STAGES - 2) * (XLOADS + WLOADS);
+  constexpr int kInFlight = (STAGES - 2) * PER * (XLOADS + WLOADS);
   static_assert(kInFlight < 64, "vmcnt");
+  static_assert(PER == 1 || !SPLIT, "parts begin at any slab");
   load_scales(slab0 >> 2);
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) load(slab0 + i, i);
+  for (int i = 0; i < (STAGES - 1) * PER; ++i) load(slab0 + i, i);
   int buf = 0, before = STAGES - 1;
   for (int quad = slab0 >> 2; 4 * quad < slab_end; ++quad) {
     uint32_t wscale[NT], xscale[MX ? MB : 1];
@@ -150,19 +161,9 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
     for (int t = 0; t < NT; ++t) wscale[t] = wnext[t];
 #pragma unroll
     for (int b = 0; b < (MX ? MB : 1); ++b) xscale[b] = xnext[b];
-    auto step = [&]<int S>() {
-      const int slab = 4 * quad + S;
-      if ((SPLIT && slab < slab0) || slab >= slab_end) return;
-      // vmcnt: this slab is in LDS; lgkmcnt: this wave has read the one before
-      __builtin_amdgcn_s_waitcnt(0x0070 | (kInFlight & 15) | (kInFlight >> 4 << 14));
-      __builtin_amdgcn_s_barrier();
-      __builtin_amdgcn_sched_barrier(0);
-      if (S == 0 || (SPLIT && slab == slab0)) load_scales(quad + 1);
-      load(slab + STAGES - 1, before);
-      const lds_t* const xl = lds + buf * STAGE + wm * MB * XBLK;
-      const lds_t* const wl = lds + buf * STAGE + XBYTES + wn * NT * kTileBytes + lane * 16;
-      before = buf;
-      buf = buf + 1 == STAGES ? 0 : buf + 1;
+    auto slab_of = [&]<int S>(int at) {  // the slab in buffer `at`
+      const lds_t* const xl = lds + at * STAGE + wm * MB * XBLK;
+      const lds_t* const wl = lds + at * STAGE + XBYTES + wn * NT * kTileBytes + lane * 16;
       u32x4_t a[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) a[t] = lds_load16(wl + t * kTileBytes);
@@ -188,12 +189,27 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
           }
         }
       }
+    };
+    auto step = [&]<int S>() {
+      const int slab = 4 * quad + S;
+      if ((SPLIT && slab < slab0) || slab >= slab_end) return;
+      // vmcnt: these slabs are in LDS; lgkmcnt: this wave has read those before
+      __builtin_amdgcn_s_waitcnt(0x0070 | (kInFlight & 15) | (kInFlight >> 4 << 14));
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      if (S == 0 || (SPLIT && slab == slab0)) load_scales(quad + 1);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) load(slab + (STAGES - 1) * PER + i, before * PER + i);
+      slab_of.template operator()<S>(buf * PER);
+      if constexpr (PER == 2) slab_of.template operator()<S + 1>(buf * PER + 1);
+      before = buf;
+      buf = buf + 1 == STAGES ? 0 : buf + 1;
       __builtin_amdgcn_sched_barrier(0);
     };
     step.template operator()<0>();
-    step.template operator()<1>();
+    if constexpr (PER == 1) step.template operator()<1>();
     step.template operator()<2>();
-    step.template operator()<3>();
+    if constexpr (PER == 1) step.template operator()<3>();
   }
 
   // Lane (g, n) holds columns 4 g .. 4 g + 3 of a tile for row n of a block.
@@ -250,7 +266,7 @@ struct Form {
   bool split;
 };
 constexpr Form kBf16Forms[] = {{32, 8, 0.45f, true}, {64, 8, 0.56f, true}, {80, 8, 0.63f, true}, {128, 8, 0.87f, true},
-                               {128, 16, 1.65f, false}};
+                               {128, 16, 1.6f, false}};
 constexpr Form kMxForms[] = {{128, 8, 0.34f, true}, {256, 16, 1.0f, false}};
 constexpr float kStartUs = 3.5f, kCombineUs = 2.5f, kCombineBytesPerUs = 4.4e6f;
 constexpr int kMaxParts = 32;
@@ -285,18 +301,18 @@ Choice choose(bool mx, bool glu, int64_t rows, int64_t n, int slabs, size_t room
 // The few-row kernel's time, from W's bytes.
 float few_us(const LinearParams& p) { return 4.f + float(p.w_tiles) * p.slabs * 1.0625e3f / 4e6f; }
 
-template <int WM, int WN, int MB, int NT, int STAGES, bool MX, bool GLU, bool SPLIT>
+template <int WM, int WN, int MB, int NT, int STAGES, bool MX, bool GLU, bool SPLIT, int PER = 1>
 void run(const LinearParams& p, int parts, hipStream_t stream) {
   constexpr int BM = WM * MB * 16, COLS = WN * NT * 16 / (GLU ? 2 : 1);
   const dim3 grid(uint32_t((p.rows + BM - 1) / BM * ((p.n + COLS - 1) / COLS)), parts);
-  hipLaunchKernelGGL((many_kernel<WM, WN, MB, NT, STAGES, MX, GLU, SPLIT>), grid, dim3(64 * WM * WN), 0, stream, p);
+  hipLaunchKernelGGL((many_kernel<WM, WN, MB, NT, STAGES, MX, GLU, SPLIT, PER>), grid, dim3(64 * WM * WN), 0, stream, p);
 }
 
 template <bool MX, bool GLU, bool SPLIT>
 void run_form(const LinearParams& p, int form, int parts, hipStream_t stream) {
   if constexpr (MX) {
     if (SPLIT || form == 0) run<2, 2, 4, 4, 4, true, GLU, SPLIT>(p, parts, stream);
-    else run<2, 4, 8, 4, 3, true, GLU, false>(p, 1, stream);
+    else run<2, 4, 8, 4, 2, true, GLU, false, 2>(p, 1, stream);
   } else {
     if (form == 0) run<1, 4, 2, 2, 4, false, GLU, SPLIT>(p, parts, stream);
     else if (form == 1) run<2, 4, 2, 2, 4, false, GLU, SPLIT>(p, parts, stream);
