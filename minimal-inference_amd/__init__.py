@@ -7,7 +7,9 @@ Public surface (mirrors what the reference's model.py / scheduler.py call):
   page.append_paged_kv_cache                        -- model.py:207-216
   decode.BatchDecodeWithPagedKVCacheWrapper         -- scheduler.py:535-539
   prefill.BatchPrefillWithPagedKVCacheWrapper       -- scheduler.py:530-534
-  sampling.sample_batch / sample                    -- scheduler.py:310-343
+  sampling.sample_batch / sample / Sampler.draw     -- scheduler.py:310-343
+  mxfp4.MXFP4 / quantize_mxfp4 / linear_mxfp4       -- 4-bit weights (no counterpart)
+  dense.post_norm_add_rms_norm                      -- norms around a block (no counterpart)
   kv_cache.PagedKVCache / build_csr_metadata        -- scheduler.py:168-302
   kv_cache.DevicePageTable                          -- GPU page table + CSR build
   engine.Scheduler / engine.AttentionBackend        -- scheduler.py:229-259, 477+

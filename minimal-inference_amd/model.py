@@ -23,7 +23,9 @@ output), the projections of a decode step's few rows on the kernel that streams
 each weight once (``dense.linear``), SiLU(gate) * up in that launch too or, for
 more rows, as a kernel of its own (``dense.linear_silu``);
 ``fused_dense=False`` keeps torch's ``F.linear``, ``F.rms_norm``, adds and
-``F.silu(g) * u``.  RoPE tables are held in the model dtype, as the reference's are after ``.to(dtype)``
+``F.silu(g) * u``.  ``Model.quantize_weights()`` turns the layers' projections into
+microscaled 4-bit matrices (``mxfp4.MXFP4``), which every step then multiplies by
+``mxfp4.linear_mxfp4`` / ``linear_silu_mxfp4``, whatever its rows.  RoPE tables are held in the model dtype, as the reference's are after ``.to(dtype)``
 (server.py:251).  Weights are random-initialised on the device (N(0, 0.02),
 norms 1) -- the benchmark configurations use random weights.
 """
@@ -39,6 +41,7 @@ import torch
 import torch.nn.functional as F
 
 from .dense import add_rms_norm, linear, linear_silu
+from .mxfp4 import MXFP4, linear_mxfp4, linear_silu_mxfp4, quantize_mxfp4
 from .page import append_paged_kv_cache, rope_append_paged_kv_cache
 
 
@@ -132,6 +135,10 @@ class Layer:
         self.w_down = w(h, cfg.intermediate_size)
 
 
+def _project(h: torch.Tensor, w: torch.Tensor | MXFP4, bias: torch.Tensor | None = None) -> torch.Tensor:
+    return linear_mxfp4(h, w, bias) if isinstance(w, MXFP4) else linear(h, w, bias)
+
+
 @dataclasses.dataclass
 class AttentionBackend:
     """What the attention layers need for one forward (scheduler.py:229-259).
@@ -182,11 +189,24 @@ class Model:
         t = self.embed.numel() + self.norm.numel()
         if self.lm_head is not self.embed:
             t += self.lm_head.numel()
+        t *= self.embed.element_size()
         for L in self.layers:
             for x in (L.in_norm, L.post_norm, L.w_qkv, L.b_qkv, L.w_o, L.w_gate_up, L.w_down):
                 if x is not None:
-                    t += x.numel()
-        return t * self.embed.element_size()
+                    t += x.nbytes
+        return t
+
+    def quantize_weights(self) -> None:
+        """The layers' projections in microscaled 4-bit floats from here on (0.53 bytes
+        per weight); embedding, LM head, norms and biases stay in bf16.  After the
+        weights are loaded and before a scheduler captures its graphs."""
+        if not self.fused_dense:
+            raise ValueError("4-bit weights need fused_dense")
+        for L in self.layers:
+            for name in ("w_qkv", "w_o", "w_gate_up", "w_down"):
+                w = getattr(L, name)
+                if not isinstance(w, MXFP4):
+                    setattr(L, name, quantize_mxfp4(w))
 
     # ------------------------------------------------------------------ forward
     def forward(self, input_ids: torch.Tensor, positions: torch.Tensor, backend: AttentionBackend,
@@ -209,7 +229,7 @@ class Model:
         backend._layer_idx = 0
         eps = cfg.rms_norm_eps
         dense = self.fused_dense
-        project = linear if dense else F.linear
+        project = _project if dense else F.linear
         if dense:
             h = add_rms_norm(x, None, self.layers[0].in_norm, eps, write_x=False)
         for li, L in enumerate(self.layers):
@@ -244,7 +264,8 @@ class Model:
                 continue
             # x += o W_o; h = rms(x); x += down(silu(g) * u); h = next layer's rms(x)
             h = add_rms_norm(x, project(o.view(t, nq * d), L.w_o), L.post_norm, eps)
-            down = project(linear_silu(h, L.w_gate_up), L.w_down)
+            gate_up = linear_silu_mxfp4 if isinstance(L.w_gate_up, MXFP4) else linear_silu
+            down = project(gate_up(h, L.w_gate_up), L.w_down)
             if li + 1 < len(self.layers):
                 h = add_rms_norm(x, down, self.layers[li + 1].in_norm, eps)
             elif last_rows is None:

@@ -247,6 +247,9 @@ def init_engine(config: dict):
         dev = torch.device("cuda", 0)
     sc = config.get("scheduler", {})
     max_seq = int(sc.get("max_seq_len", 4096))
+    weight_format = str(config.get("weight_format", "bfloat16"))
+    if weight_format not in ("bfloat16", "bf16", "mxfp4"):
+        raise ValueError(f"weight_format {weight_format!r}: bfloat16 or mxfp4")
     model_path = config.get("model_path")
     seed = int(config.get("seed", 0))
     if model_path:
@@ -263,6 +266,8 @@ def init_engine(config: dict):
         model = Model(cfg, dev, seed=seed, max_positions=max_seq + 16)
         tok = SyntheticTokenizer(cfg.vocab_size)
         name = f"{preset}-random"
+    if weight_format == "mxfp4":
+        model.quantize_weights()
     stops = stop_ids(tok)
     sch = Scheduler(model, max_batch_size=int(sc.get("max_batch_size", 40)), max_seq_len=max_seq,
                     page_size=int(sc.get("page_size", 16)), eos_token_ids=stops or None,

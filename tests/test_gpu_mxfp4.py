@@ -285,3 +285,46 @@ def test_empty_and_refused(dev):
             bad()
     with pytest.raises(TypeError):
         linear_mxfp4(x, x)
+
+
+@pytest.mark.parametrize("acts", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("silu", [False, True])
+@pytest.mark.parametrize("rows,n,k", [
+    (20, 300, 8192), (33, 520, 2080), (64, 2048, 4096), (65, 130, 18944), (80, 1000, 896), (81, 1000, 4000),
+    (128, 640, 8192), (137, 384, 1024), (256, 256, 14336), (265, 4096, 512), (521, 96, 2048), (1024, 2048, 256),
+    (2057, 4096, 160), (2304, 3000, 416), (4100, 520, 96)])
+def test_every_form_of_whole_numbers(dev, rows, n, k, silu, acts):
+    """Sizes on which the forms (blocks of 32 to 256 rows, k whole and in parts, rows
+    behind the last whole block) differ: sums exact in fp32 are the exact ones, with a
+    workspace and without one, strided rows and what lies around them included."""
+    from minimal_inference_amd import _lib
+    from minimal_inference_amd.mxfp4 import linear_mxfp4, linear_silu_mxfp4, quantize_mxfp4
+
+    g = torch.Generator(device=dev).manual_seed(rows + n + k)
+    values = torch.tensor([0, 1, 2, 3, 4, 6, -1, -2, -3, -4, -6], device=dev, dtype=torch.float32)
+
+    def whole(r):
+        m = values[torch.randint(0, 11, (r, k), device=dev, generator=g)]
+        m[:, ::32] = torch.where(m[:, ::32] < 0, -6.0, 6.0)
+        return m.to(torch.bfloat16)
+
+    x, w = whole(rows), whole(2 * n if silu else n)
+    weight = quantize_mxfp4(w)
+    xx = quantize_mxfp4(x) if acts == "mxfp4" else torch.cat([x, torch.full_like(x[:, :32], float("nan"))], 1)[:, :k]
+    sums = x.double() @ w.double().t()
+    ref = sums
+    if silu:
+        gate, up = sums.chunk(2, -1)
+        ref = gate * torch.sigmoid(gate) * up
+    out = torch.full((rows + 1, n + 8), 7.0, device=dev, dtype=torch.bfloat16)
+    (linear_silu_mxfp4 if silu else linear_mxfp4)(xx, weight, out=out[:rows, :n])
+    alone = torch.full_like(out, 7.0)  # and by the C entry, which may get no workspace
+    ptr = (xx.codes_ptr, 0, xx.scales_ptr) if acts == "mxfp4" else (xx.data_ptr(), xx.stride(0), None)
+    _lib.call("mi_linear_mxfp4", *ptr, weight.codes_ptr, weight.scales_ptr, None, alone.data_ptr(), alone.stride(0), rows, n,
+              k, int(silu), None, 0, torch.cuda.current_stream().cuda_stream)
+    for got in (out, alone):
+        if silu:  # fp32: the exponential, the quotient and the products round 8 times
+            assert bool(((got[:rows, :n].double() - ref).abs() <= (2 ** -8 + 8 * 2 ** -24) * ref.abs() + 1e-30).all())
+        else:
+            assert torch.equal(got[:rows, :n], ref.to(torch.bfloat16))
+        assert bool((got[rows] == 7).all()) and bool((got[:, n:] == 7).all())

@@ -102,3 +102,16 @@ def test_oracle_draw_by_hand():
     assert [draw_row(l, u, 1.0, top_p=0.6) for u in (0.0, 0.6)] == [1, 3]
     assert [draw_row(l, u, 1.0, min_p=0.5) for u in (0.0, 0.6)] == [1, 3]
     assert draw_row(l, 0.3, 0.0) == 1
+
+
+def test_workspace_of_the_products():
+    """k is shared between workgroups where few blocks would leave the chip idle, and
+    nowhere that the few-row kernel runs."""
+    _, lib = _lib()
+    size = lib.mi_linear_mxfp4_workspace_size
+    assert size(77, 3584, 18944, 0, 0) > 0 and size(128, 4096, 14336, 0, 1) > 0
+    assert size(77, 3584, 18944, 0, 0) % 16 == 0
+    assert size(16, 4096, 14336, 0, 0) == 0 and size(64, 4096, 14336, 0, 1) == 0
+    assert size(8192, 10240, 8192, 0, 1) == 0
+    for bad in ((-1, 32, 64), (100, 0, 64), (100, 32, 48), ((1 << 22) + 1, 32, 64)):
+        assert size(*bad, 0, 0) == 0
