@@ -129,6 +129,8 @@ extern "C" int mi_post_norm_add_rms_norm(const void* x, int64_t x_stride, const 
   uintptr_t aligned = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) |
                       reinterpret_cast<uintptr_t>(post_weight) | reinterpret_cast<uintptr_t>(weight) |
                       reinterpret_cast<uintptr_t>(x_out) | reinterpret_cast<uintptr_t>(h_out);
+  if (rows == 1) x_stride = y_stride = x_out_stride = h_stride = hidden;  // (nothing lies at a row stride)
+  if (rows == 1 && gate) gate_row_stride = 0;
   int64_t strides = x_stride | y_stride | x_out_stride | h_stride;
   if (gate && gate_per_column) aligned |= reinterpret_cast<uintptr_t>(gate), strides |= gate_row_stride;
   if ((aligned & 15) || (strides & 7) || (reinterpret_cast<uintptr_t>(gate) & 1))

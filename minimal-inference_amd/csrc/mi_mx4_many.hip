@@ -212,6 +212,8 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
     if constexpr (PER == 1) step.template operator()<3>();
   }
 
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // (the loads past the end write zeros to LDS)
+
   // Lane (g, n) holds columns 4 g .. 4 g + 3 of a tile for row n of a block.
 #pragma unroll
   for (int t = 0; t < NT; t += HALVES) {
@@ -393,6 +395,7 @@ extern "C" int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_sc
                     (long long)rows, (long long)n, (long long)k, kBlock, kMaxK);
   if (silu && bias) return mi::fail(MI_ERR_INVALID, "linear_mxfp4: no bias with the gated product");
   if (rows == 0) return MI_OK;
+  if (rows == 1) x_stride = k, out_stride = n;  // (nothing lies at a row stride)
   if (!x || !codes || !scales || !out) return mi::fail(MI_ERR_INVALID, "linear_mxfp4: null pointer argument");
   const uintptr_t aligned = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(codes) |
                             reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(x_scales) |

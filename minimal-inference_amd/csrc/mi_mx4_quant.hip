@@ -154,6 +154,7 @@ int run_matrix(const char* name, bool quantize, const void* x, int64_t stride, v
   mi::clear_error();
   if (int rc = check_shape(name, rows, cols)) return rc;
   if (rows == 0) return MI_OK;
+  if (rows == 1) stride = cols;  // (nothing lies at a row stride)
   if (!x || !codes || !scales) return mi::fail(MI_ERR_INVALID, "%s: null pointer argument", name);
   if (!aligned16(x) || !aligned16(codes) || !aligned16(scales) || stride % 8 || stride < cols)
     return mi::fail(MI_ERR_INVALID, "%s: rows, codes and scales must be 16-byte aligned, row stride at least the columns",

@@ -92,6 +92,17 @@ def test_zero_rows_infinities_and_defaults(dev):
     assert post_norm_add_rms_norm(x[:0], y[:0], post, pre, 1e-6).shape == (0, 512)
 
 
+def test_one_row_of_any_stride(dev):
+    from minimal_inference_amd.dense import post_norm_add_rms_norm
+
+    x, y, post, pre, gate = _inputs(1, 64, "full", dev)
+    want_x, odd_x = torch.empty_like(x), torch.empty_like(x)
+    want = post_norm_add_rms_norm(x, y, post, pre, 1e-6, gate=gate, x_out=want_x)
+    odd = lambda t: t.as_strided((1, 64), (5, 1))  # noqa: E731
+    assert torch.equal(post_norm_add_rms_norm(odd(x), odd(y), post, pre, 1e-6, gate=odd(gate), x_out=odd(odd_x)), want)
+    assert torch.equal(odd_x, want_x)
+
+
 def test_refused(dev):
     from minimal_inference_amd.dense import post_norm_add_rms_norm
 

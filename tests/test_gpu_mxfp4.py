@@ -259,6 +259,18 @@ def test_linear_in_a_graph_and_on_another_stream(dev):
         assert all(torch.equal(u, v) for y in ya + yb for u, v in zip(y, want))
 
 
+def test_one_row_of_any_stride(dev):
+    """A single row's stride is not looked at: rows of buffers whose width is odd."""
+    from minimal_inference_amd.mxfp4 import linear_mxfp4, quantize_mxfp4
+
+    _, _, w, _ = _weight(33, 64, dev, 8)
+    x = torch.randn(1, 64, device=dev).to(torch.bfloat16)
+    odd = x.as_strided((1, 64), (3, 1))
+    out = torch.empty(33, device=dev, dtype=torch.bfloat16).as_strided((1, 33), (1, 1))
+    assert torch.equal(linear_mxfp4(odd, w, out=out), linear_mxfp4(x, w))
+    assert torch.equal(quantize_mxfp4(odd).dequantize(), quantize_mxfp4(x).dequantize())
+
+
 def test_empty_and_refused(dev):
     from minimal_inference_amd.mxfp4 import MXFP4, linear_mxfp4, linear_silu_mxfp4, quantize_mxfp4
 
