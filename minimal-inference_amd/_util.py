@@ -17,11 +17,14 @@ def call_on(t: torch.Tensor, name: str, *args) -> None:
     """``_lib.call`` on ``t``'s device with its current stream as the last argument; the
     current device changes only where it is another (the context manager costs 3 us)."""
     device = t.get_device()
+    entry = getattr(_lib.load(), name)
     if device == torch._C._cuda_getDevice():
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+        status = entry(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+            status = entry(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        _lib.check(status, name)
 
 
 def require_gpu(name: str, t: torch.Tensor) -> None:

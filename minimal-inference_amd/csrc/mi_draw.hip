@@ -607,8 +607,8 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
       // (a bin above the maximum is empty and its power may be infinite)
       w0 = c.x ? r.weigh(key_of_bin(bin)) : 0.0;
       w1 = c.y ? r.weigh(key_of_bin(bin + 1)) : 0.0;
-      if (w0 < r.min_p) c.x = 0;
-      if (w1 < r.min_p) c.y = 0;
+      if (w0 < r.min_p) c.x = 0, w0 = 0.0;
+      if (w1 < r.min_p) c.y = 0, w1 = 0.0;
       *reinterpret_cast<uint2*>(&s.count[bin]) = c;
       n = wave_sum(int(c.x + c.y));
       m = wave_sum(whole(c.x) * w0 + whole(c.y) * w1);
@@ -618,9 +618,20 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
   }
   __syncthreads();
   if (wave == 0) {  // (in every wave alike it took three times as long)
-    Place at = find_bin(s, kBins, [&](int n, double) { return n >= r.top_k; });
-    at.kept = min(at.kept, r.top_k - at.count_before);
-    double all = at.before + at.kept * s.weight[at.bin];
+    int tokens = 0;
+    double all = 0.0;
+#pragma unroll
+    for (int part = 0; part < (kGroups + 63) / 64; ++part) {
+      const int g = part * 64 + lane;
+      tokens += wave_sum(g < kGroups ? s.group_count[g] : 0);
+      all += wave_sum(g < kGroups ? s.group_mass[g] : 0.0);
+    }
+    Place at = {kBins - 1, 0, 0, 0.0};  // (an unused bin: all that min_p keeps)
+    if (tokens > r.top_k) {
+      at = find_bin(s, kBins, [&](int n, double) { return n >= r.top_k; });
+      at.kept = min(at.kept, r.top_k - at.count_before);
+      all = at.before + at.kept * s.weight[at.bin];
+    }
     if (r.top_p < 1.0) {
       const double target = r.top_p * all;
       const Place cut = find_bin(s, at.bin + 1, [&](int, double m) { return m >= target; });

@@ -85,20 +85,23 @@ def post_norm_add_rms_norm(x: torch.Tensor, y: torch.Tensor, post_weight: torch.
     or [rows, hidden].  x_out may be x, and h_out y; other overlaps are undefined.
     """
     _rows("x", x)
-    shape = rows, hidden = x.shape
-    if x_out is None:
-        x_out = x
-    if h_out is None:
-        h_out = torch.empty(rows, hidden, dtype=x.dtype, device=x.device)
+    shape = x.shape
+    rows, hidden = shape
     device, grad = x.get_device(), torch.is_grad_enabled()
-    for name, t in (("x", x), ("y", y), ("x_out", x_out), ("h_out", h_out)):
-        if (t.shape != shape or t.dtype != torch.bfloat16 or t.get_device() != device or t.stride(1) != 1
-                or (grad and t.requires_grad)):
+    if grad and x.requires_grad:
+        _refuse("x", x, shape, x.device)
+    for name, t in (("y", y), ("x_out", x_out), ("h_out", h_out)):
+        if t is not None and (t.shape != shape or t.dtype != torch.bfloat16 or t.get_device() != device
+                              or t.stride(1) != 1 or (grad and t.requires_grad)):
             _refuse(name, t, shape, x.device)
     for name, t in (("post_weight", post_weight), ("weight", weight)):
         if (t.shape != (hidden,) or t.dtype != torch.bfloat16 or t.get_device() != device or t.stride(0) != 1
                 or (grad and t.requires_grad)):
             _refuse(name, t, (hidden,), x.device)
+    if x_out is None:
+        x_out = x
+    if h_out is None:
+        h_out = torch.empty_like(x) if x.stride(0) == hidden else torch.empty(rows, hidden, dtype=x.dtype, device=x.device)
     g_ptr, g_stride, g_column = None, 0, 0
     if gate is not None:
         if gate.dtype != torch.bfloat16 or gate.get_device() != device or (grad and gate.requires_grad):

@@ -30,11 +30,12 @@ _FEW_ROWS = 16  # no call of up to so many rows takes a workspace
 def _rows_of(name: str, t: torch.Tensor) -> tuple[int, int]:
     require_gpu(name, t)
     require_dtype(name, t, torch.bfloat16)
-    if t.dim() != 2 or t.stride(1) != 1:
-        raise ValueError(f"{name} must be [rows, width] with a contiguous last axis; got {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 2 or t.stride(1) != 1:
+        raise ValueError(f"{name} must be [rows, width] with a contiguous last axis; got {tuple(shape)}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: there is no backward pass")
-    return t.shape[0], t.shape[1]
+    return shape
 
 
 def _out(out: torch.Tensor | None, rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
