@@ -1,9 +1,10 @@
 // Projections of few rows with an MXFP4 weight (decode steps): out = x W^T (+ bias)
 // or silu(x Wg^T) * (x Wu^T), fp32 accumulation and one rounding; x bf16 or MXFP4.
 //
-// Bound: HBM, the one read of W, 0.53 bytes per weight.  A workgroup of 4 waves owns
+// Bound: HBM, the one read of W, 0.53 bytes per weight (a launch starts and ends in 3 to
+// 4 us; beyond that 62 MB, one row, stream at 6.3 TB/s).  A workgroup of 4 or 8 waves owns
 // 16 R rows of W over all of k and the waves split k: wave w takes the slabs of 128 k
-// w, w + 4, ...  A tile of W is an operand as it is loaded, so it goes from memory to
+// w, w + WAVES, ...  A tile of W is an operand as it is loaded, so it goes from memory to
 // the matrix instructions through registers alone, D slabs ahead.  With bf16 rows
 // its codes become bf16 by one instruction per pair, exactly, and x passes through a
 // wave-private LDS slot into operand order; with MXFP4 rows x's tiles are operands
@@ -14,20 +15,19 @@
 namespace mi::mx4 {
 namespace {
 
-constexpr int kWaves = 4;
 constexpr int kXSlot = 16 * kSlab * 2;  // a block of 16 bf16 rows of a slab
 
-template <int R, int MB, int D, bool MX, bool GLU>
-__global__ __launch_bounds__(64 * kWaves) void few_kernel(LinearParams p) {
+template <int R, int MB, int D, bool MX, bool GLU, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
   constexpr int HALVES = GLU ? 2 : 1, COLS = 16 * R / HALVES;
   static_assert(R % HALVES == 0, "gate and up tiles in pairs");
   constexpr int SLOT = MX ? 0 : MB * kXSlot, RED = R * MB * 1024;
-  __shared__ __attribute__((aligned(16))) char smem[kWaves * (SLOT > RED ? SLOT : RED)];
+  __shared__ __attribute__((aligned(16))) char smem[WAVES * (SLOT > RED ? SLOT : RED)];
   lds_t* const lds = (lds_t*)smem;
   const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, n = lane & 15;
   const int col0 = int(blockIdx.x) * COLS;
-  const int steps = (p.slabs - w + kWaves - 1) / kWaves;  // this wave's slabs: w, w + 4, ...
+  const int steps = (p.slabs - w + WAVES - 1) / WAVES;  // this wave's slabs: w, w + WAVES, ...
 
   const char *wbase[HALVES], *sbase[HALVES];
   int wsize[HALVES], ssize[HALVES];
@@ -51,13 +51,13 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(LinearParams p) {
   u32x4_t wr[D][R], xr[D][MX ? MB : 4 * MB];
   uint32_t wscale[D][R], xscale[D][MB];
   auto load = [&](int d, int step) {
-    const int slab = step * kWaves + w;
+    const int slab = step * WAVES + w, quad = (slab >> 2) * kQuadBytes;
     const bool ok = step < steps;
     __amdgpu_buffer_rsrc_t rw[HALVES], rs[HALVES];
 #pragma unroll
     for (int h = 0; h < HALVES; ++h) {
       rw[h] = buffer(wbase[h] + slab * kTileBytes, ok ? wsize[h] - slab * kTileBytes : 0);
-      rs[h] = buffer(sbase[h] + step * kQuadBytes, ok ? ssize[h] - step * kQuadBytes : 0);
+      rs[h] = buffer(sbase[h] + quad, ok ? ssize[h] - quad : 0);
     }
     // W is read once: non-temporal
 #pragma unroll
@@ -67,7 +67,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(LinearParams p) {
     }
     if constexpr (MX) {
       const __amdgpu_buffer_rsrc_t rx = buffer(p.x + slab * kTileBytes, ok ? xsize - slab * kTileBytes : 0);
-      const __amdgpu_buffer_rsrc_t rxs = buffer(p.xs + step * kQuadBytes, ok ? xssize - step * kQuadBytes : 0);
+      const __amdgpu_buffer_rsrc_t rxs = buffer(p.xs + quad, ok ? xssize - quad : 0);
 #pragma unroll
       for (int b = 0; b < MB; ++b) {
         xr[d][b] = __builtin_amdgcn_raw_buffer_load_b128(rx, b * p.slabs * kTileBytes + lane * 16, 0, 0);
@@ -84,6 +84,8 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(LinearParams p) {
     }
   };
 
+  static_assert(WAVES % 4 == 0, "a wave's slabs lie at one place of their groups of four");
+  const int shift = 8 * (w & 3);
   f32x4_t acc[R][MB];
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -109,9 +111,9 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(LinearParams p) {
         u32x4_t a[R], x[MB];
         uint32_t as[R], xs[MB];
 #pragma unroll
-        for (int r = 0; r < R; ++r) a[r] = wr[d][r], as[r] = wscale[d][r] >> (8 * w);
+        for (int r = 0; r < R; ++r) a[r] = wr[d][r], as[r] = wscale[d][r] >> shift;
 #pragma unroll
-        for (int b = 0; b < MB; ++b) x[b] = xr[d][b], xs[b] = xscale[d][b] >> (8 * w);
+        for (int b = 0; b < MB; ++b) x[b] = xr[d][b], xs[b] = xscale[d][b] >> shift;
         load(d, s0 + d + D);
 #pragma unroll
         for (int r = 0; r < R; ++r)
@@ -123,7 +125,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(LinearParams p) {
         u32x4_t a[R];
         float as[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) a[r] = wr[d][r], as[r] = scale_f32(wscale[d][r] >> (8 * w) & 255u);
+        for (int r = 0; r < R; ++r) a[r] = wr[d][r], as[r] = scale_f32(wscale[d][r] >> shift & 255u);
         load(d, s0 + d + D);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
@@ -154,11 +156,11 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(LinearParams p) {
   auto total = [&](int q) {
     f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int o = 0; o < kWaves; ++o)
+    for (int o = 0; o < WAVES; ++o)
       sum += __builtin_bit_cast(f32x4_t, lds_load16(lds + (o * R * MB + q) * 1024 + lane * 16));
     return sum;
   };
-  for (int q = w; q < R / HALVES * MB; q += kWaves) {
+  for (int q = w; q < R / HALVES * MB; q += WAVES) {
     const int r = q / MB, b = q - r * MB;  // r: the tile (or pair of tiles)
     const f32x4_t sum = total(HALVES * r * MB + b);
     f32x4_t up = {0.f, 0.f, 0.f, 0.f};
@@ -168,37 +170,47 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(LinearParams p) {
   }
 }
 
-template <int R, int MB, int D, bool MX, bool GLU>
+template <int R, int MB, int D, bool MX, bool GLU, int WAVES>
 void run(const LinearParams& p, hipStream_t stream) {
   constexpr int COLS = 16 * R / (GLU ? 2 : 1);
-  hipLaunchKernelGGL((few_kernel<R, MB, D, MX, GLU>), dim3((p.n + COLS - 1) / COLS), dim3(64 * kWaves), 0, stream, p);
+  hipLaunchKernelGGL((few_kernel<R, MB, D, MX, GLU, WAVES>), dim3((p.n + COLS - 1) / COLS), dim3(64 * WAVES), 0, stream, p);
 }
 
-// The form of a launch, from the tiles of W and the 16-row blocks of x (us, weights
-// rotated through 600 MB):
-//                              rows   R 1 D 4   R 2 D 2   R 4 D 2   R 8 D 1   R 8 D 2
-//   N  4096 K  4096               8     5.2       6.3       7.2       10.6      10.5
-//   N  4096 K  4096              32     7.9       8.1      10.0       14.1      15.3
-//   N  4096 K 14336               8    12.3      16.8      19.5       32.7      27.9
-//   N 10240 K  8192               8    16.2      13.1      12.8       19.7      17.9
-//   N 10240 K  8192              32    28.7      22.2      17.7       25.4      27.5
-//   gated 2 x 4864, K 896         1               4.8       4.4        5.8       6.2
-//   gated 2 x 14336, K 4096       1              15.6      13.4       14.7      14.1
-//   gated 2 x 14336, K 4096      16              18.1      14.5       14.4      14.0
-//   gated 2 x 14336, K 4096      32              24.6      18.2       15.8      17.7
-//   MXFP4 x: N 4096 K 4096        8     4.0       5.0       6.3        9.9       8.8
-//   MXFP4 x: N 10240 K 8192      48    18.7      15.8      13.7       18.2      19.4
-// Every workgroup reads x, so tiles as many as still leave a workgroup for most CUs:
-// one up to 256 tiles (loads in flight bound it then: D 4), four beyond; eight where
-// there are over 1,024 tiles and x is two blocks, whose bf16 rows are then the larger
-// part of what is read.
+// The form of a launch, from the tiles of W, the slabs and the 16-row blocks of x (us,
+// weights rotated through 600 MB; R tiles per workgroup, D slabs ahead):
+//                             waves:      4                       8
+//                              rows   R 1 D 4  R 2 D 2  R 4 D 2   R 1 D 2  R 1 D 1  R 2 D 1  R 4 D 1
+//   N  1152 K   896               8     3.6      3.1      3.7       3.5      3.1      3.2      3.8
+//   N  4096 K  4096               1     5.0      6.1      7.0       4.8      5.1      5.4      6.5
+//   N  4096 K  4096              32     8.0      8.1     10.0       7.7      7.2      8.3      9.2
+//   N  4096 K 14336               8    12.4     16.8     19.5      11.2     12.0     12.3     16.8
+//   N  6144 K  4096               8              6.5      7.4                6.7      5.6      6.7
+//   N  8192 K  8192              32             13.6     17.4               19.6     13.0     16.2
+//   N 10240 K  8192               8             13.1     13.0      16.2     15.9     14.7     11.6
+//   N 10240 K  8192              32             22.2     17.7               26.9     23.6     16.7
+//   N 28672 K  1024               1              6.7      6.2                8.1      7.0      6.5
+//   gated 2 x 4864, K 896         1              4.9      4.4                         4.6      4.7
+//   gated 2 x 18944, K 3584       8             18.5     18.0                        17.3     16.8
+//   gated 2 x 14336, K 4096      32             24.5     18.2  (R 8 D 1: 15.8)       24.3     19.4
+//   MXFP4 x: N 4096 K 14336       8     9.3     12.0               8.1      10.4      9.9     14.0
+//   MXFP4 x: N 8192 K 8192       64             11.5     14.3               15.5     10.6     14.3
+//   MXFP4 x: N 10240 K 8192      48             15.8     13.7               18.0     16.1     13.0
+// Every workgroup reads x, so tiles as many as still leave a workgroup for most of the
+// CUs; eight waves while k is long enough to feed them.  Two blocks of bf16 rows are
+// the larger part of what is read: eight tiles, while they leave no second round.
 template <int MB, bool MX, bool GLU>
 void pick(const LinearParams& p, hipStream_t stream) {
-  if constexpr (!MX && MB == 2) {
-    if (p.w_tiles > 1024) return run<8, MB, 1, MX, GLU>(p, stream);
+  constexpr int ONE = GLU ? 2 : 1;
+  if (p.w_tiles <= 256) {
+    if (MB == 1 && p.slabs >= 32) return run<ONE, MB, MB == 1 ? 2 : 1, MX, GLU, 8>(p, stream);
+    return run<ONE, MB, 1, MX, GLU, 8>(p, stream);
   }
-  if (p.w_tiles > 256) return run<4, MB, 2, MX, GLU>(p, stream);
-  run<GLU ? 2 : 1, MB, (MB > 1 && !MX ? 2 : 4), MX, GLU>(p, stream);
+  if (p.w_tiles <= 512) return run<2, MB, 1, MX, GLU, 8>(p, stream);
+  if constexpr (!MX && MB == 2) {
+    if (p.w_tiles > 1024 && p.w_tiles <= 2048) return run<8, MB, 1, MX, GLU, 4>(p, stream);
+  }
+  if (p.slabs >= 28) return run<4, MB, 1, MX, GLU, 8>(p, stream);
+  run<4, MB, 2, MX, GLU, 4>(p, stream);
 }
 
 template <bool GLU>
