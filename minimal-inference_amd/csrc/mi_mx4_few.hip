@@ -166,7 +166,7 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
     f32x4_t up = {0.f, 0.f, 0.f, 0.f};
     if constexpr (GLU) up = total((HALVES * r + 1) * MB + b);
     const int m = b * 16 + n, col = col0 + r * 16 + 4 * g;
-    if (m < rows && col < p.n) store4<GLU>(p, m, col, sum, up);
+    if (m < rows && col < p.n) store4<GLU>(p, m, col, sum, up, bias4(p, col));
   }
 }
 

@@ -35,29 +35,34 @@ __device__ __forceinline__ LaneRow lane_row(const LinearParams& p, int base_row,
   return {tile * p.slabs * kTileBytes + at * 16, tile * p.quads * kQuadBytes + at * 4};
 }
 
+// The bias of columns col .. col + 3.
+__device__ __forceinline__ f32x4_t bias4(const LinearParams& p, int col) {
+  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+  if (!p.bias) return v;
+  if (p.vec) {
+    const u32x2_t b = *reinterpret_cast<const u32x2_t*>(p.bias + col);
+    return f32x4_t{bf16_lo(b.x), bf16_hi(b.x), bf16_lo(b.y), bf16_hi(b.y)};
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (col + i < p.n) v[i] = bf16_to_f32(p.bias[col + i]);
+  return v;
+}
+
 // Columns col .. col + 3 of out's row m from a lane's sums (and, gated, those of the
 // up rows): bias or silu(gate) * up in fp32, one rounding.
 template <bool GLU>
-__device__ __forceinline__ void store4(const LinearParams& p, int64_t m, int col, f32x4_t sum, f32x4_t up) {
+__device__ __forceinline__ void store4(const LinearParams& p, int64_t m, int col, f32x4_t sum, f32x4_t up, f32x4_t bias) {
   uint16_t* const out = p.out + m * p.o_stride + col;
-  if constexpr (GLU) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] = silu(sum[i]) * up[i];
-  }
+  for (int i = 0; i < 4; ++i) sum[i] = GLU ? silu(sum[i]) * up[i] : sum[i] + bias[i];
   if (p.vec) {
-    if (!GLU && p.bias) {
-      const u32x2_t b = *reinterpret_cast<const u32x2_t*>(p.bias + col);
-      sum[0] += bf16_lo(b.x);
-      sum[1] += bf16_hi(b.x);
-      sum[2] += bf16_lo(b.y);
-      sum[3] += bf16_hi(b.y);
-    }
     *reinterpret_cast<u32x2_t*>(out) = u32x2_t{cvt_pk_bf16(sum[0], sum[1]), cvt_pk_bf16(sum[2], sum[3])};
     return;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (col + i < p.n) out[i] = cvt_bf16(!GLU && p.bias ? sum[i] + bf16_to_f32(p.bias[col + i]) : sum[i]);
+    if (col + i < p.n) out[i] = cvt_bf16(sum[i]);
 }
 
 // Slot of 16-byte chunk c in a staged row of 256 bytes: the 8 rows that an operand

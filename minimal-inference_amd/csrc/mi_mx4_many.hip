@@ -219,6 +219,7 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
   for (int t = 0; t < NT; t += HALVES) {
     const int col = col0 + (wn * NT + t) / HALVES * 16 + 4 * g;
     if (col >= p.n) continue;
+    const f32x4_t bias = SPLIT ? f32x4_t{0.f, 0.f, 0.f, 0.f} : bias4(p, col);
 #pragma unroll
     for (int b = 0; b < MB; ++b) {
       const int m = (wm * MB + b) * 16 + n;
@@ -230,7 +231,7 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
         for (int h = 0; h < HALVES; ++h)
           p.parts[((int64_t(blockIdx.y) * HALVES + h) * p.rows + m0 + m) * fours + col / 4] = acc[t + h][b];
       } else {
-        store4<GLU>(p, m0 + m, col, acc[t][b], acc[t + HALVES - 1][b]);
+        store4<GLU>(p, m0 + m, col, acc[t][b], acc[t + HALVES - 1][b], bias);
       }
     }
   }
@@ -250,7 +251,8 @@ __global__ __launch_bounds__(256) void combine_kernel(LinearParams p, int parts)
     sum += p.parts[i * HALVES * one + at];
     if constexpr (GLU) up += p.parts[(i * HALVES + 1) * one + at];
   }
-  store4<GLU>(p, at / fours, int(at % fours) * 4, sum, up);
+  const int col = int(at % fours) * 4;
+  store4<GLU>(p, at / fours, col, sum, up, bias4(p, col));
 }
 
 // ---------------------------------------------------------------- which form
