@@ -256,23 +256,25 @@ __global__ __launch_bounds__(256) void combine_kernel(LinearParams p, int parts)
 }
 
 // ---------------------------------------------------------------- which form
-// Forms of the kernel: rows of x and of W per workgroup, and the time of a slab with
-// one workgroup on every CU (us, measured; the larger the block, the fewer the bytes
-// that each product needs and the fewer the workgroups).  A launch takes its start, a
-// slab's time for every slab of every round of workgroups, and, where workgroups share
-// k, the combining launch with the parts' way to memory and back.  Model and measured
-// (us): 77 x 18,944 x 3,584, 80-row blocks, 9 parts 21.9 / 22.5, whole 95.3 / 95.5;
-// 128 x 8,192 x 10,240, 128 x 128, 3 parts 32.2 / 32.2, whole 59.2 / 57.9;
-// 512 x 14,336 x 4,096, 128 x 128, 2 parts 64.3 / 62.9, whole 100.9 / 95.9.
+// Forms of the kernel: rows of x and of W per workgroup, and the time of a slab (us,
+// measured) with one workgroup on a CU and, per workgroup, with more of them in turn or
+// side by side.  The larger the block, the fewer the bytes that each product needs and
+// the fewer the workgroups.  A launch takes its start, a slab's time for every slab of
+// every workgroup of a CU, the way of its output to memory, and, where workgroups share
+// k, the combining launch with the parts' way there and back.  Model and measured (us):
+// 77 x 18,944 x 3,584, 80-row blocks, 9 parts 22.0 / 22.5, whole 96.9 / 95.5;
+// 128 x 8,192 x 10,240, 128 x 128, 3 parts 32.3 / 32.2; bf16 1,024 x 8,192 x 10,240,
+// 128 x 128 in fours of waves 162 / 159, 128 x 256 197 / 184; in 4 bits 2,048 x 8,192 x
+// 10,240, 128 x 128 118 / 105, 128 x 256 118 / 104, 256 x 256 144 / 125.
 struct Form {
   int rows, tiles;  // 16-row tiles of W
-  float slab_us;
+  float one_us, more_us;
   bool split;
 };
-constexpr Form kBf16Forms[] = {{32, 8, 0.45f, true}, {64, 8, 0.56f, true}, {80, 8, 0.63f, true}, {128, 8, 0.87f, true},
-                               {128, 16, 1.6f, false}};
-constexpr Form kMxForms[] = {{128, 8, 0.34f, true}, {256, 16, 1.0f, false}};
-constexpr float kStartUs = 3.5f, kCombineUs = 2.5f, kCombineBytesPerUs = 4.4e6f;
+constexpr Form kBf16Forms[] = {{32, 8, 0.45f, 0.45f, true}, {64, 8, 0.56f, 0.56f, true}, {80, 8, 0.63f, 0.63f, true},
+                               {128, 8, 0.86f, 0.93f, true}, {128, 8, 1.0f, 0.8f, false}, {128, 16, 1.45f, 1.5f, false}};
+constexpr Form kMxForms[] = {{128, 8, 0.385f, 0.33f, true}, {128, 16, 0.56f, 0.53f, false}, {256, 16, 1.02f, 1.02f, false}};
+constexpr float kStartUs = 3.5f, kCombineUs = 2.5f, kBytesPerUs = 4.4e6f;
 constexpr int kMaxParts = 32;
 
 struct Choice {
@@ -284,7 +286,7 @@ struct Choice {
 // The fastest by that count within `room` bytes for parts.
 Choice choose(bool mx, bool glu, int64_t rows, int64_t n, int slabs, size_t room) {
   Choice best = {1e30f, 0, 1, slabs, 0};
-  const int cus = mi::num_cus(), forms = mx ? 2 : 5;
+  const int cus = mi::num_cus(), forms = mx ? 3 : 6;
   for (int f = 0; f < forms; ++f) {
     const Form& form = mx ? kMxForms[f] : kBf16Forms[f];
     const int64_t cols = form.tiles * kTileRows / (glu ? 2 : 1);
@@ -294,8 +296,9 @@ Choice choose(bool mx, bool glu, int64_t rows, int64_t n, int slabs, size_t room
       if (parts != want || (want > 1 && (each < 2 || tiles * (want - 1) >= 2 * cus))) continue;
       const size_t bytes = want > 1 ? size_t(want) * (glu ? 2 : 1) * rows * ((n + 3) / 4) * 16 : 0;
       if (bytes > room) continue;
-      float us = kStartUs + float((tiles * want + cus - 1) / cus) * each * form.slab_us;
-      if (want > 1) us += kCombineUs + 2 * float(bytes) / kCombineBytesPerUs;
+      const int64_t per_cu = (tiles * want + cus - 1) / cus;
+      float us = kStartUs + each * (per_cu == 1 ? form.one_us : float(per_cu) * form.more_us);
+      us += want > 1 ? kCombineUs + 2 * float(bytes) / kBytesPerUs : 2 * float(rows) * float(n) / kBytesPerUs;
       if (us < best.us) best = {us, f, want, each, bytes};
     }
   }
@@ -316,12 +319,14 @@ template <bool MX, bool GLU, bool SPLIT>
 void run_form(const LinearParams& p, int form, int parts, hipStream_t stream) {
   if constexpr (MX) {
     if (SPLIT || form == 0) run<2, 2, 4, 4, 4, true, GLU, SPLIT>(p, parts, stream);
+    else if (form == 1) run<2, 4, 4, 4, 3, true, GLU, false>(p, 1, stream);
     else run<2, 4, 8, 4, 2, true, GLU, false, 2>(p, 1, stream);
   } else {
     if (form == 0) run<1, 4, 2, 2, 4, false, GLU, SPLIT>(p, parts, stream);
     else if (form == 1) run<2, 4, 2, 2, 4, false, GLU, SPLIT>(p, parts, stream);
     else if (form == 2) run<1, 4, 5, 2, 4, false, GLU, SPLIT>(p, parts, stream);
     else if (SPLIT || form == 3) run<2, 4, 4, 2, 3, false, GLU, SPLIT>(p, parts, stream);
+    else if (form == 4) run<2, 2, 4, 4, 2, false, GLU, false>(p, 1, stream);
     else run<2, 4, 4, 4, 3, false, GLU, false>(p, 1, stream);
   }
 }
