@@ -10,6 +10,10 @@
 // wave-private LDS slot into operand order; with MXFP4 rows x's tiles are operands
 // too and one scaled instruction does a slab.  The waves meet once, at the end, where
 // their accumulators are added in wave order: the result does not depend on timing.
+// More rows than the accumulators hold (64 of MXFP4, 32 of bf16) are groups of their own
+// workgroups, which read W again, from the caches.
+#include <algorithm>
+
 #include "mi_mx4_linear.h"
 
 namespace mi::mx4 {
@@ -44,7 +48,10 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
   }
   // bf16: load i of block b takes 4 rows, lane l chunk l % 16 of row l / 16
   const int lr = lane >> 4, lc = lane & 15;
-  const int rows = int(p.rows), stride = int(p.x_stride * 2);
+  const int64_t m0 = int64_t(blockIdx.y) * (16 * MB);
+  const int rows = int(min(p.rows - m0, int64_t(16 * MB))), stride = int(p.x_stride * 2);
+  const char* const x = p.x + (MX ? m0 / kTileRows * p.slabs * kTileBytes : m0 * stride);
+  const char* const xs = p.xs + (MX ? m0 / kTileRows * p.quads * kQuadBytes : 0);
   const int xsize = MX ? (rows + 15) / 16 * p.slabs * kTileBytes : (rows - 1) * stride + p.k * 2;
   const int xssize = (rows + 15) / 16 * p.quads * kQuadBytes;
 
@@ -66,8 +73,8 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
       wscale[d][r] = __builtin_amdgcn_raw_buffer_load_b32(rs[r % HALVES], at[r].scales, 0, 0);
     }
     if constexpr (MX) {
-      const __amdgpu_buffer_rsrc_t rx = buffer(p.x + slab * kTileBytes, ok ? xsize - slab * kTileBytes : 0);
-      const __amdgpu_buffer_rsrc_t rxs = buffer(p.xs + quad, ok ? xssize - quad : 0);
+      const __amdgpu_buffer_rsrc_t rx = buffer(x + slab * kTileBytes, ok ? xsize - slab * kTileBytes : 0);
+      const __amdgpu_buffer_rsrc_t rxs = buffer(xs + quad, ok ? xssize - quad : 0);
 #pragma unroll
       for (int b = 0; b < MB; ++b) {
         xr[d][b] = __builtin_amdgcn_raw_buffer_load_b128(rx, b * p.slabs * kTileBytes + lane * 16, 0, 0);
@@ -75,7 +82,7 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
       }
     } else {
       const int off = slab * kSlab * 2;
-      const __amdgpu_buffer_rsrc_t rx = buffer(p.x + off, ok ? xsize - off : 0);
+      const __amdgpu_buffer_rsrc_t rx = buffer(x + off, ok ? xsize - off : 0);
       // past a row's end lies the next row: out of range instead
       const bool in = off + lc * 16 < p.k * 2;
 #pragma unroll
@@ -108,17 +115,17 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
 #pragma unroll
     for (int d = 0; d < D; ++d) {
       if constexpr (MX) {
-        u32x4_t a[R], x[MB];
-        uint32_t as[R], xs[MB];
+        u32x4_t a[R], xc[MB];
+        uint32_t as[R], xsc[MB];
 #pragma unroll
         for (int r = 0; r < R; ++r) a[r] = wr[d][r], as[r] = wscale[d][r] >> shift;
 #pragma unroll
-        for (int b = 0; b < MB; ++b) x[b] = xr[d][b], xs[b] = xscale[d][b] >> shift;
+        for (int b = 0; b < MB; ++b) xc[b] = xr[d][b], xsc[b] = xscale[d][b] >> shift;
         load(d, s0 + d + D);
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int b = 0; b < MB; ++b) acc[r][b] = mfma_fp4<0, 0>(a[r], as[r], x[b], xs[b], acc[r][b]);
+          for (int b = 0; b < MB; ++b) acc[r][b] = mfma_fp4<0, 0>(a[r], as[r], xc[b], xsc[b], acc[r][b]);
       } else {
 #pragma unroll
         for (int i = 0; i < 4 * MB; ++i) lds_store16(slot + i * 1024 + so[i & 1], xr[d][i]);
@@ -129,15 +136,15 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
         load(d, s0 + d + D);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          bf16x8_t x[MB];
+          bf16x8_t xv[MB];
 #pragma unroll
           for (int b = 0; b < MB; ++b)
-            x[b] = __builtin_bit_cast(bf16x8_t, lds_load16(slot + b * kXSlot + ro[s]));
+            xv[b] = __builtin_bit_cast(bf16x8_t, lds_load16(slot + b * kXSlot + ro[s]));
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const bf16x8_t v = to_bf16(a[r][s], as[r]);
 #pragma unroll
-            for (int b = 0; b < MB; ++b) acc[r][b] = mfma_16x16x32_bf16(v, x[b], acc[r][b]);
+            for (int b = 0; b < MB; ++b) acc[r][b] = mfma_16x16x32_bf16(v, xv[b], acc[r][b]);
           }
         }
       }
@@ -166,14 +173,15 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
     f32x4_t up = {0.f, 0.f, 0.f, 0.f};
     if constexpr (GLU) up = total((HALVES * r + 1) * MB + b);
     const int m = b * 16 + n, col = col0 + r * 16 + 4 * g;
-    if (m < rows && col < p.n) store4<GLU>(p, m, col, sum, up, bias4(p, col));
+    if (m < rows && col < p.n) store4<GLU>(p, m0 + m, col, sum, up, bias4(p, col));
   }
 }
 
 template <int R, int MB, int D, bool MX, bool GLU, int WAVES>
 void run(const LinearParams& p, hipStream_t stream) {
   constexpr int COLS = 16 * R / (GLU ? 2 : 1);
-  hipLaunchKernelGGL((few_kernel<R, MB, D, MX, GLU, WAVES>), dim3((p.n + COLS - 1) / COLS), dim3(64 * WAVES), 0, stream, p);
+  const dim3 grid((p.n + COLS - 1) / COLS, uint32_t((p.rows + 16 * MB - 1) / (16 * MB)));
+  hipLaunchKernelGGL((few_kernel<R, MB, D, MX, GLU, WAVES>), grid, dim3(64 * WAVES), 0, stream, p);
 }
 
 // The form of a launch, from the tiles of W, the slabs and the 16-row blocks of x (us,
@@ -215,7 +223,7 @@ void pick(const LinearParams& p, hipStream_t stream) {
 
 template <bool GLU>
 void launch(const LinearParams& p, hipStream_t stream) {
-  const int blocks = int((p.rows + 15) / 16);
+  const int blocks = int((std::min(p.rows, few_group(p.xs != nullptr)) + 15) / 16);
   if (p.xs) {
     if (blocks == 1) pick<1, true, GLU>(p, stream);
     else if (blocks == 2) pick<2, true, GLU>(p, stream);

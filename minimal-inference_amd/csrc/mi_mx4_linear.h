@@ -71,7 +71,10 @@ __device__ __forceinline__ int chunk_slot(int r, int c) { return c ^ ((r & 7) <<
 
 constexpr int64_t kMaxRows = 1 << 22, kMaxN = 1 << 24, kMaxStride = 1 << 22;
 
-// Whether the few-row kernel is the faster one.  (Two blocks of bf16 rows along a long k
+// The rows that a workgroup of the few-row kernel takes at most.
+constexpr int64_t few_group(bool mx) { return mx ? 64 : 32; }
+
+// Whether the few-row kernel is the faster one in any case.  (Two blocks of bf16 rows along a long k
 // are read by every one of its workgroups: 32 x 14,336 x 4,096 19.1 us, the blocks of
 // 128 rows of W with k in parts 14.5; 32 x 4,096 x 4,096 7.6, 10.0.)
 inline bool few(bool mx, int64_t rows, int64_t w_rows, int64_t k) {

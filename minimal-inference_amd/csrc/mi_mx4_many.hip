@@ -305,8 +305,16 @@ Choice choose(bool mx, bool glu, int64_t rows, int64_t n, int slabs, size_t room
   return best;
 }
 
-// The few-row kernel's time, from W's bytes.
-float few_us(const LinearParams& p) { return 4.f + float(p.w_tiles) * p.slabs * 1.0625e3f / 4e6f; }
+// The few-row kernel's time: W's bytes once for every group of rows, beyond the first
+// from the caches.  More groups than one are faster than blocks of 128 rows where W is
+// small (128 x 4,096 x 4,096 in 4 bits 6.0 us, in blocks 13; 64 x 4,096 x 6,144 of bf16
+// rows 11 and 13; the count's 8.4 and 13, 11 and 13); more than 512 rows are not
+// measured and not asked for.
+float few_us(bool mx, int64_t rows, int w_tiles, int slabs) {
+  if (rows > 512) return 1e30f;
+  const int64_t group = few_group(mx);
+  return 4.f + float((rows + group - 1) / group * w_tiles) * slabs * (kTileBytes + kQuadBytes / 4) / (mx ? 4e6f : 3.5e6f);
+}
 
 template <int WM, int WN, int MB, int NT, int STAGES, bool MX, bool GLU, bool SPLIT, int PER = 1>
 void run(const LinearParams& p, int parts, hipStream_t stream) {
@@ -354,18 +362,20 @@ int64_t rest_of(bool mx, int64_t rows) {
 }  // namespace
 
 size_t many_workspace(bool mx, bool glu, int64_t rows, int64_t n, int slabs) {
-  return choose(mx, glu, rows, n, slabs, size_t(1) << 28).bytes;
+  const Choice c = choose(mx, glu, rows, n, slabs, size_t(1) << 28);
+  return few_us(mx, rows, int(row_tiles(glu ? 2 * n : n)), slabs) < c.us ? 0 : c.bytes;
 }
 
 void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t stream) {
   const bool mx = p.xs != nullptr;
   LinearParams q = p;
   Choice c = choose(mx, glu, p.rows, p.n, p.slabs, room);
+  if (few_us(mx, p.rows, p.w_tiles, p.slabs) < c.us) return launch_few(p, glu, stream);
   // (4,105 x 4,096 x 6,144: 792 blocks are four rounds; 768 and nine rows of the few-row
   // kernel three and 7 us)
   if (const int64_t rest = rest_of(mx, p.rows)) {
     const Choice whole = choose(mx, glu, p.rows - rest, p.n, p.slabs, room);
-    if (whole.us + few_us(p) < c.us) {
+    if (whole.us + few_us(mx, rest, p.w_tiles, p.slabs) < c.us) {
       c = whole;
       q.rows = p.rows - rest;
     }

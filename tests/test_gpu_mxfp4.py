@@ -304,10 +304,14 @@ def test_empty_and_refused(dev):
 @pytest.mark.parametrize("rows,n,k", [
     (20, 300, 8192), (33, 520, 2080), (64, 2048, 4096), (65, 130, 18944), (80, 1000, 896), (81, 1000, 4000),
     (128, 640, 8192), (137, 384, 1024), (256, 256, 14336), (265, 4096, 512), (521, 96, 2048), (1024, 2048, 256),
-    (2057, 4096, 160), (2304, 3000, 416), (4100, 520, 96)])
+    (2057, 4096, 160), (2304, 3000, 416), (4100, 520, 96), (320, 77, 96), (512, 300, 160), (531, 124, 1184),
+    (528, 36, 1184), (649, 80, 6496), (1349, 152, 2624), (2563, 148, 5920), (1432, 34, 3680), (2179, 40, 5440),
+    (81, 1773, 7968), (591, 1676, 64), (133, 11615, 64), (165, 10884, 64), (564, 8256, 64), (1205, 6524, 64),
+    (528, 7352, 64), (1539, 7712, 64), (1284, 4530, 64), (1290, 916, 7200), (1159, 1028, 7392), (2053, 467, 10080),
+    (650, 3891, 3392), (2563, 3116, 672), (1295, 6303, 544), (4671, 1788, 1216), (4124, 4007, 928)])
 def test_every_form_of_whole_numbers(dev, rows, n, k, silu, acts):
-    """Sizes on which the forms (blocks of 32 to 256 rows, k whole and in parts, rows
-    behind the last whole block) differ: sums exact in fp32 are the exact ones, with a
+    """Sizes on which the forms (groups of 32 or 64 rows, blocks of 32 to 256 rows, k
+    whole and in parts, rows behind the last whole block) differ: sums exact in fp32 are the exact ones, with a
     workspace and without one, strided rows and what lies around them included."""
     from minimal_inference_amd import _lib
     from minimal_inference_amd.mxfp4 import linear_mxfp4, linear_silu_mxfp4, quantize_mxfp4
