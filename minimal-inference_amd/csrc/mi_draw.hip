@@ -21,11 +21,12 @@
 // other values outside the counted range takes the draw kernel's second path, which
 // finds the same boundary by bisection over the 2^16 values, a pass over the row each.
 //
-// Bound: latency.  48 rows x 152,064 (us): count 8.6, of which the LDS atomics take 3.5 (16
-// cycles a wave's, at any spread of values) and the arithmetic of a token's bin as much
-// beside them; draw 21, a chain on one CU per row: 3 until the row's counts are there,
-// 2 for the powers and sums, 1.4 for the boundary, 1 for the chunks' masses, 5 for 32,768
-// tokens' weights out of LDS, 1.5 to the token.  One row of 32,768: 3.9 and 10.
+// Bound: latency.  48 rows x 152,064 (us): count 6.6 to 7.9, of which the LDS atomics take
+// 3.5 (16 cycles a wave's, at any spread of values); draw 15.8, a chain on one CU per
+// row: 3 until the row's counts are there, 2 for the powers and sums, 1.4 for the
+// boundary, 1 for the chunks' masses, 2 for 32,768 tokens' weights out of LDS, 1.5 to the
+// token.  One row of 32,768: 3.8 and 10.  The bins of two tokens come from 16-bit
+// instructions on both: with a 32-bit one for each, 9.1 + 21.1.
 // (In the first form every thread had a contiguous run of bins, sums went through LDS
 // shuffles and all waves searched alike: 13 + 45, one row 11 + 23.)
 #include <math.h>
@@ -175,11 +176,14 @@ __device__ __forceinline__ T block_sum(T v, T* red) {
 
 typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
 typedef __attribute__((ext_vector_type(2))) short s16x2_t;
-// The keys (without the NaN rule) of a pair of tokens.
-__device__ __forceinline__ u16x2_t key_pair(uint32_t x) {
-  const s16x2_t sign = __builtin_bit_cast(s16x2_t, x) >> 15;
-  const s16x2_t mag = __builtin_bit_cast(s16x2_t, x & 0x7fff7fffu);
-  return __builtin_bit_cast(u16x2_t, (mag ^ sign) - sign) + (unsigned short)0x8000;
+// The bins of a pair of tokens, by 16-bit instructions on both at once.  As signed
+// numbers in descending order of value over all values, NaN apart and those of a
+// magnitude in (0, 2^-30), which come out as zero's; from 2^8 on negative.
+__device__ __forceinline__ s16x2_t bin_pair(uint32_t x) {
+  const u16x2_t off = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2_t, x & 0x7fff7fffu),
+                                                    u16x2_t(kLoField * 128 - 1));
+  const s16x2_t flip = __builtin_bit_cast(s16x2_t, ~x) >> 15;
+  return (__builtin_bit_cast(s16x2_t, off) ^ flip) - flip + short(kZeroBin);
 }
 
 // G groups of eight tokens per thread, 8,192 G tokens per workgroup.
@@ -209,43 +213,39 @@ __global__ __launch_bounds__(kThreads) void count_kernel(DrawParams p) {
   // the largest key (NaN 0, or highest where the row is greedy), and the counts
   auto place = [&](int i, int h) { return ((i >> 2) * kThreads + tid) * 8 + (i & 3) * 2 + h; };
   // Without a branch per token (with one it took twice as long): a value outside the
-  // bins counts in an unused one of its lane's own, since all of a wave's on one, as
-  // masked tokens are, would queue.
-  const uint32_t spare = uint32_t(kSpareBin + (tid & 63));
-  u16x2_t mags = {0, 0}, keys = {0, 0};
-  bool other = false;
+  // bins counts in one behind them, most often its lane's own, since all of a wave's on
+  // one, as masked tokens are, would queue.
+  const u16x2_t spare = u16x2_t((unsigned short)(kSpareBin + (tid & 63)));
+  u16x2_t mags = {0, 0}, least = {0xffff, 0xffff};  // magnitudes: the largest, and the least less one, zeros apart
+  s16x2_t bins = {0x7fff, 0x7fff};
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     if (base + (g * kThreads + tid) * 8 >= p.vocab) break;
 #pragma unroll
     for (int i = 4 * g; i < 4 * g + 4; ++i) {
-      mags = __builtin_elementwise_max(mags, __builtin_bit_cast(u16x2_t, v[i] & 0x7fff7fffu));
-      keys = __builtin_elementwise_max(keys, key_pair(v[i]));
+      const u16x2_t mag = __builtin_bit_cast(u16x2_t, v[i] & 0x7fff7fffu);
+      const s16x2_t pair = bin_pair(v[i]);
+      mags = __builtin_elementwise_max(mags, mag);
+      least = __builtin_elementwise_min(least, mag - (unsigned short)1);
+      bins = __builtin_elementwise_min(bins, pair);
+      if (greedy) continue;
+      const u16x2_t bin = __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, pair), spare);
+      atomicAdd(&hist[bin.x], 1u);
+      atomicAdd(&hist[bin.y], 1u);
     }
-    if (greedy) continue;
-#pragma unroll
-    for (int i = 4 * g; i < 4 * g + 4; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t mag = h ? v[i] >> 16 & 0x7fffu : v[i] & 0x7fffu;
-        const bool negative = h ? int(v[i]) < 0 : (v[i] & 0x8000u) != 0;
-        const uint32_t above = kZeroBin + (kLoField * 128 - 1) - mag, below = kZeroBin - (kLoField * 128 - 1) + mag;
-        const bool in = mag - kLoField * 128 < unsigned(kSide);
-        uint32_t bin = negative ? below : above;
-        bin = in ? bin : spare;
-        bin = mag ? bin : uint32_t(kZeroBin);
-        other |= bin == spare;
-        atomicAdd(&hist[bin], 1u);
-      }
   }
-  uint32_t top = max(uint32_t(keys.x), uint32_t(keys.y));
-  const bool nan_here = max(uint32_t(mags.x), uint32_t(mags.y)) > 0x7f80u;
+  const uint32_t most = max(uint32_t(mags.x), uint32_t(mags.y));
+  const bool tiny = min(uint32_t(least.x), uint32_t(least.y)) < kLoField * 128 - 1;
+  // NaN, or values whose bins do not say their order
+  const bool by_key = most > 0x7f80u || tiny, other = most >= kHiField * 128u || tiny;
+  const int top_bin = min(int(bins.x), int(bins.y));
+  uint32_t top = top_bin == 0x7fff ? 0u : key_of_bin(top_bin);
   const uint32_t nan = greedy ? 0xffffu : 0u;
   auto key_at = [&](int i, int h) -> uint32_t {
     const int local = place(i, h);
     return base + local < p.vocab ? key_of(h ? v[i] >> 16 : v[i] & 0xffffu, nan) : 0u;
   };
-  if (nan_here) {
+  if (by_key) {
     top = 0;
 #pragma unroll
     for (int i = 0; i < 4 * G; ++i) top = max(top, max(key_at(i, 0), key_at(i, 1)));
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(kThreads) void count_kernel(DrawParams p) {
   const int64_t slot = row * p.chunks + chunk;
   if (mine == top) {
     int at = 0;  // 0x10000 - the first place
-    if (nan_here) {
+    if (by_key) {
 #pragma unroll
       for (int i = 4 * G - 1; i >= 0; --i)
 #pragma unroll
@@ -268,9 +268,9 @@ __global__ __launch_bounds__(kThreads) void count_kernel(DrawParams p) {
     } else {
 #pragma unroll
       for (int i = 4 * G - 1; i >= 0; --i) {
-        const u16x2_t k = key_pair(v[i]);
-        if (k.y == top) at = 0x10000 - place(i, 1);
-        if (k.x == top) at = 0x10000 - place(i, 0);
+        const s16x2_t pair = bin_pair(v[i]);
+        if (pair.y == top_bin) at = 0x10000 - place(i, 1);
+        if (pair.x == top_bin) at = 0x10000 - place(i, 0);
       }
     }
     if (at) atomicMax(&first, at);
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(kThreads) void count_kernel(DrawParams p) {
   for (int i = 0; i < kPairs; ++i) {
     const int d = i * kThreads + tid;
     uint2 c = *reinterpret_cast<const uint2*>(&hist[2 * d]);
-    if (2 * d >= kSpareBin) c = make_uint2(0u, 0u);
+    if (2 * d >= 2 * kSide) c = make_uint2(2 * d == 2 * kSide ? c.x : 0u, 0u);  // (behind the last bin)
     counts[d] = c.x | c.y << 16;
   }
 }
@@ -641,7 +641,10 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
       at.bin = cut.bin;
       all = cut.before + at.kept * s.weight[at.bin];
     }
-    if (lane == 0) s.last = at, s.total = all;
+    if (lane == 0) {
+      s.last = at, s.total = all;
+      s.weight[min(at.bin, 2 * kSide) + 1] = 0.0;  // the weight of all tokens that are not kept
+    }
   }
   __syncthreads();
   // kept: the bins before last_bin and the first `ties` tokens of it
@@ -654,16 +657,18 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
 #pragma unroll
     for (int j = 0; j < kPairs; ++j) {
       const int bin = 2 * (j * kThreads + tid), group = j * kWaves + wave;
+      if (j * kThreads + tid == last_bin / 2) {
+#pragma unroll
+        for (int q = 0; q < kTogether; ++q)
+          if (c0 + q < p.chunks) s.chunk_ties[c0 + q] = int(counts[q][j] >> (16 * (last_bin & 1)) & 0xffffu);
+      }
       if (128 * group > last_bin || s.group_count[group] == 0) continue;
       double2 w = *reinterpret_cast<const double2*>(&s.weight[bin]);
       if (bin >= last_bin) w.x = 0.0;
       if (bin + 1 >= last_bin) w.y = 0.0;
 #pragma unroll
-      for (int q = 0; q < kTogether; ++q) {
+      for (int q = 0; q < kTogether; ++q)
         m[q] += whole(counts[q][j] & 0xffffu) * w.x + whole(counts[q][j] >> 16) * w.y;
-        if (j * kThreads + tid == last_bin / 2 && c0 + q < p.chunks)
-          s.chunk_ties[c0 + q] = int(counts[q][j] >> (16 * (last_bin & 1)) & 0xffffu);
-      }
     }
     const double four = wave_sum4(m[0], m[1], m[2], m[3]);
     if (lane < 4 && c0 + lane < p.chunks) s.mass[c0 + lane][wave] = four;
@@ -696,22 +701,23 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
   // Its tokens once more: wave w has 512 G of them in a row, group i of a lane the
   // eight from 512 i + 8 lane on.
   const int first = chunk * kChunk + wave * 512 * G + lane * 8;
-  uint4 v[G];
+  const u16x2_t past = u16x2_t((unsigned short)(min(last_bin, 2 * kSide) + 1));
+  u16x2_t bins[G][4];  // of its tokens, `past` for those that are not kept
 #pragma unroll
   for (int i = 0; i < G; ++i) {
-    v[i] = make_uint4(kPad, kPad, kPad, kPad);
-    if (first + i * 512 < p.vocab) v[i] = load8(r.logits, first + i * 512, p.vocab);
+    const uint4 v = first + i * 512 < p.vocab ? load8(r.logits, first + i * 512, p.vocab) : make_uint4(kPad, kPad, kPad, kPad);
+    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bins[i][j] = __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, bin_pair(x[j])), past);
   }
-  const bool some = s.chunk_ties[chunk] > room;  // not all of its tokens with the last value are kept
-  uint32_t dropped[G] = {};                      // of a group's eight, a bit each
-  if (some) {
+  if (s.chunk_ties[chunk] > room) {  // not all of its tokens with the last value are kept
     int n = 0, inc[G];
-    uint32_t same[G];
+    uint32_t same[G];  // of a group's eight, a bit each
 #pragma unroll
     for (int i = 0; i < G; ++i) {
       same[i] = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) same[i] |= uint32_t(bin_of(token(v[i], j)) == last_bin) << j;
+      for (int j = 0; j < 8; ++j) same[i] |= uint32_t(bins[i][j / 2][j & 1] == last_bin) << j;
       inc[i] = wave_scan(int(__popc(same[i])));
       const int all = last_lane(inc[i]);
       inc[i] += n;
@@ -728,15 +734,11 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
       int rank = ahead + inc[i] - int(__popc(same[i]));
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (same[i] >> j & 1) dropped[i] |= uint32_t(rank++ >= room) << j;
+        if ((same[i] >> j & 1) && rank++ >= room) bins[i][j / 2][j & 1] = past.x;
     }
   }
   // a token's kept weight
-  auto held = [&](int i, int j) -> double {
-    const unsigned bin = unsigned(bin_of(token(v[i], j)));
-    const double m = s.weight[min(bin, unsigned(kBins - 1))];  // (the last bin is an unused one)
-    return bin > unsigned(last_bin) || (dropped[i] >> j & 1) ? 0.0 : m;
-  };
+  auto held = [&](int i, int j) -> double { return s.weight[bins[i][j / 2][j & 1]]; };
   double group[G], mine = 0.0;
 #pragma unroll
   for (int i = 0; i < G; ++i) {
