@@ -18,8 +18,8 @@
 //          thread; prefix sums of count and mass give the last kept value and how many
 //          tokens of it; each chunk's kept mass gives the chunk of the draw, whose
 //          tokens are read once more.
-// Values below -2^8 weigh nothing beside a maximum that is 45 t above; a row that holds
-// other values outside the counted range takes the draw kernel's second path, which
+// Values from -2^8 down weigh nothing beside a maximum that is 45 t above; a row that
+// holds other values outside the counted range takes the draw kernel's second path, which
 // finds the same boundary by bisection over the 2^16 values, a pass over the row each.
 //
 // Bound: latency.  48 rows x 152,064 (us): count 6.6 to 7.9, of which the LDS atomics take
@@ -47,8 +47,9 @@ constexpr int kBins = kThreads * kPairs * 2;  // in descending order of value; t
 constexpr int kGroups = kBins / 128;          // a wave's share of one pair per thread
 constexpr int kSpareBin = kBins - 64;
 static_assert(2 * kSide + 1 <= kSpareBin && kSpareBin % 2 == 0, "bins");
-// what a chunk holds outside the bins
-constexpr uint32_t kTinyOrHigh = 1, kLow = 2;
+// What a chunk holds outside the bins: this and up for tiny or high values, else the key
+// of its largest finite value from -2^8 down, or 0.
+constexpr uint32_t kTinyOrHigh = 0x10000;
 // Order-preserving keys: 0x8000 + the magnitude's bits with the sign; NaN 0 (never
 // drawn) or, in greedy rows, 0xffff (above +inf).
 constexpr uint32_t kMinusInf = 0x8000 - 0x7f80;
@@ -285,9 +286,9 @@ __global__ __launch_bounds__(kThreads) void count_kernel(DrawParams p) {
       for (int h = 0; h < 2; ++h) {
         const uint32_t b = h ? v[i] >> 16 : v[i] & 0xffffu, key = key_of(b, 0);
         if (key > kMinusInf && bin_of(b) < 0)
-          seen |= key < 0x8000u && (b & 0x7fffu) >= kHiField * 128u ? kLow : kTinyOrHigh;
+          seen = max(seen, key < 0x8000u && (b & 0x7fffu) >= kHiField * 128u ? key : kTinyOrHigh);
       }
-    if (seen) atomicOr(&outside, seen);
+    if (seen) atomicMax(&outside, seen);
   }
   __syncthreads();
   if (tid == 0) {
@@ -555,7 +556,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
   load_counts(0);
   for (int o = 1; o < p.chunks; o <<= 1) {
     top = max(top, (unsigned long long)__shfl_xor((long long)top, o));
-    outside |= uint32_t(__shfl_xor(int(outside), o));
+    outside = max(outside, uint32_t(__shfl_xor(int(outside), o)));
   }
   top = (unsigned long long)__builtin_amdgcn_readfirstlane(int(top >> 32)) << 32 |
         uint32_t(__builtin_amdgcn_readfirstlane(int(top)));
@@ -575,8 +576,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
   r.top_p = pf < 1.f ? double(pf) : 2.0;
   r.min_p = mf > 0.f ? fmin(double(mf), 1.0) : 0.0;
   r.u = fmax(double(uf), 0.0);
-  const bool low_matters = (outside & kLow) && (-256.0 - r.lmax) * r.per_t > -64.0;
-  if ((outside & kTinyOrHigh) || low_matters) {
+  if (outside >= kTinyOrHigh || (outside && (value_of_key(outside) - r.lmax) * r.per_t > -64.0)) {
     const Row copy = r;  // (r itself stays in registers)
     const int drawn = draw_outside(copy, s);
     if (tid == 0) p.out[row] = drawn;

@@ -127,6 +127,23 @@ def test_values_outside_the_counted_range(dev, scale):
     _check(dev, logits, u, t, top_k=[50] * b, top_p=[0.9] * b, min_p=[0.01] * b)
 
 
+def test_low_values_at_every_temperature(dev):
+    """Values on either side of -2^8 and the type's lowest as masks, at temperatures at
+    which the ones weigh something and the others do not."""
+    v = 20000
+    logits = _logits(10, v, dev, 21)
+    logits[:, 100:15000] = torch.finfo(torch.bfloat16).min
+    logits[2:, ::3] -= 257
+    logits[4:6, 1::2] = -256
+    logits[6:8] -= 400
+    logits[8, 1:] = -255
+    u = _uniform(10, dev, 22)
+    for scale in (1.0, 6.0, 100.0):
+        t = [scale * (0.5 + 0.1 * i) for i in range(10)]
+        _check(dev, logits, u, t)
+        _check(dev, logits, u, t, top_k=[0, 6000, 40, 15000, 1, 9000, 50, 0, 3, 19999], top_p=[0.95] * 10)
+
+
 def test_extreme_temperatures(dev):
     logits, u = _logits(6, 5000, dev, 8), _uniform(6, dev, 8)
     t = [1e-30, 1e-3, 1e3, 1e30, math.inf, math.nan]
