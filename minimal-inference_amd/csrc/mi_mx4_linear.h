@@ -21,7 +21,8 @@ struct LinearParams {
   int w_tiles;  // row tiles of W
   f32x4_t* parts;   // sums of workgroups that share k
   int split_slabs;  // slabs that one of them takes
-  bool vec;     // out and bias take 8-byte accesses
+  bool vec;     // out and bias take 8-byte accesses,
+  bool wide;    // out 16-byte ones
 };
 
 // Row h n + first + i of W (i the lane's row of 16): its 16 codes' place from the
@@ -38,7 +39,7 @@ __device__ __forceinline__ LaneRow lane_row(const LinearParams& p, int base_row,
 // The bias of columns col .. col + 3.
 __device__ __forceinline__ f32x4_t bias4(const LinearParams& p, int col) {
   f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-  if (!p.bias) return v;
+  if (!p.bias || col >= p.n) return v;
   if (p.vec) {
     const u32x2_t b = *reinterpret_cast<const u32x2_t*>(p.bias + col);
     return f32x4_t{bf16_lo(b.x), bf16_hi(b.x), bf16_lo(b.y), bf16_hi(b.y)};
@@ -49,20 +50,26 @@ __device__ __forceinline__ f32x4_t bias4(const LinearParams& p, int col) {
   return v;
 }
 
-// Columns col .. col + 3 of out's row m from a lane's sums (and, gated, those of the
-// up rows): bias or silu(gate) * up in fp32, one rounding.
+// A lane's sums (and, gated, those of the up rows): bias or silu(gate) * up in fp32, one
+// rounding.
+template <bool GLU>
+__device__ __forceinline__ u32x2_t round4(f32x4_t sum, f32x4_t up, f32x4_t bias) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum[i] = GLU ? silu(sum[i]) * up[i] : sum[i] + bias[i];
+  return u32x2_t{cvt_pk_bf16(sum[0], sum[1]), cvt_pk_bf16(sum[2], sum[3])};
+}
+// They are columns col .. col + 3 of out's row m.
 template <bool GLU>
 __device__ __forceinline__ void store4(const LinearParams& p, int64_t m, int col, f32x4_t sum, f32x4_t up, f32x4_t bias) {
   uint16_t* const out = p.out + m * p.o_stride + col;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) sum[i] = GLU ? silu(sum[i]) * up[i] : sum[i] + bias[i];
+  const u32x2_t v = round4<GLU>(sum, up, bias);
   if (p.vec) {
-    *reinterpret_cast<u32x2_t*>(out) = u32x2_t{cvt_pk_bf16(sum[0], sum[1]), cvt_pk_bf16(sum[2], sum[3])};
+    *reinterpret_cast<u32x2_t*>(out) = v;
     return;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (col + i < p.n) out[i] = cvt_bf16(sum[i]);
+    if (col + i < p.n) out[i] = uint16_t(v[i / 2] >> (16 * (i & 1)));
 }
 
 // Slot of 16-byte chunk c in a staged row of 256 bytes: the 8 rows that an operand

@@ -24,13 +24,16 @@ constexpr int kGroupM = 4;
 // flight, and after the barrier its predecessor's buffer is filled again.  Loads past
 // the last slab are out of range, so that every wait counts the same loads.
 //
-// PER slabs stand between two barriers: two for the largest blocks of MXFP4 rows, so that
-// the second's operands are read while the first is multiplied (8,192 x 8,192 x 10,240
-// 342 -> 329 us; all operands a slab ahead in registers spilled).
+// AHEAD (the largest blocks of MXFP4 rows): four waves of 128 x 128 read 16 operands for 64
+// products, where eight of 128 x 64 read 12 for 32 and LDS could feed no more; the next
+// slab's tiles of W, and tiles of x AHEAD blocks before their turn, are read between the
+// products, whose sums fill the half of a SIMD's registers that the operands leave free.
+// (8,192 x 8,192 x 10,240, operands read at a slab's begin: eight waves 346 us, four 342; so
+// 316.)
 //
 // SPLIT: the workgroup takes p.split_slabs slabs and leaves its sums, in fp32, for
 // combine_kernel.
-template <int WM, int WN, int MB, int NT, int STAGES, bool MX, bool GLU, bool SPLIT, int PER = 1>
+template <int WM, int WN, int MB, int NT, int STAGES, bool MX, bool GLU, bool SPLIT, int AHEAD = 0>
 __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
   constexpr int WAVES = WM * WN, HALVES = GLU ? 2 : 1;
   constexpr int XBLK = MX ? kTileBytes : 16 * kSlab * 2;  // 16 rows of x of a slab
@@ -38,8 +41,8 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
   constexpr int XBYTES = WM * MB * XBLK, STAGE = XBYTES + TILES * kTileBytes;
   constexpr int XLOADS = XBYTES / 1024 / WAVES, WLOADS = TILES / WAVES;
   static_assert(XBYTES / 1024 % WAVES == 0 && TILES % WAVES == 0 && NT % HALVES == 0, "even shares");
-  static_assert(STAGES * PER * STAGE <= 160 * 1024, "LDS");
-  __shared__ __attribute__((aligned(16))) char smem[STAGES * PER * STAGE];
+  static_assert(STAGES * STAGE <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(16))) char smem[STAGES * STAGE];
   lds_t* const lds = (lds_t*)smem;
   const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
   const int wm = w / WN, wn = w % WN;
@@ -148,13 +151,59 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
 #pragma unroll
   for (int s = 0; s < 4; ++s) ro[s] = n * 256 + chunk_slot(n, 4 * g + s) * 16;
 
-  constexpr int kInFlight = (STAGES - 2) * PER * (XLOADS + WLOADS);
+  constexpr int kInFlight = (STAGES - (AHEAD ? 3 : 2)) * (XLOADS + WLOADS);
   static_assert(kInFlight < 64, "vmcnt");
-  static_assert(PER == 1 || !SPLIT, "parts begin at any slab");
   load_scales(slab0 >> 2);
 #pragma unroll
-  for (int i = 0; i < (STAGES - 1) * PER; ++i) load(slab0 + i, i);
+  for (int i = 0; i < STAGES - 1; ++i) load(slab0 + i, i);
   int buf = 0, before = STAGES - 1;
+  if constexpr (AHEAD) {
+    static_assert(MX && !SPLIT && NT == MB && STAGES > 3);
+    u32x4_t a[2][NT], x[MB];
+    auto w_tile = [&](int at, int t) {
+      return lds_load16(lds + at * STAGE + XBYTES + (wn * NT + t) * kTileBytes + lane * 16);
+    };
+    auto x_tile = [&](int at, int b) { return lds_load16(lds + at * STAGE + (wm * MB + b) * XBLK + lane * 16); };
+    constexpr int kFirst = (STAGES - 2) * (XLOADS + WLOADS);
+    __builtin_amdgcn_s_waitcnt(0x0070 | (kFirst & 15) | (kFirst >> 4 << 14));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) a[0][t] = w_tile(0, t);
+#pragma unroll
+    for (int b = 0; b < AHEAD; ++b) x[b] = x_tile(0, b);
+    for (int quad = 0; 4 * quad < slab_end; ++quad) {
+      uint32_t wscale[NT], xscale[MB];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) wscale[t] = wnext[t];
+#pragma unroll
+      for (int b = 0; b < MB; ++b) xscale[b] = xnext[b];
+      auto step = [&]<int S>() {
+        const int slab = 4 * quad + S;
+        __builtin_amdgcn_s_waitcnt(0x0f70 | (kInFlight & 15) | (kInFlight >> 4 << 14));
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        if (S == 0) load_scales(quad + 1);
+        load(slab + STAGES - 1, before);
+        const int next = buf + 1 == STAGES ? 0 : buf + 1;
+#pragma unroll
+        for (int b = 0; b < MB; ++b) {
+          x[(b + AHEAD) % MB] = x_tile(b + AHEAD < MB ? buf : next, (b + AHEAD) % MB);
+          a[(S + 1) & 1][b] = w_tile(next, b);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) acc[t][b] = mfma_fp4<S, S>(a[S & 1][t], wscale[t], x[b], xscale[b], acc[t][b]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        before = buf;
+        buf = next;
+      };
+      step.template operator()<0>();
+      step.template operator()<1>();
+      step.template operator()<2>();
+      step.template operator()<3>();
+    }
+  } else
   for (int quad = slab0 >> 2; 4 * quad < slab_end; ++quad) {
     uint32_t wscale[NT], xscale[MX ? MB : 1];
 #pragma unroll
@@ -193,28 +242,47 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
     auto step = [&]<int S>() {
       const int slab = 4 * quad + S;
       if ((SPLIT && slab < slab0) || slab >= slab_end) return;
-      // vmcnt: these slabs are in LDS; lgkmcnt: this wave has read those before
+      // vmcnt: this slab is in LDS; lgkmcnt: this wave has read the one before
       __builtin_amdgcn_s_waitcnt(0x0070 | (kInFlight & 15) | (kInFlight >> 4 << 14));
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_sched_barrier(0);
       if (S == 0 || (SPLIT && slab == slab0)) load_scales(quad + 1);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) load(slab + (STAGES - 1) * PER + i, before * PER + i);
-      slab_of.template operator()<S>(buf * PER);
-      if constexpr (PER == 2) slab_of.template operator()<S + 1>(buf * PER + 1);
+      load(slab + STAGES - 1, before);
+      slab_of.template operator()<S>(buf);
       before = buf;
       buf = buf + 1 == STAGES ? 0 : buf + 1;
       __builtin_amdgcn_sched_barrier(0);
     };
     step.template operator()<0>();
-    if constexpr (PER == 1) step.template operator()<1>();
+    step.template operator()<1>();
     step.template operator()<2>();
-    if constexpr (PER == 1) step.template operator()<3>();
+    step.template operator()<3>();
   }
 
   __builtin_amdgcn_s_waitcnt(0x0f70);  // (the loads past the end write zeros to LDS)
 
-  // Lane (g, n) holds columns 4 g .. 4 g + 3 of a tile for row n of a block.
+  // Lane (g, n) holds columns 4 g .. 4 g + 3 of a tile for row n of a block.  Two tiles'
+  // lanes change places, so that a lane has eight columns and four lanes 64 bytes of a row.
+  if constexpr (!SPLIT && NT / HALVES % 2 == 0) {
+    if (p.wide) {
+#pragma unroll
+      for (int t = 0; t < NT; t += 2 * HALVES) {
+        const int first = col0 + (wn * NT + t) / HALVES * 16, col = first + (g & 1) * 16 + (g >> 1) * 8;
+        const f32x4_t bias0 = bias4(p, first + 4 * g), bias1 = bias4(p, first + 16 + 4 * g);
+#pragma unroll
+        for (int b = 0; b < MB; ++b) {
+          const u32x2_t u = round4<GLU>(acc[t][b], acc[t + HALVES - 1][b], bias0);
+          const u32x2_t v = round4<GLU>(acc[t + HALVES][b], acc[t + 2 * HALVES - 1][b], bias1);
+          const auto s0 = __builtin_amdgcn_permlane16_swap(u.x, v.x, false, false);
+          const auto s1 = __builtin_amdgcn_permlane16_swap(u.y, v.y, false, false);
+          const int m = (wm * MB + b) * 16 + n;
+          if (m < rows && col < p.n)
+            *reinterpret_cast<u32x4_t*>(p.out + (m0 + m) * p.o_stride + col) = u32x4_t{s0[0], s1[0], s0[1], s1[1]};
+        }
+      }
+      return;
+    }
+  }
 #pragma unroll
   for (int t = 0; t < NT; t += HALVES) {
     const int col = col0 + (wn * NT + t) / HALVES * 16 + 4 * g;
@@ -316,11 +384,11 @@ float few_us(bool mx, int64_t rows, int w_tiles, int slabs) {
   return 4.f + float((rows + group - 1) / group * w_tiles) * slabs * (kTileBytes + kQuadBytes / 4) / (mx ? 4e6f : 3.5e6f);
 }
 
-template <int WM, int WN, int MB, int NT, int STAGES, bool MX, bool GLU, bool SPLIT, int PER = 1>
+template <int WM, int WN, int MB, int NT, int STAGES, bool MX, bool GLU, bool SPLIT, int AHEAD = 0>
 void run(const LinearParams& p, int parts, hipStream_t stream) {
   constexpr int BM = WM * MB * 16, COLS = WN * NT * 16 / (GLU ? 2 : 1);
   const dim3 grid(uint32_t((p.rows + BM - 1) / BM * ((p.n + COLS - 1) / COLS)), parts);
-  hipLaunchKernelGGL((many_kernel<WM, WN, MB, NT, STAGES, MX, GLU, SPLIT, PER>), grid, dim3(64 * WM * WN), 0, stream, p);
+  hipLaunchKernelGGL((many_kernel<WM, WN, MB, NT, STAGES, MX, GLU, SPLIT, AHEAD>), grid, dim3(64 * WM * WN), 0, stream, p);
 }
 
 template <bool MX, bool GLU, bool SPLIT>
@@ -328,7 +396,7 @@ void run_form(const LinearParams& p, int form, int parts, hipStream_t stream) {
   if constexpr (MX) {
     if (SPLIT || form == 0) run<2, 2, 4, 4, 4, true, GLU, SPLIT>(p, parts, stream);
     else if (form == 1) run<2, 4, 4, 4, 3, true, GLU, false>(p, 1, stream);
-    else run<2, 4, 8, 4, 2, true, GLU, false, 2>(p, 1, stream);
+    else run<2, 2, 8, 8, 4, true, GLU, false, 3>(p, 1, stream);
   } else {
     if (form == 0) run<1, 4, 2, 2, 4, false, GLU, SPLIT>(p, parts, stream);
     else if (form == 1) run<2, 4, 2, 2, 4, false, GLU, SPLIT>(p, parts, stream);
@@ -440,6 +508,7 @@ extern "C" int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_sc
   p.w_tiles = int(row_tiles(silu ? 2 * n : n));
   p.vec = n % 4 == 0 && out_stride % 4 == 0 &&
           ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) & 7) == 0;
+  p.wide = p.vec && n % 8 == 0 && out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   p.parts = static_cast<mi::f32x4_t*>(workspace);
   if (few(x_scales != nullptr, rows, silu ? 2 * n : n, k)) launch_few(p, silu != 0, s);
