@@ -331,17 +331,18 @@ __global__ __launch_bounds__(256) void combine_kernel(LinearParams p, int parts)
 // every workgroup of a CU, the way of its output to memory, and, where workgroups share
 // k, the combining launch with the parts' way there and back.  Model and measured (us):
 // 77 x 18,944 x 3,584, 80-row blocks, 9 parts 22.0 / 22.5, whole 96.9 / 95.5;
-// 128 x 8,192 x 10,240, 128 x 128, 3 parts 32.3 / 32.2; bf16 1,024 x 8,192 x 10,240,
-// 128 x 128 in fours of waves 162 / 159, 128 x 256 197 / 184; in 4 bits 2,048 x 8,192 x
-// 10,240, 128 x 128 118 / 105, 128 x 256 118 / 104, 256 x 256 144 / 125.
+// 128 x 8,192 x 10,240, 128 x 128, 3 parts 31.7 / 32.2; bf16 1,024 x 8,192 x 10,240,
+// 128 x 128 in fours of waves 153 / 154, 128 x 256 190 / 179; in 4 bits 2,048 x 8,192 x
+// 10,240, 128 x 128 98 / 100, 128 x 256 99 / 98, 256 x 256 122 / 112; 8,192 rows of it 381 /
+// 378, 326 / 321, 314 / 312.
 struct Form {
   int rows, tiles;  // 16-row tiles of W
   float one_us, more_us;
   bool split;
 };
 constexpr Form kBf16Forms[] = {{32, 8, 0.45f, 0.45f, true}, {64, 8, 0.56f, 0.56f, true}, {80, 8, 0.63f, 0.63f, true},
-                               {128, 8, 0.86f, 0.93f, true}, {128, 8, 1.0f, 0.8f, false}, {128, 16, 1.45f, 1.5f, false}};
-constexpr Form kMxForms[] = {{128, 8, 0.385f, 0.33f, true}, {128, 16, 0.56f, 0.53f, false}, {256, 16, 1.02f, 1.02f, false}};
+                               {128, 8, 0.84f, 0.885f, true}, {128, 8, 0.96f, 0.755f, false}, {128, 16, 1.35f, 1.42f, false}};
+constexpr Form kMxForms[] = {{128, 8, 0.345f, 0.265f, true}, {128, 16, 0.51f, 0.445f, false}, {256, 16, 0.78f, 0.85f, false}};
 constexpr float kStartUs = 3.5f, kCombineUs = 2.5f, kBytesPerUs = 4.4e6f;
 constexpr int kMaxParts = 32;
 

@@ -308,7 +308,11 @@ def test_empty_and_refused(dev):
     (528, 36, 1184), (649, 80, 6496), (1349, 152, 2624), (2563, 148, 5920), (1432, 34, 3680), (2179, 40, 5440),
     (81, 1773, 7968), (591, 1676, 64), (133, 11615, 64), (165, 10884, 64), (564, 8256, 64), (1205, 6524, 64),
     (528, 7352, 64), (1539, 7712, 64), (1284, 4530, 64), (1290, 916, 7200), (1159, 1028, 7392), (2053, 467, 10080),
-    (650, 3891, 3392), (2563, 3116, 672), (1295, 6303, 544), (4671, 1788, 1216), (4124, 4007, 928)])
+    (650, 3891, 3392), (2563, 3116, 672), (1295, 6303, 544), (4671, 1788, 1216), (4124, 4007, 928),
+    (263, 1836, 64), (288, 5555, 64), (1281, 5936, 64), (771, 4957, 64), (1923, 2064, 544), (2568, 1588, 704),
+    (4109, 916, 1216), (1671, 1179, 1664), (1284, 2040, 3520), (645, 1878, 4032), (1295, 1004, 6560),
+    (646, 1020, 8224), (1538, 385, 7424), (2621, 3078, 1056), (3360, 4820, 1088), (4127, 2019, 2080),
+    (4657, 858, 2144), (3596, 1060, 4064), (3604, 554, 3584)])
 def test_every_form_of_whole_numbers(dev, rows, n, k, silu, acts):
     """Sizes on which the forms (groups of 32 or 64 rows, blocks of 32 to 256 rows, k
     whole and in parts, rows behind the last whole block) differ: sums exact in fp32 are the exact ones, with a
