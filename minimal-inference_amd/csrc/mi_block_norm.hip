@@ -7,7 +7,7 @@
 //
 // Bound: HBM, 8 bytes per element (10 with a full gate), half of them writes: 18,240 x
 // 4,096 107 us = 5.6 TB/s, where a copy of 1 GiB reaches 5.2.  One workgroup per row,
-// one to four 16-byte chunks per thread; every load of the row is issued before anything
+// one, two or four 16-byte chunks per thread; every load of the row is issued before anything
 // is computed or stored, and the row stays in registers over both sums.
 #include "mi_common.h"
 
@@ -15,6 +15,7 @@ namespace {
 
 constexpr int kMaxThreads = 512;
 constexpr int kMaxHidden = 16384;
+constexpr int64_t kMaxRows = 1 << 22;  // (a launch counts its threads in 32 bits)
 
 struct BlockNormParams {
   const uint16_t* x;
@@ -120,8 +121,8 @@ extern "C" int mi_post_norm_add_rms_norm(const void* x, int64_t x_stride, const 
                                          int64_t x_out_stride, void* h_out, int64_t h_stride, int64_t rows,
                                          int32_t hidden, float eps, float scale, mi_stream_t stream) {
   mi::clear_error();
-  if (rows < 0 || rows > 0x7fffffff || hidden <= 0 || hidden % 8 || hidden > kMaxHidden)
-    return mi::fail(MI_ERR_INVALID, "post_norm_add_rms_norm: %lld rows, hidden %d (multiple of 8, <= %d)",
+  if (rows < 0 || rows > kMaxRows || hidden <= 0 || hidden % 8 || hidden > kMaxHidden)
+    return mi::fail(MI_ERR_INVALID, "post_norm_add_rms_norm: %lld rows (0..2^22), hidden %d (multiple of 8, <= %d)",
                     (long long)rows, hidden, kMaxHidden);
   if (rows == 0) return MI_OK;
   if (!x || !y || !post_weight || !weight || !x_out || !h_out)
@@ -135,6 +136,9 @@ extern "C" int mi_post_norm_add_rms_norm(const void* x, int64_t x_stride, const 
   if (gate && gate_per_column) aligned |= reinterpret_cast<uintptr_t>(gate), strides |= gate_row_stride;
   if ((aligned & 15) || (strides & 7) || (reinterpret_cast<uintptr_t>(gate) & 1))
     return mi::fail(MI_ERR_INVALID, "post_norm_add_rms_norm: rows must be 16-byte aligned");
+  if (x_out_stride < hidden || h_stride < hidden)
+    return mi::fail(MI_ERR_INVALID, "post_norm_add_rms_norm: output row strides %lld, %lld for hidden %d",
+                    (long long)x_out_stride, (long long)h_stride, hidden);
   BlockNormParams p;
   p.x = static_cast<const uint16_t*>(x);
   p.x_stride = x_stride;

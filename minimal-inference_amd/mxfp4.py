@@ -76,7 +76,9 @@ class MXFP4:
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "MXFP4":
         """From row-major codes [rows, cols / 2] (the even column in a byte's lower
-        half) and scale bytes [rows, cols / 32], both uint8."""
+        half) and scale bytes [rows, cols / 32], both uint8.  Every scale byte is kept;
+        bf16 holds values of 2^128 and up (bytes 253 and 254) as infinities, in
+        ``dequantize`` and beside bf16 rows."""
         _check_codes(codes, scales)
         m = cls(codes.shape[0], 2 * codes.shape[1], codes.device)
         call_on(codes, "mi_mxfp4_pack", codes.data_ptr(), scales.data_ptr(), m.codes_ptr, m.scales_ptr,
@@ -148,6 +150,10 @@ def _linear(x, weight: MXFP4, bias, out, silu: bool) -> torch.Tensor:
         require_dtype("bias", bias, torch.bfloat16)
         if bias.shape != (n,) or not bias.is_contiguous() or bias.device != like.device:
             raise ValueError(f"bias must be a contiguous [{n}] tensor on {like.device}")
+        if bias.requires_grad and torch.is_grad_enabled():
+            raise ValueError("bias requires a gradient: there is no backward pass")
+    if out is not None and out is x:
+        raise ValueError("out is x, which other workgroups still read")
     out = _out(out, rows, n, like)
     if rows and n:
         room = _workspace_size(rows, n, k, silu, scales is not None) if rows > _FEW_ROWS else 0
@@ -166,7 +172,8 @@ def _workspace_size(rows: int, n: int, k: int, silu: bool, x_mxfp4: bool) -> int
 
 def linear_mxfp4(x: torch.Tensor | MXFP4, weight: MXFP4, bias: torch.Tensor | None = None,
                  out: torch.Tensor | None = None) -> torch.Tensor:
-    """``x @ weight.T + bias`` as bf16 [rows, n]; x is bf16 [rows, k] or MXFP4."""
+    """``x @ weight.T + bias`` as bf16 [rows, n]; x is bf16 [rows, k] or MXFP4.  out must
+    not overlap x."""
     return _linear(x, weight, bias, out, False)
 
 

@@ -103,6 +103,7 @@ class Sampler:
         the lowest id whose cumulative kept weight, in order of ids, exceeds u times
         the kept total.  In 64 bits; temperatures are taken as they are (not rounded to
         bf16).  Rows with temperature <= 0, or with no logit above -inf, give argmax.
+        A sampler's draws share its workspace: one at a time.
         """
         if logits.dim() == 3:
             logits = logits[:, -1, :]

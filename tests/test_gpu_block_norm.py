@@ -112,7 +112,8 @@ def test_refused(dev):
                   ((x, y, post, pre), {"gate": gate.float()}), ((x, y, post, pre), {"x_out": x[:2]}),
                   ((x, y, post, pre), {"h_out": y[:, ::2]}), ((x[:, :60], y[:, :60], post[:60], pre[:60]), {}),
                   ((x.cpu(), y, post, pre), {}), ((x, y, post.clone().requires_grad_(), pre), {}),
-                  ((x[:, 4:], y[:, 4:], post[4:], pre[4:]), {})]:
+                  ((x[:, 4:], y[:, 4:], post[4:], pre[4:]), {}), ((x[:1].expand(4, 64), y, post, pre), {}),
+                  ((x, y, post, pre), {"h_out": y[:1].expand(4, 64)})]:
         with pytest.raises(ValueError):
             post_norm_add_rms_norm(*a, 1e-6, **kw)
 

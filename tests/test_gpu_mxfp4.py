@@ -283,6 +283,7 @@ def test_empty_and_refused(dev):
     bias = torch.zeros(32, device=dev, dtype=torch.bfloat16)
     odd = torch.zeros(4, 65, device=dev, dtype=torch.bfloat16)[:, 1:]
     far = torch.zeros(1, device=dev, dtype=torch.bfloat16).expand(2, 64)
+    square = _weight(64, 64, dev, 7)[2]
     grad = x.clone().requires_grad_()
     for bad in [lambda: linear_mxfp4(x[:, :32], w), lambda: linear_mxfp4(x.float(), w), lambda: linear_mxfp4(odd, w),
                 lambda: linear_mxfp4(x, w, bias[:16]), lambda: linear_mxfp4(x, w, bias.float()),
@@ -292,7 +293,8 @@ def test_empty_and_refused(dev):
                 lambda: quantize_mxfp4(x[:, :48]), lambda: quantize_mxfp4(x, out=w), lambda: MXFP4(4, 33, dev),
                 lambda: MXFP4.from_codes(torch.zeros(4, 32, dtype=torch.uint8, device=dev),
                                          torch.zeros(4, 1, dtype=torch.uint8, device=dev)),
-                lambda: linear_silu_mxfp4(x, _weight(31, 64, dev, 6)[2]), lambda: w.dequantize(x)]:
+                lambda: linear_silu_mxfp4(x, _weight(31, 64, dev, 6)[2]), lambda: w.dequantize(x),
+                lambda: linear_mxfp4(x, w, bias.clone().requires_grad_()), lambda: linear_mxfp4(x, square, out=x)]:
         with pytest.raises(ValueError):
             bad()
     with pytest.raises(TypeError):

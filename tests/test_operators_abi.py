@@ -57,7 +57,7 @@ def test_mxfp4_matrix_calls_refuse():
 
 
 @pytest.mark.parametrize("change", [
-    {"rows": -1}, {"rows": 1 << 31}, {"hidden": 12}, {"hidden": 0}, {"hidden": 16392}, {"x": None}, {"y": None},
+    {"rows": -1}, {"rows": 1 << 31}, {"rows": (1 << 22) + 1}, {"xos": 0}, {"xos": 56}, {"hs": 0}, {"hidden": 12}, {"hidden": 0}, {"hidden": 16392}, {"x": None}, {"y": None},
     {"post": None}, {"weight": None}, {"x_out": None}, {"h_out": None}, {"x": FAKE + 8}, {"ys": 68}, {"hs": 60},
     {"gate": FAKE + 8, "col": 1}, {"gate": FAKE, "gs": 4, "col": 1}, {"gate": FAKE + 1}])
 def test_post_norm_refuses(change):
