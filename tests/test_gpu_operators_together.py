@@ -142,3 +142,51 @@ def test_refuses_unfused(dev):
     model.fused_dense = False
     with pytest.raises(ValueError):
         model.quantize_weights()
+
+
+def test_matrices_past_32_bits(dev):
+    """More than 2^32 bytes of rows, of codes and of output: the last rows are those of
+    the same rows alone."""
+    from minimal_inference_amd.dense import post_norm_add_rms_norm
+    from minimal_inference_amd.mxfp4 import MXFP4, linear_mxfp4, quantize_mxfp4
+
+    rows, cols = 600_000, 4096
+    g = torch.Generator(device=dev).manual_seed(0)
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=dev).normal_(generator=g)
+    q = quantize_mxfp4(x)
+    back = q.dequantize()
+    for part in (slice(0, 40), slice(rows - 40, rows)):
+        assert torch.equal(back[part], quantize_mxfp4(x[part]).dequantize())
+    del q
+    w = torch.ones(cols, dtype=torch.bfloat16, device=dev)
+    tail = slice(rows - 40, rows)
+    want_x = torch.empty(40, cols, dtype=torch.bfloat16, device=dev)
+    want_h = post_norm_add_rms_norm(x[tail], back[tail], w, w, 1e-6, x_out=want_x)
+    h = post_norm_add_rms_norm(x, back, w, w, 1e-6, h_out=back)
+    assert torch.equal(x[tail], want_x) and torch.equal(h[tail], want_h)
+    del x, back, h
+    # whole numbers: the sums are exact, whatever the form of the launch
+    values = torch.tensor([0, 1, 2, 3, 4, 6, -1, -2, -3, -4, -6], dtype=torch.bfloat16, device=dev)
+    for rows, n, k in ((270_000, 10_240, 64), (3, 1 << 20, 8192)):
+        x = values[torch.randint(0, 11, (rows, k), device=dev, generator=g)]
+        x[:, ::32] = 6.0
+        wc = torch.randint(0, 256, (n, k // 2), device=dev, generator=g, dtype=torch.uint8)
+        weight = MXFP4.from_codes(wc, torch.full((n, k // 32), 128, dtype=torch.uint8, device=dev))
+        one = MXFP4.from_codes(wc[-50:].contiguous(), torch.full((50, k // 32), 128, dtype=torch.uint8, device=dev))
+        ref = (x[-40:].double() @ one.dequantize().double().t()).to(torch.bfloat16)
+        for a in (x, quantize_mxfp4(x)):
+            assert torch.equal(linear_mxfp4(a, weight)[-40:, -50:], ref)
+
+
+def test_draws_from_rows_far_apart(dev):
+    from minimal_inference_amd.sampling import Sampler
+
+    b, v, apart = 40, 32768, 1 << 26
+    wide = torch.empty(b * apart, dtype=torch.bfloat16, device=dev)
+    logits = wide.as_strided((b, v), (apart, 1))
+    logits.normal_(std=3.0, generator=torch.Generator(device=dev).manual_seed(1))
+    u = torch.rand(b, device=dev, generator=torch.Generator(device=dev).manual_seed(2))
+    s = Sampler(dev, b, vocab=v)
+    s.set_params([0.8] * b, [0.95] * b, top_k=[100] * b, min_p=[0.01] * b)
+    near = s.draw(logits.contiguous(), u).clone()
+    assert torch.equal(s.draw(logits, u), near)
