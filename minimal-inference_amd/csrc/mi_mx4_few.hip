@@ -185,40 +185,64 @@ void run(const LinearParams& p, hipStream_t stream) {
 }
 
 // The form of a launch, from the tiles of W, the slabs and the 16-row blocks of x (us,
-// weights rotated through 600 MB; R tiles per workgroup, D slabs ahead):
-//                             waves:      4                       8
-//                              rows   R 1 D 4  R 2 D 2  R 4 D 2   R 1 D 2  R 1 D 1  R 2 D 1  R 4 D 1
-//   N  1152 K   896               8     3.6      3.1      3.7       3.5      3.1      3.2      3.8
-//   N  4096 K  4096               1     5.0      6.1      7.0       4.8      5.1      5.4      6.5
-//   N  4096 K  4096              32     8.0      8.1     10.0       7.7      7.2      8.3      9.2
-//   N  4096 K 14336               8    12.4     16.8     19.5      11.2     12.0     12.3     16.8
-//   N  6144 K  4096               8              6.5      7.4                6.7      5.6      6.7
-//   N  8192 K  8192              32             13.6     17.4               19.6     13.0     16.2
-//   N 10240 K  8192               8             13.1     13.0      16.2     15.9     14.7     11.6
-//   N 10240 K  8192              32             22.2     17.7               26.9     23.6     16.7
-//   N 28672 K  1024               1              6.7      6.2                8.1      7.0      6.5
-//   gated 2 x 4864, K 896         1              4.9      4.4                         4.6      4.7
-//   gated 2 x 18944, K 3584       8             18.5     18.0                        17.3     16.8
-//   gated 2 x 14336, K 4096      32             24.5     18.2  (R 8 D 1: 15.8)       24.3     19.4
-//   MXFP4 x: N 4096 K 14336       8     9.3     12.0               8.1      10.4      9.9     14.0
-//   MXFP4 x: N 8192 K 8192       64             11.5     14.3               15.5     10.6     14.3
-//   MXFP4 x: N 10240 K 8192      48             15.8     13.7               18.0     16.1     13.0
-// Every workgroup reads x, so tiles as many as still leave a workgroup for most of the
-// CUs; eight waves while k is long enough to feed them.  Two blocks of bf16 rows are
-// the larger part of what is read: eight tiles, while they leave no second round.
+// weights rotated through 600 MB; R tiles and 4 or 8 waves per workgroup, 1 slab ahead, 2
+// where marked):
+//                             waves:      4                                  8
+//                              rows   R 2*   R 3   R 4   R 5   R 7   R 8   R 1   R 2   R 3   R 4   R 5   R 6
+//   N  1152 K   896               8   3.1                                  3.1   3.2         3.8
+//   N  4096 K  4096               1   6.1                                  5.1   5.4         6.5
+//   N  4096 K  4096              32   8.1                                  7.2   8.3         9.2
+//   N  6144 K  4096               8   6.5                                  6.7   5.6         6.7
+//   N  8192 K  8192              32  13.6                                       13.0        16.2
+//   N 10240 K   896               8          3.8   3.9                                 3.9   4.1
+//   N 10240 K  2048              32          6.4   6.6                                 6.7   6.9
+//   N 10240 K  8192               8  13.1                     18.1  19.7       14.7  10.7  11.7  13.4  14.3
+//   N 10240 K  8192              32  22.2                     21.7  25.1       23.6  15.4  16.9  18.4  19.6
+//   N 18432 K  4096              32                           13.6  15.4             15.9  17.9  12.3  12.9
+//   N 28672 K  4096               8                     13.7  16.0                   14.7  13.2  14.9  17.6
+//   N 28672 K  2048               8                7.7         8.5                         8.7
+//   N 28672 K  4096              32                           15.3  17.9             21.2  18.9  21.2  23.1
+//   N 59136 K  8192               8               46.0  41.1        49.0                   46.2  40.4
+//   N 59136 K  8192              32               59.5              53.4                   62.7
+//   gated 2 x 11008, K 4096      32                                 15.4                   19.2        14.1
+//   gated 2 x 14336, K 4096       1               12.9              14.7                   13.8
+//   gated 2 x 14336, K 4096      32                                 16.3                   19.4
+//   MXFP4 x: N 10240 K 8192      64                           19.1  20.6             13.0  14.7  16.4
+//   MXFP4 x: N 18432 K 4096      48                           11.5  13.2             12.5  14.7  10.5  11.2
+//   MXFP4 x: N 28672 K 4096      48                           13.8  16.4             17.1  15.9  18.3  20.0
+// Every workgroup reads x, so as many tiles as make one round of workgroups; eight waves
+// while k is long enough to feed them and their sums fit in LDS.  Seven and eight tiles
+// pay from two blocks of x on; beyond one round of eight, a single block takes three
+// rounds and more blocks two.  (More slabs ahead are slower: gated 2 x 14,336, 32 rows 18.1.)
+template <int R, int MB, bool MX, bool GLU>
+void waves(const LinearParams& p, hipStream_t stream) {
+  if constexpr (R == (GLU ? 2 : 1) && MB == 1) {
+    if (p.w_tiles <= mi::num_cus() && p.slabs >= 32) return run<R, MB, 2, MX, GLU, 8>(p, stream);
+  }
+  if constexpr (R <= 6 && R * MB * 8 <= 160) {
+    if (R <= 2 || p.slabs >= 28) return run<R, MB, 1, MX, GLU, 8>(p, stream);
+  }
+  run<R, MB, 1, MX, GLU, 4>(p, stream);
+}
 template <int MB, bool MX, bool GLU>
 void pick(const LinearParams& p, hipStream_t stream) {
-  constexpr int ONE = GLU ? 2 : 1;
-  if (p.w_tiles <= 256) {
-    if (MB == 1 && p.slabs >= 32) return run<ONE, MB, MB == 1 ? 2 : 1, MX, GLU, 8>(p, stream);
-    return run<ONE, MB, 1, MX, GLU, 8>(p, stream);
+  const int cus = mi::num_cus();
+  auto rounds = [&](int n) { return (p.w_tiles + n * cus - 1) / (n * cus); };
+  int tiles = rounds(1);
+  if (MB == 1 && tiles > 6) tiles = tiles <= 8 ? 4 : std::min(rounds(3), 6);
+  else if (tiles > 8) tiles = std::min(rounds(2), 8);
+  if constexpr (!GLU) {
+    if (tiles == 1) return waves<1, MB, MX, GLU>(p, stream);
+    if (tiles == 3) return waves<3, MB, MX, GLU>(p, stream);
+    if (tiles == 5) return waves<5, MB, MX, GLU>(p, stream);
+    if constexpr (MB > 1) {
+      if (tiles == 7) return waves<7, MB, MX, GLU>(p, stream);
+    }
   }
-  if (p.w_tiles <= 512) return run<2, MB, 1, MX, GLU, 8>(p, stream);
-  if constexpr (!MX && MB == 2) {
-    if (p.w_tiles > 1024 && p.w_tiles <= 2048) return run<8, MB, 1, MX, GLU, 4>(p, stream);
-  }
-  if (p.slabs >= 28) return run<4, MB, 1, MX, GLU, 8>(p, stream);
-  run<4, MB, 2, MX, GLU, 4>(p, stream);
+  if (tiles <= 2) return waves<2, MB, MX, GLU>(p, stream);
+  if (tiles <= 4) return waves<4, MB, MX, GLU>(p, stream);
+  if (MB == 1 || tiles <= 6) return waves<6, MB, MX, GLU>(p, stream);
+  if constexpr (MB > 1) waves<8, MB, MX, GLU>(p, stream);
 }
 
 template <bool GLU>

@@ -6,6 +6,8 @@
 // buffers, the next slab's while this one is multiplied) and from there, as operands,
 // to the waves.  MXFP4 tiles are operands as they lie; the codes of W become bf16 in
 // registers, exactly, where x is bf16, whose rows are staged with permuted chunks.
+#include <algorithm>
+
 #include "mi_mx4_linear.h"
 
 namespace mi::mx4 {
@@ -375,14 +377,19 @@ Choice choose(bool mx, bool glu, int64_t rows, int64_t n, int slabs, size_t room
 }
 
 // The few-row kernel's time: W's bytes once for every group of rows, beyond the first
-// from the caches.  More groups than one are faster than blocks of 128 rows where W is
-// small (128 x 4,096 x 4,096 in 4 bits 6.0 us, in blocks 13; 64 x 4,096 x 6,144 of bf16
-// rows 11 and 13; the count's 8.4 and 13, 11 and 13); more than 512 rows are not
-// measured and not asked for.
+// from the caches, or where that is longer the rows of x into each of its workgroups.
+// More groups than one are faster than blocks of 128 rows where W is small (128 x 4,096 x
+// 4,096 in 4 bits 6.0 us, in blocks 13; 64 x 4,096 x 6,144 of bf16 rows 11 and 13; the
+// count's 8.4 and 13, 11.6 and 13); one is slower along a long k (32 x 18,944 x 3,584 21,
+// in blocks 17; the count's 19 and 17).  More than 512 rows are not measured and not asked
+// for.
 float few_us(bool mx, int64_t rows, int w_tiles, int slabs) {
   if (rows > 512) return 1e30f;
-  const int64_t group = few_group(mx);
-  return 4.f + float((rows + group - 1) / group * w_tiles) * slabs * (kTileBytes + kQuadBytes / 4) / (mx ? 4e6f : 3.5e6f);
+  const int64_t group = few_group(mx), groups = (rows + group - 1) / group;
+  const int cus = mi::num_cus(), each = (w_tiles + cus - 1) / cus, wgs = (w_tiles + each - 1) / each;
+  const float w = float(groups * w_tiles) * slabs * (kTileBytes + kQuadBytes / 4) / (mx ? 4e6f : 3.5e6f);
+  const float x = float(std::min(rows, group) * slabs * (mx ? kSlab / 2 : 2 * kSlab)) / 8e4f;
+  return 4.f + std::max(w, x * float((wgs * groups + cus - 1) / cus));
 }
 
 template <int WM, int WN, int MB, int NT, int STAGES, bool MX, bool GLU, bool SPLIT, int AHEAD = 0>

@@ -350,3 +350,29 @@ def test_every_form_of_whole_numbers(dev, rows, n, k, silu, acts):
         else:
             assert torch.equal(got[:rows, :n], ref.to(torch.bfloat16))
         assert bool((got[rows] == 7).all()) and bool((got[:, n:] == 7).all())
+
+
+@pytest.mark.parametrize("silu", [False, True])
+@pytest.mark.parametrize("rows,acts", [(1, "bf16"), (20, "bf16"), (7, "mxfp4"), (20, "mxfp4"), (40, "mxfp4"), (64, "mxfp4")])
+@pytest.mark.parametrize("k", [160, 3616])
+@pytest.mark.parametrize("w_rows", [4000, 8190, 10_234, 16_002, 18_420, 22_004, 28_660, 32_002, 40_006, 59_000, 70_002])
+def test_few_rows_of_every_width(dev, w_rows, k, rows, acts, silu):
+    """One to eight tiles of W per workgroup, one round of them and several, four waves
+    and eight: whole numbers whose sums are exact in fp32."""
+    from minimal_inference_amd.mxfp4 import MXFP4, linear_mxfp4, linear_silu_mxfp4, quantize_mxfp4
+
+    g = torch.Generator(device=dev).manual_seed(rows + w_rows + k)
+    values = torch.tensor([0, 1, 2, 3, 4, 6, -1, -2, -3, -4, -6], device=dev, dtype=torch.bfloat16)
+    x = values[torch.randint(0, 11, (rows, k), device=dev, generator=g)]
+    x[:, ::32] = 6.0
+    codes = torch.randint(0, 256, (w_rows, k // 2), device=dev, generator=g, dtype=torch.uint8)
+    weight = MXFP4.from_codes(codes, torch.full((w_rows, k // 32), 128, device=dev, dtype=torch.uint8))
+    sums = x.float() @ weight.dequantize().float().t()  # (whole numbers below 2^24)
+    xx = quantize_mxfp4(x) if acts == "mxfp4" else x
+    if silu:
+        gate, up = sums.double().chunk(2, -1)
+        ref = gate * torch.sigmoid(gate) * up
+        got = linear_silu_mxfp4(xx, weight).double()  # fp32: 8 roundings, then one to bf16
+        assert bool(((got - ref).abs() <= (2 ** -8 + 8 * 2 ** -24) * ref.abs() + 1e-30).all())
+    else:
+        assert torch.equal(linear_mxfp4(xx, weight), sums.to(torch.bfloat16))
