@@ -314,7 +314,8 @@ def test_empty_and_refused(dev):
     (263, 1836, 64), (288, 5555, 64), (1281, 5936, 64), (771, 4957, 64), (1923, 2064, 544), (2568, 1588, 704),
     (4109, 916, 1216), (1671, 1179, 1664), (1284, 2040, 3520), (645, 1878, 4032), (1295, 1004, 6560),
     (646, 1020, 8224), (1538, 385, 7424), (2621, 3078, 1056), (3360, 4820, 1088), (4127, 2019, 2080),
-    (4657, 858, 2144), (3596, 1060, 4064), (3604, 554, 3584)])
+    (4657, 858, 2144), (3596, 1060, 4064), (3604, 554, 3584), (648, 1936, 7808), (2307, 1688, 2752), (24, 76, 13120),
+    (79, 50, 4128), (92, 84, 11616)])
 def test_every_form_of_whole_numbers(dev, rows, n, k, silu, acts):
     """Sizes on which the forms (groups of 32 or 64 rows, blocks of 32 to 256 rows, k
     whole and in parts, rows behind the last whole block) differ: sums exact in fp32 are the exact ones, with a
