@@ -8,8 +8,8 @@
 //
 // A bf16 logit is one of few values, so a row is a histogram of whole numbers: counts
 // per value say all that order and mass need, one exp per value in 64 bits is enough,
-// and nothing depends on the order of additions.  Two launches, no atomics on memory
-// and nothing kept between calls:
+// and nothing depends on the order of additions.  One or two launches, no atomics on
+// memory and nothing kept between calls:
 //   count  one workgroup per 8,192 to 32,768 tokens, on the XCD of the row's draw (its L2
 //          then holds the counts: 0.4 us): largest value with its lowest index, and
 //          the counts of the 2 x 38 x 128 values of magnitude [2^-30, 2^8) and of zero
@@ -189,33 +189,41 @@ __device__ __forceinline__ s16x2_t bin_pair(uint32_t x) {
   return (__builtin_bit_cast(s16x2_t, off) ^ flip) - flip + short(kZeroBin);
 }
 
-// G groups of eight tokens per thread, 8,192 G tokens per workgroup.
+// What a chunk's tokens come to, beside their counts.
+struct Seen {
+  uint32_t best[kWaves];
+  uint32_t outside;
+  int first;  // 0x10000 - the first place of the largest
+};
+
+// A thread's G groups of eight tokens, wave by wave: a wave has 512 G in a row, group i of
+// a lane the eight from 512 i + 8 lane on.  Past the row's end: NaN bits.
 template <int G>
-__global__ __launch_bounds__(kThreads) void count_kernel(DrawParams p) {
-  constexpr int kChunk = kThreads * 8 * G;
-  __shared__ uint32_t hist[kBins];
-  __shared__ uint32_t best[kWaves];
-  __shared__ uint32_t outside;
-  __shared__ int first;
-  const int tid = threadIdx.x, chunk = blockIdx.x >> 3;
-  const int64_t row = blockIdx.y * 8 + (blockIdx.x & 7);
-  if (row >= p.batch) return;
-  const uint16_t* logits = p.logits + row * p.stride;
-  const int base = chunk * kChunk;
-  uint32_t v[4 * G];
+__device__ __forceinline__ int place_of(int i) {
+  return int(threadIdx.x >> 6) * 512 * G + i * 512 + int(threadIdx.x & 63) * 8;
+}
+template <int G>
+__device__ __forceinline__ void load_tokens(uint32_t (&v)[4 * G], const uint16_t* logits, int base, int vocab) {
 #pragma unroll
   for (int i = 0; i < G; ++i) {
-    const int at = base + (i * kThreads + tid) * 8;
-    const uint4 x = at < p.vocab ? load8(logits, at, p.vocab) : make_uint4(kPad, kPad, kPad, kPad);
+    const int at = base + place_of<G>(i);
+    const uint4 x = at < vocab ? load8(logits, at, vocab) : make_uint4(kPad, kPad, kPad, kPad);
     v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
   }
-  const bool greedy = !(p.temperature[row] > 0.f);
+}
+
+// The counts of a workgroup's tokens (none of a greedy row's) into `hist`, and the key of
+// the largest with NaN 0 (highest where the row is greedy); the workgroup's sums are
+// complete behind the last barrier.
+template <int G>
+__device__ __forceinline__ uint32_t count_tokens(const uint32_t (&v)[4 * G], int base, int vocab, bool greedy, uint32_t* hist,
+                                                 Seen& seen) {
+  const int tid = threadIdx.x;
 #pragma unroll
   for (int i = 0; i < kBins / kThreads; ++i) hist[i * kThreads + tid] = 0;
-  if (tid == 0) outside = 0, first = 0;
+  if (tid == 0) seen.outside = 0, seen.first = 0;
   __syncthreads();
-  // the largest key (NaN 0, or highest where the row is greedy), and the counts
-  auto place = [&](int i, int h) { return ((i >> 2) * kThreads + tid) * 8 + (i & 3) * 2 + h; };
+  auto place = [&](int i, int h) { return place_of<G>(i >> 2) + (i & 3) * 2 + h; };
   // Without a branch per token (with one it took twice as long): a value outside the
   // bins counts in one behind them, most often its lane's own, since all of a wave's on
   // one, as masked tokens are, would queue.
@@ -224,7 +232,7 @@ __global__ __launch_bounds__(kThreads) void count_kernel(DrawParams p) {
   s16x2_t bins = {0x7fff, 0x7fff};
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    if (base + (g * kThreads + tid) * 8 >= p.vocab) break;
+    if (base + place_of<G>(g) >= vocab) break;
 #pragma unroll
     for (int i = 4 * g; i < 4 * g + 4; ++i) {
       const u16x2_t mag = __builtin_bit_cast(u16x2_t, v[i] & 0x7fff7fffu);
@@ -246,8 +254,7 @@ __global__ __launch_bounds__(kThreads) void count_kernel(DrawParams p) {
   uint32_t top = top_bin == 0x7fff ? 0u : key_of_bin(top_bin);
   const uint32_t nan = greedy ? 0xffffu : 0u;
   auto key_at = [&](int i, int h) -> uint32_t {
-    const int local = place(i, h);
-    return base + local < p.vocab ? key_of(h ? v[i] >> 16 : v[i] & 0xffffu, nan) : 0u;
+    return base + place(i, h) < vocab ? key_of(h ? v[i] >> 16 : v[i] & 0xffffu, nan) : 0u;
   };
   if (by_key) {
     top = 0;
@@ -256,19 +263,18 @@ __global__ __launch_bounds__(kThreads) void count_kernel(DrawParams p) {
   }
   const uint32_t mine = top;
   top = wave_max(top);
-  if ((tid & 63) == 0) best[tid >> 6] = top;
+  if ((tid & 63) == 0) seen.best[tid >> 6] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) top = max(top, best[w]);
-  const int64_t slot = row * p.chunks + chunk;
+  for (int w = 0; w < kWaves; ++w) top = max(top, seen.best[w]);
   if (mine == top) {
-    int at = 0;  // 0x10000 - the first place
+    int at = 0;
     if (by_key) {
 #pragma unroll
       for (int i = 4 * G - 1; i >= 0; --i)
 #pragma unroll
         for (int h = 1; h >= 0; --h)
-          if (key_at(i, h) == top && base + place(i, h) < p.vocab) at = 0x10000 - place(i, h);
+          if (key_at(i, h) == top && base + place(i, h) < vocab) at = 0x10000 - place(i, h);
     } else {
 #pragma unroll
       for (int i = 4 * G - 1; i >= 0; --i) {
@@ -277,33 +283,57 @@ __global__ __launch_bounds__(kThreads) void count_kernel(DrawParams p) {
         if (pair.x == top_bin) at = 0x10000 - place(i, 0);
       }
     }
-    if (at) atomicMax(&first, at);
+    if (at) atomicMax(&seen.first, at);
   }
   if (other) {
-    uint32_t seen = 0;
+    uint32_t out = 0;
 #pragma unroll
     for (int i = 0; i < 4 * G; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint32_t b = h ? v[i] >> 16 : v[i] & 0xffffu, key = key_of(b, 0);
         if (key > kMinusInf && bin_of(b) < 0)
-          seen = max(seen, key < 0x8000u && (b & 0x7fffu) >= kHiField * 128u ? key : kTinyOrHigh);
+          out = max(out, key < 0x8000u && (b & 0x7fffu) >= kHiField * 128u ? key : kTinyOrHigh);
       }
-    if (seen) atomicMax(&outside, seen);
+    if (out) atomicMax(&seen.outside, out);
   }
   __syncthreads();
+  return top;
+}
+// (what lies in `hist` behind the last bin is nobody's)
+__device__ __forceinline__ uint2 pair_of(const uint32_t* hist, int d) {
+  uint2 c = *reinterpret_cast<const uint2*>(&hist[2 * d]);
+  if (2 * d >= 2 * kSide) c = make_uint2(2 * d == 2 * kSide ? c.x : 0u, 0u);
+  return c;
+}
+__device__ __forceinline__ unsigned long long winner_of(uint32_t top, int base, const Seen& seen) {
+  return (unsigned long long)top << 32 | (0xffffffffu - uint32_t(base + 0x10000 - seen.first));
+}
+
+// G groups of eight tokens per thread, 8,192 G tokens per workgroup.
+template <int G>
+__global__ __launch_bounds__(kThreads) void count_kernel(DrawParams p) {
+  __shared__ __attribute__((aligned(16))) uint32_t hist[kBins];
+  __shared__ Seen seen;
+  const int tid = threadIdx.x, chunk = blockIdx.x >> 3;
+  const int64_t row = blockIdx.y * 8 + (blockIdx.x & 7);
+  if (row >= p.batch) return;
+  const int base = chunk * kThreads * 8 * G;
+  uint32_t v[4 * G];
+  load_tokens<G>(v, p.logits + row * p.stride, base, p.vocab);
+  const bool greedy = !(p.temperature[row] > 0.f);
+  const uint32_t top = count_tokens<G>(v, base, p.vocab, greedy, hist, seen);
+  const int64_t slot = row * p.chunks + chunk;
   if (tid == 0) {
-    p.winner[slot] = (unsigned long long)top << 32 | (0xffffffffu - uint32_t(base + 0x10000 - first));
-    p.outside[slot] = outside;
+    p.winner[slot] = winner_of(top, base, seen);
+    p.outside[slot] = seen.outside;
   }
   if (greedy) return;
   uint32_t* counts = p.counts + slot * (kBins / 2);
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) {
-    const int d = i * kThreads + tid;
-    uint2 c = *reinterpret_cast<const uint2*>(&hist[2 * d]);
-    if (2 * d >= 2 * kSide) c = make_uint2(2 * d == 2 * kSide ? c.x : 0u, 0u);  // (behind the last bin)
-    counts[d] = c.x | c.y << 16;
+    const uint2 c = pair_of(hist, i * kThreads + tid);
+    counts[i * kThreads + tid] = c.x | c.y << 16;
   }
 }
 
@@ -350,6 +380,7 @@ struct Place {
 };
 
 struct Shared {
+  Seen seen;
   Place last;
   double total;
   double weight[kBins];
@@ -527,7 +558,8 @@ __device__ __noinline__ int draw_outside(const Row& r, Shared& s) {
   return drawn;
 }
 
-template <int G>
+// ONE: the row is one chunk, whose tokens are counted here.
+template <int G, bool ONE>
 __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
   constexpr int kChunk = kThreads * 8 * G;
   __shared__ __attribute__((aligned(16))) Shared s;
@@ -541,7 +573,13 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
   const float pf = p.top_p ? p.top_p[row] : 1.f, mf = p.min_p ? p.min_p[row] : 0.f;
   unsigned long long top = 0;
   uint32_t outside = 0;
-  if (lane < p.chunks) {
+  uint32_t tokens[4 * G];
+  if constexpr (ONE) {
+    load_tokens<G>(tokens, p.logits + row * p.stride, 0, p.vocab);
+    const uint32_t key = count_tokens<G>(tokens, 0, p.vocab, !(tf > 0.f), s.count, s.seen);
+    top = winner_of(key, 0, s.seen);
+    outside = s.seen.outside;
+  } else if (lane < p.chunks) {
     top = p.winner[row * p.chunks + lane];
     outside = p.outside[row * p.chunks + lane];
   }
@@ -554,10 +592,12 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
       for (int j = 0; j < kPairs; ++j)
         counts[q][j] = c0 + q < p.chunks ? row_counts[(c0 + q) * (kBins / 2) + j * kThreads] : 0u;
   };
-  load_counts(0);
-  for (int o = 1; o < p.chunks; o <<= 1) {
-    top = max(top, (unsigned long long)__shfl_xor((long long)top, o));
-    outside = max(outside, uint32_t(__shfl_xor(int(outside), o)));
+  if constexpr (!ONE) {
+    load_counts(0);
+    for (int o = 1; o < p.chunks; o <<= 1) {
+      top = max(top, (unsigned long long)__shfl_xor((long long)top, o));
+      outside = max(outside, uint32_t(__shfl_xor(int(outside), o)));
+    }
   }
   top = (unsigned long long)__builtin_amdgcn_readfirstlane(int(top >> 32)) << 32 |
         uint32_t(__builtin_amdgcn_readfirstlane(int(top)));
@@ -585,7 +625,13 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
   }
 
   // pair d = 1,024 j + tid: this thread's bins 2 d and 2 d + 1, group 16 j + wave
-  {
+  if constexpr (ONE) {
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+      const int d = j * kThreads + tid;
+      if (d >= kSide) *reinterpret_cast<uint2*>(&s.count[2 * d]) = pair_of(s.count, d);
+    }
+  } else {
     uint2 cnt[kPairs] = {};
     for (int c0 = 0; c0 < p.chunks; c0 += kTogether) {
       if (c0) load_counts(c0);
@@ -653,67 +699,70 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
   // kept: the bins before last_bin and the first `ties` tokens of it
   const int last_bin = s.last.bin, ties = s.last.kept;
   const double target = r.u * s.total, w_last = s.weight[last_bin];
-  // each chunk's mass above the last kept value, and its tokens with it
-  for (int c0 = 0; c0 < p.chunks; c0 += kTogether) {
-    if (c0 || p.chunks > kTogether) load_counts(c0);
-    double m[kTogether] = {};
+  int chunk = 0, room = ties;
+  double cum = 0.0, sum = 0.0;
+  bool some = ONE && int(s.count[last_bin]) > ties;  // not all of the chunk's tokens with the last value are kept
+  if constexpr (!ONE) {
+    // each chunk's mass above the last kept value, and its tokens with it
+    for (int c0 = 0; c0 < p.chunks; c0 += kTogether) {
+      if (c0 || p.chunks > kTogether) load_counts(c0);
+      double m[kTogether] = {};
 #pragma unroll
-    for (int j = 0; j < kPairs; ++j) {
-      const int bin = 2 * (j * kThreads + tid), group = j * kWaves + wave;
-      if (j * kThreads + tid == last_bin / 2) {
+      for (int j = 0; j < kPairs; ++j) {
+        const int bin = 2 * (j * kThreads + tid), group = j * kWaves + wave;
+        if (j * kThreads + tid == last_bin / 2) {
+#pragma unroll
+          for (int q = 0; q < kTogether; ++q)
+            if (c0 + q < p.chunks) s.chunk_ties[c0 + q] = int(counts[q][j] >> (16 * (last_bin & 1)) & 0xffffu);
+        }
+        if (128 * group > last_bin || s.group_count[group] == 0) continue;
+        double2 w = *reinterpret_cast<const double2*>(&s.weight[bin]);
+        if (bin >= last_bin) w.x = 0.0;
+        if (bin + 1 >= last_bin) w.y = 0.0;
 #pragma unroll
         for (int q = 0; q < kTogether; ++q)
-          if (c0 + q < p.chunks) s.chunk_ties[c0 + q] = int(counts[q][j] >> (16 * (last_bin & 1)) & 0xffffu);
+          m[q] += whole(counts[q][j] & 0xffffu) * w.x + whole(counts[q][j] >> 16) * w.y;
       }
-      if (128 * group > last_bin || s.group_count[group] == 0) continue;
-      double2 w = *reinterpret_cast<const double2*>(&s.weight[bin]);
-      if (bin >= last_bin) w.x = 0.0;
-      if (bin + 1 >= last_bin) w.y = 0.0;
-#pragma unroll
-      for (int q = 0; q < kTogether; ++q)
-        m[q] += whole(counts[q][j] & 0xffffu) * w.x + whole(counts[q][j] >> 16) * w.y;
+      const double four = wave_sum4(m[0], m[1], m[2], m[3]);
+      if (lane < 4 && c0 + lane < p.chunks) s.mass[c0 + lane][wave] = four;
+      if (c0 + 4 < p.chunks) {
+        m[4] = wave_sum(m[4]);
+        if (lane == 0) s.mass[c0 + 4][wave] = m[4];
+      }
     }
-    const double four = wave_sum4(m[0], m[1], m[2], m[3]);
-    if (lane < 4 && c0 + lane < p.chunks) s.mass[c0 + lane][wave] = four;
-    if (c0 + 4 < p.chunks) {
-      m[4] = wave_sum(m[4]);
-      if (lane == 0) s.mass[c0 + 4][wave] = m[4];
-    }
-  }
-  __syncthreads();
-  if (tid < p.chunks) {
-    double m = 0.0;
+    __syncthreads();
+    if (tid < p.chunks) {
+      double m = 0.0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m += s.mass[tid][w];
-    s.chunk_mass[tid] = m;
-  }
-  __syncthreads();
-  // The chunk of the draw: the first whose mass takes the sum over the target, or, with u
-  // so near 1 that none does, the last that has any.
-  int chunk = 0, room = ties, left = ties;
-  double cum = 0.0, sum = 0.0;
-  for (int c = 0; c < p.chunks; ++c) {
-    const int here = min(s.chunk_ties[c], left);
-    const double m = s.chunk_mass[c] + here * w_last;
-    if (m > 0.0) chunk = c, room = left, cum = sum;
-    if (sum + m > target) break;
-    sum += m;
-    left -= here;
+      for (int w = 0; w < kWaves; ++w) m += s.mass[tid][w];
+      s.chunk_mass[tid] = m;
+    }
+    __syncthreads();
+    // The chunk of the draw: the first whose mass takes the sum over the target, or, with u
+    // so near 1 that none does, the last that has any.
+    int left = ties;
+    for (int c = 0; c < p.chunks; ++c) {
+      const int here = min(s.chunk_ties[c], left);
+      const double m = s.chunk_mass[c] + here * w_last;
+      if (m > 0.0) chunk = c, room = left, cum = sum;
+      if (sum + m > target) break;
+      sum += m;
+      left -= here;
+    }
+    some = s.chunk_ties[chunk] > room;
   }
 
-  // Its tokens once more: wave w has 512 G of them in a row, group i of a lane the
-  // eight from 512 i + 8 lane on.
-  const int first = chunk * kChunk + wave * 512 * G + lane * 8;
+  // Its tokens, once more where another workgroup counted them.
+  if constexpr (!ONE) load_tokens<G>(tokens, r.logits, chunk * kChunk, p.vocab);
+  const int first = chunk * kChunk + place_of<G>(0);
   const u16x2_t past = u16x2_t((unsigned short)(min(last_bin, 2 * kSide) + 1));
-  u16x2_t bins[G][4];  // of its tokens, `past` for those that are not kept
+  u16x2_t bins[G][4];  // `past` for those that are not kept
 #pragma unroll
-  for (int i = 0; i < G; ++i) {
-    const uint4 v = first + i * 512 < p.vocab ? load8(r.logits, first + i * 512, p.vocab) : make_uint4(kPad, kPad, kPad, kPad);
-    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+  for (int i = 0; i < G; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) bins[i][j] = __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, bin_pair(x[j])), past);
-  }
-  if (s.chunk_ties[chunk] > room) {  // not all of its tokens with the last value are kept
+    for (int j = 0; j < 4; ++j)
+      bins[i][j] = __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, bin_pair(tokens[4 * i + j])), past);
+  if (some) {
     int n = 0, inc[G];
     uint32_t same[G];  // of a group's eight, a bit each
 #pragma unroll
@@ -799,10 +848,14 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
   p.out[row] = drawn;
 }
 
-// Tokens of a workgroup: few enough that a small batch takes more CUs (and a thread
-// looks up fewer weights at the end), as long as the counts of a row's chunks, 20 KB
-// each, stay few.
+// Tokens of a workgroup.  A short row is one chunk, counted and drawn in one launch (us, in
+// a graph, against two launches: 1 x 5,000 9.2 and 12.1, 300 x 5,000 18 and 30, 1 x 16,384
+// 10.3 and 12.9; 32 x 32,768 15.6 and 15.5, 256 rows of it 16.6 and 22.2, one 15.2 and 14.0).
+// Else few enough that a small batch takes more CUs (and a thread looks up fewer weights
+// at the end), as long as the counts of a row's chunks, 20 KB each, stay few.
 int groups_for(int64_t batch, int64_t vocab) {
+  if (vocab <= 16384) return vocab <= 8192 ? 1 : 2;  // one chunk
+  if (vocab <= 32768 && batch >= 32) return 4;
   if (vocab <= 8 * 8192 && batch * ((vocab + 8191) / 8192) <= 256) return 1;
   if (vocab <= 32 * 16384 && batch * ((vocab + 16383) / 16384) <= 256) return 2;
   return 4;
@@ -858,15 +911,16 @@ extern "C" int mi_draw(const void* logits, int64_t logits_row_stride, int32_t ba
   p.outside = reinterpret_cast<uint32_t*>(p.winner + used);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 chunks(8 * p.chunks, (batch_size + 7) / 8), rows(batch_size), threads(kThreads);
-  if (groups == 1) {
-    hipLaunchKernelGGL(count_kernel<1>, chunks, threads, 0, s, p);
-    hipLaunchKernelGGL(draw_kernel<1>, rows, threads, 0, s, p);
-  } else if (groups == 2) {
-    hipLaunchKernelGGL(count_kernel<2>, chunks, threads, 0, s, p);
-    hipLaunchKernelGGL(draw_kernel<2>, rows, threads, 0, s, p);
-  } else {
-    hipLaunchKernelGGL(count_kernel<4>, chunks, threads, 0, s, p);
-    hipLaunchKernelGGL(draw_kernel<4>, rows, threads, 0, s, p);
-  }
+  auto run = [&]<int G>() {
+    if (p.chunks == 1) {
+      hipLaunchKernelGGL((draw_kernel<G, true>), rows, threads, 0, s, p);
+      return;
+    }
+    hipLaunchKernelGGL(count_kernel<G>, chunks, threads, 0, s, p);
+    hipLaunchKernelGGL((draw_kernel<G, false>), rows, threads, 0, s, p);
+  };
+  if (groups == 1) run.template operator()<1>();
+  else if (groups == 2) run.template operator()<2>();
+  else run.template operator()<4>();
   return mi::check_launch("draw_kernel");
 }

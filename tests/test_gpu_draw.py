@@ -63,6 +63,30 @@ def test_every_filter(dev, vocab):
     _check(dev, logits, u, off)
 
 
+@pytest.mark.parametrize("b,v", [(12, 5000), (12, 8192), (12, 8193), (12, 16384), (32, 16385), (36, 32761), (36, 32768), (31, 32768)])
+def test_rows_of_one_chunk_and_beside_them(dev, b, v):
+    """Short rows, which one launch counts and draws, up to the sizes where two begin:
+    ties cut inside a value, masks, NaN, infinities, values outside the counted range,
+    greedy rows."""
+    logits = _logits(b, v, dev, v + b)
+    logits[0] = 0
+    logits[1] = torch.randint(0, 3, (v,), device=dev, generator=torch.Generator(device=dev).manual_seed(1))
+    logits[2, 17:] = -math.inf
+    logits[3, 5:v - 3] = torch.finfo(torch.bfloat16).min
+    logits[4, ::2] = math.nan
+    logits[5, v // 2] = math.inf
+    logits[6] *= 300
+    logits[7, 9] = 2.0 ** -40
+    logits[8] = -math.inf
+    logits[9] = math.nan
+    u = _uniform(b, dev, v)
+    t = [0.0 if i in (10, 11) else 0.4 + 0.1 * (i % 9) for i in range(b)]
+    _check(dev, logits, u, t)
+    _check(dev, logits, u, t, top_k=[v // 3, 7, 3, 50][:4] * (b // 4) + [1] * (b % 4))
+    _check(dev, logits, u, t, top_p=[0.3, 0.9, 1.0] * (b // 3) + [0.5] * (b % 3), min_p=[0.0, 0.02] * (b // 2) + [0.1] * (b % 2))
+    _check(dev, logits, u, [50.0] * b, top_k=[1000] * b, top_p=[0.7] * b, min_p=[0.001] * b)
+
+
 def test_ties_go_to_the_lowest_index(dev):
     """Rows of one value and of three, cut inside a value by top-k and by top-p, over
     several chunks."""
