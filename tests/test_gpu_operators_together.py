@@ -190,3 +190,35 @@ def test_draws_from_rows_far_apart(dev):
     s.set_params([0.8] * b, [0.95] * b, top_k=[100] * b, min_p=[0.01] * b)
     near = s.draw(logits.contiguous(), u).clone()
     assert torch.equal(s.draw(logits, u), near)
+
+
+def test_server_engine_with_4_bit_layers(dev):
+    """weight_format: mxfp4 in the server's configuration: the loop's greedy tokens are
+    those of a scheduler over the same model quantised by hand."""
+    import queue
+
+    from minimal_inference_amd.engine import Request, Scheduler
+    from minimal_inference_amd.model import PRESETS, Model
+    from minimal_inference_amd.mxfp4 import MXFP4
+    from minimal_inference_amd.server import init_engine
+
+    sizes = {"max_batch_size": 4, "max_seq_len": 256}
+    sch, _, _, stops = init_engine({"model_preset": "qwen2.5-0.5b", "weight_format": "mxfp4", "seed": 5, "scheduler": sizes})
+    try:
+        assert all(isinstance(w, MXFP4) for layer in sch.model.layers
+                   for w in (layer.w_qkv, layer.w_o, layer.w_gate_up, layer.w_down))
+        prompt = list(range(40, 100))
+        got: queue.Queue = queue.Queue()
+        sch.submit_request(Request("a", prompt, 12, 0.0, sink=got.put))
+        served = []
+        while (token := got.get(timeout=60)) is not None:
+            served.append(token)
+    finally:
+        sch.stop()
+    model = Model(PRESETS["qwen2.5-0.5b"], dev, seed=5, max_positions=256 + 16)
+    model.quantize_weights()
+    other = Scheduler(model, eos_token_ids=stops or None, seed=5, **sizes)
+    request = Request("b", prompt, 12, 0.0)
+    other.submit(request)
+    other.run()
+    assert served == request.generated_tokens

@@ -115,3 +115,10 @@ def test_workspace_of_the_products():
     assert size(8192, 10240, 8192, 0, 1) == 0
     for bad in ((-1, 32, 64), (100, 0, 64), (100, 32, 48), ((1 << 22) + 1, 32, 64)):
         assert size(*bad, 0, 0) == 0
+
+
+def test_server_refuses_other_weight_formats():
+    from minimal_inference_amd.server import init_engine
+
+    with pytest.raises(ValueError, match="weight_format"):
+        init_engine({"weight_format": "int4"})
