@@ -18,10 +18,12 @@
 //          thread; prefix sums of count and mass give the last kept value and how many
 //          tokens of it; each chunk's kept mass gives the chunk of the draw, whose
 //          tokens are read once more.
-// Values from -2^8 down weigh nothing beside a maximum that is 45 t above; a row that
-// holds other values outside the counted range takes the draw kernel's second path, which
-// finds the same boundary by bisection over the 2^16 values, a pass over the row each (48
-// such rows of 152,064: up to 1.1 ms).
+// Values from -2^8 down are left out of a row where all of them together would weigh less
+// than the rounding of u times the total does (the total is 1 at least: 66 t below the
+// maximum for u from 2^-24 on; at u = 0 only those whose power is 0 in 64 bits).  A row
+// that holds other values outside the counted range takes the draw kernel's second path,
+// which finds the same boundary by bisection over the 2^16 values, a pass over the row each
+// (48 such rows of 152,064: up to 1.1 ms).
 //
 // Bound: latency.  48 rows x 152,064 (us): count 6.6 to 7.9, of which the LDS atomics take
 // 3.5 (16 cycles a wave's, at any spread of values); draw 15.8, a chain on one CU per
@@ -617,7 +619,9 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
   r.top_p = pf < 1.f ? double(pf) : 2.0;
   r.min_p = mf > 0.f ? fmin(double(mf), 1.0) : 0.0;
   r.u = fmax(double(uf), 0.0);
-  if (outside >= kTinyOrHigh || (outside && (value_of_key(outside) - r.lmax) * r.per_t > -64.0)) {
+  // (the largest of the low values stands for all; -1,100: from there on a power is 0)
+  if (outside >= kTinyOrHigh || (outside && (value_of_key(outside) - r.lmax) * r.per_t > -1100.0 &&
+                                 r.weigh(outside) * r.vocab > r.u * 0x1p-53)) {
     const Row copy = r;  // (r itself stays in registers)
     const int drawn = draw_outside(copy, s);
     if (tid == 0) p.out[row] = drawn;
