@@ -834,8 +834,10 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(DrawParams p) {
     if (gi == i) g = group[i];
   const unsigned long long over = __ballot(g > 0.0 && ahead + inc > target), any = __ballot(g > 0.0);
   const int the_lane = over ? __builtin_ctzll(over) : any ? 63 - __builtin_clzll(any) : 0;
+  // (the lane's own sum less its own weights would lose what is small beside them)
+  const double before = the_lane ? lane_value(inc, the_lane - 1) : 0.0;
   if (lane != the_lane) return;
-  double at = ahead + (inc - g);
+  double at = ahead + before;
   int drawn = first + gi * 512;
   bool stop = false;
 #pragma unroll

@@ -59,3 +59,18 @@ def test_zero_and_small_u_beside_low_values(dev, v):
         _check(dev, logits, uniforms, t)
         _check(dev, logits, uniforms, t, top_k=[0, 1, 2, v // 2] * 4, top_p=[1.0, 1.0, 0.9, 1.0] * 4,
                min_p=[0.0, 0.0, 0.0, 1e-30] * 4)
+
+
+@pytest.mark.parametrize("v", [100, 40000])
+def test_small_u_inside_a_lane(dev, v):
+    """u between the sums of tokens that weigh next to nothing, some of them beside one
+    that holds nearly all of the weight."""
+    logits = torch.full((64, v), -200.0, device=dev, dtype=torch.bfloat16)
+    u = torch.empty(64, dtype=torch.float64)
+    for i in range(64):
+        logits[i, : i + 1] = -80.0
+        logits[i, i + 1] = 0.0
+        u[i] = (i + 0.5) * math.exp(-80.0)  # the last of those i + 1
+    _check(dev, logits, u.float().to(dev), [1.0] * 64)
+    _check(dev, logits, (u / 2).float().to(dev), [1.0] * 64, min_p=[1e-35] * 64)
+    _check(dev, logits, u.float().to(dev), [1.0] * 64, top_k=[50] * 64)
