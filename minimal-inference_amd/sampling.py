@@ -10,10 +10,11 @@ final ``.tolist()``, as in the reference.
 
 ``Sampler`` is the allocation-free form for graph capture: it owns device
 buffers for per-row temperature / top-p, the output ids, the Philox counter
-and the kernels' workspace (sized at construction for ``vocab`` when given,
-else for the largest vocabulary seen; a workspace that grows is replaced but
-kept alive, so a graph captured with the old one never writes into freed
-memory), so a captured decode step can include the draw.
+and the kernels' workspaces, one of ``sample`` and one of ``draw`` (sized at
+construction for ``vocab`` when given, else for the largest vocabulary seen, which
+takes one call before a capture; a workspace that grows is replaced but kept alive,
+so a graph captured with the old one never writes into freed memory), so a captured
+decode step can include the draw.
 
 ``Sampler.draw`` draws from given uniform numbers, one per row, with top-k and min-p
 beside temperature and top-p (``set_params(top_k=, min_p=)``): the same numbers give
@@ -50,6 +51,7 @@ class Sampler:
         self._retired: list[torch.Tensor] = []  # replaced workspaces a captured graph may still use
         if vocab is not None:
             self._workspace_for(vocab)
+            self._draw_workspace_for(vocab)
 
     def _workspace_for(self, vocab: int) -> torch.Tensor:
         need = int(_lib.load().mi_sample_workspace_size(self.max_batch, vocab))

@@ -74,3 +74,24 @@ def test_small_u_inside_a_lane(dev, v):
     _check(dev, logits, u.float().to(dev), [1.0] * 64)
     _check(dev, logits, (u / 2).float().to(dev), [1.0] * 64, min_p=[1e-35] * 64)
     _check(dev, logits, u.float().to(dev), [1.0] * 64, top_k=[50] * 64)
+
+
+@pytest.mark.parametrize("b,v", [(3, 500), (2, 50000)])
+def test_first_draw_of_a_sampler_in_a_graph(dev, b, v):
+    """A sampler that knows its vocabulary is ready for a captured draw as it stands."""
+    from minimal_inference_amd.sampling import Sampler
+
+    s = Sampler(dev, b, vocab=v)
+    s.set_params([0.9] * b, [0.9] * b, top_k=[40] * b, min_p=[0.01] * b)
+    logits, u = _logits(b, v, dev, 1), _uniform(b, dev, 2)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ids = s.draw(logits, u)
+    f = lambda x: torch.tensor(x).double().item()  # noqa: E731
+    for seed in range(3):
+        logits.copy_(_logits(b, v, dev, 10 + seed))
+        u.copy_(_uniform(b, dev, 20 + seed))
+        graph.replay()
+        held = ids.tolist()
+        assert held == [draw_row(logits[i].cpu(), u[i].item(), f(0.9), 40, f(0.9), f(0.01)) for i in range(b)]
+        assert s.draw(logits, u).tolist() == held
