@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -37,6 +38,17 @@ def require_gpu(name: str, t: torch.Tensor) -> None:
 def require_dtype(name: str, t: torch.Tensor, dtype: torch.dtype) -> None:
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype} (got {t.dtype})")
+
+
+def refuse_derivatives(name: str, t: torch.Tensor | None) -> None:
+    """Of an operator without a backward pass: a tensor that asks for a gradient, or that
+    carries a forward-mode tangent (which a kernel of the library would drop)."""
+    if t is None:
+        return
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: there is no backward pass")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} has a forward-mode tangent: there is no derivative")
 
 
 def require_i32_vector(name: str, t: torch.Tensor) -> None:

@@ -23,7 +23,7 @@ from torch.autograd import forward_ad
 from torch.overrides import has_torch_function
 
 from . import _lib
-from ._util import call_on, require_dtype, require_gpu, stream_of
+from ._util import call_on, refuse_derivatives, require_dtype, require_gpu, stream_of
 
 
 def _rows(name: str, t: torch.Tensor, width: int | None = None) -> None:
@@ -66,8 +66,7 @@ def add_rms_norm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tens
 
 
 def _refuse(name: str, t: torch.Tensor, shape, device) -> None:
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient: there is no backward pass")
+    refuse_derivatives(name, t)
     raise ValueError(f"{name} must be {tuple(shape)} bfloat16 on {device} with a contiguous last axis; got "
                      f"{tuple(t.shape)} {t.dtype} on {t.device}")
 
@@ -83,6 +82,7 @@ def post_norm_add_rms_norm(x: torch.Tensor, y: torch.Tensor, post_weight: torch.
 
     in fp32, the second norm from s before its rounding.  ``gate``: [hidden], [rows, 1]
     or [rows, hidden].  x_out may be x, and h_out y; other overlaps are undefined.
+    Tensors that ask for gradients or carry forward-mode tangents are refused.
     """
     _rows("x", x)
     shape = x.shape
@@ -98,6 +98,10 @@ def post_norm_add_rms_norm(x: torch.Tensor, y: torch.Tensor, post_weight: torch.
         if (t.shape != (hidden,) or t.dtype != torch.bfloat16 or t.get_device() != device or t.stride(0) != 1
                 or (grad and t.requires_grad)):
             _refuse(name, t, (hidden,), x.device)
+    if forward_ad._current_level >= 0:
+        for name, t in (("x", x), ("y", y), ("post_weight", post_weight), ("weight", weight), ("gate", gate),
+                        ("x_out", x_out), ("h_out", h_out)):
+            refuse_derivatives(name, t)
     if x_out is None:
         x_out = x
     if h_out is None:

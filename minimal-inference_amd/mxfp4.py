@@ -10,7 +10,7 @@ the matrix instructions' operand order; ``quantize_mxfp4(x)`` makes one of bf16 
 x bf16, or MXFP4 too.  ``linear_silu_mxfp4(x, gate_up)`` is
 ``silu(x @ gate.T) * (x @ up.T)`` of a fused gate and up weight in the same launch.
 Both accumulate in fp32 and round once.  There is no torch fallback and no backward
-pass: inputs that ask for gradients are refused.
+pass: tensors that ask for gradients or carry forward-mode tangents are refused.
 """
 
 from __future__ import annotations
@@ -20,7 +20,7 @@ import functools
 import torch
 
 from . import _lib
-from ._util import call_on, require_dtype, require_gpu
+from ._util import call_on, refuse_derivatives, require_dtype, require_gpu
 
 BLOCK = 32
 _TILE_ROWS, _SLAB, _TILE_BYTES, _QUAD_BYTES = 16, 128, 1024, 256
@@ -33,8 +33,7 @@ def _rows_of(name: str, t: torch.Tensor) -> tuple[int, int]:
     shape = t.shape
     if len(shape) != 2 or t.stride(1) != 1:
         raise ValueError(f"{name} must be [rows, width] with a contiguous last axis; got {tuple(shape)}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient: there is no backward pass")
+    refuse_derivatives(name, t)
     return shape
 
 
@@ -150,8 +149,7 @@ def _linear(x, weight: MXFP4, bias, out, silu: bool) -> torch.Tensor:
         require_dtype("bias", bias, torch.bfloat16)
         if bias.shape != (n,) or not bias.is_contiguous() or bias.device != like.device:
             raise ValueError(f"bias must be a contiguous [{n}] tensor on {like.device}")
-        if bias.requires_grad and torch.is_grad_enabled():
-            raise ValueError("bias requires a gradient: there is no backward pass")
+        refuse_derivatives("bias", bias)
     if out is not None and out is x:
         raise ValueError("out is x, which other workgroups still read")
     out = _out(out, rows, n, like)

@@ -1,0 +1,45 @@
+"""GPU: what the operators over 4-bit matrices and the norms around a block refuse, and
+their largest forms with a bias, infinities and NaN."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def test_tangents_are_refused(dev):
+    """A forward-mode tangent would be dropped: it is refused like a gradient, on every
+    argument; tensors without one pass inside a level, and after it all do."""
+    from torch.autograd import forward_ad
+
+    from minimal_inference_amd.dense import post_norm_add_rms_norm
+    from minimal_inference_amd.mxfp4 import linear_mxfp4, linear_silu_mxfp4, quantize_mxfp4
+
+    x = torch.randn(4, 64, device=dev).to(torch.bfloat16)
+    w = quantize_mxfp4(torch.randn(32, 64, device=dev).to(torch.bfloat16))
+    bias, norm = torch.ones(32, device=dev, dtype=torch.bfloat16), torch.ones(64, device=dev, dtype=torch.bfloat16)
+    want = linear_mxfp4(x, w, bias), linear_silu_mxfp4(x, w), quantize_mxfp4(x).dequantize()
+    norms = post_norm_add_rms_norm(x, x, norm, norm, 1e-6, gate=norm, x_out=torch.empty_like(x))
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        out = dual(torch.empty_like(want[0]))
+        for bad in [lambda: linear_mxfp4(dual(x), w), lambda: linear_mxfp4(x, w, dual(bias)),
+                    lambda: linear_mxfp4(x, w, out=out), lambda: linear_silu_mxfp4(dual(x), w),
+                    lambda: quantize_mxfp4(dual(x)), lambda: w.dequantize(dual(torch.empty(32, 64, device=dev, dtype=x.dtype))),
+                    lambda: post_norm_add_rms_norm(dual(x), x, norm, norm, 1e-6, x_out=torch.empty_like(x)),
+                    lambda: post_norm_add_rms_norm(x, dual(x), norm, norm, 1e-6, x_out=torch.empty_like(x)),
+                    lambda: post_norm_add_rms_norm(x, x, dual(norm), norm, 1e-6, x_out=torch.empty_like(x)),
+                    lambda: post_norm_add_rms_norm(x, x, norm, dual(norm), 1e-6, x_out=torch.empty_like(x)),
+                    lambda: post_norm_add_rms_norm(x, x, norm, norm, 1e-6, gate=dual(norm), x_out=torch.empty_like(x)),
+                    lambda: post_norm_add_rms_norm(x, x, norm, norm, 1e-6, x_out=dual(torch.empty_like(x))),
+                    lambda: post_norm_add_rms_norm(x, x, norm, norm, 1e-6, x_out=torch.empty_like(x), h_out=dual(x.clone()))]:
+            with pytest.raises(ValueError, match="tangent"):
+                bad()
+        assert torch.equal(linear_mxfp4(x, w, bias), want[0])
+        with torch.inference_mode():  # (no derivatives are asked for there)
+            assert torch.equal(linear_silu_mxfp4(dual(x), w), want[1])
+        x2 = dual(x)
+    assert torch.equal(quantize_mxfp4(x2).dequantize(), want[2])
+    assert torch.equal(post_norm_add_rms_norm(x, x, norm, norm, 1e-6, gate=norm, x_out=torch.empty_like(x)), norms)
