@@ -65,6 +65,9 @@ def add_rms_norm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tens
     return h_out if norm else None
 
 
+_NORM_MAX_HIDDEN = 16384
+
+
 def _refuse(name: str, t: torch.Tensor, shape, device) -> None:
     refuse_derivatives(name, t)
     raise ValueError(f"{name} must be {tuple(shape)} bfloat16 on {device} with a contiguous last axis; got "
@@ -87,6 +90,8 @@ def post_norm_add_rms_norm(x: torch.Tensor, y: torch.Tensor, post_weight: torch.
     _rows("x", x)
     shape = x.shape
     rows, hidden = shape
+    if hidden > _NORM_MAX_HIDDEN:  # (the entry takes 32 bits of it)
+        raise ValueError(f"hidden is {hidden}: multiples of 8 up to {_NORM_MAX_HIDDEN}")
     device, grad = x.get_device(), torch.is_grad_enabled()
     if grad and x.requires_grad:
         _refuse("x", x, shape, x.device)

@@ -30,6 +30,7 @@ from . import _lib
 from ._util import call_on, require_dtype, require_gpu, stream_of
 
 _DEFAULT_SEED = 0x6D69616D64  # "miamd"
+_DRAW_MAX_VOCAB = 1 << 20
 
 
 class Sampler:
@@ -113,6 +114,8 @@ class Sampler:
         require_dtype("logits", logits, torch.bfloat16)
         if logits.dim() != 2 or logits.stride(1) != 1:
             raise ValueError("logits must be [B, V] with a contiguous vocab axis")
+        if logits.shape[1] > _DRAW_MAX_VOCAB:  # (the entry takes 32 bits of it)
+            raise ValueError(f"rows of {logits.shape[1]} tokens: at most {_DRAW_MAX_VOCAB}")
         n = logits.shape[0] if n is None else n
         if not 0 <= n <= min(logits.shape[0], self.max_batch):
             raise ValueError(f"{n} rows: logits have {logits.shape[0]}, the sampler takes {self.max_batch}")

@@ -43,3 +43,17 @@ def test_tangents_are_refused(dev):
         x2 = dual(x)
     assert torch.equal(quantize_mxfp4(x2).dequantize(), want[2])
     assert torch.equal(post_norm_add_rms_norm(x, x, norm, norm, 1e-6, gate=norm, x_out=torch.empty_like(x)), norms)
+
+
+def test_widths_past_32_bits_are_refused(dev):
+    """Sizes whose lower 32 bits are a width that the kernels take."""
+    from minimal_inference_amd.dense import post_norm_add_rms_norm
+    from minimal_inference_amd.sampling import Sampler
+
+    wide = torch.empty(1, (1 << 32) + 64, device=dev, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="hidden"):
+        post_norm_add_rms_norm(wide, wide, wide[0], wide[0], 1e-6, h_out=wide)
+    s = Sampler(dev, 1, vocab=64)
+    s.set_params([1.0])
+    with pytest.raises(ValueError, match="tokens"):
+        s.draw(wide, torch.zeros(1, device=dev))
