@@ -18,6 +18,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._util import call_on, refuse_derivatives, require_dtype, require_gpu
@@ -33,7 +34,8 @@ def _rows_of(name: str, t: torch.Tensor) -> tuple[int, int]:
     shape = t.shape
     if len(shape) != 2 or t.stride(1) != 1:
         raise ValueError(f"{name} must be [rows, width] with a contiguous last axis; got {tuple(shape)}")
-    refuse_derivatives(name, t)
+    if t.requires_grad or forward_ad._current_level >= 0:
+        refuse_derivatives(name, t)
     return shape
 
 
@@ -149,7 +151,8 @@ def _linear(x, weight: MXFP4, bias, out, silu: bool) -> torch.Tensor:
         require_dtype("bias", bias, torch.bfloat16)
         if bias.shape != (n,) or not bias.is_contiguous() or bias.device != like.device:
             raise ValueError(f"bias must be a contiguous [{n}] tensor on {like.device}")
-        refuse_derivatives("bias", bias)
+        if bias.requires_grad or forward_ad._current_level >= 0:
+            refuse_derivatives("bias", bias)
     if out is not None and out is x:
         raise ValueError("out is x, which other workgroups still read")
     out = _out(out, rows, n, like)
