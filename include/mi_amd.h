@@ -428,7 +428,8 @@ int mi_mxfp4_unpack(const void* codes, const void* scales, void* row_codes, void
  * not read.  silu != 0: W is [2 n][k], n gate rows and then n up rows, and
  * out = silu(x Wg^T) * (x Wu^T) (MLP, model.py:301-311); no bias then.
  * rows 0..2^22, n 1..2^24 (any), k a multiple of 32 up to 2^20, x_stride at most
- * 2^22; bias [n] or null.  The result does not depend on timing.
+ * 2^22; bias [n] or null.  An out that overlaps x, W or the bias is refused (rows of
+ * one buffer whose columns lie apart do not).  The result does not depend on timing.
  * workspace (16-byte aligned; may be null) holds partial sums of workgroups that
  * share k: mi_linear_mxfp4_workspace_size bytes are what the fastest form takes
  * (often 0); with fewer, one that takes no more is run, with the same results

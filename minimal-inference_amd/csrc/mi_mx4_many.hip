@@ -9,6 +9,7 @@
 #include <algorithm>
 
 #include "mi_mx4_linear.h"
+#include "mi_overlap.h"
 
 namespace mi::mx4 {
 namespace {
@@ -500,6 +501,17 @@ extern "C" int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_sc
   if (out_stride < n || (!x_scales && (x_stride < k || x_stride > kMaxStride)))
     return mi::fail(MI_ERR_INVALID, "linear_mxfp4: row strides %lld (at most 2^22) / %lld for k %lld, n %lld",
                     (long long)x_stride, (long long)out_stride, (long long)k, (long long)n);
+  // (a workgroup's rows of out are written while others still read all of x, W and bias)
+  const int64_t w_rows = silu ? 2 * n : n;
+  const mi::Rows to = {out, out_stride * 2, rows, n * 2};
+  const mi::Rows from[] = {
+      x_scales ? mi::Rows{x, 0, 1, row_tiles(rows) * slabs(k) * kTileBytes} : mi::Rows{x, x_stride * 2, rows, k * 2},
+      {x_scales, 0, x_scales ? 1 : 0, row_tiles(rows) * quads(k) * kQuadBytes},
+      {codes, 0, 1, row_tiles(w_rows) * slabs(k) * kTileBytes},
+      {scales, 0, 1, row_tiles(w_rows) * quads(k) * kQuadBytes},
+      {bias, 0, bias ? 1 : 0, n * 2}};
+  for (const mi::Rows& r : from)
+    if (mi::rows_meet(to, r)) return mi::fail(MI_ERR_INVALID, "linear_mxfp4: out overlaps x, the weight or the bias");
   LinearParams p;
   p.x = static_cast<const char*>(x);
   p.x_stride = x_stride;

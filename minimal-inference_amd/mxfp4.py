@@ -153,8 +153,6 @@ def _linear(x, weight: MXFP4, bias, out, silu: bool) -> torch.Tensor:
             raise ValueError(f"bias must be a contiguous [{n}] tensor on {like.device}")
         if bias.requires_grad or forward_ad._current_level >= 0:
             refuse_derivatives("bias", bias)
-    if out is not None and out is x:
-        raise ValueError("out is x, which other workgroups still read")
     out = _out(out, rows, n, like)
     if rows and n:
         room = _workspace_size(rows, n, k, silu, scales is not None) if rows > _FEW_ROWS else 0
@@ -173,8 +171,8 @@ def _workspace_size(rows: int, n: int, k: int, silu: bool, x_mxfp4: bool) -> int
 
 def linear_mxfp4(x: torch.Tensor | MXFP4, weight: MXFP4, bias: torch.Tensor | None = None,
                  out: torch.Tensor | None = None) -> torch.Tensor:
-    """``x @ weight.T + bias`` as bf16 [rows, n]; x is bf16 [rows, k] or MXFP4.  out must
-    not overlap x."""
+    """``x @ weight.T + bias`` as bf16 [rows, n]; x is bf16 [rows, k] or MXFP4.  An out
+    that overlaps x, the weight or the bias is refused (columns of one buffer need not)."""
     return _linear(x, weight, bias, out, False)
 
 

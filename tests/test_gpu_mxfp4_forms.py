@@ -57,3 +57,25 @@ def test_widths_past_32_bits_are_refused(dev):
     s.set_params([1.0])
     with pytest.raises(ValueError, match="tokens"):
         s.draw(wide, torch.zeros(1, device=dev))
+
+
+@pytest.mark.parametrize("acts", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("rows", [1, 20, 200])
+def test_linear_into_the_columns_beside_x(dev, rows, acts):
+    """x, out and the bias in one buffer, columns and rows apart: as with tensors of their own."""
+    from minimal_inference_amd.mxfp4 import linear_mxfp4, quantize_mxfp4
+
+    n, k = 96, 160
+    w = quantize_mxfp4(torch.randn(n, k, device=dev).to(torch.bfloat16))
+    buffer = torch.randn(rows + 1, k + n + 8, device=dev).to(torch.bfloat16)
+    x, out, bias = buffer[:rows, :k], buffer[:rows, k:k + n], buffer[rows, :n]
+    xx = quantize_mxfp4(x) if acts == "mxfp4" else x
+    want = linear_mxfp4(xx, w, bias.clone())
+    around = buffer.clone()
+    assert linear_mxfp4(xx, w, bias, out=out).data_ptr() == out.data_ptr()
+    around[:rows, k:k + n] = want
+    assert torch.equal(buffer, around)
+    for bad in (buffer[:rows, k - 1:k - 1 + n], buffer[1:rows + 1, :n], buffer[rows:, :n].expand(rows, n)):
+        if acts == "bf16" or bad.data_ptr() == bias.data_ptr():
+            with pytest.raises(ValueError):
+                linear_mxfp4(xx, w, bias, out=bad)

@@ -27,3 +27,32 @@ def test_derivatives():
         with torch.inference_mode():
             refuse_derivatives("x", dual)
     refuse_derivatives("x", dual)
+
+
+FAKE = 1 << 30  # an aligned address that no refused call reads
+
+
+def _lib():
+    from minimal_inference_amd import _lib
+
+    return _lib, _lib.load()
+
+
+@pytest.mark.parametrize("change", [
+    {"out": 0}, {"out": 2}, {"out": -2 * 64 * 3 - 62}, {"out": 2 * 64 * 4 - 2}, {"out_stride": 96, "out": 96 * 2 + 32},
+    {"x_stride": 96, "out_stride": 96, "out": 2 * 63}, {"x_stride": 96, "out_stride": 96, "out": -2 * 63},
+    {"x_stride": 96, "out_stride": 96, "out": -3 * 96 * 2 - 2}, {"n": 64, "out_stride": 64, "out": 0}, {"rows": 1, "out": 126},
+    {"codes": 1 << 20}, {"codes": (1 << 20) - 2048 + 16}, {"codes": (1 << 20) + 448 - 16},
+    {"scales": (1 << 20) - 512 + 16}, {"bias": (1 << 20) + 66}, {"bias": (1 << 20) - 62}, {"silu": 1, "codes": (1 << 20) - 4096 + 16},
+    {"x_scales": (1 << 20) - 240}, {"x_scales": 1 << 24, "x": (1 << 20) - 1008},
+    {"rows": 1 << 22, "x_stride": 128, "out_stride": 136, "out": 136}])
+def test_linear_mxfp4_refuses_an_out_over_its_inputs(change):
+    """Rows of out that share a byte with x, either of the weight's parts or the bias; the
+    weight's rows past its last are part of its tile."""
+    mod, lib = _lib()
+    a = dict(x=0, x_stride=64, x_scales=None, codes=1 << 28, scales=1 << 29, bias=None, out=1 << 20, out_stride=64, rows=4,
+             n=32, k=64, silu=0, ws=None, ws_bytes=0) | change
+    for name in ("x", "x_scales", "codes", "scales", "bias", "out"):
+        a[name] = None if a[name] is None else a[name] + FAKE
+    assert lib.mi_linear_mxfp4(*a.values(), None) == mod.MI_ERR_INVALID
+    assert "overlaps" in mod.last_error()
