@@ -384,7 +384,8 @@ int mi_linear_silu(const void* x, int64_t x_stride, const void* weight, void* ou
  * value per column (gate_per_column != 0; row stride 0: the same for all rows)
  * or one value per row (gate_per_column 0: gate[row * gate_row_stride]).
  * At most 2^22 rows; hidden: multiple of 8, <= 16384; rows, weights and a gate per column 16-byte
- * aligned.  x_out may be x and h_out may be y; no other overlap. */
+ * aligned.  x_out may be x and h_out may be y; a row of an output that overlaps the
+ * other output, a weight, or another row of x, y or gate is refused. */
 int mi_post_norm_add_rms_norm(const void* x, int64_t x_stride, const void* y, int64_t y_stride,
                               const void* post_weight, const void* weight, const void* gate,
                               int64_t gate_row_stride, int32_t gate_per_column, void* x_out,

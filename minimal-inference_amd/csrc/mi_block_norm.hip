@@ -10,6 +10,7 @@
 // one, two or four 16-byte chunks per thread; every load of the row is issued before anything
 // is computed or stored, and the row stays in registers over both sums.
 #include "mi_common.h"
+#include "mi_overlap.h"
 
 namespace {
 
@@ -139,6 +140,18 @@ extern "C" int mi_post_norm_add_rms_norm(const void* x, int64_t x_stride, const 
   if (x_out_stride < hidden || h_stride < hidden)
     return mi::fail(MI_ERR_INVALID, "post_norm_add_rms_norm: output row strides %lld, %lld for hidden %d",
                     (long long)x_out_stride, (long long)h_stride, hidden);
+  // (a row's workgroup has read all of x, y and gate that it takes when it writes; the other
+  // rows' have not, nor has anyone the weights)
+  const int64_t width = int64_t(hidden) * 2;
+  const mi::Rows xo = {x_out, x_out_stride * 2, rows, width}, ho = {h_out, h_stride * 2, rows, width};
+  const mi::Rows in[] = {{x, x_stride * 2, rows, width}, {y, y_stride * 2, rows, width},
+                         {gate, gate_row_stride * 2, gate ? rows : 0, gate_per_column ? width : 2}};
+  const mi::Rows w[] = {{post_weight, 0, 1, width}, {weight, 0, 1, width}};
+  bool meet = mi::rows_meet(xo, ho);
+  for (const mi::Rows& r : in) meet = meet || mi::rows_meet(xo, r, true) || mi::rows_meet(ho, r, true);
+  for (const mi::Rows& r : w) meet = meet || mi::rows_meet(xo, r) || mi::rows_meet(ho, r);
+  if (meet)
+    return mi::fail(MI_ERR_INVALID, "post_norm_add_rms_norm: an output overlaps the other, a weight or another row's input");
   BlockNormParams p;
   p.x = static_cast<const uint16_t*>(x);
   p.x_stride = x_stride;

@@ -84,7 +84,8 @@ def post_norm_add_rms_norm(x: torch.Tensor, y: torch.Tensor, post_weight: torch.
         return bf16(rms_norm(s, weight))
 
     in fp32, the second norm from s before its rounding.  ``gate``: [hidden], [rows, 1]
-    or [rows, hidden].  x_out may be x, and h_out y; other overlaps are undefined.
+    or [rows, hidden].  x_out may be x, and h_out y; outputs that overlap
+    each other, a weight or another row of an input are refused.
     Tensors that ask for gradients or carry forward-mode tangents are refused.
     """
     _rows("x", x)

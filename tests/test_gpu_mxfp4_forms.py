@@ -79,3 +79,31 @@ def test_linear_into_the_columns_beside_x(dev, rows, acts):
         if acts == "bf16" or bad.data_ptr() == bias.data_ptr():
             with pytest.raises(ValueError):
                 linear_mxfp4(xx, w, bias, out=bad)
+
+
+@pytest.mark.parametrize("rows", [1, 7, 300])
+def test_norms_in_place_of_any_input(dev, rows):
+    """Outputs over x, y or a full gate, over a column of a wider buffer and beside x in one:
+    the bits of a call with tensors of their own; overlaps between rows are refused."""
+    from minimal_inference_amd.dense import post_norm_add_rms_norm
+
+    hidden = 264
+    randn = lambda *s: torch.randn(*s, device=dev).to(torch.bfloat16)  # noqa: E731
+    x, y, gate, post, pre = randn(rows, hidden), randn(rows, hidden), randn(rows, hidden), randn(hidden), randn(hidden)
+    want_x = torch.empty_like(x)
+    want = post_norm_add_rms_norm(x, y, post, pre, 1e-6, gate=gate, x_out=want_x)
+    for xo, ho in (("x", "y"), ("y", "x"), ("gate", "x"), ("x", "gate"), ("beside", "x"), ("y", "beside")):
+        wide = randn(rows, 2 * hidden + 8)
+        wide[:, :hidden] = x
+        at = {"x": wide[:, :hidden], "y": y.clone(), "gate": gate.clone(), "beside": wide[:, hidden:2 * hidden]}
+        got = post_norm_add_rms_norm(at["x"], at["y"], post, pre, 1e-6, gate=at["gate"], x_out=at[xo], h_out=at[ho])
+        assert got is at[ho] and torch.equal(got, want) and torch.equal(at[xo], want_x)
+    buffer = randn(rows + 1, hidden)
+    buffer[:rows] = x
+    for bad in [dict(x_out=buffer[:rows], h_out=buffer[:rows])] + ([dict(x_out=buffer[1:]), dict(h_out=buffer[1:])] if rows > 1 else []):
+        with pytest.raises(ValueError, match="overlaps"):
+            post_norm_add_rms_norm(buffer[:rows], y, post, pre, 1e-6, **bad)
+    with pytest.raises(ValueError, match="overlaps"):
+        post_norm_add_rms_norm(x, y, post, buffer[rows], 1e-6, x_out=buffer[1:])
+    with pytest.raises(ValueError, match="overlaps"):
+        post_norm_add_rms_norm(x, x, post, pre, 1e-6, h_out=x)

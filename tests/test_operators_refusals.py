@@ -56,3 +56,21 @@ def test_linear_mxfp4_refuses_an_out_over_its_inputs(change):
         a[name] = None if a[name] is None else a[name] + FAKE
     assert lib.mi_linear_mxfp4(*a.values(), None) == mod.MI_ERR_INVALID
     assert "overlaps" in mod.last_error()
+
+
+@pytest.mark.parametrize("change", [
+    {"h_out": 1 << 24}, {"h_out": (1 << 24) + 3 * 128 + 112}, {"x_out": 16}, {"x_out": -16}, {"x_out": 128}, {"h_out": 16},
+    {"x_out": 1 << 20, "xos": 72}, {"h_out": (1 << 20) - 3 * 128}, {"h_out": (1 << 28) + 112}, {"x_out": (1 << 27) - 496},
+    {"gate": (1 << 24) + 64, "gs": 0, "col": 1}, {"gate": (1 << 24) + 64, "gs": 72, "col": 1}, {"gate": (1 << 24) + 64, "gs": 0},
+    {"gate": (1 << 25) + 128 + 2, "gs": 1}, {"xs": 0, "x_out": 0}, {"xs": 128, "x_out": 0}, {"rows": 1, "h_out": (1 << 24) + 16},
+    {"rows": 1, "x_out": 1 << 27}, {"rows": 1 << 22, "h_out": 128}])
+def test_post_norm_refuses_outputs_over_other_rows(change):
+    """x at 0, y at 2^20, x_out at 2^24, h_out at 2^25, post at 2^27, weight at 2^28: rows of 64
+    values, 4 of them."""
+    mod, lib = _lib()
+    a = dict(x=0, xs=64, y=1 << 20, ys=64, post=1 << 27, weight=1 << 28, gate=None, gs=0, col=0, x_out=1 << 24, xos=64,
+             h_out=1 << 25, hs=64, rows=4, hidden=64, eps=1e-6, scale=1.0) | change
+    for name in ("x", "y", "post", "weight", "gate", "x_out", "h_out"):
+        a[name] = None if a[name] is None else a[name] + FAKE
+    assert lib.mi_post_norm_add_rms_norm(*a.values(), None) == mod.MI_ERR_INVALID
+    assert "overlaps" in mod.last_error()
