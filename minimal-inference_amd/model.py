@@ -41,7 +41,7 @@ import torch
 import torch.nn.functional as F
 
 from .dense import add_rms_norm, linear, linear_silu
-from .mxfp4 import MXFP4, linear_mxfp4, linear_silu_mxfp4, quantize_mxfp4
+from .mxfp4 import BLOCK, MXFP4, linear_mxfp4, linear_silu_mxfp4, quantize_mxfp4
 from .page import append_paged_kv_cache, rope_append_paged_kv_cache
 
 
@@ -199,14 +199,19 @@ class Model:
     def quantize_weights(self) -> None:
         """The layers' projections in microscaled 4-bit floats from here on (0.53 bytes
         per weight); embedding, LM head, norms and biases stay in bf16.  After the
-        weights are loaded and before a scheduler captures its graphs."""
+        weights are loaded and before a scheduler captures its graphs.  Weights that have
+        no such form leave the model as it was."""
         if not self.fused_dense:
             raise ValueError("4-bit weights need fused_dense")
-        for L in self.layers:
-            for name in ("w_qkv", "w_o", "w_gate_up", "w_down"):
-                w = getattr(L, name)
-                if not isinstance(w, MXFP4):
-                    setattr(L, name, quantize_mxfp4(w))
+        weights = [(L, name) for L in self.layers for name in ("w_qkv", "w_o", "w_gate_up", "w_down")
+                   if not isinstance(getattr(L, name), MXFP4)]
+        for L, name in weights:
+            w = getattr(L, name)
+            if not w.is_cuda or w.dtype != torch.bfloat16 or w.shape[1] % BLOCK:
+                raise ValueError(f"4-bit weights are made of bf16 on a GPU with columns in blocks of {BLOCK}; {name} is "
+                                 f"{tuple(w.shape)} {w.dtype} on {w.device}")
+        for L, name in weights:  # (one by one: both forms of all weights need not fit together)
+            setattr(L, name, quantize_mxfp4(getattr(L, name)))
 
     # ------------------------------------------------------------------ forward
     def forward(self, input_ids: torch.Tensor, positions: torch.Tensor, backend: AttentionBackend,
