@@ -53,7 +53,7 @@ import torch
 
 from .decode import BatchDecodeWithPagedKVCacheWrapper
 from .kv_cache import DevicePageTable, PagedKVCache
-from .model import AttentionBackend, Model
+from .model import AttentionBackend, Model, capturers
 from .prefill import BatchPrefillWithPagedKVCacheWrapper
 from .sampling import Sampler
 
@@ -326,6 +326,7 @@ class Scheduler:
                                  cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, self.page_size)
 
     def _capture_graphs(self) -> None:
+        capturers.add(self)
         for bs in self.graph_sizes:
             # all rows are padding rows: they own only the scratch page
             self.pt.step([], [], bs, self.d_indptr, self.d_indices, self.d_last, self.d_batch, self.d_pos)

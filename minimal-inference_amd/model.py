@@ -33,9 +33,11 @@ norms 1) -- the benchmark configurations use random weights.
 from __future__ import annotations
 
 import dataclasses
+import gc
 import json
 import math
 import os
+import weakref
 
 import torch
 import torch.nn.functional as F
@@ -135,6 +137,10 @@ class Layer:
         self.w_down = w(h, cfg.intermediate_size)
 
 
+# Schedulers with captured graphs, which hold the addresses of their model's weights.
+capturers: weakref.WeakSet = weakref.WeakSet()
+
+
 def _project(h: torch.Tensor, w: torch.Tensor | MXFP4, bias: torch.Tensor | None = None) -> torch.Tensor:
     return linear_mxfp4(h, w, bias) if isinstance(w, MXFP4) else linear(h, w, bias)
 
@@ -199,12 +205,16 @@ class Model:
     def quantize_weights(self) -> None:
         """The layers' projections in microscaled 4-bit floats from here on (0.53 bytes
         per weight); embedding, LM head, norms and biases stay in bf16.  After the
-        weights are loaded and before a scheduler captures its graphs.  Weights that have
-        no such form leave the model as it was."""
+        weights are loaded and before a scheduler captures its graphs, which read the
+        weights of their time.  Weights that have no such form leave the model as it was."""
         if not self.fused_dense:
             raise ValueError("4-bit weights need fused_dense")
         weights = [(L, name) for L in self.layers for name in ("w_qkv", "w_o", "w_gate_up", "w_down")
                    if not isinstance(getattr(L, name), MXFP4)]
+        if weights and any(s.model is self for s in capturers):
+            gc.collect()  # (one that nobody holds any more may be part of a cycle)
+            if any(s.model is self for s in capturers):
+                raise RuntimeError("a scheduler's captured graphs read the weights: quantize_weights() comes before it")
         for L, name in weights:
             w = getattr(L, name)
             if not w.is_cuda or w.dtype != torch.bfloat16 or w.shape[1] % BLOCK:

@@ -34,3 +34,29 @@ def test_quantizing_twice_changes_nothing(dev):
     before = [getattr(L, n) for L in model.layers for n in NAMES]
     model.quantize_weights()
     assert all(a is b for a, b in zip(before, [getattr(L, n) for L in model.layers for n in NAMES]))
+
+
+def test_refused_under_captured_graphs(dev):
+    """A scheduler's graphs hold the addresses of the weights that they were captured with,
+    which a change would free: refused while such a scheduler lives, and not after it, nor
+    for one without graphs, nor where nothing would change."""
+    from minimal_inference_amd.engine import Request, Scheduler
+
+    model = _model(dev)
+    plain = Scheduler(model, max_batch_size=2, max_seq_len=64, use_graphs=False)
+    sch = Scheduler(model, max_batch_size=2, max_seq_len=64)
+    before = [getattr(L, n) for L in model.layers for n in NAMES]
+    with pytest.raises(RuntimeError, match="captured"):
+        model.quantize_weights()
+    assert all(a is b for a, b in zip(before, [getattr(L, n) for L in model.layers for n in NAMES]))
+    del sch
+    model.quantize_weights()
+    sch = Scheduler(model, max_batch_size=2, max_seq_len=64)
+    model.quantize_weights()  # (nothing to change)
+    tokens = []
+    for s in (plain, sch):
+        s.submit(Request("a", [1, 2, 3], 5, 0.0))
+        request = s.waiting[0]
+        s.run()
+        tokens.append(request.generated_tokens)
+    assert tokens[0] == tokens[1] and len(tokens[0]) == 5
