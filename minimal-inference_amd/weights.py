@@ -29,6 +29,8 @@ import re
 
 import torch
 
+from .mxfp4 import MXFP4
+
 _LAYER = re.compile(r"^model\.layers\.(\d+)\.(.+)$")
 
 
@@ -76,6 +78,9 @@ def load_weights(model, model_path: str) -> None:
     """Copy a checkpoint's tensors into ``model`` (cast to the model dtype)."""
     from safetensors import safe_open
 
+    for L in model.layers:
+        if any(isinstance(w, MXFP4) for w in (L.w_qkv, L.w_o, L.w_gate_up, L.w_down)):
+            raise ValueError("the model holds 4-bit weights: load a checkpoint before quantize_weights()")
     targets = _targets(model)
     seen: set[str] = set()
     for path in checkpoint_files(model_path):

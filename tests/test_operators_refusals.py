@@ -74,3 +74,24 @@ def test_post_norm_refuses_outputs_over_other_rows(change):
         a[name] = None if a[name] is None else a[name] + FAKE
     assert lib.mi_post_norm_add_rms_norm(*a.values(), None) == mod.MI_ERR_INVALID
     assert "overlaps" in mod.last_error()
+
+
+def test_a_checkpoint_is_not_loaded_into_4_bit_weights(tmp_path):
+    """Refused before a tensor of the model changes."""
+    from safetensors.torch import save_file
+
+    from minimal_inference_amd.model import Model, ModelConfig
+    from minimal_inference_amd.mxfp4 import MXFP4
+    from minimal_inference_amd.weights import load_weights
+
+    cfg = ModelConfig(hidden_size=64, num_attention_heads=2, num_key_value_heads=1, head_dim=32, num_hidden_layers=1,
+                      intermediate_size=96, vocab_size=100, max_position_embeddings=64)
+    model = Model(cfg, "cpu", max_positions=64)
+    save_file({"model.embed_tokens.weight": torch.ones(100, 64, dtype=torch.bfloat16),
+               "model.layers.0.mlp.down_proj.weight": torch.ones(64, 96, dtype=torch.bfloat16)},
+              str(tmp_path / "model.safetensors"))
+    model.layers[0].w_down = MXFP4(64, 96, "cpu")
+    before = model.embed.clone()
+    with pytest.raises(ValueError, match="4-bit"):
+        load_weights(model, str(tmp_path))
+    assert torch.equal(model.embed, before)
