@@ -95,3 +95,90 @@ def test_first_draw_of_a_sampler_in_a_graph(dev, b, v):
         held = ids.tolist()
         assert held == [draw_row(logits[i].cpu(), u[i].item(), f(0.9), 40, f(0.9), f(0.01)) for i in range(b)]
         assert s.draw(logits, u).tolist() == held
+
+
+# (rows, vocabulary) of two launches: workgroups of 8,192 tokens up to 8 of them, of 16,384 up to
+# 32, and of 32,768 from 256 workgroups of the others on and up to 32, the last of them whole or not
+TWO_LAUNCHES = [(2, 65536), (3, 65530), (3, 200000), (2, 524288), (24, 180225), (48, 152064), (48, 151929), (30, 151929),
+                (64, 65536), (20, 400003), (2, 524289), (2, 1 << 20), (3, (1 << 20) - 3)]
+
+
+@pytest.mark.parametrize("b,v", TWO_LAUNCHES)
+def test_every_form_of_two_launches(dev, b, v):
+    """Random rows with all filters, ties that reach over the workgroups of a row, rows of one
+    value (a workgroup's count at its largest), masks on either side, the largest at the end."""
+    logits = _logits(b, v, dev, v + b)
+    logits[0] = 0.5
+    logits[1] = torch.randint(0, 3, (v,), device=dev, generator=torch.Generator(device=dev).manual_seed(v))
+    if b > 2:
+        logits[2, : v - 40000] = torch.finfo(torch.bfloat16).min
+    if b > 8:
+        logits[3, 40000:] = -math.inf
+        logits[4, v - 1] = 90.0
+        logits[5] = -1.0
+        logits[5, ::7] = math.nan
+        logits[6] = -250.0
+        logits[6, 3::32768] = 1.0
+        logits[7, v // 2] = 300.0  # (the second path)
+    u = _uniform(b, dev, v)
+    t = [0.0 if i == 9 else 0.5 + 0.1 * (i % 8) for i in range(b)]
+    k = [v // 2 + 7, v // 3, 0, 50, 1000, v - 5, 30, 20][:b] + [[0, 1, 40, 5000][i % 4] for i in range(b - 8)]
+    p = [[0.7, 0.95, 1.0, 0.3][i % 4] for i in range(b)]
+    _check(dev, logits, u, t)
+    _check(dev, logits, u, t, top_k=k)
+    _check(dev, logits, u, t, top_p=p, top_k=k, min_p=[[0.0, 0.02, 0.001][i % 3] for i in range(b)])
+
+
+def test_rows_far_apart_of_two_launches(dev):
+    """Rows whose offsets pass 2^32 bytes, in workgroups of 32,768 tokens."""
+    b, v, apart = 34, 250007, 1 << 26
+    wide = torch.empty((b - 1) * apart + v, dtype=torch.bfloat16, device=dev)
+    logits = wide.as_strided((b, v), (apart, 1))
+    logits.normal_(std=3.0, generator=torch.Generator(device=dev).manual_seed(1))
+    u = _uniform(b, dev, 2)
+    _check(dev, logits, u, [0.8] * b, top_p=[0.95] * b, top_k=[100] * b, min_p=[0.01] * b)
+
+
+def test_on_a_side_stream_and_two_samplers_at_once(dev):
+    """A draw on a stream of its own, in order with what made its logits there; two samplers
+    on two streams at once, eager and replayed: each the ids that it draws alone."""
+    from minimal_inference_amd.sampling import Sampler
+
+    b, v = 12, 152064
+    made = [(_logits(b, v, dev, i), _uniform(b, dev, i)) for i in range(2)]
+    samplers, want = [], []
+    for logits, u in made:
+        s = Sampler(dev, b, vocab=v)
+        s.set_params([0.7] * b, [0.9] * b, top_k=[60] * b, min_p=[0.01] * b)
+        samplers.append(s)
+        want.append(s.draw(logits, u).tolist())
+    f = lambda x: torch.tensor(x).double().item()  # noqa: E731
+    assert want[0] == [draw_row(made[0][0][i].cpu(), made[0][1][i].item(), f(0.7), 60, f(0.9), f(0.01)) for i in range(b)]
+    streams = [torch.cuda.Stream() for _ in made]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (s, stream, (logits, u)) in enumerate(zip(samplers, streams, made)):
+            with torch.cuda.stream(stream):
+                there = (logits + 1).sub_(1)  # (rounds: other logits, made on this stream)
+                got[i].append((there, s.draw(there, u).clone(), s.draw(logits, u).clone()))
+    torch.cuda.synchronize()
+    for i, (s, (logits, u)) in enumerate(zip(samplers, made)):
+        for there, moved, same in got[i]:
+            assert same.tolist() == want[i]
+            assert torch.equal(s.draw(there, u), moved)
+    graphs, ids = [], []
+    for s, stream, (logits, u) in zip(samplers, streams, made):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            ids.append(s.draw(logits, u))
+        graphs.append(g)
+    for _ in range(5):
+        for t in ids:
+            t.fill_(-1)
+        torch.cuda.synchronize()
+        for g, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                g.replay()
+        torch.cuda.synchronize()
+        assert [t.tolist() for t in ids] == want
