@@ -338,7 +338,14 @@ __global__ __launch_bounds__(256) void combine_kernel(LinearParams p, int parts)
 // 128 x 8,192 x 10,240, 128 x 128, 3 parts 31.7 / 32.2; bf16 1,024 x 8,192 x 10,240,
 // 128 x 128 in fours of waves 153 / 154, 128 x 256 190 / 179; in 4 bits 2,048 x 8,192 x
 // 10,240, 128 x 128 98 / 100, 128 x 256 99 / 98, 256 x 256 122 / 112; 8,192 rows of it 381 /
-// 378, 326 / 321, 314 / 312.
+// 378, 326 / 321, 314 / 312: most within 3 %, some blocks of 256 columns counted 6 to 9 % slow.
+//
+// Blocks of bf16 rows: 32, 64 and 128 rows, and one rung between the last two, of 80, for 65 to
+// 80 rows and for twice as many and more where 128 would leave a block half empty (us, with
+// that rung and without: 72 x 3,584 x 18,944 21.9 and 24.5, 72 x 10,240 x 8,192 24.4 and 27.8,
+// 72 x 8,192 x 29,568 51 and 60, 144 x 4,096 x 14,336 28.8 and 34.2, 144 x 8,192 x 29,568 88
+// and 112; along a short k it gains nothing: 72 x 6,144 x 4,096 16.0 and 15.6).  81 to 96 rows
+// have no rung of their own: they take blocks of 128 (96 x 10,240 x 8,192 29.8; 80 rows 25.1).
 struct Form {
   int rows, tiles;  // 16-row tiles of W
   float one_us, more_us;
