@@ -12,7 +12,7 @@ Kinds of case:
   norm     x + delta, its root-mean-square norm, and that in 8 bits: blocks of 32 with a
            power of two each; returns the sum and the values that the blocks stand for
   linear   a projection with both operands in 8 bits; with ``silu`` the fused gate and up
-           projection followed by silu(gate) * up, which leaves 8-bit blocks again
+           projection followed by silu(gate) * up
   adapter  y + scale B (A x) with the row's own adapter, of several requests at once; the
            outputs are one piece (o, down) or several with factors of their own (q, k, v);
            x is bf16 or (``acts`` "mxfp8") 8-bit rows; an eighth of the requests has none
@@ -102,7 +102,7 @@ def draw(rng):
     if kind == "linear":
         k, n, silu = rng.choice(PROJECTIONS)
         if rng.random() < 0.3:  # widths that fill no whole tile
-            k, n = k - BLOCK * rng.randrange(4), n - (BLOCK * rng.randrange(4) if silu else rng.randrange(16))
+            k, n = k - BLOCK * rng.randrange(4), n - rng.randrange(16)
         wide = n * (2 if silu else 1) * k
         rows = _log_int(rng, 1, max(1, min(8201, 8201 * 8192 * 10240 // wide)))
         return _linear(rows, k, n, silu, rng.random() < 0.3 and not silu)
@@ -225,7 +225,7 @@ def _plain_linear(s):
         y = y + s["bias"].float()
     if s["case"]["silu"]:
         gate, up = y.chunk(2, dim=-1)
-        y = _values(*_quantized(gate / (1 + torch.exp(-gate)) * up))
+        y = gate / (1 + torch.exp(-gate)) * up
     return y.to(torch.bfloat16)
 
 
@@ -262,7 +262,7 @@ def run(state):
     from minimal_inference_amd.mxfp8 import linear_mxfp8, linear_silu_mxfp8
 
     if case["silu"]:
-        return linear_silu_mxfp8(state["rows8"], state["weight8"]).dequantize()
+        return linear_silu_mxfp8(state["rows8"], state["weight8"])
     return linear_mxfp8(state["rows8"], state["weight8"], state["bias"])
 
 
@@ -321,7 +321,7 @@ def exact(case, seed):
             y += s["bias"].double()
         if case["silu"]:
             gate, up = y.chunk(2, dim=-1)
-            y = _exact_quantized((gate * torch.sigmoid(gate)).mul_(up))
+            y = (gate * torch.sigmoid(gate)).mul_(up)
         return y
     # adapter by adapter, on the rows that are its own
     x = s["x"].double() if case["acts"] == "bf16" else _exact_values(s["codes"], s["scales"])
