@@ -443,6 +443,87 @@ int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_scales, const
                     size_t workspace_bytes, mi_stream_t stream);
 
 /* ------------------------------------------------------------------------ *
+ * MXFP8: 8-bit floating point (e4m3) in blocks of 32 along a row, each with a
+ * power of two (e8m0), after the OCP Microscaling Formats v1.0; the residual
+ * sum and norm that leaves such rows, and linear layers with both operands in
+ * them.  No counterpart in the reference.
+ *
+ * A matrix [rows][cols] (cols a multiple of 32, at most 2^20) is row-major as
+ * checkpoints hold it: codes, a byte each (16-byte aligned rows), and a scale
+ * byte per block.  Strides are in bytes.  mi_linear_mxfp8 reads scale rows in pieces
+ * of 16 bytes: aligned to 16, and readable to a multiple of 16 (what lies behind a
+ * row's last block is not used).
+ *
+ * Quantisation of a block: the least power of two u with max|x| <= 448 u, each
+ * code the e4m3 value nearest to x / u (ties to even), the scale byte
+ * log2 u + 127 (0 at least).  A block with an infinity or a NaN becomes NaN as a
+ * whole (scale byte 255, zero codes).  Values below 2^-133 come back to bf16 as
+ * its roundings, all others exactly.
+ * ------------------------------------------------------------------------ */
+int mi_mxfp8_quantize(const void* x, int64_t x_stride, void* codes, int64_t codes_stride,
+                      void* scales, int64_t scales_stride, int64_t rows, int64_t cols,
+                      mi_stream_t stream);
+int mi_mxfp8_dequantize(const void* codes, int64_t codes_stride, const void* scales,
+                        int64_t scales_stride, void* out, int64_t out_stride, int64_t rows,
+                        int64_t cols, mi_stream_t stream);
+
+/* x' = bf16(x + delta) (x where delta is null), stored to x_out unless that is null,
+ * and x' * rsqrt(mean(x'^2) + eps) * weight in fp32, quantised from there.  hidden a
+ * multiple of 32 up to 16384, at most 2^22 rows, 16-byte aligned rows of bf16.  x_out may be x or
+ * delta; outputs that overlap each other, the weight or another row's input are refused. */
+int mi_add_rms_norm_mxfp8(const void* x, int64_t x_stride, const void* delta, int64_t delta_stride,
+                          const void* weight, void* x_out, int64_t x_out_stride, void* codes,
+                          int64_t codes_stride, void* scales, int64_t scales_stride, int64_t rows,
+                          int32_t hidden, float eps, mi_stream_t stream);
+
+/* out = x W^T (+ bias) with x [rows][k] and W [n][k] in MXFP8, fp32 accumulation, one
+ * rounding to bf16.  silu != 0: W is [2 n][k], n gate rows and then n up rows, and
+ * out = silu(x Wg^T) * (x Wu^T); no bias then, and with out_scales not null out is MXFP8 too
+ * (codes and scale bytes, strides in bytes, n a multiple of 32), quantised from fp32.
+ * rows 0..2^22, n 1..2^24 (any), k a multiple of 32 up to 2^20, strides at most 2^22;
+ * out_stride in elements.  An out that overlaps x, W, the bias or its scales is refused.
+ * The result does not depend on timing.  workspace (16-byte aligned; may be null) as in
+ * mi_linear_mxfp4. */
+size_t mi_linear_mxfp8_workspace_size(int64_t rows, int64_t n, int64_t k, int32_t silu);
+int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void* x_scales,
+                    int64_t x_scales_stride, const void* w_codes, int64_t w_stride,
+                    const void* w_scales, int64_t w_scales_stride, const void* bias, void* out,
+                    int64_t out_stride, void* out_scales, int64_t out_scales_stride, int64_t rows,
+                    int64_t n, int64_t k, int32_t silu, void* workspace, size_t workspace_bytes,
+                    mi_stream_t stream);
+
+/* ------------------------------------------------------------------------ *
+ * Low-rank adapters of many requests beside a shared projection.  No
+ * counterpart in the reference.
+ *
+ * mi_adapter_plan sorts a batch's rows by adapter, once for all its projections:
+ * slot_of_row [rows] int32, an id outside 0..slots-1 (as -1) for none; at most 2^22
+ * rows, 1,023 adapters.  plan: mi_adapter_plan_size bytes, 16-byte aligned, written
+ * here and read by runs with the same rows and slots.
+ *
+ * mi_add_adapters: out = y + scale[s] * B[s] (A[s] x), one rounding to bf16, with row
+ * t's adapter s; rows without one are y's.  y, out [rows][n] bf16; x [rows][k] bf16, or,
+ * x_scales not null, MXFP8 (any alignment of scale rows).  The n columns are
+ * pieces (1..8, piece_columns on the host, multiples of 16 up to 2^20) with factors of
+ * their own: a [slots][pieces * rank][k], b [slots][n][rank] bf16 contiguous, scale
+ * [slots] fp32.  rank a multiple of 8 up to 128 (smaller ones padded with zeros), k of 32 up
+ * to 2^20; rows of x, y and out 16-byte aligned.  out may be y itself; otherwise an out that
+ * overlaps another argument is refused.  workspace: mi_add_adapters_workspace_size bytes,
+ * need not be initialised, one call at a time.  A row's result depends on no other row.
+ * ------------------------------------------------------------------------ */
+size_t mi_adapter_plan_size(int64_t rows, int64_t slots);
+int mi_adapter_plan(void* plan, size_t plan_bytes, const int32_t* slot_of_row, int64_t rows,
+                    int64_t slots, mi_stream_t stream);
+size_t mi_add_adapters_workspace_size(int64_t rows, int64_t slots, int64_t k, int64_t rank,
+                                      int64_t pieces);
+int mi_add_adapters(const void* y, int64_t y_stride, const void* x, int64_t x_stride,
+                    const void* x_scales, int64_t x_scales_stride, const void* a, const void* b,
+                    const float* scale, int64_t slots, int64_t k, int64_t rank,
+                    const int32_t* piece_columns, int64_t pieces, void* out, int64_t out_stride,
+                    const void* plan, int64_t rows, void* workspace, size_t workspace_bytes,
+                    mi_stream_t stream);
+
+/* ------------------------------------------------------------------------ *
  * One draw per row from given uniform numbers, with top-k, top-p and min-p.
  * Beside mi_sample (scheduler.py:310-343), for callers that bring their own
  * random numbers or filter by more than top-p.

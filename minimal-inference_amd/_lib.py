@@ -102,6 +102,26 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _c_i32,
         [_vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _vp, _c_sz, _vp],
     ),
+    "mi_mxfp8_quantize": (_c_i32, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp]),
+    "mi_mxfp8_dequantize": (_c_i32, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp]),
+    "mi_add_rms_norm_mxfp8": (
+        _c_i32,
+        [_vp, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_i32, _c_f32, _vp],
+    ),
+    "mi_linear_mxfp8_workspace_size": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_i32]),
+    "mi_linear_mxfp8": (
+        _c_i32,
+        [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_i64,
+         _c_i32, _vp, _c_sz, _vp],
+    ),
+    "mi_adapter_plan_size": (_c_sz, [_c_i64, _c_i64]),
+    "mi_adapter_plan": (_c_i32, [_vp, _c_sz, _vp, _c_i64, _c_i64, _vp]),
+    "mi_add_adapters_workspace_size": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64]),
+    "mi_add_adapters": (
+        _c_i32,
+        [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp,
+         _c_i64, _vp, _c_sz, _vp],
+    ),
     "mi_draw_workspace_size": (_c_sz, [_c_i32, _c_i32]),
     "mi_draw": (
         _c_i32,

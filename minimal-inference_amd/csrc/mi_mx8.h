@@ -1,0 +1,91 @@
+// Device helpers of MXFP8 matrices: 8-bit floating point (e4m3) in blocks of 32 along a
+// row with one shared power of two (e8m0) each, after the OCP Microscaling Formats (MX) v1.0.
+//
+// A matrix [rows][k] is row-major as checkpoints hold it: codes, a byte each, at a row
+// stride of whole 16 bytes, and a scale byte per block, whose rows are readable to a
+// multiple of 16 bytes.  The matrix instructions' operand order is made on the way
+// through LDS, where a row of a slab of 128 k is 8 chunks of 16 bytes.
+#pragma once
+
+#include "mi_common.h"
+
+namespace mi::mx8 {
+
+constexpr int kBlock = 32;
+constexpr int kSlab = 128;  // k per matrix instruction
+constexpr int kMaxK = 1 << 20;
+
+inline __host__ __device__ int64_t slabs(int64_t k) { return (k + kSlab - 1) / kSlab; }
+
+typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2_t;
+typedef __attribute__((ext_vector_type(8))) int i32x8_t;
+typedef __attribute__((address_space(3))) char lds_t;
+
+constexpr int kBufferWord3 = 0x00020000;
+constexpr int kCacheNT = 2;
+constexpr int kOutOfRange = 0x7ffffff0;  // an offset past every buffer's end
+
+__device__ __forceinline__ u32x4_t lds_load16(const lds_t* p) {
+  return *(const __attribute__((address_space(3))) u32x4_t*)p;
+}
+__device__ __forceinline__ uint32_t lds_load1(const lds_t* p) { return *(const __attribute__((address_space(3))) uint8_t*)p; }
+__device__ __forceinline__ void lds_store16(lds_t* p, u32x4_t v) { *(__attribute__((address_space(3))) u32x4_t*)p = v; }
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, kBufferWord3);
+}
+
+// The power of two of a scale byte as the conversions take it: they read the
+// exponent field alone (0 is 2^-127, 255 NaN).
+__device__ __forceinline__ float scale_f32(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// The scale byte of a block from the largest magnitude's bits: the least power of two of
+// which 448, e4m3's largest value, is no less.  448 is 1.75 2^8: a mantissa above 1.75
+// carries into the exponent.  A block that holds an infinity or a NaN gets byte 255.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
+  const uint32_t field = (top + 0x1fffffu) >> 23;
+  return top >= 0x7f800000u ? 255u : max(field, 8u) - 8u;
+}
+
+// Four values over a scale, rounded to e4m3 (to nearest even).  Codes of a block
+// that is NaN are zeros.
+__device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d, uint32_t byte) {
+  typedef __attribute__((ext_vector_type(2))) short pair_t;
+  const float s = scale_f32(byte);
+  pair_t v = {0, 0};
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(v, a, b, s, false);
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(v, c, d, s, true);
+  return byte == 255u ? 0u : __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// Four codes to bf16: exact but below 2^-133, bf16's least.
+__device__ __forceinline__ u32x2_t to_bf16(uint32_t codes, float scale) {
+  return u32x2_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true))};
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t max_dpp(uint32_t v) {
+  return max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, 0xf, 0xf, false)));
+}
+// Over aligned groups of four lanes, and of eight.
+__device__ __forceinline__ uint32_t max4(uint32_t v) { return max_dpp<kDppQuadSwap2>(max_dpp<kDppQuadSwap1>(v)); }
+__device__ __forceinline__ uint32_t max8(uint32_t v) { return max_dpp<kDppRowHalfMirror>(max4(v)); }
+
+// D(16x16 fp32) += A(16x128) * B(128x16), both e4m3.  Lane l supplies row (column) l % 16:
+// chunk l / 16 of its slab of eight 16-byte chunks in lo, chunk 4 + l / 16 in hi, and
+// the scale byte of block l / 16.
+//
+// Precision: products that the instruction adds side by side are aligned to the largest
+// of them and cut some 14 bits below it; across such groups and from slab to slab the sum is
+// fp32.  On normal values the sum over k = 8,192 is 1.5e-5 off the exact one (relative to
+// the result's norm; the unscaled 8-bit instructions are alike), 1 / 100 of its rounding to bf16.
+__device__ __forceinline__ f32x4_t mfma_fp8(u32x4_t alo, u32x4_t ahi, uint32_t sa, u32x4_t blo, u32x4_t bhi, uint32_t sb,
+                                            f32x4_t c) {
+  const i32x8_t x = {int(alo[0]), int(alo[1]), int(alo[2]), int(alo[3]), int(ahi[0]), int(ahi[1]), int(ahi[2]), int(ahi[3])};
+  const i32x8_t y = {int(blo[0]), int(blo[1]), int(blo[2]), int(blo[3]), int(bhi[0]), int(bhi[1]), int(bhi[2]), int(bhi[3])};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 0, 0, int(sa), 0, int(sb));
+}
+
+}  // namespace mi::mx8
