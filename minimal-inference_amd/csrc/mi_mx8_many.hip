@@ -23,6 +23,107 @@ __device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t rs, lds_t* dst,
 
 constexpr int kGroupM = 4;
 
+// Which block of out a workgroup owns.  Workgroups go to the eight XCDs in turn.  Each XCD
+// gets a run of tiles, in groups of kGroupM down the rows of x, so that those it holds at a
+// time share rows of x and of W in its L2.
+__device__ __forceinline__ void place(const LinearParams& p, int bm, int cols, int& col0, int64_t& m0) {
+  const int mt = int((p.rows + bm - 1) / bm), nt = (p.n + cols - 1) / cols, all = mt * nt;
+  const int id = int(blockIdx.x), xcd = id & 7, each = all / 8, more = all % 8;
+  const int tile_id = xcd * each + min(xcd, more) + (id >> 3);
+  const int group = tile_id / (kGroupM * nt), in = tile_id - group * kGroupM * nt;
+  const int high = min(kGroupM, mt - group * kGroupM);
+  col0 = in / high * cols;
+  m0 = int64_t(group * kGroupM + in % high) * bm;
+}
+
+// Scales of four slabs: 64 rows a load, XS loads of x's and the rest of W's rows (16 of
+// each half in turn).
+template <int WAVES, int BM, int BN, bool GLU>
+__device__ __forceinline__ void load_scales(const LinearParams& p, lds_t* to, int quad, int w, int col0, int64_t m0, int rows) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int HALVES = GLU ? 2 : 1, XS = (BM + 63) / 64, LOADS = XS + (BN + 63) / 64;
+  const char *const xsbase = p.xs + m0 * p.xs_stride, *const wsbase = p.ws + col0 * p.ws_stride;
+  const int off = quad * 16, lane = threadIdx.x & 63;
+  for (int i = w; i < LOADS; i += WAVES) {
+    const bool of_x = i < XS;
+    const int at = (of_x ? i : i - XS) * 64 + lane, tile = at / 16;
+    const int row = of_x ? at : tile / HALVES * 16 + at % 16;
+    const char* from = of_x ? xsbase + row * p.xs_stride : wsbase + (tile % HALVES * int64_t(p.n) + row) * p.ws_stride;
+    // (anything readable in the place of rows past the matrix's and of blocks past a row's)
+    if (off * kBlock >= p.k || (of_x ? at >= rows : at >= BN || col0 + row >= p.n)) from = p.ws;
+    else from += off;
+    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)const_cast<char*>(from),
+                                     (__attribute__((address_space(3))) void*)(to + i * 1024), 16, 0, 0);
+  }
+#endif
+}
+
+// A wave's sums to memory: tile t of W's rows is columns col0 + 16 (first_tile + t) / HALVES
+// on, block b rows m0 + row0 + 16 b on.  Lane (g, n) holds columns 4 g .. 4 g + 3 of a tile for row n of a block.
+template <int MB, int NT, bool GLU, bool OUT8, bool SPLIT>
+__device__ __forceinline__ void end_of_product(const LinearParams& p, const f32x4_t (&acc)[NT][MB], int col0, int first_tile,
+                                               int64_t m0, int row0, int rows) {
+  constexpr int HALVES = GLU ? 2 : 1;
+  const int g = (threadIdx.x & 63) >> 4, n = threadIdx.x & 15;
+  if constexpr (OUT8 && !SPLIT) {
+#pragma unroll
+    for (int t = 0; t < NT; t += 4) {
+      const int first = col0 + (first_tile + t) / 2 * 16;
+      const f32x4_t none = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int b = 0; b < MB; ++b) {
+        const int m = row0 + b * 16 + n;
+        store_block(p, m0 + m, m < rows && first < p.n, first, g, finish<true>(acc[t][b], acc[t + 1][b], none),
+                    finish<true>(acc[t + 2][b], acc[t + 3][b], none));
+      }
+    }
+    return;
+  }
+  // Two tiles' lanes change places, so that a lane has eight columns and four lanes 64
+  // bytes of a row.
+  if constexpr (!SPLIT && !OUT8 && NT / HALVES % 2 == 0) {
+    if (p.wide) {
+#pragma unroll
+      for (int t = 0; t < NT; t += 2 * HALVES) {
+        const int first = col0 + (first_tile + t) / HALVES * 16, col = first + (g & 1) * 16 + (g >> 1) * 8;
+        const f32x4_t bias0 = bias4(p, first + 4 * g), bias1 = bias4(p, first + 16 + 4 * g);
+#pragma unroll
+        for (int b = 0; b < MB; ++b) {
+          const u32x2_t u = round4(finish<GLU>(acc[t][b], acc[t + HALVES - 1][b], bias0));
+          const u32x2_t v = round4(finish<GLU>(acc[t + HALVES][b], acc[t + 2 * HALVES - 1][b], bias1));
+          const auto s0 = __builtin_amdgcn_permlane16_swap(u.x, v.x, false, false);
+          const auto s1 = __builtin_amdgcn_permlane16_swap(u.y, v.y, false, false);
+          const int m = row0 + b * 16 + n;
+          if (m < rows && col < p.n)
+            *reinterpret_cast<u32x4_t*>(reinterpret_cast<uint16_t*>(p.out) + (m0 + m) * p.o_stride + col) =
+                u32x4_t{s0[0], s1[0], s0[1], s1[1]};
+        }
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; t += HALVES) {
+    const int col = col0 + (first_tile + t) / HALVES * 16 + 4 * g;
+    if (col >= p.n) continue;
+    const f32x4_t bias = SPLIT ? f32x4_t{0.f, 0.f, 0.f, 0.f} : bias4(p, col);
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+      const int m = row0 + b * 16 + n;
+      if (m >= rows) continue;
+      if constexpr (SPLIT) {
+        // [part][half][row][columns, in fours]
+        const int64_t fours = (p.n + 3) / 4;
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+          p.parts[((int64_t(blockIdx.y) * HALVES + h) * p.rows + m0 + m) * fours + col / 4] = acc[t + h][b];
+      } else if constexpr (!OUT8) {
+        store4(p, m0 + m, col, finish<GLU>(acc[t][b], acc[t + HALVES - 1][b], bias));
+      }
+    }
+  }
+}
+
 // MB blocks of 16 rows of x and NT tiles of 16 rows of W per wave.  Slabs are staged STAGES
 // deep: before slab s is multiplied the loads of the STAGES - 2 slabs behind it may be in
 // flight, and after the barrier its predecessor's buffer is filled again.  Loads past the last slab
@@ -36,7 +137,6 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
   constexpr int BM = WM * MB * 16, BN = WN * NT * 16, COLS = BN / HALVES;  // BN rows of W
   constexpr int XBYTES = BM * kSlab, STAGE = XBYTES + BN * kSlab;
   constexpr int XLOADS = XBYTES / 1024 / WAVES, WLOADS = BN * kSlab / 1024 / WAVES;
-  // scales of four slabs: 64 rows a load
   constexpr int XS = (BM + 63) / 64, SLOADS = XS + (BN + 63) / 64, SBYTES = SLOADS * 1024;
   static_assert(XBYTES / 1024 % WAVES == 0 && BN * kSlab / 1024 % WAVES == 0 && NT % HALVES == 0, "even shares");
   static_assert(!OUT8 || (GLU && NT % 4 == 0), "whole blocks");
@@ -46,16 +146,9 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
   const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
   const int wm = w / WN, wn = w % WN;
   const int g = lane >> 4, n = lane & 15;
-  // Workgroups go to the eight XCDs in turn.  Each XCD gets a run of tiles, in groups of
-  // kGroupM down the rows of x, so that those it holds at a time share rows of x and of
-  // W in its L2.
-  const int mt = int((p.rows + BM - 1) / BM), nt = (p.n + COLS - 1) / COLS, all = mt * nt;
-  const int id = int(blockIdx.x), xcd = id & 7, each = all / 8, more = all % 8;
-  const int tile_id = xcd * each + min(xcd, more) + (id >> 3);
-  const int group = tile_id / (kGroupM * nt), in = tile_id - group * kGroupM * nt;
-  const int high = min(kGroupM, mt - group * kGroupM);
-  const int col0 = in / high * COLS;
-  const int64_t m0 = int64_t(group * kGroupM + in % high) * BM;
+  int col0;
+  int64_t m0;
+  place(p, BM, COLS, col0, m0);
   const int rows = int(min(int64_t(BM), p.rows - m0));
   const int slab0 = SPLIT ? int(blockIdx.y) * p.split_slabs : 0;
   const int slab_end = SPLIT ? min(slab0 + p.split_slabs, p.slabs) : p.slabs;
@@ -98,23 +191,8 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
       lds_dma16(rw[(w * WLOADS + i) / 2 % HALVES], stage + XBYTES + (w * WLOADS + i) * 1024, inside ? wv[i] : kOutOfRange);
   };
   lds_t* const scales = lds + STAGES * STAGE;
-  auto load_scales = [&](int quad) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    lds_t* const to = scales + (quad & 1) * SBYTES;
-    const char *const xsbase = p.xs + m0 * p.xs_stride, *const wsbase = p.ws + col0 * p.ws_stride;
-    const int off = quad * 16;
-    for (int i = w; i < SLOADS; i += WAVES) {
-      const bool of_x = i < XS;
-      const int at = (of_x ? i : i - XS) * 64 + lane, tile = at / 16;
-      const int row = of_x ? at : tile / HALVES * 16 + at % 16;
-      const char* from = of_x ? xsbase + row * p.xs_stride : wsbase + (tile % HALVES * int64_t(p.n) + row) * p.ws_stride;
-      // (anything readable in the place of rows past the matrix's and of blocks past a row's)
-      if (off >= blocks || (of_x ? at >= rows : at >= BN || col0 + row >= p.n)) from = p.ws;
-      else from += off;
-      __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)const_cast<char*>(from),
-                                       (__attribute__((address_space(3))) void*)(to + i * 1024), 16, 0, 0);
-    }
-#endif
+  auto stage_scales = [&](int quad) {
+    load_scales<WAVES, BM, BN, GLU>(p, scales + (quad & 1) * SBYTES, quad, w, col0, m0, rows);
   };
 
   f32x4_t acc[NT][MB];
@@ -127,8 +205,8 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
 
   constexpr int kInFlight = (STAGES - 2) * (XLOADS + WLOADS);
   static_assert(kInFlight < 64, "vmcnt");
-  load_scales(slab0 >> 2);
-  load_scales((slab0 >> 2) + 1);
+  stage_scales(slab0 >> 2);
+  stage_scales((slab0 >> 2) + 1);
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) load(slab0 + i, i);
   int buf = 0, before = STAGES - 1;
@@ -139,7 +217,7 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     const int quad = slab >> 2;
-    if ((slab & 3) == 0 && slab != slab0) load_scales(quad + 1);  // (four slabs ahead: done by any wait before them)
+    if ((slab & 3) == 0 && slab != slab0) stage_scales(quad + 1);  // (four slabs ahead: done by any wait before them)
     load(slab + STAGES - 1, before);
     const lds_t* const xl = lds + buf * STAGE + wm * MB * 16 * kSlab;
     const lds_t* const wl = lds + buf * STAGE + XBYTES + wn * NT * 16 * kSlab;
@@ -169,64 +247,177 @@ __global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
   }
   __builtin_amdgcn_s_waitcnt(0x0f70);  // (the loads past the end write to LDS)
 
-  // Lane (g, n) holds columns 4 g .. 4 g + 3 of a tile for row n of a block.
-  if constexpr (OUT8 && !SPLIT) {
+  end_of_product<MB, NT, GLU, OUT8, SPLIT>(p, acc, col0, wn * NT, m0, wm * MB * 16, rows);
+}
+
+// The product into accumulation registers that stay where they are: 64 sums fill all of them, and
+// left to choose, the compiler moves a quarter of the sums about in every slab.  The sums may be read 18
+// cycles after the last of these at the earliest.
+__device__ __forceinline__ void mfma_in_place(u32x4_t alo, u32x4_t ahi, uint32_t sa, u32x4_t blo, u32x4_t bhi, uint32_t sb,
+                                              f32x4_t& c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const i32x8_t x = {int(alo[0]), int(alo[1]), int(alo[2]), int(alo[3]), int(ahi[0]), int(ahi[1]), int(ahi[2]), int(ahi[3])};
+  const i32x8_t y = {int(blo[0]), int(blo[1]), int(blo[2]), int(blo[3]), int(bhi[0]), int(bhi[1]), int(bhi[2]), int(bhi[3])};
+  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]" : "+a"(c) : "v"(x), "v"(y), "v"(sa), "v"(sb));
+#endif
+}
+
+// The largest blocks: 256 rows of x by 256 of W, four waves of 128 x 128, whose sums are half of
+// a SIMD's registers.  One wave per SIMD hides nothing, so everything is read before its turn.
+// A slab is four units of 128 rows (16 KB): the first and the second 64 of every wave's rows
+// of W (W0, W1) and of x (X0, X1), and its products four phases of 16 instructions:
+//   even slabs  X0 W0, X1 W0, X1 W1, X0 W1     odd slabs  X1 W0, X0 W0, X0 W1, X1 W1
+// so that a unit's registers are free two phases before the next slab needs them, and each
+// phase reads one unit from LDS for the next phase or the one after.  Units go through a ring of
+// eight buffers, two slabs', in the order in which they are read (W0, X, X, W1): a phase
+// waits for its unit, and after the barrier fills the buffer that the phase before has read,
+// seven phases before that unit's turn.  Between two matrix instructions stands one read or load:
+// an instruction leaves a wave seven issue slots, and what does not fit in them is lost.
+template <bool GLU, bool OUT8>
+__global__ __launch_bounds__(256) void wide_kernel(LinearParams p) {
+  constexpr int HALVES = GLU ? 2 : 1, BM = 256, BN = 256, COLS = BN / HALVES;
+  constexpr int UNITS = 8, UNIT = 128 * kSlab, SBYTES = 8 * 1024, LOADS = UNIT / 1024 / 4;
+  static_assert(UNITS * UNIT + 2 * SBYTES <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(16))) char smem[UNITS * UNIT + 2 * SBYTES];
+  lds_t* const lds = (lds_t*)smem;
+  lds_t* const scales = lds + UNITS * UNIT;
+  const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
+  const int wm = w / 2, wn = w % 2;
+  const int g = lane >> 4, n = lane & 15;
+  int col0;
+  int64_t m0;
+  place(p, BM, COLS, col0, m0);
+  const int rows = int(min(int64_t(BM), p.rows - m0)), blocks = p.k / kBlock;
+  const int wstride = int(p.w_stride), xstride = int(p.x_stride);
+  const char* const xbase = p.x + m0 * p.x_stride;
+  const char* const wbase = p.w + col0 * p.w_stride;
+  const char* const ubase = p.w + (int64_t(p.n) + col0) * p.w_stride;
+  const int xsize = (rows - 1) * xstride + p.k, wsize = (min(COLS, p.w_rows - col0) - 1) * wstride + p.k;
+  const int usize = GLU ? (min(COLS, p.n - col0) - 1) * wstride + p.k : 0;
+  // load i of a wave: 8 rows of a unit, lane l chunk slot l % 8 of row l / 8; rows r on of
+  // wave `of`'s 64 of the unit
+  const int r8 = lane >> 3, chunk = ((lane & 7) ^ r8) * 16;
+  int xv[2][LOADS], wv[2][LOADS];
 #pragma unroll
-    for (int t = 0; t < NT; t += 4) {
-      const int first = col0 + (wn * NT + t) / 2 * 16;
-      const f32x4_t none = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int b = 0; b < MB; ++b) {
-        const int m = (wm * MB + b) * 16 + n;
-        store_block(p, m0 + m, m < rows && first < p.n, first, g, finish<true>(acc[t][b], acc[t + 1][b], none),
-                    finish<true>(acc[t + 2][b], acc[t + 3][b], none));
-      }
+    for (int i = 0; i < LOADS; ++i) {
+      const int of = w >> 1, r = (w & 1) * 32 + i * 8, tile = j * 4 + r / 16;
+      xv[j][i] = (of * 128 + j * 64 + r + r8) * xstride + chunk;
+      wv[j][i] = (of * (128 / HALVES) + tile / HALVES * 16 + r % 16 + r8) * wstride + chunk;
     }
-    return;
-  }
-  // Two tiles' lanes change places, so that a lane has eight columns and four lanes 64
-  // bytes of a row.
-  if constexpr (!SPLIT && !OUT8 && NT / HALVES % 2 == 0) {
-    if (p.wide) {
+  // The loads of a unit: of slab u / 4, W0, X, X, W1 (`part`).
+  auto loads = [&](int slab, int part, int odd, int slot, auto each) {
+    const int off = slab * kSlab;
+    const bool ok = slab < p.slabs;
+    lds_t* const to = lds + slot * UNIT + w * LOADS * 1024;
+    const int past = off + chunk < p.k ? 0 : kOutOfRange;  // past the row's end lies the next row
+    const bool of_x = part == 1 || part == 2;
+    const int j = part == 1 ? odd : part == 2 ? 1 - odd : part == 3;
+    const __amdgpu_buffer_rsrc_t rs = of_x ? buffer(xbase + off, ok ? xsize - off : 0) : buffer(wbase + off, ok ? wsize - off : 0);
+    const __amdgpu_buffer_rsrc_t ru = GLU && !of_x ? buffer(ubase + off, ok ? usize - off : 0) : rs;
+    each([=, &xv, &wv](int i) {
+      lds_dma16(GLU && i / 2 ? ru : rs, to + i * 1024, (of_x ? xv[j][i] : wv[j][i]) | past);
+    });
+  };
+  struct Set {
+    u32x4_t v[4][2];
+    uint32_t s[4];
+  };
+  // a lane's two chunks of row n of 16 (and 64 of `wave`'s rows of a unit)
+  const lds_t* const xread = lds + wm * 64 * kSlab + n * kSlab;
+  const lds_t* const wread = lds + wn * 64 * kSlab + n * kSlab;
+  const int lo = (g ^ (n & 7)) * 16, hi = ((4 + g) ^ (n & 7)) * 16;
+  const lds_t* const xr[2] = {xread + lo, xread + hi};
+  const lds_t* const wr[2] = {wread + lo, wread + hi};
+  const lds_t* const xsr = scales + (wm * 128 + n) * 16;
+  const lds_t* const wsr = scales + (BM + wn * 128 + n) * 16;
+  // Where a slab's scale bytes lie in a staged row: behind the last block (whose codes are
+  // zeros) the last one's, since a row's padding may hold anything.
+  auto scale_at = [&](int slab) { return (slab >> 2 & 1) * SBYTES + (slab & 3) * 4 + min(g, max(blocks - 1 - slab * 4, 0)); };
+
+  f32x4_t acc[8][8];
 #pragma unroll
-      for (int t = 0; t < NT; t += 2 * HALVES) {
-        const int first = col0 + (wn * NT + t) / HALVES * 16, col = first + (g & 1) * 16 + (g >> 1) * 8;
-        const f32x4_t bias0 = bias4(p, first + 4 * g), bias1 = bias4(p, first + 16 + 4 * g);
+  for (int t = 0; t < 8; ++t)
 #pragma unroll
-        for (int b = 0; b < MB; ++b) {
-          const u32x2_t u = round4(finish<GLU>(acc[t][b], acc[t + HALVES - 1][b], bias0));
-          const u32x2_t v = round4(finish<GLU>(acc[t + HALVES][b], acc[t + 2 * HALVES - 1][b], bias1));
-          const auto s0 = __builtin_amdgcn_permlane16_swap(u.x, v.x, false, false);
-          const auto s1 = __builtin_amdgcn_permlane16_swap(u.y, v.y, false, false);
-          const int m = (wm * MB + b) * 16 + n;
-          if (m < rows && col < p.n)
-            *reinterpret_cast<u32x4_t*>(reinterpret_cast<uint16_t*>(p.out) + (m0 + m) * p.o_stride + col) =
-                u32x4_t{s0[0], s1[0], s0[1], s1[1]};
-        }
-      }
-      return;
+    for (int b = 0; b < 8; ++b) acc[t][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  Set x[2], a[2];
+  load_scales<4, BM, BN, GLU>(p, scales, 0, w, col0, m0, rows);
+  load_scales<4, BM, BN, GLU>(p, scales + SBYTES, 1, w, col0, m0, rows);
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u)
+    loads(u / 4, u & 3, u / 4, u, [&](auto load) { for (int i = 0; i < LOADS; ++i) load(i); });
+  constexpr int kFirst = (UNITS - 2) * LOADS;
+  __builtin_amdgcn_s_waitcnt(0x0070 | (kFirst & 15) | (kFirst >> 4 << 14));
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  const int s0 = scale_at(0);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      a[0].v[t][h] = lds_load16(wr[h] + t * 16 * kSlab);
+      x[0].v[t][h] = lds_load16(xr[h] + UNIT + t * 16 * kSlab);
     }
+    a[0].s[t] = lds_load1(wsr + s0 + t * 256);
+    x[0].s[t] = lds_load1(xsr + s0 + t * 256);
   }
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt: the first buffer is read
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  loads(2, 0, 0, 0, [&](auto load) { for (int i = 0; i < LOADS; ++i) load(i); });
+
+  constexpr int kInFlight = (UNITS - 2) * LOADS;
+  static_assert(kInFlight < 64, "vmcnt");
+  // Phase P of a slab of parity ODD; `at`: the scales of the slab whose unit it reads.
+  auto phase = [&]<int P, int ODD>(int slab, int at) {
+    constexpr int XH = (P == 0 || P == 3) ? ODD : 1 - ODD, WH = P < 2 ? 0 : 1;  // halves multiplied
+    // halves read: the slab's other x, its W1, the next slab's W0 and first x (by its parity)
+    constexpr bool READ_X = P == 0 || P == 3;
+    constexpr int HALF = P == 0 ? 1 - ODD : P == 1 ? 1 : P == 2 ? 0 : 1 - ODD;
+    constexpr int SLOT = (4 * ODD + P + 2) % UNITS, BEFORE = (SLOT + UNITS - 1) % UNITS;
+    // the unit seven behind: the part before this one's, two slabs on or, from its W0 back, one
+    constexpr int PART = (P + 1) & 3, ON = P + 2 + UNITS - 1;
+    __builtin_amdgcn_s_waitcnt(0x0070 | (kInFlight & 15) | (kInFlight >> 4 << 14));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    loads(slab + ON / 4, PART, ODD ^ (ON / 4 & 1), BEFORE, [&](auto load) {
 #pragma unroll
-  for (int t = 0; t < NT; t += HALVES) {
-    const int col = col0 + (wn * NT + t) / HALVES * 16 + 4 * g;
-    if (col >= p.n) continue;
-    const f32x4_t bias = SPLIT ? f32x4_t{0.f, 0.f, 0.f, 0.f} : bias4(p, col);
-#pragma unroll
-    for (int b = 0; b < MB; ++b) {
-      const int m = (wm * MB + b) * 16 + n;
-      if (m >= rows) continue;
-      if constexpr (SPLIT) {
-        // [part][half][row][columns, in fours]
-        const int64_t fours = (p.n + 3) / 4;
-#pragma unroll
-        for (int h = 0; h < HALVES; ++h)
-          p.parts[((int64_t(blockIdx.y) * HALVES + h) * p.rows + m0 + m) * fours + col / 4] = acc[t + h][b];
-      } else if constexpr (!OUT8) {
-        store4(p, m0 + m, col, finish<GLU>(acc[t][b], acc[t + HALVES - 1][b], bias));
+      for (int e = 0; e < 16; ++e) {
+        const int t = e / 4, b = e % 4;
+        mfma_in_place(a[WH].v[t][0], a[WH].v[t][1], a[WH].s[t], x[XH].v[b][0], x[XH].v[b][1], x[XH].s[b],
+                      acc[WH * 4 + t][XH * 4 + b]);
+        Set& to = READ_X ? x[HALF] : a[HALF];
+        if (e < 8) to.v[e / 2][e % 2] = lds_load16((READ_X ? xr : wr)[e % 2] + SLOT * UNIT + e / 2 * 16 * kSlab);
+        else if (e < 12) to.s[e - 8] = lds_load1((READ_X ? xsr : wsr) + at + (HALF * 64 + (e - 8) * 16) * 16);
+        else load(e - 12);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    }
+    });
+  };
+  auto slab_of = [&]<int ODD>(int slab) {
+    if ((slab & 3) == 0 && slab)
+      load_scales<4, BM, BN, GLU>(p, scales + ((slab >> 2) + 1 & 1) * SBYTES, (slab >> 2) + 1, w, col0, m0, rows);
+    const int at = scale_at(slab), next = scale_at(slab + 1);
+    phase.template operator()<0, ODD>(slab, at);
+    phase.template operator()<1, ODD>(slab, at);
+    phase.template operator()<2, ODD>(slab, next);
+    phase.template operator()<3, ODD>(slab, next);
+  };
+  int slab = 0;
+  for (; slab + 1 < p.slabs; slab += 2) {
+    slab_of.template operator()<0>(slab);
+    slab_of.template operator()<1>(slab + 1);
   }
+  if (slab < p.slabs) slab_of.template operator()<0>(slab);
+  __builtin_amdgcn_s_waitcnt(0x0070);  // (the loads past the end write to LDS)
+  // (the last products' sums are written some cycles after their issue)
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+#pragma unroll
+    for (int b = 0; b < 8; ++b) asm volatile("" : "+a"(acc[t][b]));
+  end_of_product<8, 8, GLU, OUT8, false>(p, acc, col0, wn * 8, m0, wm * 128, rows);
 }
 
 // The sum of the parts in their order, and the end of the product.
@@ -304,7 +495,11 @@ template <bool GLU, bool OUT8, bool SPLIT>
 void run_form(const LinearParams& p, int form, int parts, hipStream_t stream) {
   if (form == 0) run<1, 2, 4, 4, 4, GLU, OUT8, SPLIT>(p, parts, stream);
   else if (SPLIT || form == 1) run<2, 2, 4, 4, 4, GLU, OUT8, SPLIT>(p, parts, stream);
-  else run<2, 2, 8, 8, 2, GLU, OUT8, false>(p, 1, stream);
+  else {
+    constexpr int COLS = GLU ? 128 : 256;
+    hipLaunchKernelGGL((wide_kernel<GLU, OUT8>), dim3(uint32_t((p.rows + 255) / 256 * ((p.n + COLS - 1) / COLS))), dim3(256), 0,
+                       stream, p);
+  }
 }
 
 template <bool GLU, bool OUT8>
