@@ -35,6 +35,14 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* base, int b
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, kBufferWord3);
 }
 
+// 16 bytes a lane straight to LDS, lane after lane.
+template <int AUX = 0>
+__device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t rs, lds_t* dst, int voffset) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16, voffset, 0, 0, AUX);
+#endif
+}
+
 // The power of two of a scale byte as the conversions take it: they read the
 // exponent field alone (0 is 2^-127, 255 NaN).
 __device__ __forceinline__ float scale_f32(uint32_t byte) { return __uint_as_float(byte << 23); }

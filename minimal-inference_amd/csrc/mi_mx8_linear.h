@@ -81,8 +81,11 @@ __device__ __forceinline__ void store_block(const LinearParams& p, int64_t m, bo
   if (g == 0) p.scales[m * p.s_stride + first / kBlock] = uint8_t(byte);
 }
 
+// The rows that the few-row kernel takes.
+constexpr int64_t kFewRows = 64;
 constexpr int64_t kMaxRows = 1 << 22, kMaxN = 1 << 24, kMaxStride = 1 << 22;
 
+// (rows at most kFewRows)
 void launch_few(const LinearParams& p, bool glu, hipStream_t stream);
 void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t stream);
 

@@ -1,12 +1,11 @@
 // Projections of many rows with both operands in MXFP8 (prompts): out = x W^T (+ bias) or
 // silu(x Wg^T) * (x Wu^T), fp32 accumulation and one rounding.
 //
-// Bound: the matrix instructions.  A workgroup of WM x WN waves owns a block of out; per
-// slab of 128 k its rows of W and of x go straight from memory to LDS (one of STAGES
-// buffers, the later slabs' while this one is multiplied) and from there, as operands, to the
-// waves.  A row of a slab is 128 bytes, eight chunks whose places are permuted by the row,
-// so that the rows an operand read touches together fall on distinct banks.  The scale
-// bytes of four slabs (16 bytes a row) are staged alike.
+// Bound: the matrix instructions.  A workgroup of four waves owns a block of out; per slab
+// of 128 k its rows of W and of x go straight from memory to LDS, into a ring of buffers,
+// and from there, as operands, to the waves.  A row of a slab is 128 bytes, eight chunks whose
+// places are permuted by the row, so that the rows an operand read touches together fall on
+// distinct banks.  The scale bytes of four slabs (16 bytes a row) are staged alike.
 #include <algorithm>
 
 #include "mi_mx8_linear.h"
@@ -14,12 +13,6 @@
 
 namespace mi::mx8 {
 namespace {
-
-__device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t rs, lds_t* dst, int voffset) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16, voffset, 0, 0, 0);
-#endif
-}
 
 constexpr int kGroupM = 4;
 
@@ -124,132 +117,6 @@ __device__ __forceinline__ void end_of_product(const LinearParams& p, const f32x
   }
 }
 
-// MB blocks of 16 rows of x and NT tiles of 16 rows of W per wave.  Slabs are staged STAGES
-// deep: before slab s is multiplied the loads of the STAGES - 2 slabs behind it may be in
-// flight, and after the barrier its predecessor's buffer is filled again.  Loads past the last slab
-// are out of range, so that every wait counts the same loads.
-//
-// SPLIT: the workgroup takes p.split_slabs slabs and leaves its sums, in fp32, for
-// combine_kernel.
-template <int WM, int WN, int MB, int NT, int STAGES, bool GLU, bool OUT8, bool SPLIT>
-__global__ __launch_bounds__(64 * WM * WN) void many_kernel(LinearParams p) {
-  constexpr int WAVES = WM * WN, HALVES = GLU ? 2 : 1;
-  constexpr int BM = WM * MB * 16, BN = WN * NT * 16, COLS = BN / HALVES;  // BN rows of W
-  constexpr int XBYTES = BM * kSlab, STAGE = XBYTES + BN * kSlab;
-  constexpr int XLOADS = XBYTES / 1024 / WAVES, WLOADS = BN * kSlab / 1024 / WAVES;
-  constexpr int XS = (BM + 63) / 64, SLOADS = XS + (BN + 63) / 64, SBYTES = SLOADS * 1024;
-  static_assert(XBYTES / 1024 % WAVES == 0 && BN * kSlab / 1024 % WAVES == 0 && NT % HALVES == 0, "even shares");
-  static_assert(!OUT8 || (GLU && NT % 4 == 0), "whole blocks");
-  static_assert(STAGES * STAGE + 2 * SBYTES <= 160 * 1024, "LDS");
-  __shared__ __attribute__((aligned(16))) char smem[STAGES * STAGE + 2 * SBYTES];
-  lds_t* const lds = (lds_t*)smem;
-  const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
-  const int wm = w / WN, wn = w % WN;
-  const int g = lane >> 4, n = lane & 15;
-  int col0;
-  int64_t m0;
-  place(p, BM, COLS, col0, m0);
-  const int rows = int(min(int64_t(BM), p.rows - m0));
-  const int slab0 = SPLIT ? int(blockIdx.y) * p.split_slabs : 0;
-  const int slab_end = SPLIT ? min(slab0 + p.split_slabs, p.slabs) : p.slabs;
-  const int blocks = p.k / kBlock;
-
-  // Row r of the workgroup's rows of W: 16 of each half in turn (gate, up, gate, ...).
-  const int wstride = int(p.w_stride), xstride = int(p.x_stride);
-  const char* wbase[HALVES];
-  int wsize[HALVES];
-#pragma unroll
-  for (int h = 0; h < HALVES; ++h) {
-    const int row = h * p.n + col0, count = min(COLS, p.w_rows - row);
-    wbase[h] = p.w + row * p.w_stride;
-    wsize[h] = (count - 1) * wstride + p.k;
-  }
-  const char* const xbase = p.x + m0 * p.x_stride;
-  const int xsize = (rows - 1) * xstride + p.k;
-  // load i: 8 rows, lane l chunk slot l % 8 of row l / 8
-  const int r8 = lane >> 3, chunk = ((lane & 7) ^ r8) * 16;
-  int xv[XLOADS], wv[WLOADS];
-#pragma unroll
-  for (int i = 0; i < XLOADS; ++i) xv[i] = ((w * XLOADS + i) * 8 + r8) * xstride + chunk;
-#pragma unroll
-  for (int i = 0; i < WLOADS; ++i) {
-    const int at = (w * WLOADS + i) * 8 + r8, tile = at / 16;
-    wv[i] = (tile / HALVES * 16 + at % 16) * wstride + chunk;
-  }
-  auto load = [&](int slab, int buf) {
-    lds_t* const stage = lds + buf * STAGE;
-    const int off = slab * kSlab;
-    const bool ok = slab < slab_end, inside = off + chunk < p.k;  // past the row's end lies the next row
-    const __amdgpu_buffer_rsrc_t rx = buffer(xbase + off, ok ? xsize - off : 0);
-#pragma unroll
-    for (int i = 0; i < XLOADS; ++i) lds_dma16(rx, stage + (w * XLOADS + i) * 1024, inside ? xv[i] : kOutOfRange);
-    __amdgpu_buffer_rsrc_t rw[HALVES];
-#pragma unroll
-    for (int h = 0; h < HALVES; ++h) rw[h] = buffer(wbase[h] + off, ok ? wsize[h] - off : 0);
-#pragma unroll
-    for (int i = 0; i < WLOADS; ++i)
-      lds_dma16(rw[(w * WLOADS + i) / 2 % HALVES], stage + XBYTES + (w * WLOADS + i) * 1024, inside ? wv[i] : kOutOfRange);
-  };
-  lds_t* const scales = lds + STAGES * STAGE;
-  auto stage_scales = [&](int quad) {
-    load_scales<WAVES, BM, BN, GLU>(p, scales + (quad & 1) * SBYTES, quad, w, col0, m0, rows);
-  };
-
-  f32x4_t acc[NT][MB];
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int b = 0; b < MB; ++b) acc[t][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  // a lane's two chunks of row n of 16
-  const int lo = n * kSlab + (g ^ (n & 7)) * 16, hi = n * kSlab + ((4 + g) ^ (n & 7)) * 16;
-
-  constexpr int kInFlight = (STAGES - 2) * (XLOADS + WLOADS);
-  static_assert(kInFlight < 64, "vmcnt");
-  stage_scales(slab0 >> 2);
-  stage_scales((slab0 >> 2) + 1);
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) load(slab0 + i, i);
-  int buf = 0, before = STAGES - 1;
-  for (int slab = slab0; slab < slab_end; ++slab) {
-    // vmcnt: this slab (and the scales, older than its successors') is in LDS; lgkmcnt: this
-    // wave has read the one before
-    __builtin_amdgcn_s_waitcnt(0x0070 | (kInFlight & 15) | (kInFlight >> 4 << 14));
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    const int quad = slab >> 2;
-    if ((slab & 3) == 0 && slab != slab0) stage_scales(quad + 1);  // (four slabs ahead: done by any wait before them)
-    load(slab + STAGES - 1, before);
-    const lds_t* const xl = lds + buf * STAGE + wm * MB * 16 * kSlab;
-    const lds_t* const wl = lds + buf * STAGE + XBYTES + wn * NT * 16 * kSlab;
-    const lds_t* const sl = scales + (quad & 1) * SBYTES + n * 16 + (slab & 3) * 4 + g;
-    const bool known = slab * 4 + g < blocks;  // (a row's padding may hold anything)
-    u32x4_t a[NT][2], x[MB][2];
-    uint32_t as[NT], xs[MB];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      a[t][0] = lds_load16(wl + t * 16 * kSlab + lo);
-      a[t][1] = lds_load16(wl + t * 16 * kSlab + hi);
-      as[t] = known ? lds_load1(sl + (XS * 64 + (wn * NT + t) * 16) * 16) : 0u;
-    }
-#pragma unroll
-    for (int b = 0; b < MB; ++b) {
-      x[b][0] = lds_load16(xl + b * 16 * kSlab + lo);
-      x[b][1] = lds_load16(xl + b * 16 * kSlab + hi);
-      xs[b] = known ? lds_load1(sl + (wm * MB + b) * 16 * 16) : 0u;
-    }
-#pragma unroll
-    for (int b = 0; b < MB; ++b)
-#pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t][b] = mfma_fp8(a[t][0], a[t][1], as[t], x[b][0], x[b][1], xs[b], acc[t][b]);
-    before = buf;
-    buf = buf + 1 == STAGES ? 0 : buf + 1;
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // (the loads past the end write to LDS)
-
-  end_of_product<MB, NT, GLU, OUT8, SPLIT>(p, acc, col0, wn * NT, m0, wm * MB * 16, rows);
-}
-
 // The product into accumulation registers that stay where they are: 64 sums fill all of them, and
 // left to choose, the compiler moves a quarter of the sums about in every slab.  The sums may be read 18
 // cycles after the last of these at the earliest.
@@ -269,10 +136,14 @@ __device__ __forceinline__ void mfma_in_place(u32x4_t alo, u32x4_t ahi, uint32_t
 //   even slabs  X0 W0, X1 W0, X1 W1, X0 W1     odd slabs  X1 W0, X0 W0, X0 W1, X1 W1
 // so that a unit's registers are free two phases before the next slab needs them, and each
 // phase reads one unit from LDS for the next phase or the one after.  Units go through a ring of
-// eight buffers, two slabs', in the order in which they are read (W0, X, X, W1): a phase
-// waits for its unit, and after the barrier fills the buffer that the phase before has read,
-// seven phases before that unit's turn.  Between two matrix instructions stands one read or load:
-// an instruction leaves a wave seven issue slots, and what does not fit in them is lost.
+// eight buffers, two slabs', in the order in which they are read (W0, X, X, W1): every
+// second phase waits for its unit and the next, and after the barrier the two phases fill
+// the buffers that the two before have read, six phases before those units' turn.  Between
+// two matrix instructions stand two reads or a load: an instruction leaves a wave seven issue
+// slots, and what does not fit in them is lost.
+// (us, 8,192 x 8,192 x 10,240 of normal values: two whole slabs staged and read at once 649;
+// these phases with addresses computed in place 649, with constants and pinned sums 503, a
+// barrier in every second phase 482; zeros 417: the clock follows the power that the products take.)
 template <bool GLU, bool OUT8>
 __global__ __launch_bounds__(256) void wide_kernel(LinearParams p) {
   constexpr int HALVES = GLU ? 2 : 1, BM = 256, BN = 256, COLS = BN / HALVES;
@@ -362,12 +233,8 @@ __global__ __launch_bounds__(256) void wide_kernel(LinearParams p) {
     a[0].s[t] = lds_load1(wsr + s0 + t * 256);
     x[0].s[t] = lds_load1(xsr + s0 + t * 256);
   }
-  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt: the first buffer is read
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_sched_barrier(0);
-  loads(2, 0, 0, 0, [&](auto load) { for (int i = 0; i < LOADS; ++i) load(i); });
 
-  constexpr int kInFlight = (UNITS - 2) * LOADS;
+  constexpr int kInFlight = (UNITS - 4) * LOADS;
   static_assert(kInFlight < 64, "vmcnt");
   // Phase P of a slab of parity ODD; `at`: the scales of the slab whose unit it reads.
   auto phase = [&]<int P, int ODD>(int slab, int at) {
@@ -375,22 +242,24 @@ __global__ __launch_bounds__(256) void wide_kernel(LinearParams p) {
     // halves read: the slab's other x, its W1, the next slab's W0 and first x (by its parity)
     constexpr bool READ_X = P == 0 || P == 3;
     constexpr int HALF = P == 0 ? 1 - ODD : P == 1 ? 1 : P == 2 ? 0 : 1 - ODD;
-    constexpr int SLOT = (4 * ODD + P + 2) % UNITS, BEFORE = (SLOT + UNITS - 1) % UNITS;
-    // the unit seven behind: the part before this one's, two slabs on or, from its W0 back, one
-    constexpr int PART = (P + 1) & 3, ON = P + 2 + UNITS - 1;
-    __builtin_amdgcn_s_waitcnt(0x0070 | (kInFlight & 15) | (kInFlight >> 4 << 14));
-    __builtin_amdgcn_s_barrier();
+    constexpr int SLOT = (4 * ODD + P + 2) % UNITS, BEFORE = (SLOT + UNITS - 2) % UNITS;
+    if constexpr (P % 2 == 0) {
+      __builtin_amdgcn_s_waitcnt(0x0070 | (kInFlight & 15) | (kInFlight >> 4 << 14));
+      __builtin_amdgcn_s_barrier();
+    }
     __builtin_amdgcn_sched_barrier(0);
-    loads(slab + ON / 4, PART, ODD ^ (ON / 4 & 1), BEFORE, [&](auto load) {
+    loads(slab + 2, P, ODD, BEFORE, [&](auto load) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int t = e / 4, b = e % 4;
         mfma_in_place(a[WH].v[t][0], a[WH].v[t][1], a[WH].s[t], x[XH].v[b][0], x[XH].v[b][1], x[XH].s[b],
                       acc[WH * 4 + t][XH * 4 + b]);
         Set& to = READ_X ? x[HALF] : a[HALF];
-        if (e < 8) to.v[e / 2][e % 2] = lds_load16((READ_X ? xr : wr)[e % 2] + SLOT * UNIT + e / 2 * 16 * kSlab);
-        else if (e < 12) to.s[e - 8] = lds_load1((READ_X ? xsr : wsr) + at + (HALF * 64 + (e - 8) * 16) * 16);
-        else load(e - 12);
+        if (e < 4) {
+          to.v[e][0] = lds_load16((READ_X ? xr : wr)[0] + SLOT * UNIT + e * 16 * kSlab);
+          to.v[e][1] = lds_load16((READ_X ? xr : wr)[1] + SLOT * UNIT + e * 16 * kSlab);
+        } else if (e < 8) to.s[e - 4] = lds_load1((READ_X ? xsr : wsr) + at + (HALF * 64 + (e - 4) * 16) * 16);
+        else if (e < 12) load(e - 8);
         __builtin_amdgcn_sched_barrier(0);
       }
     });
@@ -420,6 +289,155 @@ __global__ __launch_bounds__(256) void wide_kernel(LinearParams p) {
   end_of_product<8, 8, GLU, OUT8, false>(p, acc, col0, wn * 8, m0, wm * 128, rows);
 }
 
+// Blocks of 128 rows of x by 128 of W, four waves of 64 x 64: as wide_kernel, with one unit of x and
+// one of W to a slab, one phase, and one barrier.  The products of slab s read from LDS the
+// units of s + 1, into registers of their own; after the barrier of slab s the buffers are
+// filled again that slab s - 1 has read, four slabs ahead.
+//
+// Bound: the way from L2 to LDS, 32 KB for 16 products a wave; at 0.58 us a slab 256 workgroups take 14.5 TB/s of it
+// (2,048 x 8,192 x 10,240 212 us; without the loads 133, without the reads from LDS 208).
+//
+// SPLIT: the workgroup takes p.split_slabs slabs (a multiple of four) and leaves its sums, in
+// fp32, for combine_kernel.
+template <bool GLU, bool OUT8, bool SPLIT>
+__global__ __launch_bounds__(256) void block_kernel(LinearParams p) {
+  constexpr int HALVES = GLU ? 2 : 1, BM = 128, BN = 128, COLS = BN / HALVES;
+  constexpr int RING = 4, UNIT = 128 * kSlab, SBYTES = (BM + BN) * 16, LOADS = UNIT / 1024 / 4;
+  static_assert(RING * 2 * UNIT + 2 * SBYTES <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(16))) char smem[RING * 2 * UNIT + 2 * SBYTES];
+  lds_t* const lds = (lds_t*)smem;
+  lds_t* const scales = lds + RING * 2 * UNIT;
+  const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
+  const int wm = w / 2, wn = w % 2;
+  const int g = lane >> 4, n = lane & 15;
+  int col0;
+  int64_t m0;
+  place(p, BM, COLS, col0, m0);
+  const int rows = int(min(int64_t(BM), p.rows - m0)), blocks = p.k / kBlock;
+  const int slab0 = SPLIT ? int(blockIdx.y) * p.split_slabs : 0;
+  const int slab_end = SPLIT ? min(slab0 + p.split_slabs, p.slabs) : p.slabs;
+  const int wstride = int(p.w_stride), xstride = int(p.x_stride);
+  // load i of a wave: 8 rows of a unit, lane l chunk slot l % 8 of row l / 8
+  const int r8 = lane >> 3, chunk = ((lane & 7) ^ r8) * 16;
+  int xv[LOADS], wv[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int of = w >> 1, r = (w & 1) * 32 + i * 8;
+    xv[i] = (of * 64 + r + r8) * xstride + chunk;
+    wv[i] = (of * (64 / HALVES) + r / 16 / HALVES * 16 + r % 16 + r8) * wstride + chunk;
+  }
+  const char* const xbase = p.x + m0 * p.x_stride;
+  const char* const wbase = p.w + col0 * p.w_stride;
+  const char* const ubase = p.w + (int64_t(p.n) + col0) * p.w_stride;
+  const int xsize = (rows - 1) * xstride + p.k, wsize = (min(COLS, p.w_rows - col0) - 1) * wstride + p.k;
+  const int usize = GLU ? (min(COLS, p.n - col0) - 1) * wstride + p.k : 0;
+  struct Source {
+    __amdgpu_buffer_rsrc_t first, second;  // the rows of a unit's first two loads and of the others
+    int past;
+  };
+  auto source = [&](int slab, bool of_x) {
+    const int off = slab * kSlab;
+    const bool ok = slab < slab_end;
+    const __amdgpu_buffer_rsrc_t r = of_x ? buffer(xbase + off, ok ? xsize - off : 0) : buffer(wbase + off, ok ? wsize - off : 0);
+    const __amdgpu_buffer_rsrc_t u = GLU && !of_x ? buffer(ubase + off, ok ? usize - off : 0) : r;
+    return Source{r, u, off + chunk < p.k ? 0 : kOutOfRange};  // past the row's end lies the next row
+  };
+  // Load i of a slab's unit (0: x, 1: W) into place `ring` of the ring.
+  auto load = [&](const Source& s, int unit, int ring, int i) {
+    lds_dma16(i / 2 ? s.second : s.first, lds + (ring * 2 + unit) * UNIT + (w * LOADS + i) * 1024, (unit ? wv[i] : xv[i]) | s.past);
+  };
+  auto load_slab = [&](int slab, int ring) {
+    const Source sx = source(slab, true), sw = source(slab, false);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load(sx, 0, ring, i);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load(sw, 1, ring, i);
+  };
+  struct Set {
+    u32x4_t v[4][2];
+    uint32_t s[4];
+  };
+  const int lo = n * kSlab + (g ^ (n & 7)) * 16, hi = n * kSlab + ((4 + g) ^ (n & 7)) * 16;
+  const lds_t* const xr[2] = {lds + wm * 64 * kSlab + lo, lds + wm * 64 * kSlab + hi};
+  const lds_t* const wr[2] = {lds + wn * 64 * kSlab + lo, lds + wn * 64 * kSlab + hi};
+  const lds_t* const xsr = scales + (wm * 64 + n) * 16;
+  const lds_t* const wsr = scales + (BM + wn * 64 + n) * 16;
+  // Where a slab's scale bytes lie in a staged row: behind the last block (whose codes are
+  // zeros) the last one's, since a row's padding may hold anything.
+  auto scale_at = [&](int slab) { return (slab >> 2 & 1) * SBYTES + (slab & 3) * 4 + min(g, max(blocks - 1 - slab * 4, 0)); };
+  // Read e of 12 of a unit: eight of operands, four of scales.
+  auto read = [&](Set& to, int unit, int ring, int at, int e) {
+    if (e < 8) to.v[e / 2][e % 2] = lds_load16((unit ? wr : xr)[e % 2] + (ring * 2 + unit) * UNIT + e / 2 * 16 * kSlab);
+    else to.s[e - 8] = lds_load1((unit ? wsr : xsr) + at + (e - 8) * 256);
+  };
+
+  f32x4_t acc[4][4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) acc[t][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  Set x[2], a[2];
+  load_scales<4, BM, BN, GLU>(p, scales + (slab0 >> 2 & 1) * SBYTES, slab0 >> 2, w, col0, m0, rows);
+  load_scales<4, BM, BN, GLU>(p, scales + ((slab0 >> 2) + 1 & 1) * SBYTES, (slab0 >> 2) + 1, w, col0, m0, rows);
+#pragma unroll
+  for (int i = 0; i < RING; ++i) load_slab(slab0 + i, i);
+  constexpr int kFirst = (RING - 1) * 2 * LOADS, kInFlight = (RING - 2) * 2 * LOADS;
+  static_assert(kFirst < 64, "vmcnt");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (kFirst & 15) | (kFirst >> 4 << 14));
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  int at = scale_at(slab0);
+#pragma unroll
+  for (int e = 0; e < 12; ++e) {
+    read(x[0], 0, 0, at, e);
+    read(a[0], 1, 0, at, e);
+  }
+  auto slab_of = [&]<int I>(int slab) {
+    constexpr int HERE = I & 1, NEXT = 1 - HERE, RNEXT = (I + 1) % RING;
+    __builtin_amdgcn_s_waitcnt(0x0070 | (kInFlight & 15) | (kInFlight >> 4 << 14));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    int at_next = 0;
+    Source sx, sw;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int t = e / 4, b = e % 4;
+      mfma_in_place(a[HERE].v[t][0], a[HERE].v[t][1], a[HERE].s[t], x[HERE].v[b][0], x[HERE].v[b][1], x[HERE].s[b], acc[t][b]);
+      if (e == 2) sx = source(slab + RING, true);
+      if (e == 4) sw = source(slab + RING, false);
+      if (e == 6) at_next = scale_at(slab + 1);
+      if (e < 12) {
+        read(x[NEXT], 0, RNEXT, at_next, e);
+        read(a[NEXT], 1, RNEXT, at_next, e);
+      }
+      if (e >= 8 && e < 12) load(sx, 0, I, e - 8);
+      if (e >= 12) load(sw, 1, I, e - 12);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if ((slab & 3) == 0 && slab != slab0)  // (three slabs ahead: done by the waits before them)
+      load_scales<4, BM, BN, GLU>(p, scales + ((slab >> 2) + 1 & 1) * SBYTES, (slab >> 2) + 1, w, col0, m0, rows);
+    at = at_next;
+  };
+  for (int slab = slab0;;) {
+    slab_of.template operator()<0>(slab);
+    if (++slab >= slab_end) break;
+    slab_of.template operator()<1>(slab);
+    if (++slab >= slab_end) break;
+    slab_of.template operator()<2>(slab);
+    if (++slab >= slab_end) break;
+    slab_of.template operator()<3>(slab);
+    if (++slab >= slab_end) break;
+  }
+  __builtin_amdgcn_s_waitcnt(0x0070);  // (the loads past the end write to LDS)
+  // (the last products' sums are written some cycles after their issue)
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) asm volatile("" : "+a"(acc[t][b]));
+  end_of_product<4, 4, GLU, OUT8, SPLIT>(p, acc, col0, wn * 4, m0, wm * 64, rows);
+}
+
 // The sum of the parts in their order, and the end of the product.
 template <bool GLU, bool OUT8>
 __global__ __launch_bounds__(256) void combine_kernel(LinearParams p, int parts) {
@@ -447,78 +465,80 @@ __global__ __launch_bounds__(256) void combine_kernel(LinearParams p, int parts)
 }
 
 // ---------------------------------------------------------------- which form
-struct Form {
-  int rows, w_rows;
-  float one_us, more_us;
-  bool split;
-};
-constexpr Form kForms[] = {{64, 128, 0.45f, 0.45f, true}, {128, 128, 0.6f, 0.5f, true}, {256, 256, 1.5f, 1.5f, false}};
+// The time of a launch, counted: its start, and for every round of workgroups their own start and end
+// and a slab's time for every slab; the last round is the faster, the fewer CUs it takes (they
+// share the power).  Workgroups that share k add the combining launch with the parts' way to memory and
+// back.  Counted and measured (us): 8,192 x 8,192 x 10,240 wide 498 / 482, 2,048 x 8,192 x
+// 10,240 wide 184 / 175, block 213 / 212; 1,000 x 4,096 x 6,144 wide 49 / 46, block 45 / 46; 600 x 14,336 x 4,096
+// block 75 / 73, in 3 parts 72 / 71, wide 143 / 131; 512 x 3,584 x 4,608 block 22 / 23; 200 x 4,096 x
+// 6,144 in 2 parts 22 / 21; 77 x 18,944 x 3,584 in 8 parts 24 / 27, whole 94 / 89; 128 x
+// 4,096 x 4,096 in 4 parts 17 / 19.  (Blocks of 128 x 256 were no faster than either in any of
+// these, nor two workgroups of 128 x 128 on a CU.)
 constexpr float kStartUs = 3.5f, kCombineUs = 2.5f, kBytesPerUs = 4.4e6f;
 constexpr int kMaxParts = 32;
+enum class Form { few, block, wide };
 
 struct Choice {
   float us;
-  int form, parts, split_slabs;
+  Form form;
+  int parts, split_slabs;
   size_t bytes;  // of the parts
+  int64_t rest;  // rows behind the last whole block, for a launch of their own
 };
+
+float rounds_us(int64_t workgroups, int slabs, float own, float least, float more) {
+  const int cus = mi::num_cus();
+  const int64_t whole = workgroups / cus, last = workgroups % cus;
+  return kStartUs + float(whole) * (own + slabs * (least + more)) +
+         (last ? own + slabs * (least + more * float(last) / float(cus)) : 0.f);
+}
+// The few-row kernel's (up to 64 rows): W's bytes from memory, x's into every workgroup.
+float few_us(int64_t rows, int64_t w_rows, int slabs) {
+  const float k = float(slabs) * kSlab, workgroups = std::max(1.f, std::min(float(w_rows) / 16, float(w_rows) / 64));
+  return kStartUs + float(w_rows) * k * 33 / 32 / 5.2e6f + float(rows) * k * workgroups / 15e6f;
+}
 
 // The fastest by that count within `room` bytes for parts.
 Choice choose(bool glu, int64_t rows, int64_t n, int slabs, size_t room) {
-  Choice best = {1e30f, 0, 1, slabs, 0};
-  const int cus = mi::num_cus();
-  for (int f = 0; f < int(sizeof(kForms) / sizeof(kForms[0])); ++f) {
-    const Form& form = kForms[f];
-    const int64_t cols = form.w_rows / (glu ? 2 : 1);
-    const int64_t tiles = (rows + form.rows - 1) / form.rows * ((n + cols - 1) / cols);
-    for (int want = 1; want <= (form.split ? kMaxParts : 1); ++want) {
-      const int each = (slabs + want - 1) / want, parts = (slabs + each - 1) / each;
-      if (parts != want || (want > 1 && (each < 2 || tiles * (want - 1) >= 2 * cus))) continue;
-      const size_t bytes = want > 1 ? size_t(want) * (glu ? 2 : 1) * rows * ((n + 3) / 4) * 16 : 0;
-      if (bytes > room) continue;
-      const int64_t per_cu = (tiles * want + cus - 1) / cus;
-      float us = kStartUs + each * (per_cu == 1 ? form.one_us : float(per_cu) * form.more_us);
-      us += want > 1 ? kCombineUs + 2 * float(bytes) / kBytesPerUs : 2 * float(rows) * float(n) / kBytesPerUs;
-      if (us < best.us) best = {us, f, want, each, bytes};
-    }
+  if (rows <= kFewRows) return {0.f, Form::few, 1, slabs, 0, 0};
+  const int64_t w_rows = glu ? 2 * n : n, across = (w_rows + 255) / 256;
+  Choice best = {rounds_us((rows + 255) / 256 * across, slabs, 6.f, 1.1f, 0.35f), Form::wide, 1, slabs, 0, 0};
+  // (8,201 x 8,192 x 10,240: 33 rows of blocks are a round more than 32 and a launch of nine rows)
+  if (const int64_t rest = rows % 256; rest && rest <= kFewRows && rest < rows) {
+    const float us = rounds_us(rows / 256 * across, slabs, 6.f, 1.1f, 0.35f) + few_us(rest, w_rows, slabs);
+    if (us < best.us) best.us = us, best.rest = rest;
+  }
+  const int64_t block = (rows + 127) / 128 * ((w_rows + 127) / 128);
+  for (int want = 1; want <= kMaxParts; ++want) {
+    const int each = want == 1 ? slabs : ((slabs + want - 1) / want + 3) / 4 * 4, parts = (slabs + each - 1) / each;
+    if (parts != want || (want > 1 && block * (want - 1) >= 2 * mi::num_cus())) continue;
+    const size_t bytes = want > 1 ? size_t(want) * (glu ? 2 : 1) * rows * ((n + 3) / 4) * 16 : 0;
+    if (bytes > room) continue;
+    const float us = rounds_us(block * want, each, 1.5f, 0.53f, 0.07f) +
+                     (want > 1 ? kCombineUs + 2 * float(bytes) / kBytesPerUs : 0.f);
+    if (us < best.us) best = {us, Form::block, want, each, bytes, 0};
   }
   return best;
 }
 
-template <int WM, int WN, int MB, int NT, int STAGES, bool GLU, bool OUT8, bool SPLIT>
-void run(const LinearParams& p, int parts, hipStream_t stream) {
-  constexpr int BM = WM * MB * 16, COLS = WN * NT * 16 / (GLU ? 2 : 1);
-  const dim3 grid(uint32_t((p.rows + BM - 1) / BM * ((p.n + COLS - 1) / COLS)), parts);
-  hipLaunchKernelGGL((many_kernel<WM, WN, MB, NT, STAGES, GLU, OUT8, SPLIT>), grid, dim3(64 * WM * WN), 0, stream, p);
-}
-
-template <bool GLU, bool OUT8, bool SPLIT>
-void run_form(const LinearParams& p, int form, int parts, hipStream_t stream) {
-  if (form == 0) run<1, 2, 4, 4, 4, GLU, OUT8, SPLIT>(p, parts, stream);
-  else if (SPLIT || form == 1) run<2, 2, 4, 4, 4, GLU, OUT8, SPLIT>(p, parts, stream);
-  else {
-    constexpr int COLS = GLU ? 128 : 256;
-    hipLaunchKernelGGL((wide_kernel<GLU, OUT8>), dim3(uint32_t((p.rows + 255) / 256 * ((p.n + COLS - 1) / COLS))), dim3(256), 0,
-                       stream, p);
-  }
-}
-
 template <bool GLU, bool OUT8>
 void launch(const LinearParams& p, const Choice& c, hipStream_t stream) {
+  const int size = c.form == Form::wide ? 256 : 128, cols = size / (GLU ? 2 : 1);
+  const dim3 grid(uint32_t((p.rows + size - 1) / size * ((p.n + cols - 1) / cols)), c.parts), block(256);
   LinearParams q = p;
   q.split_slabs = c.split_slabs;
-  if (c.parts == 1) {
-    run_form<GLU, OUT8, false>(q, c.form, 1, stream);
-    return;
+  if (c.form == Form::wide) {
+    hipLaunchKernelGGL((wide_kernel<GLU, OUT8>), grid, block, 0, stream, q);
+  } else if (c.parts == 1) {
+    hipLaunchKernelGGL((block_kernel<GLU, OUT8, false>), grid, block, 0, stream, q);
+  } else {
+    hipLaunchKernelGGL((block_kernel<GLU, false, true>), grid, block, 0, stream, q);
+    const int64_t fours = p.rows * ((p.n + 3) / 4);
+    hipLaunchKernelGGL((combine_kernel<GLU, OUT8>), dim3(uint32_t((fours + 255) / 256)), dim3(256), 0, stream, q, c.parts);
   }
-  run_form<GLU, false, true>(q, c.form, c.parts, stream);
-  const int64_t fours = p.rows * ((p.n + 3) / 4);
-  hipLaunchKernelGGL((combine_kernel<GLU, OUT8>), dim3(uint32_t((fours + 255) / 256)), dim3(256), 0, stream, q, c.parts);
 }
 
 }  // namespace
-
-// Whether the few-row kernel is the faster one.
-bool few(int64_t rows) { return rows <= 64; }
 
 size_t many_workspace(bool glu, int64_t rows, int64_t n, int slabs) {
   return choose(glu, rows, n, slabs, size_t(1) << 28).bytes;
@@ -526,15 +546,25 @@ size_t many_workspace(bool glu, int64_t rows, int64_t n, int slabs) {
 
 void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t stream) {
   const Choice c = choose(glu, p.rows, p.n, p.slabs, room);
-  if (!glu) launch<false, false>(p, c, stream);
-  else p.scales ? launch<true, true>(p, c, stream) : launch<true, false>(p, c, stream);
+  LinearParams q = p;
+  q.rows = p.rows - c.rest;
+  if (!glu) launch<false, false>(q, c, stream);
+  else p.scales ? launch<true, true>(q, c, stream) : launch<true, false>(q, c, stream);
+  if (!c.rest) return;
+  LinearParams rest = p;
+  rest.rows = c.rest;
+  rest.x += q.rows * p.x_stride;
+  rest.xs += q.rows * p.xs_stride;
+  rest.out += q.rows * p.o_stride * (p.scales ? 1 : 2);
+  if (p.scales) rest.scales += q.rows * p.s_stride;
+  launch_few(rest, glu, stream);
 }
 
 }  // namespace mi::mx8
 
 extern "C" size_t mi_linear_mxfp8_workspace_size(int64_t rows, int64_t n, int64_t k, int32_t silu) {
   using namespace mi::mx8;
-  if (rows <= 0 || rows > kMaxRows || n <= 0 || n > kMaxN || k <= 0 || k % kBlock || k > kMaxK || few(rows)) return 0;
+  if (rows <= 0 || rows > kMaxRows || n <= 0 || n > kMaxN || k <= 0 || k % kBlock || k > kMaxK || rows <= kFewRows) return 0;
   return many_workspace(silu != 0, rows, n, int(slabs(k)));
 }
 
@@ -609,7 +639,7 @@ extern "C" int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void
           ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) & 7) == 0;
   p.wide = p.vec && n % 8 == 0 && out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (few(rows)) launch_few(p, silu != 0, s);
+  if (rows <= kFewRows) launch_few(p, silu != 0, s);
   else launch_many(p, silu != 0, workspace ? workspace_bytes : 0, s);
   return mi::check_launch(name);
 }
