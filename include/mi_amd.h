@@ -498,12 +498,12 @@ int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void* x_scales,
  *
  * mi_adapter_plan sorts a batch's rows by adapter, once for all its projections:
  * slot_of_row [rows] int32, an id outside 0..slots-1 (as -1) for none; at most 2^22
- * rows, 1,023 adapters.  plan: mi_adapter_plan_size bytes, 16-byte aligned, written
- * here and read by runs with the same rows and slots.
+ * rows, 1,023 adapters.  plan: mi_adapter_plan_size bytes (of rows or more), 16-byte
+ * aligned, written here and read by runs with the same rows and slots.
  *
  * mi_add_adapters: out = y + scale[s] * B[s] (A[s] x), one rounding to bf16, with row
  * t's adapter s; rows without one are y's.  y, out [rows][n] bf16; x [rows][k] bf16, or,
- * x_scales not null, MXFP8 (any alignment of scale rows).  The n columns are
+ * x_scales not null, MXFP8 (scale rows as mi_linear_mxfp8 takes them).  The n columns are
  * pieces (1..8, piece_columns on the host, multiples of 16 up to 2^20) with factors of
  * their own: a [slots][pieces * rank][k], b [slots][n][rank] bf16 contiguous, scale
  * [slots] fp32.  rank a multiple of 8 up to 128 (smaller ones padded with zeros), k of 32 up

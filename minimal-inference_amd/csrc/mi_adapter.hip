@@ -2,8 +2,8 @@
 // A [r][k] and B [n][r] of the row's own adapter.  The projection's outputs are one to
 // eight pieces (q, k, v), each with r rows of A of its own.
 //
-//   plan   : rows sorted by adapter into tiles of up to 64 rows of one adapter, once per
-//            batch.  Which row comes where in its adapter's tiles is of no matter: a row's
+//   plan   : rows sorted by adapter into tiles of up to 16 or 64 rows of one adapter, once
+//            per batch.  Which row comes where in its adapter's tiles is of no matter: a row's
 //            result depends on its own operands alone.
 //   shrink : v = A x of a tile, k in parts over workgroups; sums in fp32.
 //   expand : the parts' sum, times scale, as a pair of bf16 (v and what its rounding left: 16
@@ -23,22 +23,26 @@ using mi::f32x4_t;
 using mi::mx8::u32x2_t;
 using mi::mx8::u32x4_t;
 
-constexpr int kTile = 64;        // rows of a tile
+// Rows of a tile: 16 up to 512 rows, 64 beyond (see mi_add_adapters).
+constexpr int64_t kFewRows = 512;
+constexpr int tile_rows(int64_t rows) { return rows <= kFewRows ? 16 : 64; }
 constexpr int kMaxSlots = 1023;  // (and one more count for the rows without)
 constexpr int kMaxRank = 128;
 constexpr int kMaxPieces = 8;
 constexpr int64_t kMaxRows = 1 << 22;
 constexpr int kWaves = 4;
+constexpr int kManyWaves = 2;  // of a shrink workgroup of 64 rows: two of them share a CU's LDS
 constexpr int kStep = 64;  // k of a wave's step
 constexpr int kMaxParts = 16;
-constexpr int kGroup = 4;  // 16-rank tiles of a workgroup
+constexpr int kGroup = 4;  // 16-rank tiles of a workgroup; of 8-bit rows in tiles of 64 half as many
 
 struct Tile {
   int slot, first, count, unused;  // slot -1: rows without an adapter
 };
 
 // A plan: the number of tiles in 16 bytes, the tiles, the rows in their order.
-int64_t max_tiles(int64_t rows, int64_t slots) { return std::min(rows, slots + 1) + rows / kTile; }
+int64_t max_tiles(int64_t rows, int64_t slots) { return std::min(rows, slots + 1) + rows / tile_rows(rows); }
+size_t plan_size(int64_t rows, int64_t slots) { return 16 + 16 * size_t(max_tiles(rows, slots)) + 4 * size_t(rows); }
 struct PlanView {
   int* count;
   Tile* tiles;
@@ -52,7 +56,7 @@ PlanView view(void* plan, int64_t rows, int64_t slots) {
 
 constexpr int kPlanThreads = 1024;
 
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* slot_of_row, int rows, int slots, PlanView p) {
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* slot_of_row, int rows, int slots, int tile_rows, PlanView p) {
   __shared__ int count[kPlanThreads], first[kPlanThreads], tiles[kPlanThreads];
   const int tid = threadIdx.x, lane = tid & 63;
   count[tid] = 0;
@@ -74,7 +78,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* slot_of_r
   };
   for (int row = tid; row < rows; row += kPlanThreads) places(at(row), count);
   __syncthreads();
-  const int mine = count[tid], need = (mine + kTile - 1) / kTile;
+  const int mine = count[tid], need = (mine + tile_rows - 1) / tile_rows;
   first[tid] = mine;
   tiles[tid] = need;
   __syncthreads();
@@ -87,7 +91,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* slot_of_r
   }
   const int begin = first[tid] - mine, tile = tiles[tid] - need;
   for (int i = 0; i < need; ++i)
-    p.tiles[tile + i] = {tid < slots ? tid : -1, begin + i * kTile, min(kTile, mine - i * kTile), 0};
+    p.tiles[tile + i] = {tid < slots ? tid : -1, begin + i * tile_rows, min(tile_rows, mine - i * tile_rows), 0};
   if (tid == kPlanThreads - 1) *p.count = tiles[tid];
   count[tid] = begin;
   __syncthreads();
@@ -97,7 +101,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* slot_of_r
 struct AdapterParams {
   const char* x;      // bf16 rows, or codes
   int64_t x_stride;   // bytes
-  const uint8_t* xs;  // scale bytes; null: x is bf16
+  const char* xs;     // scale bytes, rows of whole 16 bytes; null: x is bf16
   int64_t xs_stride;
   const uint16_t* a;  // [slots][pieces * rank][k]
   const uint16_t* b;  // [slots][n][rank]
@@ -107,42 +111,62 @@ struct AdapterParams {
   uint16_t* out;
   int64_t o_stride;
   PlanView plan;
-  float* parts;  // [part][tile][row of 64][ranks, padded]
+  float* parts;  // [part][tile][row of the tile][ranks, padded]
   int k, n, rank, ranks, padded;  // ranks = pieces * rank, padded to 16
-  int n_parts, part_steps, max_tiles;
+  int n_parts, part_steps, max_tiles, group_ranks;
   int pieces, chunk;  // columns of an expand workgroup
   int end[kMaxPieces];       // columns,
   int end_chunk[kMaxPieces]; // chunks up to and with each piece
 };
 
-// In a step of 64 k, lane (g, n) holds row n's k from 16 g on: its first eight are one
-// product's operand, the other eight the next one's.  (Which k comes where is of no matter
-// as long as both operands agree.)
-template <bool X8, int RT, int NB>
-__device__ void shrink(const AdapterParams& p, const Tile& tile, char* smem) {
+// The waves' sums of a tile's ranks to memory: lane (g, n) holds ranks 4 g .. 4 g + 3 of
+// tile t for row n of block b.
+template <int WAVES, int RT, int NB>
+__device__ __forceinline__ void store_ranks(const AdapterParams& p, const f32x4_t (&acc)[RT][NB], f32x4_t* red, int count,
+                                            int rank0) {
   const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, n = lane & 15;
-  const int rank0 = int(blockIdx.z) * kGroup * 16;
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) red[(w * RT * NB + t * NB + b) * 64 + lane] = acc[t][b];
+  __syncthreads();
+  for (int q = w; q < RT * NB; q += WAVES) {
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int o = 0; o < WAVES; ++o) sum += red[(o * RT * NB + q) * 64 + lane];
+    const int row = q % NB * 16 + n, r = rank0 + q / NB * 16 + 4 * g;
+    if (row < count && r < p.padded)
+      *reinterpret_cast<f32x4_t*>(p.parts + ((int64_t(blockIdx.y) * p.max_tiles + blockIdx.x) * (16 * NB) + row) * p.padded + r) = sum;
+  }
+}
+
+// Tiles of 16 rows: a wave takes steps of 64 k in turn, straight from memory to registers, the
+// next step's while this one is multiplied.  In a step lane (g, n) holds row n's k from 16 g on: its
+// first eight are one product's operand, the other eight the next one's.  (Which k comes
+// where is of no matter as long as both operands agree.)
+template <bool X8, int RT>
+__global__ __launch_bounds__(64 * kWaves) void shrink_few_kernel(AdapterParams p) {
+  __shared__ __attribute__((aligned(16))) f32x4_t red[kWaves * RT * 64];
+  const int tiles = *p.plan.count;
+  const Tile tile = p.plan.tiles[blockIdx.x];
+  if (int(blockIdx.x) >= tiles || tile.slot < 0) return;
+  const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
+  const int g = lane >> 4, n = lane & 15;
+  const int rank0 = int(blockIdx.z) * p.group_ranks;
+  const int64_t row = p.plan.order[tile.first + (n < tile.count ? n : 0)];
+  const char* const x = p.x + row * p.x_stride + (X8 ? 16 : 32) * g;
+  const char* const xs = X8 ? p.xs + row * p.xs_stride + g / 2 : nullptr;
   const uint16_t* a[RT];
-  const char* x[NB];
-  const uint8_t* xs[NB];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int r = rank0 + t * 16 + n;  // (past the last rank any row will do: its sums are not kept)
     a[t] = p.a + (int64_t(tile.slot) * p.ranks + (r < p.ranks ? r : 0)) * p.k + 16 * g;
   }
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    const int i = b * 16 + n;
-    const int64_t row = p.plan.order[tile.first + (i < tile.count ? i : 0)];
-    x[b] = p.x + row * p.x_stride + (X8 ? 16 : 32) * g;
-    if constexpr (X8) xs[b] = p.xs + row * p.xs_stride + g / 2;
-  }
-  const int all = (p.k + kStep - 1) / kStep;
-  const int end = min(all, int(blockIdx.y + 1) * p.part_steps);
+  const int end = min((p.k + kStep - 1) / kStep, int(blockIdx.y + 1) * p.part_steps);
   struct Set {
-    uint4 a[RT][2], x[NB][2];
-    float s[NB];
+    uint4 a[RT][2], x[2];
+    float s;
   };
   auto load = [&](Set& s, int step) {
     const int k0 = step * kStep;
@@ -153,168 +177,315 @@ __device__ void shrink(const AdapterParams& p, const Tile& tile, char* smem) {
       s.a[t][0] = in ? mi::load16(a[t] + k0) : none;
       s.a[t][1] = in ? mi::load16(a[t] + k0 + 8) : none;
     }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      if constexpr (X8) {
-        s.x[b][0] = in ? mi::load16(x[b] + k0) : none;
-        s.s[b] = in ? mi::mx8::scale_f32(xs[b][k0 / 32]) : 0.f;
-      } else {
-        s.x[b][0] = in ? mi::load16(x[b] + 2 * k0) : none;
-        s.x[b][1] = in ? mi::load16(x[b] + 2 * k0 + 16) : none;
-      }
-    }
+    s.x[0] = in ? mi::load16(x + (X8 ? 1 : 2) * k0) : none;
+    if constexpr (X8) s.s = in ? mi::mx8::scale_f32(uint8_t(xs[k0 / 32])) : 0.f;
+    else s.x[1] = in ? mi::load16(x + 2 * k0 + 16) : none;
   };
-  f32x4_t acc[RT][NB];
+  f32x4_t acc[RT][1];
 #pragma unroll
-  for (int t = 0; t < RT; ++t)
-#pragma unroll
-    for (int b = 0; b < NB; ++b) acc[t][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < RT; ++t) acc[t][0] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   Set cur, next;
   int step = int(blockIdx.y) * p.part_steps + w;
   load(cur, step);
   for (; step < end; step += kWaves) {
     load(next, step + kWaves);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        bf16x8_t v;
-        if constexpr (X8) {
-          const u32x2_t lo = mi::mx8::to_bf16(h ? cur.x[b][0].z : cur.x[b][0].x, cur.s[b]);
-          const u32x2_t hi = mi::mx8::to_bf16(h ? cur.x[b][0].w : cur.x[b][0].y, cur.s[b]);
-          v = mi::as_bf16x8(make_uint4(lo.x, lo.y, hi.x, hi.y));
-        } else {
-          v = mi::as_bf16x8(cur.x[b][h]);
-        }
-#pragma unroll
-        for (int t = 0; t < RT; ++t) acc[t][b] = mi::mfma_16x16x32_bf16(mi::as_bf16x8(cur.a[t][h]), v, acc[t][b]);
+    for (int h = 0; h < 2; ++h) {
+      bf16x8_t v;
+      if constexpr (X8) {
+        const u32x2_t lo = mi::mx8::to_bf16(h ? cur.x[0].z : cur.x[0].x, cur.s);
+        const u32x2_t hi = mi::mx8::to_bf16(h ? cur.x[0].w : cur.x[0].y, cur.s);
+        v = mi::as_bf16x8(make_uint4(lo.x, lo.y, hi.x, hi.y));
+      } else {
+        v = mi::as_bf16x8(cur.x[h]);
       }
+#pragma unroll
+      for (int t = 0; t < RT; ++t) acc[t][0] = mi::mfma_16x16x32_bf16(mi::as_bf16x8(cur.a[t][h]), v, acc[t][0]);
+    }
     cur = next;
   }
-  // Lane (g, n) holds ranks 4 g .. 4 g + 3 of a tile for row n of a block.
-  f32x4_t* const red = reinterpret_cast<f32x4_t*>(smem);
+  store_ranks<kWaves, RT, 1>(p, acc, red, tile.count, rank0);
+}
+
+// Tiles of 64 rows: as the few-row projections, a wave's rows go through a ring of its own in
+// LDS, two steps deep, eight rows of 128 bytes by an instruction (rows read as operands
+// straight from memory are 64 places an instruction, which the address unit takes one by one).
+// A step is 128 bytes of x: 64 k of bf16, 128 of 8 bits, which take two lots of A.
+template <bool X8, int RT>
+__global__ __launch_bounds__(64 * kManyWaves) void shrink_many_kernel(AdapterParams p) {
+  using namespace mi::mx8;
+  constexpr int WAVES = kManyWaves, NB = 4, LOTS = X8 ? 2 : 1, DEPTH = 2;
+  constexpr int XBYTES = NB * 2048, SLOT = XBYTES + RT * LOTS * 2048, SBYTES = X8 ? 1024 : 0;
+  constexpr int WAVE = DEPTH * SLOT + 2 * SBYTES, LOADS = SLOT / 1024;
+  static_assert(WAVES * WAVE <= 80 * 1024 && RT * NB * 1024 <= WAVE, "LDS");
+  __shared__ __attribute__((aligned(16))) char smem[WAVES * WAVE];
+  const int tiles = *p.plan.count;
+  const Tile tile = p.plan.tiles[blockIdx.x];
+  if (int(blockIdx.x) >= tiles || tile.slot < 0) return;
+  const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
+  lds_t* const lds = (lds_t*)smem + w * WAVE;
+  lds_t* const scales = lds + DEPTH * SLOT;
+  const int g = lane >> 4, n = lane & 15;
+  const int rank0 = int(blockIdx.z) * p.group_ranks, width = X8 ? p.k : 2 * p.k;  // bytes of a row of x
+  // a load: 8 rows, lane l chunk slot l % 8 of row l / 8
+  const int r8 = lane >> 3, chunk = ((lane & 7) ^ r8) * 16;
+  const char* x[2 * NB];
+#pragma unroll
+  for (int i = 0; i < 2 * NB; ++i) {
+    const int at = i * 8 + r8;
+    x[i] = p.x + int64_t(p.plan.order[tile.first + (at < tile.count ? at : 0)]) * p.x_stride + chunk;
+  }
+  const char* a[2 * RT];
+#pragma unroll
+  for (int i = 0; i < 2 * RT; ++i) {
+    const int r = rank0 + i * 8 + r8;  // (past the last rank any row will do: its sums are not kept)
+    a[i] = reinterpret_cast<const char*>(p.a + (int64_t(tile.slot) * p.ranks + (r < p.ranks ? r : 0)) * p.k) + chunk;
+  }
+  const char* const xs = X8 ? p.xs + int64_t(p.plan.order[tile.first + (lane < tile.count ? lane : 0)]) * p.xs_stride : nullptr;
+  auto dma = [&](const char* from, lds_t* to) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)const_cast<char*>(from),
+                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+#endif
+  };
+  const int steps = (width + 127) / 128, first = int(blockIdx.y) * p.part_steps, end = min(steps, first + p.part_steps);
+  // (behind the last k anything readable: it meets zeros, below)
+  auto load = [&](int step, int slot) {
+    lds_t* const to = lds + slot * SLOT;
+    const int off = step < end ? step * 128 : 0;
+    const int xo = off + chunk < width ? off : 0;
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) dma(x[i] + xo, to + i * 1024);
+#pragma unroll
+    for (int l = 0; l < LOTS; ++l) {
+      const int ao = off * LOTS + l * 128;
+#pragma unroll
+      for (int i = 0; i < 2 * RT; ++i) dma(a[i] + (ao + chunk < 2 * p.k ? ao : 0), to + XBYTES + (l * 2 * RT + i) * 1024);
+    }
+  };
+  // (8 bits: the scale bytes of four steps, 16 a row; a wave takes groups of four in turn)
+  auto load_scales = [&](int quad) { dma(xs + (quad * 512 < p.k ? quad * 16 : 0), scales + (quad / WAVES & 1) * SBYTES); };
+  auto step_at = [&](int i) { return X8 ? first + 4 * (w + i / 4 * WAVES) + i % 4 : first + w + i * WAVES; };
+  const int lo = n * 128 + (g ^ (n & 7)) * 16, hi = n * 128 + ((4 + g) ^ (n & 7)) * 16;
+  const int even = n * 128 + ((2 * g) ^ (n & 7)) * 16, odd = n * 128 + ((2 * g + 1) ^ (n & 7)) * 16;
+
+  f32x4_t acc[RT][NB];
 #pragma unroll
   for (int t = 0; t < RT; ++t)
 #pragma unroll
-    for (int b = 0; b < NB; ++b) red[(w * RT * NB + t * NB + b) * 64 + lane] = acc[t][b];
-  __syncthreads();
-  for (int q = w; q < RT * NB; q += kWaves) {
-    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int o = 0; o < kWaves; ++o) sum += red[(o * RT * NB + q) * 64 + lane];
-    const int row = q % NB * 16 + n, r = rank0 + q / NB * 16 + 4 * g;
-    if (row < tile.count && r < p.padded)
-      *reinterpret_cast<f32x4_t*>(p.parts + ((int64_t(blockIdx.y) * p.max_tiles + blockIdx.x) * kTile + row) * p.padded + r) = sum;
+    for (int b = 0; b < NB; ++b) acc[t][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  constexpr int kInFlight = (DEPTH - 1) * LOADS;
+  static_assert(kInFlight < 64, "vmcnt");
+  const int quad0 = first / 4 + w;
+  if constexpr (X8) {
+    load_scales(quad0);
+    load_scales(quad0 + WAVES);
   }
+#pragma unroll
+  for (int i = 0; i < DEPTH; ++i) load(step_at(i), i);
+  for (int i = 0; X8 ? step_at(i & ~3) < end : step_at(i) < end; i += DEPTH) {
+    if constexpr (X8) {  // (a group ahead: done by the waits before it)
+      if (i && (i & 3) == 0) load_scales(quad0 + (i / 4 + 1) * WAVES);
+    }
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const int step = step_at(i + d);
+      __builtin_amdgcn_s_waitcnt(0x0f70 | (kInFlight & 15) | (kInFlight >> 4 << 14));
+      __builtin_amdgcn_sched_barrier(0);
+      const lds_t* const xl = lds + d * SLOT;
+      const lds_t* const al = xl + XBYTES;
+      u32x4_t v[NB][2], f[LOTS][RT][2];
+      float s[NB][2];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        v[b][0] = lds_load16(xl + b * 2048 + lo);
+        v[b][1] = lds_load16(xl + b * 2048 + hi);
+        if constexpr (X8) {
+          const lds_t* const sl = scales + (((first / 4 + w + i / 4 * WAVES) / WAVES) & 1) * SBYTES + (b * 16 + n) * 16 + (i + d) % 4 * 4;
+          s[b][0] = scale_f32(lds_load1(sl + g / 2));
+          s[b][1] = scale_f32(lds_load1(sl + 2 + g / 2));
+        }
+      }
+#pragma unroll
+      for (int l = 0; l < LOTS; ++l)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          f[l][t][0] = lds_load16(al + (l * RT + t) * 2048 + (X8 ? even : lo));
+          f[l][t][1] = lds_load16(al + (l * RT + t) * 2048 + (X8 ? odd : hi));
+        }
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // read: the place may be filled again
+      __builtin_amdgcn_sched_barrier(0);
+      load(step_at(i + d + DEPTH), d);
+      // the operands' k of x's two chunks; A's behind the last k (and in no step) are made zeros
+      const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool in = step < end && step * 128 + h * 64 + g * 16 < width;
+#pragma unroll
+        for (int l = 0; l < LOTS; ++l) {
+          bf16x8_t u[NB];
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            uint4 q = __builtin_bit_cast(uint4, v[b][h]);
+            if constexpr (X8) {
+              const u32x2_t c = to_bf16(l ? q.z : q.x, s[b][h]), d2 = to_bf16(l ? q.w : q.y, s[b][h]);
+              q = make_uint4(c.x, c.y, d2.x, d2.y);
+            }
+            u[b] = mi::as_bf16x8(in ? q : none);
+          }
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            // 8 bits: chunk h of x is lot h of A, its halves A's even and odd chunks
+            const u32x4_t fa = X8 ? f[X8 ? h : 0][t][l] : f[0][t][h];
+            const bf16x8_t m = mi::as_bf16x8(in ? __builtin_bit_cast(uint4, fa) : none);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) acc[t][b] = mi::mfma_16x16x32_bf16(m, u[b], acc[t][b]);
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0x0070);  // (the loads past the end write to LDS)
+  __syncthreads();
+  store_ranks<WAVES, RT, NB>(p, acc, reinterpret_cast<f32x4_t*>(smem), tile.count, rank0);
 }
 
-template <bool X8, int RT>
-__global__ __launch_bounds__(64 * kWaves) void shrink_kernel(AdapterParams p) {
-  __shared__ __attribute__((aligned(16))) char smem[kWaves * RT * (kTile / 16) * 1024];
-  if (int(blockIdx.x) >= *p.plan.count) return;
-  const Tile tile = p.plan.tiles[blockIdx.x];
-  if (tile.slot < 0) return;
-  if (tile.count <= 16) shrink<X8, RT, 1>(p, tile, smem);
-  else shrink<X8, RT, kTile / 16>(p, tile, smem);
-}
-
-// J: products of 32 that a piece's pairs of ranks take.
-template <int J>
+// out = y + B v of a tile of 16 NB rows and a chunk of columns.  J: products of 32 that the
+// pairs of a piece's ranks take.  A unit of work is 16 rows by 128 columns, eight products
+// side by side: column c of product t is column 8 c + t of the unit, so that lane (g, n) ends with
+// columns 8 n .. 8 n + 7 of rows 4 g .. 4 g + 3, 16 bytes of y and out in the order of the lanes.
+template <int NB, int J>
 __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
-  constexpr int kMaxPair = 4 * J * 8;  // pairs of bf16 of a row, side by side: the roundings, then what they left
-  __shared__ __attribute__((aligned(16))) uint16_t vs[kTile * (kMaxPair + 8)];
-  if (int(blockIdx.x) >= *p.plan.count) return;
+  constexpr int ROWS = 16 * NB, kPair = 32 * J;  // a row's ranks in bf16, and what the rounding left of them
+  constexpr int VSTRIDE = kPair + 8;              // (the rows of an operand on distinct banks)
+  constexpr int kMaxWeights = 128 * (kPair / 2) + 128;  // a unit's columns of B: eight of them, then 16 bytes apart
+  __shared__ __attribute__((aligned(16))) uint16_t vs[ROWS * VSTRIDE];
+  __shared__ __attribute__((aligned(16))) uint16_t ws[2][kMaxWeights];
+  const int tiles = *p.plan.count;
   const Tile tile = p.plan.tiles[blockIdx.x];
-  if (tile.slot < 0 && p.out == p.y) return;
+  if (int(blockIdx.x) >= tiles || (tile.slot < 0 && p.out == p.y)) return;
+  const bool adds = tile.slot >= 0;
   int piece = 0;
   while (int(blockIdx.y) >= p.end_chunk[piece]) ++piece;
   const int begin = piece ? p.end[piece - 1] : 0, before = piece ? p.end_chunk[piece - 1] : 0;
   const int c0 = begin + (int(blockIdx.y) - before) * p.chunk, c1 = min(c0 + p.chunk, p.end[piece]);
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int g = lane >> 4, n = lane & 15;
-  const int stride = kMaxPair + 8;  // (the rows of an operand on distinct banks)
-  const int nb = (tile.count + 15) / 16;
-  if (tile.slot >= 0) {
+  const int nb = (tile.count + 15) / 16, groups = (c1 - c0 + 127) / 128;
+  const int eighths = p.rank / 8;
+  const uint16_t* const weights = p.b + int64_t(max(tile.slot, 0)) * p.n * p.rank;
+
+  // the weights of a unit's 128 columns, 16 bytes a thread and lot
+  constexpr int LOTS = (128 * (kPair / 2) / 8 + 64 * kWaves - 1) / (64 * kWaves);
+  uint4 wv[LOTS];
+  auto fetch = [&](int group) {
+#pragma unroll
+    for (int i = 0; i < LOTS; ++i) {
+      const int e = i * 64 * kWaves + tid, col = c0 + group * 128 + e / eighths;
+      wv[i] = adds && e < 128 * eighths && col < c1 ? mi::load16(weights + int64_t(col) * p.rank + e % eighths * 8)
+                                                    : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  auto keep = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < LOTS; ++i) {
+      const int e = i * 64 * kWaves + tid, col = e / eighths;
+      if (e < 128 * eighths) mi::store16(ws[buf] + col * p.rank + col / 8 * 8 + e % eighths * 8, wv[i]);
+    }
+  };
+  fetch(0);
+  // wave w takes row block w
+  struct Rows {
+    uint4 y[4];
+  };
+  int64_t row[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = w * 16 + 4 * g + i;
+    row[i] = w < nb ? p.plan.order[tile.first + (at < tile.count ? at : 0)] : 0;
+  }
+  auto load_rows = [&](Rows& r, int col) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r.y[i] = w < nb && col < c1 ? mi::load16_nt(p.y + row[i] * p.y_stride + col) : make_uint4(0u, 0u, 0u, 0u);
+  };
+  Rows rows, next_rows;
+  load_rows(rows, c0 + 8 * n);
+  if (adds) {
     const float scale = p.scale[tile.slot];
     const int fours = p.rank / 4;
-    const int64_t part = int64_t(p.max_tiles) * kTile * p.padded;
+    const int64_t part = int64_t(p.max_tiles) * ROWS * p.padded;
     for (int i = tid; i < tile.count * fours; i += 64 * kWaves) {
       const int row = i / fours, r = i % fours * 4;
-      const float* const from = p.parts + (int64_t(blockIdx.x) * kTile + row) * p.padded + piece * p.rank + r;
-      f32x4_t sum = *reinterpret_cast<const f32x4_t*>(from);
-      for (int o = 1; o < p.n_parts; ++o) sum += *reinterpret_cast<const f32x4_t*>(from + o * part);
+      const float* const from = p.parts + (int64_t(blockIdx.x) * ROWS + row) * p.padded + piece * p.rank + r;
+      f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+      auto add = [&](int first) {  // eight on their way at once, added in their order
+        f32x4_t v[8];
+#pragma unroll
+        for (int o = 0; o < 8; ++o)
+          v[o] = first + o < p.n_parts ? *reinterpret_cast<const f32x4_t*>(from + (first + o) * part) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int o = 0; o < 8; ++o) sum += v[o];
+      };
+      static_assert(kMaxParts == 16);
+      add(0);
+      if (p.n_parts > 8) add(8);
       uint32_t hi[2], lo[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float u = sum[2 * j] * scale, v = sum[2 * j + 1] * scale;
-        hi[j] = mi::cvt_pk_bf16(u, v);
-        const float du = u - mi::bf16_lo(hi[j]), dv = v - mi::bf16_hi(hi[j]);
+        const float s = sum[2 * j] * scale, t = sum[2 * j + 1] * scale;
+        hi[j] = mi::cvt_pk_bf16(s, t);
+        const float ds = s - mi::bf16_lo(hi[j]), dt = t - mi::bf16_hi(hi[j]);
         // (an infinity leaves nothing)
-        lo[j] = mi::cvt_pk_bf16(isfinite(mi::bf16_lo(hi[j])) ? du : 0.f, isfinite(mi::bf16_hi(hi[j])) ? dv : 0.f);
+        lo[j] = mi::cvt_pk_bf16(isfinite(mi::bf16_lo(hi[j])) ? ds : 0.f, isfinite(mi::bf16_hi(hi[j])) ? dt : 0.f);
       }
-      *reinterpret_cast<uint2*>(vs + row * stride + r) = make_uint2(hi[0], hi[1]);
-      *reinterpret_cast<uint2*>(vs + row * stride + p.rank + r) = make_uint2(lo[0], lo[1]);
+      *reinterpret_cast<uint2*>(vs + row * VSTRIDE + r) = make_uint2(hi[0], hi[1]);
+      *reinterpret_cast<uint2*>(vs + row * VSTRIDE + p.rank + r) = make_uint2(lo[0], lo[1]);
     }
-    __syncthreads();
   }
-  const int eighths = p.rank / 8;
   int from[J];  // of a lane's eight ranks of product j, -1: past the last pair
 #pragma unroll
   for (int j = 0; j < J; ++j) from[j] = 4 * j + g < 2 * eighths ? (4 * j + g) % eighths * 8 : -1;
-  int64_t row[kTile / 16];
-#pragma unroll
-  for (int b = 0; b < kTile / 16; ++b) {
-    const int i = b * 16 + n;
-    row[b] = p.plan.order[tile.first + (i < tile.count ? i : 0)];
-  }
-  const uint16_t* const weights = p.b + int64_t(max(tile.slot, 0)) * p.n * p.rank;
-  for (int c = c0 + w * 32; c < c1; c += 32 * kWaves) {  // two tiles of 16 columns
-    const int col = c + (g & 1) * 16 + (g >> 1) * 8;
-    const bool mine = col < c1;
-    uint4 yv[kTile / 16];
-#pragma unroll
-    for (int b = 0; b < kTile / 16; ++b)
-      if (b < nb && mine) yv[b] = mi::load16_nt(p.y + row[b] * p.y_stride + col);
-    bf16x8_t wt[2][J];
-    if (tile.slot >= 0) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int r = c + 16 * t + n;  // (the second tile may lie past the piece: not kept)
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-          wt[t][j] = mi::as_bf16x8(from[j] >= 0 ? mi::load16(weights + int64_t(r < c1 ? r : c) * p.rank + from[j])
-                                                : make_uint4(0u, 0u, 0u, 0u));
-      }
+  for (int group = 0; group < groups; ++group) {
+    const int col = c0 + group * 128 + 8 * n, buf = group & 1;
+    keep(buf);
+    if (group + 1 < groups) {
+      fetch(group + 1);
+      load_rows(next_rows, col + 128);
     }
+    __syncthreads();
+    if (w < nb) {
+      f32x4_t d[8];
 #pragma unroll
-    for (int b = 0; b < kTile / 16; ++b) {
-      if (b >= nb) break;
-      uint4 o = yv[b];
-      if (tile.slot >= 0) {
-        f32x4_t s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      for (int t = 0; t < 8; ++t) d[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      if (adds) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-          const uint4 q = *reinterpret_cast<const uint4*>(vs + (b * 16 + n) * stride + (4 * j + g) * 8);
-          const bf16x8_t v = mi::as_bf16x8(from[j] >= 0 ? q : make_uint4(0u, 0u, 0u, 0u));
-          s[0] = mi::mfma_16x16x32_bf16(wt[0][j], v, s[0]);
-          s[1] = mi::mfma_16x16x32_bf16(wt[1][j], v, s[1]);
-        }
-        // Lane (g, n) holds columns 4 g .. 4 g + 3 of either tile; lanes change places, so that
-        // each has eight columns side by side.
-        float d[8];
+          const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+          const uint4 q = *reinterpret_cast<const uint4*>(vs + (w * 16 + n) * VSTRIDE + (4 * j + g) * 8);
+          const bf16x8_t v = mi::as_bf16x8(from[j] >= 0 ? q : none);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const auto e = __builtin_amdgcn_permlane16_swap(__float_as_uint(s[0][i]), __float_as_uint(s[1][i]), false, false);
-          d[i] = __uint_as_float(e[0]);
-          d[4 + i] = __uint_as_float(e[1]);
+          for (int t = 0; t < 8; ++t) {
+            const int at = (8 * n + t) * p.rank + n * 8 + (from[j] >= 0 ? from[j] : 0);
+            const uint4 m = *reinterpret_cast<const uint4*>(ws[buf] + at);
+            d[t] = mi::mfma_16x16x32_bf16(v, mi::as_bf16x8(from[j] >= 0 ? m : none), d[t]);
+          }
         }
-        o.x = mi::cvt_pk_bf16(mi::bf16_lo(o.x) + d[0], mi::bf16_hi(o.x) + d[1]);
-        o.y = mi::cvt_pk_bf16(mi::bf16_lo(o.y) + d[2], mi::bf16_hi(o.y) + d[3]);
-        o.z = mi::cvt_pk_bf16(mi::bf16_lo(o.z) + d[4], mi::bf16_hi(o.z) + d[5]);
-        o.w = mi::cvt_pk_bf16(mi::bf16_lo(o.w) + d[6], mi::bf16_hi(o.w) + d[7]);
       }
-      if (mine && b * 16 + n < tile.count) mi::store16(p.out + row[b] * p.o_stride + col, o);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint4 o = rows.y[i];
+        if (adds) {
+          o.x = mi::cvt_pk_bf16(mi::bf16_lo(o.x) + d[0][i], mi::bf16_hi(o.x) + d[1][i]);
+          o.y = mi::cvt_pk_bf16(mi::bf16_lo(o.y) + d[2][i], mi::bf16_hi(o.y) + d[3][i]);
+          o.z = mi::cvt_pk_bf16(mi::bf16_lo(o.z) + d[4][i], mi::bf16_hi(o.z) + d[5][i]);
+          o.w = mi::cvt_pk_bf16(mi::bf16_lo(o.w) + d[6][i], mi::bf16_hi(o.w) + d[7][i]);
+        }
+        if (col < c1 && w * 16 + 4 * g + i < tile.count) mi::store16(p.out + row[i] * p.o_stride + col, o);
+      }
     }
+    rows = next_rows;
   }
 }
 
@@ -332,17 +503,49 @@ int check_shape(const char* name, int64_t rows, int64_t slots, int64_t k, int64_
   return MI_OK;
 }
 
-int parts_of(int64_t tiles, int64_t k, int64_t groups) {
-  const int64_t steps = (k + kStep - 1) / kStep, most = std::min<int64_t>(kMaxParts, (steps + kWaves - 1) / kWaves);
-  const int64_t want = (2 * mi::num_cus() + tiles * groups - 1) / (tiles * groups);
-  return int(std::max<int64_t>(1, std::min(most, want)));
+// How a shrink launch shares k.  `steps` of a wave and `part_steps` of a workgroup are of 64 k,
+// or of 128 bytes of x in tiles of 64 rows, whose workgroups share a CU by two.
+struct Split {
+  int64_t tiles;
+  int groups, parts, part_steps;
+  size_t bytes;
+};
+Split split_of(int64_t rows, int64_t slots, int64_t k, int64_t padded, bool x8) {
+  Split s;
+  const bool many = tile_rows(rows) == 64;
+  const int64_t cus = mi::num_cus(), rank_tiles = padded / 16;
+  const int64_t width = many && x8 ? 128 : kStep, unit = many && x8 ? 4 : 1;
+  const int64_t steps = (k + width - 1) / width, waves = many ? kManyWaves : kWaves;
+  const int64_t each = (steps + unit * waves - 1) / (unit * waves) * unit;
+  int64_t best = 1, group = many && x8 ? kGroup / 2 : kGroup;
+  s.tiles = max_tiles(rows, slots);
+  if (!many) {
+    // two steps a wave at least; then ranks apart, until every CU has two workgroups (32 rows, 8
+    // adapters of rank 64, k 14,336: 4 rank tiles a workgroup 8.0 us, one 7.1)
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxParts, (each + 1) / 2));
+    while (group > 1 && s.tiles * ((rank_tiles + group - 1) / group) * most < 2 * cus) group /= 2;
+    s.groups = int((rank_tiles + group - 1) / group);
+    best = std::max<int64_t>(1, std::min<int64_t>(most, (2 * cus + s.tiles * s.groups - 1) / (s.tiles * s.groups)));
+  } else {
+    s.groups = int((rank_tiles + group - 1) / group);
+    int64_t least = INT64_MAX;  // rounds of workgroups, of their steps and a start of twelve
+    for (int64_t parts = 1; parts <= std::min<int64_t>(kMaxParts, each / unit); ++parts) {
+      const int64_t rounds = (s.tiles * s.groups * parts + 2 * cus - 1) / (2 * cus), cost = rounds * ((each + parts - 1) / parts + 12);
+      if (cost < least) least = cost, best = parts;
+    }
+  }
+  s.part_steps = int(((steps + best - 1) / best + unit - 1) / unit * unit);
+  s.parts = int((steps + s.part_steps - 1) / s.part_steps);
+  s.bytes = size_t(s.parts) * size_t(s.tiles) * tile_rows(rows) * size_t(padded) * 4;
+  return s;
 }
 
 }  // namespace
 
 extern "C" size_t mi_adapter_plan_size(int64_t rows, int64_t slots) {
   if (check_plan("adapter_plan_size", rows, slots)) return 0;
-  return 16 + 16 * size_t(max_tiles(rows, slots)) + 4 * size_t(rows);
+  // (of fewer rows too: those in tiles of 16 may take more)
+  return std::max(plan_size(rows, slots), plan_size(std::min(rows, kFewRows), slots));
 }
 
 extern "C" int mi_adapter_plan(void* plan, size_t plan_bytes, const int32_t* slot_of_row, int64_t rows, int64_t slots,
@@ -354,21 +557,20 @@ extern "C" int mi_adapter_plan(void* plan, size_t plan_bytes, const int32_t* slo
   if (!plan || !slot_of_row) return mi::fail(MI_ERR_INVALID, "%s: null pointer argument", name);
   if ((reinterpret_cast<uintptr_t>(plan) & 15) || (reinterpret_cast<uintptr_t>(slot_of_row) & 3))
     return mi::fail(MI_ERR_INVALID, "%s: the plan must be 16-byte aligned, the slots 4-byte", name);
-  const size_t need = mi_adapter_plan_size(rows, slots);
+  const size_t need = plan_size(rows, slots);
   if (plan_bytes < need)
     return mi::fail(MI_ERR_WORKSPACE, "%s: the plan takes %zu bytes, %zu given", name, need, plan_bytes);
   const mi::Rows to = {plan, 0, 1, int64_t(need)}, from = {slot_of_row, 0, 1, rows * 4};
   if (mi::rows_meet(to, from)) return mi::fail(MI_ERR_INVALID, "%s: the plan overlaps the slots", name);
   hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 0, static_cast<hipStream_t>(stream), slot_of_row, int(rows),
-                     int(slots), view(plan, rows, slots));
+                     int(slots), tile_rows(rows), view(plan, rows, slots));
   return mi::check_launch(name);
 }
 
 extern "C" size_t mi_add_adapters_workspace_size(int64_t rows, int64_t slots, int64_t k, int64_t rank, int64_t pieces) {
   if (check_shape("add_adapters_workspace_size", rows, slots, k, rank, pieces) || rows == 0) return 0;
-  const int64_t tiles = max_tiles(rows, slots), padded = (pieces * rank + 15) / 16 * 16;
-  const int64_t groups = (padded / 16 + kGroup - 1) / kGroup;
-  return size_t(parts_of(tiles, k, groups)) * size_t(tiles) * kTile * size_t(padded) * 4;
+  const int64_t padded = (pieces * rank + 15) / 16 * 16;
+  return std::max(split_of(rows, slots, k, padded, false).bytes, split_of(rows, slots, k, padded, true).bytes);
 }
 
 extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, int64_t x_stride, const void* x_scales,
@@ -390,21 +592,23 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
   }
   if (rows == 0) return MI_OK;
   const int64_t each = x_scales ? 1 : 2;
-  if (rows == 1) y_stride = out_stride = n, x_stride = (k + 15) & ~int64_t(15), x_scales_stride = k / 32;
+  const int64_t scale_bytes = (k / 32 + 15) & ~int64_t(15);
+  if (rows == 1) y_stride = out_stride = n, x_stride = (k + 15) & ~int64_t(15), x_scales_stride = scale_bytes;
   if (!y || !x || !a || !b || !scale || !out || !plan || !workspace)
     return mi::fail(MI_ERR_INVALID, "%s: null pointer argument", name);
   const uintptr_t aligned = reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(a) |
                             reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(out) |
-                            reinterpret_cast<uintptr_t>(plan) | reinterpret_cast<uintptr_t>(workspace);
-  if ((aligned & 15) || ((y_stride | out_stride) & 7) || (x_stride * each) % 16 || (reinterpret_cast<uintptr_t>(scale) & 3))
+                            reinterpret_cast<uintptr_t>(plan) | reinterpret_cast<uintptr_t>(workspace) |
+                            reinterpret_cast<uintptr_t>(x_scales);
+  if ((aligned & 15) || ((y_stride | out_stride) & 7) || (x_scales && x_scales_stride % 16) || (x_stride * each) % 16 || (reinterpret_cast<uintptr_t>(scale) & 3))
     return mi::fail(MI_ERR_INVALID, "%s: rows, factors, plan and workspace must be 16-byte aligned", name);
-  if (out_stride < n || x_stride < 0 || y_stride < 0 || x_scales_stride < 0)
+  if (out_stride < n || x_stride < 0 || y_stride < 0 || (x_scales && x_scales_stride < scale_bytes))
     return mi::fail(MI_ERR_INVALID, "%s: row strides %lld, %lld, %lld, %lld for %lld columns", name, (long long)y_stride,
                     (long long)x_stride, (long long)x_scales_stride, (long long)out_stride, (long long)n);
-  const int64_t tiles = max_tiles(rows, slots), padded = (pieces * rank + 15) / 16 * 16;
-  const int groups = int((padded / 16 + kGroup - 1) / kGroup);
-  const int parts = parts_of(tiles, k, groups);
-  const size_t need = size_t(parts) * size_t(tiles) * kTile * size_t(padded) * 4;
+  const int64_t padded = (pieces * rank + 15) / 16 * 16;
+  const Split split = split_of(rows, slots, k, padded, x_scales != nullptr);
+  const int64_t tiles = split.tiles;
+  const size_t need = split.bytes;
   if (workspace_bytes < need)
     return mi::fail(MI_ERR_WORKSPACE, "%s: the workspace takes %zu bytes, %zu given", name, need, workspace_bytes);
   // (rows of out are written while others are still read; a row of y only by who writes it)
@@ -416,13 +620,13 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
                            {a, 0, 1, slots * pieces * rank * k * 2},
                            {b, 0, 1, slots * n * rank * 2},
                            {scale, 0, 1, slots * 4},
-                           {plan, 0, 1, int64_t(mi_adapter_plan_size(rows, slots))},
+                           {plan, 0, 1, int64_t(plan_size(rows, slots))},
                            {workspace, 0, 1, int64_t(need)}};
   for (const mi::Rows& r : from)
     if (mi::rows_meet(to, r)) return mi::fail(MI_ERR_INVALID, "%s: out overlaps another argument (it may be y itself)", name);
   p.x = static_cast<const char*>(x);
   p.x_stride = x_stride * each;
-  p.xs = static_cast<const uint8_t*>(x_scales);
+  p.xs = static_cast<const char*>(x_scales);
   p.xs_stride = x_scales_stride;
   p.a = static_cast<const uint16_t*>(a);
   p.b = static_cast<const uint16_t*>(b);
@@ -440,23 +644,29 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
   p.padded = int(padded);
   p.max_tiles = int(tiles);
   p.pieces = int(pieces);
-  const int steps = int((k + kStep - 1) / kStep);
-  p.part_steps = (steps + parts - 1) / parts;
-  p.n_parts = (steps + p.part_steps - 1) / p.part_steps;
+  p.part_steps = split.part_steps;
+  p.n_parts = split.parts;
+  p.group_ranks = int(((padded / 16 + split.groups - 1) / split.groups) * 16);
   // columns of a workgroup: few where there are few tiles, so that every CU has some
   p.chunk = 128;
   while (p.chunk < 1024 && tiles * ((n + p.chunk - 1) / p.chunk) > 8 * mi::num_cus()) p.chunk *= 2;
   int chunks = 0;
   for (int i = 0; i < pieces; ++i) p.end_chunk[i] = chunks += (piece_columns[i] + p.chunk - 1) / p.chunk;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid(uint32_t(tiles), uint32_t(p.n_parts), uint32_t(groups)), block(64 * kWaves);
-  const int rt = int(std::min<int64_t>(padded / 16, kGroup));
-  const auto shrink = p.xs ? (rt == 1 ? shrink_kernel<true, 1> : rt == 2 ? shrink_kernel<true, 2>
-                              : rt == 3 ? shrink_kernel<true, 3> : shrink_kernel<true, 4>)
-                           : (rt == 1 ? shrink_kernel<false, 1> : rt == 2 ? shrink_kernel<false, 2>
-                              : rt == 3 ? shrink_kernel<false, 3> : shrink_kernel<false, 4>);
-  hipLaunchKernelGGL(shrink, grid, block, 0, s, p);
-  const auto expand = rank <= 16 ? expand_kernel<1> : rank <= 32 ? expand_kernel<2> : rank <= 64 ? expand_kernel<4> : expand_kernel<8>;
-  hipLaunchKernelGGL(expand, dim3(uint32_t(tiles), uint32_t(chunks)), block, 0, s, p);
+  const dim3 grid(uint32_t(tiles), uint32_t(p.n_parts), uint32_t(split.groups)), block(64 * kWaves);
+  const int rt = p.group_ranks / 16;
+  const bool x8 = p.xs != nullptr, many = tile_rows(rows) == 64;
+  using Kernel = void (*)(AdapterParams);
+  const Kernel few[2][kGroup] = {
+      {shrink_few_kernel<false, 1>, shrink_few_kernel<false, 2>, shrink_few_kernel<false, 3>, shrink_few_kernel<false, 4>},
+      {shrink_few_kernel<true, 1>, shrink_few_kernel<true, 2>, shrink_few_kernel<true, 3>, shrink_few_kernel<true, 4>}};
+  const Kernel wide[2][kGroup] = {
+      {shrink_many_kernel<false, 1>, shrink_many_kernel<false, 2>, shrink_many_kernel<false, 3>, shrink_many_kernel<false, 4>},
+      {shrink_many_kernel<true, 1>, shrink_many_kernel<true, 2>, nullptr, nullptr}};
+  hipLaunchKernelGGL((many ? wide : few)[x8][rt - 1], grid, dim3(64 * (many ? kManyWaves : kWaves)), 0, s, p);
+  const int j = rank <= 16 ? 0 : rank <= 32 ? 1 : rank <= 64 ? 2 : 3;
+  const Kernel expand[2][4] = {{expand_kernel<1, 1>, expand_kernel<1, 2>, expand_kernel<1, 4>, expand_kernel<1, 8>},
+                               {expand_kernel<4, 1>, expand_kernel<4, 2>, expand_kernel<4, 4>, expand_kernel<4, 8>}};
+  hipLaunchKernelGGL(expand[many][j], dim3(uint32_t(tiles), uint32_t(chunks)), block, 0, s, p);
   return mi::check_launch(name);
 }

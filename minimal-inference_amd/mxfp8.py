@@ -69,6 +69,18 @@ class MXFP8:
         self.codes_ptr = self.anchor.data_ptr()
         self.scales_ptr = self.codes_ptr + rows * cols
 
+    @classmethod
+    def _room(cls, rows: int, cols: int, device) -> "MXFP8":
+        """``MXFP8(rows, cols, device)`` of sizes that an entry has checked or will."""
+        m = cls.__new__(cls)
+        m.rows, m.cols, m.device, m._held = rows, cols, device, None
+        m.codes_stride = cols
+        stride = m.scales_stride = (cols + 511 >> 9) * _PIECE
+        m.anchor = torch.empty(rows * (cols + stride), dtype=torch.uint8, device=device)
+        m.codes_ptr = at = m.anchor.data_ptr()
+        m.scales_ptr = at + rows * cols
+        return m
+
     @property
     def shape(self) -> tuple[int, int]:
         return self.rows, self.cols
@@ -144,7 +156,9 @@ def _check_codes(codes: torch.Tensor, scales: torch.Tensor) -> tuple[torch.Tenso
 
 def _rows8(out: "MXFP8 | None", rows: int, cols: int, device) -> MXFP8:
     if out is None:
-        return MXFP8(rows, cols, device)
+        if cols % BLOCK or cols <= 0 or cols > 1 << 20:
+            raise ValueError(f"an MXFP8 matrix has columns in blocks of {BLOCK}, at most 2^20; got [{rows}, {cols}]")
+        return MXFP8._room(rows, cols, device)
     if not isinstance(out, MXFP8) or out.shape != (rows, cols) or out.device != device:
         raise ValueError(f"out must be an MXFP8 matrix [{rows}, {cols}] on {device}")
     return out
@@ -166,19 +180,28 @@ def add_rms_norm_mxfp8(x: torch.Tensor, delta: torch.Tensor | None, weight: torc
     in place in ``x`` when that is not given; without ``delta`` x itself, which is then not written),
     and its ``rms_norm(...) * weight`` in fp32, quantised from there as ``quantize_mxfp8`` does.
     Outputs that overlap each other, the weight or another row's input are refused."""
-    rows, hidden = _rows_of("x", x)
-    device = x.device
+    shape, grad = x.shape, torch.is_grad_enabled()
+    if len(shape) != 2:
+        raise ValueError(f"x must be [rows, hidden]; got {tuple(shape)}")
+    rows, hidden = shape
     if hidden > 16384:  # (the entry takes 32 bits of it)
         raise ValueError(f"hidden is {hidden}: multiples of {BLOCK} up to 16384")
+    at, device = x.get_device(), x.device
+    if (x.dtype != torch.bfloat16 or at < 0 or x.stride(1) != 1 or (grad and x.requires_grad)):
+        _rows_of("x", x)
     for name, t in (("delta", delta), ("x_out", x_out)):
-        if t is not None and (_rows_of(name, t) != (rows, hidden) or t.device != device):
+        if t is not None and (t.shape != shape or t.dtype != torch.bfloat16 or t.get_device() != at or t.stride(1) != 1
+                              or (grad and t.requires_grad)):
+            _rows_of(name, t)
             raise ValueError(f"{name} must be [{rows}, {hidden}] on {device}; got {tuple(t.shape)} on {t.device}")
-    require_gpu("weight", weight)
-    require_dtype("weight", weight, torch.bfloat16)
-    if weight.shape != (hidden,) or weight.stride(0) != 1 or weight.device != device:
-        raise ValueError(f"weight must be a contiguous [{hidden}] tensor on {device}")
-    if weight.requires_grad or forward_ad._current_level >= 0:
+    if (weight.shape != (hidden,) or weight.dtype != torch.bfloat16 or weight.get_device() != at or weight.stride(0) != 1
+            or (grad and weight.requires_grad)):
         refuse_derivatives("weight", weight)
+        raise ValueError(f"weight must be a contiguous bfloat16 [{hidden}] tensor on {device}; got {tuple(weight.shape)} "
+                         f"{weight.dtype} on {weight.device}")
+    if forward_ad._current_level >= 0:
+        for name, t in (("x", x), ("delta", delta), ("weight", weight), ("x_out", x_out)):
+            refuse_derivatives(name, t)
     if x_out is None and delta is not None:
         x_out = x
     out = _rows8(out, rows, hidden, device)

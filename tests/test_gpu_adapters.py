@@ -61,7 +61,8 @@ def _want(values, ad, slot, y):
 @pytest.mark.parametrize("k,pieces,rank", [(32, [16], 8), (96, [48, 16], 16), (896, [896, 128, 128], 16), (1056, [304], 24),
                                            (544, [64, 32, 16], 64), (4864, [896], 32), (256, [160, 160], 128),
                                            (160, [16] * 8, 8)])
-@pytest.mark.parametrize("rows,slots", [(1, 1), (3, 5), (17, 2), (64, 1), (65, 1), (130, 7), (300, 40)])
+@pytest.mark.parametrize("rows,slots", [(1, 1), (3, 5), (17, 2), (64, 1), (130, 7), (300, 40), (512, 3), (513, 3), (1000, 1),
+                                        (900, 30)])
 def test_add_adapters(dev, rows, slots, k, pieces, rank, x8):
     """Odd numbers of rows and adapters, rows without one among them; in place and into an out, whose
     surroundings stay; strided rows."""
@@ -111,7 +112,8 @@ def test_plan_lists_every_row_once(dev):
         if rows == 0:
             assert int(words[0]) == 0
             continue
-        most = min(rows, slots + 1) + rows // 64
+        height = 16 if rows <= 512 else 64
+        most = min(rows, slots + 1) + rows // height
         order = words[4 + 4 * most:]
         assert torch.equal(order.sort()[0], torch.arange(rows, dtype=torch.int32))
         tiles = words[4: 4 + 4 * int(words[0])].view(-1, 4)
@@ -120,7 +122,7 @@ def test_plan_lists_every_row_once(dev):
         for s, first, count, _ in tiles.tolist():
             mine = slot[order[first: first + count].long()]
             own = (mine == s) if s >= 0 else (mine < 0) | (mine >= slots)
-            assert 0 < count <= 64 and first == seen and bool(own.all())
+            assert 0 < count <= height and first == seen and bool(own.all())
             seen += count
         assert seen == rows
 
