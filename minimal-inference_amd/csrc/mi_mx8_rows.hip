@@ -5,8 +5,10 @@
 //              the e4m3 value nearest to x / u (ties to even), scale byte log2 u + 127, at
 //              least 0.  A block that holds an infinity or a NaN gets byte 255, the
 //              format's NaN, and zero codes: all of it reads back as NaN.
-//   add_rms  : x' = bf16(x + d), stored when asked; h = x' rsqrt(mean(x'^2) + eps) w in
-//              fp32, quantised from there: one rounding between the norm and the code.
+//   add_rms  : x' = bf16(x + d), stored when asked; h = x' rsqrt(mean(x'^2) + eps) w, quantised.
+//              The sum and the root are taken in 64 bits and the product x' w (exact in
+//              fp32) times the root is rounded to odd, so that the codes are those of the exact
+//              norm (in fp32 alone some 4e-7 of them fall on the other side of a border).
 //
 // Bound: HBM.  add_rms reads x and d once, writes x' and 1.03 bytes of h per element.
 #include "mi_mx8.h"
@@ -91,12 +93,38 @@ struct AddRmsParams {
   float eps;
 };
 
+// Sum over the wave in 64 bits; every lane gets it.
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u)), CTRL, 0xf, 0xf, false));
+  const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u >> 32)), CTRL, 0xf, 0xf, false));
+  return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+  v += dpp<mi::kDppQuadSwap1>(v);
+  v += dpp<mi::kDppQuadSwap2>(v);
+  v += dpp<mi::kDppRowHalfMirror>(v);
+  v += dpp<mi::kDppRowMirror>(v);
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// a (hi + lo), rounded to odd: cut, with the last bit set where something was cut off.  Rounded
+// again to the four bits of a code this is the exact product's rounding.  So is a hi rounded to
+// nearest, unless that lies halfway between two codes, with 19 zeros behind its leading bits.
+__device__ __forceinline__ float product_to_odd(float a, float hi, float lo) {
+  const float h = a * hi, rest = fmaf(a, lo, fmaf(a, hi, -h));
+  const uint32_t u = __float_as_uint(h);
+  return rest == 0.f ? h : __uint_as_float((u - ((u ^ __float_as_uint(rest)) >> 31)) | 1u);
+}
+
 // One workgroup per row, CH 16-byte chunks per thread; every load of the row is issued
 // before anything is computed, all of it is read before any of it is written (x_out may
 // lie over x or delta), and the row stays in registers between the sum of squares and the codes.
 template <int CH>
 __global__ __launch_bounds__(kMaxThreads) void add_rms_kernel(AddRmsParams p) {
-  __shared__ float red[kMaxThreads / 64];
+  __shared__ double red[kMaxThreads / 64];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, nt = blockDim.x, nch = p.hidden / 8;
   uint4 xv[CH], dv[CH], wv[CH];
@@ -111,44 +139,63 @@ __global__ __launch_bounds__(kMaxThreads) void add_rms_kernel(AddRmsParams p) {
     }
   }
   float v[CH][8];
-  float ss = 0.f;
+  uint32_t xo[CH][4];
+  double ss = 0.;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const uint32_t xw[4] = {xv[c].x, xv[c].y, xv[c].z, xv[c].w}, dw[4] = {dv[c].x, dv[c].y, dv[c].z, dv[c].w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const uint32_t o = p.delta ? mi::cvt_pk_bf16(mi::bf16_lo(xw[k]) + mi::bf16_lo(dw[k]), mi::bf16_hi(xw[k]) + mi::bf16_hi(dw[k]))
+      const uint32_t o = xo[c][k] = p.delta ? mi::cvt_pk_bf16(mi::bf16_lo(xw[k]) + mi::bf16_lo(dw[k]), mi::bf16_hi(xw[k]) + mi::bf16_hi(dw[k]))
                                  : xw[k];
       const float a = mi::bf16_lo(o), b = mi::bf16_hi(o);
       v[c][2 * k] = a;
       v[c][2 * k + 1] = b;
-      ss = fmaf(a, a, ss);
-      ss = fmaf(b, b, ss);
+      ss = fma(double(a), double(a), ss);
+      ss = fma(double(b), double(b), ss);
     }
   }
-  ss = mi::wave_sum(ss);
+  ss = wave_sum(ss);
   if ((tid & 63) == 0) red[tid >> 6] = ss;
   __syncthreads();
-  float tot = 0.f;
+  double tot = 0.;
   for (int w = 0; w < nt / 64; ++w) tot += red[w];
-  const float rstd = rsqrtf(tot / float(p.hidden) + p.eps);
+  // 1 / sqrt(m) from an estimate and a step in 64 bits, of m's mantissa where fp32 does not hold m: the
+  // row takes the power of two then
+  double m = tot / p.hidden + p.eps;
+  if (!(m > 0x1p-100 && m < 0x1p100) && m < 1e300) {
+    const int e = (__builtin_amdgcn_frexp_exp(m) - 1) & ~1;
+    m = ldexp(m, -e);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[c][k] = ldexpf(v[c][k], -e / 2);
+  }
+  const double r0 = rsqrtf(float(m)), off = fma(-m * r0, r0, 1.);
+  const double r = m < 1e300 ? fma(r0 * off, fma(0.375, off, 0.5), r0) : r0;  // (else 0 or NaN)
+  const float hi = float(r), lo = float(r - double(hi));
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int ch = tid + c * nt;
     const uint32_t ww[4] = {wv[c].x, wv[c].y, wv[c].z, wv[c].w};
+    if (ch >= nch) break;
+    if (p.x_out)
+      mi::store16(p.x_out + row * p.xo_stride + ch * 8, make_uint4(xo[c][0], xo[c][1], xo[c][2], xo[c][3]));
     float h[8];
+    uint32_t zeros = ~0u;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      h[2 * k] = v[c][2 * k] * rstd * mi::bf16_lo(ww[k]);
-      h[2 * k + 1] = v[c][2 * k + 1] * rstd * mi::bf16_hi(ww[k]);
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t w16 = ww[k / 2];
+      v[c][k] *= k % 2 ? mi::bf16_hi(w16) : mi::bf16_lo(w16);
+      h[k] = v[c][k] * hi;
+      zeros = min(zeros, __float_as_uint(h[k]) & 0x7ffffu);
+    }
+    if (zeros == 0) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) h[k] = product_to_odd(v[c][k], hi, lo);
     }
     uint32_t byte;
     const u32x2_t code = quantize8(h, byte);
-    if (ch >= nch) break;
-    if (p.x_out)  // (exact: the values are bf16's)
-      mi::store16(p.x_out + row * p.xo_stride + ch * 8,
-                  make_uint4(mi::cvt_pk_bf16(v[c][0], v[c][1]), mi::cvt_pk_bf16(v[c][2], v[c][3]),
-                             mi::cvt_pk_bf16(v[c][4], v[c][5]), mi::cvt_pk_bf16(v[c][6], v[c][7])));
     *reinterpret_cast<u32x2_t*>(p.codes + row * p.c_stride + ch * 8) = code;
     if ((ch & 3) == 0) p.scales[row * p.s_stride + ch / 4] = uint8_t(byte);
   }
