@@ -31,6 +31,9 @@ carries the device page table's sticky error word and the decode plan's
 error word; a nonzero one (host mirror and device state disagree, a plan
 that did not fit) raises RuntimeError.
 
+Requests of a model with adapters name theirs (``Request.adapter``): the rows of a prefill and of a
+window are planned once by adapter; a window none of whose rows has one replays a graph without them.
+
 Serving: ``start()`` runs the step loop in a daemon thread and
 ``submit_request()`` hands requests to it from any thread
 (scheduler.py:569-604); every token, then ``None`` once the request is
@@ -51,6 +54,7 @@ from typing import Callable
 
 import torch
 
+from .adapters import AdapterPlan
 from .decode import BatchDecodeWithPagedKVCacheWrapper
 from .kv_cache import DevicePageTable, PagedKVCache
 from .model import AttentionBackend, Model, capturers
@@ -81,6 +85,8 @@ class Request:
     finish_reason: str | None = None
     prefill_done_time: float = 0.0
     last_token_time: float = 0.0
+    # of the model's adapters (Model.enable_adapters), -1 for none
+    adapter: int = -1
     # receives each token id, then None when the request is retired
     sink: Callable[[int | None], None] | None = None
 
@@ -184,6 +190,12 @@ class Scheduler:
         self.active: list[Request] = []
         self.free_slots: deque[int] = deque(range(max_batch_size))
         self.graphs: dict[int, tuple[torch.cuda.CUDAGraph, torch.Tensor]] = {}
+        # adapters: the decode rows' plan, and the graphs of windows with adapters
+        self.adapter_slots = model.adapter_slots
+        self.adapter_plan = AdapterPlan(bmax, self.adapter_slots, dev) if self.adapter_slots else None
+        self.d_adapter = torch.full((bmax,), -1, dtype=torch.int32, device=dev)
+        self._up_adapter = _Pinned(bmax, torch.int32)
+        self.adapter_graphs: dict[int, tuple[torch.cuda.CUDAGraph, torch.Tensor]] = {}
         self.steps = 0
         # background loop state
         self._inbox: list[Request] = []
@@ -197,7 +209,12 @@ class Scheduler:
             self._capture_graphs()
 
     # ------------------------------------------------------------------ API
+    def _check_adapter(self, req: Request) -> None:
+        if not -1 <= req.adapter < self.adapter_slots:
+            raise ValueError(f"adapter {req.adapter}: the scheduler's model has {self.adapter_slots}")
+
     def submit(self, req: Request) -> None:
+        self._check_adapter(req)
         self.waiting.append(req)
 
     def has_work(self) -> bool:
@@ -247,6 +264,7 @@ class Scheduler:
             raise ValueError(f"prompt of {n} tokens (allowed 1..{self.max_seq_len})")
         if self.pt.pages_needed(n) > self.pt.num_pages - 1:
             raise ValueError(f"prompt of {n} tokens needs more pages than the pool holds")
+        self._check_adapter(req)
         with self._lock:
             self._inbox.append(req)
         self._wake.set()
@@ -309,12 +327,12 @@ class Scheduler:
             req.sink(token)
 
     # ------------------------------------------------------------------ graphs
-    def _backend(self, wrapper, mode, indptr, indices, last, batch, pos):
-        return AttentionBackend(self.kv, wrapper, mode, indptr, indices, last, None, batch, pos)
+    def _backend(self, wrapper, mode, indptr, indices, last, batch, pos, adapter_plan=None):
+        return AttentionBackend(self.kv, wrapper, mode, indptr, indices, last, None, batch, pos, adapter_plan=adapter_plan)
 
-    def _decode_forward(self, bs: int) -> torch.Tensor:
+    def _decode_forward(self, bs: int, adapters: bool = False) -> torch.Tensor:
         be = self._backend(self.decode_wrapper, "decode", self.d_indptr[: bs + 1], self.d_indices,
-                           self.d_last[:bs], self.d_batch[:bs], self.d_pos[:bs])
+                           self.d_last[:bs], self.d_batch[:bs], self.d_pos[:bs], self.adapter_plan if adapters else None)
         logits = self.model.forward(self.d_ids[:bs], self.d_pos[:bs], be)
         if self.keep_logits:
             self.d_logits[:bs].copy_(logits)
@@ -332,17 +350,23 @@ class Scheduler:
             self.pt.step([], [], bs, self.d_indptr, self.d_indices, self.d_last, self.d_batch, self.d_pos)
             self._plan_decode(bs)
             self.sampler.temperature[:bs].fill_(0.0)
-            s = torch.cuda.Stream(self.device)
-            s.wait_stream(torch.cuda.current_stream(self.device))
-            with torch.cuda.stream(s):
-                for _ in range(2):
-                    self._decode_forward(bs)
-            torch.cuda.current_stream(self.device).wait_stream(s)
-            g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g):
-                out = self._decode_forward(bs)
-            self.graphs[bs] = (g, out)
+            self._capture(bs, self.graphs, False)
+            if self.adapter_plan is not None:
+                self.adapter_plan.plan(self.d_adapter[:bs])
+                self._capture(bs, self.adapter_graphs, True)
         torch.cuda.synchronize(self.device)
+
+    def _capture(self, bs: int, graphs: dict, adapters: bool) -> None:
+        s = torch.cuda.Stream(self.device)
+        s.wait_stream(torch.cuda.current_stream(self.device))
+        with torch.cuda.stream(s):
+            for _ in range(2):
+                self._decode_forward(bs, adapters)
+        torch.cuda.current_stream(self.device).wait_stream(s)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = self._decode_forward(bs, adapters)
+        graphs[bs] = (g, out)
 
     # ------------------------------------------------------------------ step
     def step(self) -> list[tuple[Request, int]]:
@@ -408,8 +432,13 @@ class Scheduler:
         self.prefill_wrapper.plan(qo_d, self.p_indptr[: n + 1], self.p_indices, self.p_last[:n],
                                   cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, self.page_size,
                                   causal=True, max_total_q=total)
+        plan = None
+        if any(r.adapter >= 0 for r in reqs):
+            slot = torch.tensor([r.adapter for r, x in zip(reqs, lens) for _ in range(x)], dtype=torch.int32)
+            plan = AdapterPlan(total, self.adapter_slots, dev)
+            plan.plan(slot.to(dev, non_blocking=True))
         be = self._backend(self.prefill_wrapper, "prefill", self.p_indptr[: n + 1], self.p_indices,
-                           self.p_last[:n], bidx, pos)
+                           self.p_last[:n], bidx, pos, plan)
         logits = self.model.forward(ids, pos, be, last_rows=last_rows)
         if self.keep_logits:
             self.p_logits[:n].copy_(logits)
@@ -480,7 +509,8 @@ class Scheduler:
         sampled ids, taken on the GPU."""
         b = len(reqs)
         bs = next((g for g in self.graph_sizes if g >= b), None)
-        graph = self.graphs.get(bs) if bs is not None else None
+        adapters = any(r.adapter >= 0 for r in reqs)
+        graph = (self.adapter_graphs if adapters else self.graphs).get(bs) if bs is not None else None
         padded = bs if graph is not None else b
         if padded > self.d_batch.numel():
             raise RuntimeError(f"decode batch {b} exceeds the static buffers ({self.d_batch.numel()})")
@@ -495,6 +525,9 @@ class Scheduler:
         if prev is None:
             self._up_t.upload([r.temperature for r in reqs] + [0.0] * (padded - b), self.sampler.temperature)
             self._up_p.upload([r.top_p for r in reqs] + [1.0] * (padded - b), self.sampler.top_p)
+            if adapters:
+                self._up_adapter.upload([r.adapter for r in reqs] + [-1] * (padded - b), self.d_adapter)
+                self.adapter_plan.plan(self.d_adapter[:padded])
         cfg = self.model.cfg
         plan = (self.decode_wrapper, cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim)
         toks = prev.last if prev is not None else None
@@ -513,7 +546,7 @@ class Scheduler:
                 g.replay()
                 toks = out
             else:
-                toks = self._decode_forward(padded)
+                toks = self._decode_forward(padded, adapters)
             if w > 1:
                 self.d_ring[j, :padded].copy_(toks[:padded])
         k = self._slot

@@ -25,7 +25,12 @@ more rows, as a kernel of its own (``dense.linear_silu``);
 ``fused_dense=False`` keeps torch's ``F.linear``, ``F.rms_norm``, adds and
 ``F.silu(g) * u``.  ``Model.quantize_weights()`` turns the layers' projections into
 microscaled 4-bit matrices (``mxfp4.MXFP4``), which every step then multiplies by
-``mxfp4.linear_mxfp4`` / ``linear_silu_mxfp4``, whatever its rows.  RoPE tables are held in the model dtype, as the reference's are after ``.to(dtype)``
+``mxfp4.linear_mxfp4`` / ``linear_silu_mxfp4``, whatever its rows; ``quantize_weights("mxfp8")``
+into 8-bit ones (``mxfp8.MXFP8``), whose inputs are 8-bit rows too: the norms leave such rows
+(``add_rms_norm_mxfp8``), SiLU(gate) * up does in its projection's launch, and the attention's
+outputs are quantised.  ``Model.enable_adapters()`` makes room for low-rank adapters beside the
+projections (``adapters.add_adapters``), which the rows of a step take by their backend's
+``adapter_plan``.  RoPE tables are held in the model dtype, as the reference's are after ``.to(dtype)``
 (server.py:251).  Weights are random-initialised on the device (N(0, 0.02),
 norms 1) -- the benchmark configurations use random weights.
 """
@@ -42,8 +47,10 @@ import weakref
 import torch
 import torch.nn.functional as F
 
-from .dense import add_rms_norm, linear, linear_silu
+from .adapters import Adapters, add_adapters
+from .dense import add_rms_norm, linear, linear_silu, silu_mul
 from .mxfp4 import BLOCK, MXFP4, linear_mxfp4, linear_silu_mxfp4, quantize_mxfp4
+from .mxfp8 import MXFP8, add_rms_norm_mxfp8, linear_mxfp8, linear_silu_mxfp8, quantize_mxfp8
 from .page import append_paged_kv_cache, rope_append_paged_kv_cache
 
 
@@ -135,14 +142,22 @@ class Layer:
         self.w_o = w(h, nq * d)
         self.w_gate_up = w(2 * cfg.intermediate_size, h)
         self.w_down = w(h, cfg.intermediate_size)
+        self.adapters: dict[str, Adapters] = {}
 
 
 # Schedulers with captured graphs, which hold the addresses of their model's weights.
 capturers: weakref.WeakSet = weakref.WeakSet()
 
 
-def _project(h: torch.Tensor, w: torch.Tensor | MXFP4, bias: torch.Tensor | None = None) -> torch.Tensor:
+def _project(h: torch.Tensor | MXFP8, w: torch.Tensor | MXFP4 | MXFP8, bias: torch.Tensor | None = None) -> torch.Tensor:
+    if isinstance(w, MXFP8):
+        return linear_mxfp8(h if isinstance(h, MXFP8) else quantize_mxfp8(h), w, bias)
     return linear_mxfp4(h, w, bias) if isinstance(w, MXFP4) else linear(h, w, bias)
+
+
+# The projections that may have adapters, and the pieces of their outputs, by the names of checkpoints.
+ADAPTED = {"w_qkv": ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj"), "w_o": ("self_attn.o_proj",),
+           "w_gate_up": ("mlp.gate_proj", "mlp.up_proj"), "w_down": ("mlp.down_proj",)}
 
 
 @dataclasses.dataclass
@@ -166,6 +181,8 @@ class AttentionBackend:
     batch_indices: torch.Tensor
     positions: torch.Tensor
     _layer_idx: int = 0
+    # an ``adapters.AdapterPlan`` of the forward's rows; None: no row has an adapter
+    adapter_plan: object | None = None
 
     def next_layer(self) -> int:
         idx = self._layer_idx
@@ -202,26 +219,56 @@ class Model:
                     t += x.nbytes
         return t
 
-    def quantize_weights(self) -> None:
-        """The layers' projections in microscaled 4-bit floats from here on (0.53 bytes
-        per weight); embedding, LM head, norms and biases stay in bf16.  After the
+    def quantize_weights(self, weight_format: str = "mxfp4") -> None:
+        """The layers' projections in microscaled floats of 4 bits ("mxfp4", 0.53 bytes per weight) or
+        8 ("mxfp8", 1.03) from here on; embedding, LM head, norms and biases stay in bf16.  After the
         weights are loaded and before a scheduler captures its graphs, which read the
         weights of their time.  Weights that have no such form leave the model as it was."""
+        if weight_format not in ("mxfp4", "mxfp8"):
+            raise ValueError(f"weight_format {weight_format!r}: mxfp4 or mxfp8")
+        made, quantize = (MXFP4, quantize_mxfp4) if weight_format == "mxfp4" else (MXFP8, quantize_mxfp8)
+        bits = weight_format[-1]
         if not self.fused_dense:
-            raise ValueError("4-bit weights need fused_dense")
-        weights = [(L, name) for L in self.layers for name in ("w_qkv", "w_o", "w_gate_up", "w_down")
-                   if not isinstance(getattr(L, name), MXFP4)]
+            raise ValueError(f"{bits}-bit weights need fused_dense")
+        weights = [(L, name) for L in self.layers for name in ADAPTED if not isinstance(getattr(L, name), made)]
         if weights and any(s.model is self for s in capturers):
             gc.collect()  # (one that nobody holds any more may be part of a cycle)
             if any(s.model is self for s in capturers):
                 raise RuntimeError("a scheduler's captured graphs read the weights: quantize_weights() comes before it")
         for L, name in weights:
             w = getattr(L, name)
+            if not isinstance(w, torch.Tensor):
+                raise ValueError(f"{name} is held in another microscaled format: weights are quantised from bf16")
             if not w.is_cuda or w.dtype != torch.bfloat16 or w.shape[1] % BLOCK:
-                raise ValueError(f"4-bit weights are made of bf16 on a GPU with columns in blocks of {BLOCK}; {name} is "
+                raise ValueError(f"{bits}-bit weights are made of bf16 on a GPU with columns in blocks of {BLOCK}; {name} is "
                                  f"{tuple(w.shape)} {w.dtype} on {w.device}")
         for L, name in weights:  # (one by one: both forms of all weights need not fit together)
-            setattr(L, name, quantize_mxfp4(getattr(L, name)))
+            setattr(L, name, quantize(getattr(L, name)))
+
+    # ------------------------------------------------------------------ adapters
+    @property
+    def adapter_slots(self) -> int:
+        """How many adapters there is room for."""
+        return next((a.slots for L in self.layers for a in L.adapters.values()), 0)
+
+    def enable_adapters(self, slots: int, rank: int, projections=tuple(ADAPTED)) -> None:
+        """Room for ``slots`` adapters of up to ``rank`` beside the layers' projections (any of ADAPTED's
+        names), which add nothing until ``weights.load_adapter`` or ``Adapters.set`` fills them.  Before a
+        scheduler of this model is made."""
+        if not self.fused_dense:
+            raise ValueError("adapters need fused_dense")
+        unknown = set(projections) - set(ADAPTED)
+        if unknown or not projections:
+            raise ValueError(f"projections {sorted(unknown)}: any of {sorted(ADAPTED)}")
+        if self.adapter_slots:
+            raise ValueError("the model has adapters already")
+        cfg = self.cfg
+        q, kv = cfg.num_attention_heads * cfg.head_dim, cfg.num_key_value_heads * cfg.head_dim
+        h, inter = cfg.hidden_size, cfg.intermediate_size
+        shapes = {"w_qkv": (h, [q, kv, kv]), "w_o": (q, [h]), "w_gate_up": (h, [inter, inter]), "w_down": (inter, [h])}
+        made = [{name: Adapters.empty(slots, *shapes[name], rank, self.device) for name in projections} for _ in self.layers]
+        for L, adapters in zip(self.layers, made):
+            L.adapters = adapters
 
     # ------------------------------------------------------------------ forward
     def forward(self, input_ids: torch.Tensor, positions: torch.Tensor, backend: AttentionBackend,
@@ -245,13 +292,24 @@ class Model:
         eps = cfg.rms_norm_eps
         dense = self.fused_dense
         project = _project if dense else F.linear
+        plan = backend.adapter_plan
+
+        def adapted(y, h, L, name):  # y, with what the rows' adapters add to it
+            adapters = L.adapters.get(name) if plan is not None else None
+            return y if adapters is None else add_adapters(y, h, adapters, plan)
+
+        def norm(x, delta, weight, w):  # the norm that w's projection reads
+            if isinstance(w, MXFP8):
+                return add_rms_norm_mxfp8(x, delta, weight, eps)
+            return add_rms_norm(x, delta, weight, eps, write_x=delta is not None)
+
         if dense:
-            h = add_rms_norm(x, None, self.layers[0].in_norm, eps, write_x=False)
+            h = norm(x, None, self.layers[0].in_norm, self.layers[0].w_qkv)
         for li, L in enumerate(self.layers):
             layer_idx = backend.next_layer()
             if not dense:
                 h = F.rms_norm(x, (cfg.hidden_size,), L.in_norm, eps)
-            qkv = project(h, L.w_qkv, L.b_qkv)
+            qkv = adapted(project(h, L.w_qkv, L.b_qkv), h, L, "w_qkv")
             kv_data = backend.paged_kv_cache.kv_data[layer_idx]
             if fused and backend.mode == "decode" and self.fused_decode:
                 # RoPE, append and attention in one launch (one new token per
@@ -278,11 +336,22 @@ class Model:
                 x = x + F.linear(F.silu(g) * u, L.w_down)
                 continue
             # x += o W_o; h = rms(x); x += down(silu(g) * u); h = next layer's rms(x)
-            h = add_rms_norm(x, project(o.view(t, nq * d), L.w_o), L.post_norm, eps)
-            gate_up = linear_silu_mxfp4 if isinstance(L.w_gate_up, MXFP4) else linear_silu
-            down = project(gate_up(h, L.w_gate_up), L.w_down)
+            o = o.view(t, nq * d)
+            if isinstance(L.w_o, MXFP8):
+                o = quantize_mxfp8(o)
+            h = norm(x, adapted(project(o, L.w_o), o, L, "w_o"), L.post_norm, L.w_gate_up)
+            if plan is not None and "w_gate_up" in L.adapters:
+                act = silu_mul(adapted(project(h, L.w_gate_up), h, L, "w_gate_up"))
+                if isinstance(L.w_down, MXFP8):
+                    act = quantize_mxfp8(act)
+            elif isinstance(L.w_gate_up, MXFP8):
+                act = linear_silu_mxfp8(h, L.w_gate_up, quantize=True)
+            else:
+                act = (linear_silu_mxfp4 if isinstance(L.w_gate_up, MXFP4) else linear_silu)(h, L.w_gate_up)
+            down = adapted(project(act, L.w_down), act, L, "w_down")
             if li + 1 < len(self.layers):
-                h = add_rms_norm(x, down, self.layers[li + 1].in_norm, eps)
+                nxt = self.layers[li + 1]
+                h = norm(x, down, nxt.in_norm, nxt.w_qkv)
             elif last_rows is None:
                 h = add_rms_norm(x, down, self.norm, eps)
             else:

@@ -22,7 +22,9 @@ architecture, with the synthetic tokenizer), ``device``, ``dtype``
 (bfloat16), ``seed``, ``server.host`` / ``server.port``,
 ``scheduler.max_seq_len`` / ``max_batch_size`` / ``page_size`` /
 ``decode_window`` / ``pipeline`` / ``use_graphs`` (``use_flashinfer`` is
-accepted and ignored: the HIP path is the only one).
+accepted and ignored: the HIP path is the only one), ``weight_format`` (bfloat16,
+mxfp4 or mxfp8), and ``adapters`` (name -> directory of a low-rank adapter) with
+``adapter_rank``: a request whose ``model`` is an adapter's name is served with it.
 """
 
 from __future__ import annotations
@@ -118,10 +120,10 @@ class ChatCompletionChunk(BaseModel):
 
 
 # ---------------------------------------------------------------- app
-def create_app(scheduler, tokenizer, model_name: str, stop_ids: set[int]) -> FastAPI:
+def create_app(scheduler, tokenizer, model_name: str, stop_ids: set[int], adapters: dict[str, int] | None = None) -> FastAPI:
     """``scheduler`` needs ``submit_request(Request)`` and a running loop
     (``engine.Scheduler`` after ``start()``); tokens reach each request
-    through its ``sink``."""
+    through its ``sink``.  ``adapters``: the slots of the model's adapters by name."""
     app = FastAPI(title="minimal-inference (MI355X)")
     app.add_middleware(CORSMiddleware, allow_origins=["*"], allow_methods=["*"], allow_headers=["*"])
     stops = set(stop_ids)
@@ -140,7 +142,8 @@ def create_app(scheduler, tokenizer, model_name: str, stop_ids: set[int]) -> Fas
 
     @app.get("/v1/models")
     async def models():
-        return {"object": "list", "data": [{"id": model_name, "object": "model", "owned_by": "local"}]}
+        return {"object": "list", "data": [{"id": name, "object": "model", "owned_by": "local"}
+                                           for name in (model_name, *(adapters or {}))]}
 
     @app.post("/v1/chat/completions")
     async def chat_completions(body: ChatCompletionRequest):
@@ -148,6 +151,7 @@ def create_app(scheduler, tokenizer, model_name: str, stop_ids: set[int]) -> Fas
         queue: asyncio.Queue = asyncio.Queue()
         req = Request(request_id=f"chatcmpl-{uuid.uuid4().hex[:12]}", input_ids=prompt_ids(body.messages),
                       max_new_tokens=body.max_tokens, temperature=body.temperature, top_p=body.top_p,
+                      adapter=(adapters or {}).get(body.model, -1),
                       sink=lambda t: loop.call_soon_threadsafe(queue.put_nowait, t))
         try:
             scheduler.submit_request(req)
@@ -231,12 +235,13 @@ def create_app(scheduler, tokenizer, model_name: str, stop_ids: set[int]) -> Fas
 # ---------------------------------------------------------------- engine from a config
 def init_engine(config: dict):
     """(scheduler started, tokenizer, model name, stop ids) from a config
-    dict shaped like the reference's config.yaml (server.py:235-285)."""
+    dict (slot i of its adapters is the i-th of ``adapters``) shaped like the reference's config.yaml (server.py:235-285)."""
     import torch
 
     from .engine import Scheduler
     from .model import PRESETS, Model, ModelConfig
     from .tokenizer import SyntheticTokenizer, load_tokenizer, stop_ids
+    from .weights import load_adapter, load_weights
 
     if str(config.get("dtype", "bfloat16")) not in ("bfloat16", "bf16"):
         raise ValueError("the HIP path computes in bfloat16; set dtype: bfloat16")
@@ -248,13 +253,12 @@ def init_engine(config: dict):
     sc = config.get("scheduler", {})
     max_seq = int(sc.get("max_seq_len", 4096))
     weight_format = str(config.get("weight_format", "bfloat16"))
-    if weight_format not in ("bfloat16", "bf16", "mxfp4"):
-        raise ValueError(f"weight_format {weight_format!r}: bfloat16 or mxfp4")
+    if weight_format not in ("bfloat16", "bf16", "mxfp4", "mxfp8"):
+        raise ValueError(f"weight_format {weight_format!r}: bfloat16, mxfp4 or mxfp8")
+    adapters = dict(config.get("adapters") or {})
     model_path = config.get("model_path")
     seed = int(config.get("seed", 0))
     if model_path:
-        from .weights import load_weights
-
         cfg = ModelConfig.from_pretrained(model_path)
         model = Model(cfg, dev, seed=seed, max_positions=max_seq + 16)
         load_weights(model, model_path)
@@ -266,8 +270,14 @@ def init_engine(config: dict):
         model = Model(cfg, dev, seed=seed, max_positions=max_seq + 16)
         tok = SyntheticTokenizer(cfg.vocab_size)
         name = f"{preset}-random"
-    if weight_format == "mxfp4":
-        model.quantize_weights()
+    if weight_format in ("mxfp4", "mxfp8"):
+        model.quantize_weights(weight_format)
+    if adapters:
+        if name in adapters:
+            raise ValueError(f"an adapter has the model's name {name!r}")
+        model.enable_adapters(len(adapters), int(config.get("adapter_rank", 16)))
+        for slot, path in enumerate(adapters.values()):
+            load_adapter(model, slot, str(path))
     stops = stop_ids(tok)
     sch = Scheduler(model, max_batch_size=int(sc.get("max_batch_size", 40)), max_seq_len=max_seq,
                     page_size=int(sc.get("page_size", 16)), eos_token_ids=stops or None,
@@ -293,7 +303,8 @@ def main(argv=None) -> int:
     srv = config.get("server", {})
     log.info("engine ready: model=%s, max_batch_size=%d, page_size=%d, decode_window=%d", name,
              sch.max_batch_size, sch.page_size, sch.decode_window)
-    uvicorn.run(create_app(sch, tok, name, stops), host=args.host or srv.get("host", "127.0.0.1"),
+    slots = {str(adapter): i for i, adapter in enumerate(config.get("adapters") or {})}
+    uvicorn.run(create_app(sch, tok, name, stops, slots), host=args.host or srv.get("host", "127.0.0.1"),
                 port=args.port or int(srv.get("port", 8000)), log_level="warning")
     sch.stop()
     return 0

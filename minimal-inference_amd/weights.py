@@ -29,7 +29,7 @@ import re
 
 import torch
 
-from .mxfp4 import MXFP4
+from .model import ADAPTED
 
 _LAYER = re.compile(r"^model\.layers\.(\d+)\.(.+)$")
 
@@ -79,8 +79,10 @@ def load_weights(model, model_path: str) -> None:
     from safetensors import safe_open
 
     for L in model.layers:
-        if any(isinstance(w, MXFP4) for w in (L.w_qkv, L.w_o, L.w_gate_up, L.w_down)):
-            raise ValueError("the model holds 4-bit weights: load a checkpoint before quantize_weights()")
+        for name in ADAPTED:
+            if not isinstance(getattr(L, name), torch.Tensor):
+                bits = 4 if type(getattr(L, name)).__name__ == "MXFP4" else 8
+                raise ValueError(f"the model holds {bits}-bit weights: load a checkpoint before quantize_weights()")
     targets = _targets(model)
     seen: set[str] = set()
     for path in checkpoint_files(model_path):
@@ -103,3 +105,46 @@ def load_weights(model, model_path: str) -> None:
     missing = sorted(set(targets) - seen)
     if missing:
         raise ValueError(f"checkpoint lacks {len(missing)} tensors, e.g. {missing[:3]}")
+
+
+_FACTOR = re.compile(r"^(?:base_model\.model\.)?model\.layers\.(\d+)\.(.+)\.lora_([AB])(?:\.default)?\.weight$")
+
+
+def load_adapter(model, slot: int, path: str) -> None:
+    """A low-rank adapter's directory (``adapter_config.json`` and ``adapter_model.safetensors``) into
+    ``slot`` of a model after ``enable_adapters``.  The factors add ``lora_alpha / r`` (with
+    ``use_rslora`` ``lora_alpha / sqrt(r)``) of their product; modules that it lacks add nothing.  Modules
+    that the model has no room for, and adapters of another kind, are refused before anything changes."""
+    from safetensors import safe_open
+
+    if not 0 <= slot < model.adapter_slots:
+        raise ValueError(f"slot {slot}: the model has room for {model.adapter_slots} adapters (enable_adapters)")
+    with open(os.path.join(path, "adapter_config.json")) as f:
+        cfg = json.load(f)
+    if cfg.get("peft_type", "LORA") != "LORA" or cfg.get("use_dora") or cfg.get("bias", "none") != "none" \
+            or cfg.get("rank_pattern") or cfg.get("alpha_pattern") or cfg.get("modules_to_save") or cfg.get("fan_in_fan_out"):
+        raise ValueError(f"{path}: a plain low-rank adapter of one rank without biases expected")
+    r = int(cfg["r"])
+    scale = float(cfg["lora_alpha"]) / (r ** 0.5 if cfg.get("use_rslora") else r)
+    place = {piece: (name, i) for name, pieces in ADAPTED.items() for i, piece in enumerate(pieces)}
+    found: dict[tuple[int, str, int], dict[str, torch.Tensor]] = {}
+    with safe_open(os.path.join(path, "adapter_model.safetensors"), framework="pt", device="cpu") as f:
+        for key in f.keys():
+            m = _FACTOR.match(key)
+            if not m or m.group(2) not in place:
+                raise ValueError(f"{path}: {key} is no factor of a layer's projection")
+            layer, (name, i) = int(m.group(1)), place[m.group(2)]
+            if layer >= len(model.layers) or name not in model.layers[layer].adapters:
+                raise ValueError(f"{path}: the model has no room for {key}")
+            found.setdefault((layer, name, i), {})[m.group(3)] = f.get_tensor(key)
+    for (layer, name, i), f in found.items():
+        a = model.layers[layer].adapters[name]
+        if set(f) != {"A", "B"}:
+            raise ValueError(f"{path}: layer {layer}, {ADAPTED[name][i]}: A and B expected")
+        if tuple(f["A"].shape) != (r, a.k) or tuple(f["B"].shape) != (a.pieces[i], r) or r > a.rank:
+            raise ValueError(f"{path}: layer {layer}, {ADAPTED[name][i]}: A [{r}, {a.k}] and B [{a.pieces[i]}, {r}], a rank "
+                             f"of up to {a.rank} expected; got {tuple(f['A'].shape)} and {tuple(f['B'].shape)}")
+    for layer, L in enumerate(model.layers):
+        for name, a in L.adapters.items():
+            factors = [found.get((layer, name, i)) for i in range(len(a.pieces))]
+            a.set(slot, [None if f is None else (f["A"], f["B"]) for f in factors], scale)
