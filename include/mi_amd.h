@@ -468,8 +468,8 @@ int mi_mxfp8_dequantize(const void* codes, int64_t codes_stride, const void* sca
                         int64_t cols, mi_stream_t stream);
 
 /* x' = bf16(x + delta) (x where delta is null), stored to x_out unless that is null,
- * and x' * rsqrt(mean(x'^2) + eps) * weight in fp32, quantised from there.  hidden a
- * multiple of 32 up to 16384, at most 2^22 rows, 16-byte aligned rows of bf16.  x_out may be x or
+ * and x' * rsqrt(mean(x'^2) + eps) * weight, quantised as its exact value would be (the sum of
+ * squares and the root are held in 64 bits).  hidden a multiple of 32 up to 16384, at most 2^22 rows, 16-byte aligned rows of bf16.  x_out may be x or
  * delta; outputs that overlap each other, the weight or another row's input are refused. */
 int mi_add_rms_norm_mxfp8(const void* x, int64_t x_stride, const void* delta, int64_t delta_stride,
                           const void* weight, void* x_out, int64_t x_out_stride, void* codes,

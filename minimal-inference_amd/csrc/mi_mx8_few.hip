@@ -9,6 +9,9 @@
 // directly are 64 separate places an instruction, and the address unit takes them one by
 // one: 32 x 14,336 x 4,096 32 us.)  The waves meet once, at the end, where their
 // accumulators are added in wave order: the result does not depend on timing.
+// SPLIT: the workgroup takes p.split_slabs slabs (a multiple of four) and leaves its sums for launch_combine.
+#include <algorithm>
+
 #include "mi_mx8_linear.h"
 
 namespace mi::mx8 {
@@ -20,11 +23,12 @@ constexpr int few_lds(int r, int mb, int depth, int waves) {
   return waves * (ring > sums ? ring : sums);
 }
 
-template <int R, int MB, int DEPTH, bool GLU, bool OUT8, int WAVES>
+template <int R, int MB, int DEPTH, bool GLU, bool OUT8, int WAVES, bool SPLIT>
 __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
   constexpr int HALVES = GLU ? 2 : 1, COLS = 16 * R / HALVES, TILES = R + MB;
   constexpr int SLOT = TILES * 2048, SLOADS = (TILES * 16 + 63) / 64, SBYTES = SLOADS * 1024, LOADS = 2 * TILES;
   constexpr int WAVE = few_lds(R, MB, DEPTH, 1);
+  static_assert(!SPLIT || (!GLU && !OUT8), "parts are of plain products");
   static_assert(R % HALVES == 0 && (!OUT8 || COLS % kBlock == 0), "gate and up tiles in pairs, whole blocks");
   static_assert(4 % DEPTH == 0 && DEPTH * SLOT + 2 * SBYTES <= WAVE && WAVES * WAVE <= 160 * 1024, "LDS");
   __shared__ __attribute__((aligned(16))) char smem[WAVES * WAVE];
@@ -34,6 +38,7 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
   const int g = lane >> 4, n = lane & 15;
   const int col0 = int(blockIdx.x) * COLS, blocks = p.k / kBlock;
   const int rows = int(p.rows);
+  const int slab0 = SPLIT ? int(blockIdx.y) * p.split_slabs : 0, slab_end = SPLIT ? min(slab0 + p.split_slabs, p.slabs) : p.slabs;
   const int wstride = int(p.w_stride), xstride = int(p.x_stride);
   const char* const xbase = p.x;
   const char* const wbase = p.w + col0 * p.w_stride;
@@ -45,7 +50,7 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
   auto load = [&](int slab, int slot) {
     const int xlane = r8 * xstride + chunk, wlane = r8 * wstride + chunk;
     const int off = slab * kSlab;
-    const bool ok = slab < p.slabs;
+    const bool ok = slab < slab_end;
     const int past = off + chunk < p.k ? 0 : kOutOfRange;  // past the row's end lies the next row
     const __amdgpu_buffer_rsrc_t rw = buffer(wbase + off, ok ? wsize - off : 0), rx = buffer(xbase + off, ok ? xsize - off : 0);
     const __amdgpu_buffer_rsrc_t ru = GLU ? buffer(ubase + off, ok ? usize - off : 0) : rw;
@@ -58,10 +63,11 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
     for (int i = 0; i < 2 * MB; ++i)
       lds_dma16(rx, to + (2 * R + i) * 1024, (xlane + i * 8 * xstride) | past);
   };
+  const int quad0 = slab0 / 4, first = quad0 + w;
   // The scale bytes of four slabs, 16 a row: the tiles' rows of W, then x's.
   auto load_scales = [&](int quad) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    lds_t* const to = scales + (quad / WAVES & 1) * SBYTES;
+    lds_t* const to = scales + ((quad - quad0) / WAVES & 1) * SBYTES;
 #pragma unroll
     for (int i = 0; i < SLOADS; ++i) {
       const int at = i * 64 + lane, tile = at / 16, r = at % 16;
@@ -85,18 +91,18 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
   const int lo = n * kSlab + (g ^ (n & 7)) * 16, hi = n * kSlab + ((4 + g) ^ (n & 7)) * 16;
   auto slab_at = [&](int quad, int s) { return 4 * (quad + s / 4 * WAVES) + s % 4; };  // s steps into a group
 
-  if (4 * w < p.slabs) {
-    load_scales(w);
-    load_scales(w + WAVES);
+  if (4 * first < slab_end) {
+    load_scales(first);
+    load_scales(first + WAVES);
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) load(slab_at(w, d), d);
+    for (int d = 0; d < DEPTH; ++d) load(slab_at(first, d), d);
   }
   constexpr int kInFlight = (DEPTH - 1) * LOADS;
   static_assert(kInFlight < 64, "vmcnt");
-  for (int quad = w; 4 * quad < p.slabs; quad += WAVES) {
+  for (int quad = first; 4 * quad < slab_end; quad += WAVES) {
     // (a group ahead: done by the waits of the four steps before it)
-    if (quad != w) load_scales(quad + WAVES);
-    const lds_t* const sl = scales + (quad / WAVES & 1) * SBYTES + n * 16 + g;
+    if (quad != first) load_scales(quad + WAVES);
+    const lds_t* const sl = scales + ((quad - quad0) / WAVES & 1) * SBYTES + n * 16 + g;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const int slab = 4 * quad + s;
@@ -152,7 +158,11 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
   constexpr int STEP = OUT8 ? 2 : 1;
   for (int q = w; q < COLS / 16 / STEP * MB; q += WAVES) {
     const int r = q / MB * STEP, b = q % MB, m = b * 16 + n, col = col0 + r * 16;
-    if constexpr (OUT8) {
+    if constexpr (SPLIT) {
+      // [part][row][columns, in fours]
+      if (m < rows && col + 4 * g < p.n)
+        p.parts[(int64_t(blockIdx.y) * rows + m) * ((p.n + 3) / 4) + col / 4 + g] = total(q);
+    } else if constexpr (OUT8) {
       store_block(p, m, m < rows && col < p.n, col, g, result(r, b), result(r + 1, b));
     } else {
       const f32x4_t v = result(r, b);
@@ -161,11 +171,11 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
   }
 }
 
-template <int R, int MB, int DEPTH, bool GLU, bool OUT8, int WAVES>
+template <int R, int MB, int DEPTH, bool GLU, bool OUT8, int WAVES, bool SPLIT = false>
 void run(const LinearParams& p, hipStream_t stream) {
   constexpr int COLS = 16 * R / (GLU ? 2 : 1);
-  const dim3 grid((p.n + COLS - 1) / COLS);
-  hipLaunchKernelGGL((few_kernel<R, MB, DEPTH, GLU, OUT8, WAVES>), grid, dim3(64 * WAVES), 0, stream, p);
+  const dim3 grid((p.n + COLS - 1) / COLS, SPLIT ? (p.slabs + p.split_slabs - 1) / p.split_slabs : 1);
+  hipLaunchKernelGGL((few_kernel<R, MB, DEPTH, GLU, OUT8, WAVES, SPLIT>), grid, dim3(64 * WAVES), 0, stream, p);
 }
 
 // The form of a launch, from the tiles of W and the 16-row blocks of x (us, weights rotated
@@ -222,9 +232,55 @@ void launch(const LinearParams& p, hipStream_t stream) {
   else pick<4, GLU, OUT8>(p, stream);
 }
 
+// Workgroups that share k (S of them, four tiles each) read an S-th of x's bytes where
+// one by itself reads all; their sums go through memory in fp32, and another launch adds them in
+// order. The count, in us: the way into LDS of a CU (56.6 GB/s, half of it hidden behind
+// HBM) against the launch and the sums' way. Measured (calls in a graph, alone / shared):
+//   N  4096 K 14336   16 rows 17.4 / 17.5 (S 4)   32 rows 20.5 / 18.7 (4)   64 rows 25.7 / 21.3 (4)
+//   N  3584 K 18944   32 rows 24.6 / 22.1 (4)     64 rows 32.6 / 25.6 (4)
+//   N  8192 K 29568   32 rows 62.4 / 57.6 (2)     64 rows 72.6 / 64.3 (2)
+//   N  4096 K  4096   64 rows  9.8 / 11.5 (4)     N 6144 K 4096   64 rows 12.1 / 13.7 (2)
+//   N  8192 K  8192   64 rows 22.6 / 24.9 (2)
+// (other tiles and S were slower than the better of the two; a single block of x gains nothing)
+int split_slabs_of(bool glu, int64_t rows, int64_t n, int slabs, size_t room) {
+  const int tiles = int((n + 15) / 16), blocks = int((rows + 15) / 16), cus = mi::num_cus();
+  if (glu || blocks == 1) return slabs;
+  const int rounds = std::min((tiles + cus - 1) / cus, 4);
+  const float k = float(slabs) * kSlab, per_us = 2 * 56.6e3f;
+  float best = (rounds + blocks) * 16 * k / per_us;
+  int found = slabs;
+  for (int s = 2; s <= 4; s += 2) {
+    const int each = ((slabs + s - 1) / s + 3) / 4 * 4;
+    if ((tiles + 3) / 4 * s > cus || each * (s - 1) >= slabs || room < size_t(s) * rows * ((n + 3) / 4) * 16) continue;
+    const float us = (4 + blocks) * 16 * float(each) * kSlab / per_us + 1.f + 2.f * 4 * s * float(rows) * float(n) / 4.4e6f;
+    if (us < best) best = us, found = each;
+  }
+  return found;
+}
+
+template <int MB>
+void run_shared(const LinearParams& p, hipStream_t stream) {
+  run<4, MB, 2, false, false, 4, true>(p, stream);
+}
+
 }  // namespace
 
-void launch_few(const LinearParams& p, bool glu, hipStream_t stream) {
+size_t few_workspace(bool glu, int64_t rows, int64_t n, int slabs) {
+  const int each = split_slabs_of(glu, rows, n, slabs, size_t(1) << 28);
+  return each < slabs ? size_t((slabs + each - 1) / each) * rows * ((n + 3) / 4) * 16 : 0;
+}
+
+void launch_few(const LinearParams& p, bool glu, size_t room, hipStream_t stream) {
+  LinearParams q = p;
+  q.split_slabs = split_slabs_of(glu, p.rows, p.n, p.slabs, room);
+  if (q.split_slabs < p.slabs) {
+    const int blocks = int((p.rows + 15) / 16);
+    if (blocks == 2) run_shared<2>(q, stream);
+    else if (blocks == 3) run_shared<3>(q, stream);
+    else run_shared<4>(q, stream);
+    launch_combine(q, false, (p.slabs + q.split_slabs - 1) / q.split_slabs, stream);
+    return;
+  }
   if (!glu) launch<false, false>(p, stream);
   else p.scales ? launch<true, true>(p, stream) : launch<true, false>(p, stream);
 }

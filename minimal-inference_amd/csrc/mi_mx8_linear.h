@@ -85,8 +85,11 @@ __device__ __forceinline__ void store_block(const LinearParams& p, int64_t m, bo
 constexpr int64_t kFewRows = 64;
 constexpr int64_t kMaxRows = 1 << 22, kMaxN = 1 << 24, kMaxStride = 1 << 22;
 
-// (rows at most kFewRows)
-void launch_few(const LinearParams& p, bool glu, hipStream_t stream);
+// (rows at most kFewRows; `room` bytes for parts)
+size_t few_workspace(bool glu, int64_t rows, int64_t n, int slabs);
+void launch_few(const LinearParams& p, bool glu, size_t room, hipStream_t stream);
+// The sum of parts [part][half][row][columns in fours], and the end of the product.
+void launch_combine(const LinearParams& p, bool glu, int parts, hipStream_t stream);
 void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t stream);
 
 }  // namespace mi::mx8

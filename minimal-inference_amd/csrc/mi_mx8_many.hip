@@ -533,12 +533,19 @@ void launch(const LinearParams& p, const Choice& c, hipStream_t stream) {
     hipLaunchKernelGGL((block_kernel<GLU, OUT8, false>), grid, block, 0, stream, q);
   } else {
     hipLaunchKernelGGL((block_kernel<GLU, false, true>), grid, block, 0, stream, q);
-    const int64_t fours = p.rows * ((p.n + 3) / 4);
-    hipLaunchKernelGGL((combine_kernel<GLU, OUT8>), dim3(uint32_t((fours + 255) / 256)), dim3(256), 0, stream, q, c.parts);
+    launch_combine(q, GLU, c.parts, stream);
   }
 }
 
 }  // namespace
+
+void launch_combine(const LinearParams& p, bool glu, int parts, hipStream_t stream) {
+  const int64_t fours = p.rows * ((p.n + 3) / 4);
+  const dim3 grid(uint32_t((fours + 255) / 256)), block(256);
+  if (!glu) hipLaunchKernelGGL((combine_kernel<false, false>), grid, block, 0, stream, p, parts);
+  else if (p.scales) hipLaunchKernelGGL((combine_kernel<true, true>), grid, block, 0, stream, p, parts);
+  else hipLaunchKernelGGL((combine_kernel<true, false>), grid, block, 0, stream, p, parts);
+}
 
 size_t many_workspace(bool glu, int64_t rows, int64_t n, int slabs) {
   return choose(glu, rows, n, slabs, size_t(1) << 28).bytes;
@@ -557,14 +564,15 @@ void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t strea
   rest.xs += q.rows * p.xs_stride;
   rest.out += q.rows * p.o_stride * (p.scales ? 1 : 2);
   if (p.scales) rest.scales += q.rows * p.s_stride;
-  launch_few(rest, glu, stream);
+  launch_few(rest, glu, 0, stream);
 }
 
 }  // namespace mi::mx8
 
 extern "C" size_t mi_linear_mxfp8_workspace_size(int64_t rows, int64_t n, int64_t k, int32_t silu) {
   using namespace mi::mx8;
-  if (rows <= 0 || rows > kMaxRows || n <= 0 || n > kMaxN || k <= 0 || k % kBlock || k > kMaxK || rows <= kFewRows) return 0;
+  if (rows <= 0 || rows > kMaxRows || n <= 0 || n > kMaxN || k <= 0 || k % kBlock || k > kMaxK) return 0;
+  if (rows <= kFewRows) return few_workspace(silu != 0, rows, n, int(slabs(k)));
   return many_workspace(silu != 0, rows, n, int(slabs(k)));
 }
 
@@ -639,7 +647,8 @@ extern "C" int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void
           ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) & 7) == 0;
   p.wide = p.vec && n % 8 == 0 && out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (rows <= kFewRows) launch_few(p, silu != 0, s);
-  else launch_many(p, silu != 0, workspace ? workspace_bytes : 0, s);
+  const size_t room = workspace ? workspace_bytes : 0;
+  if (rows <= kFewRows) launch_few(p, silu != 0, room, s);
+  else launch_many(p, silu != 0, room, s);
   return mi::check_launch(name);
 }

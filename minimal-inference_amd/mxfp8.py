@@ -28,7 +28,6 @@ from ._util import call_on, refuse_derivatives, require_dtype, require_gpu
 
 BLOCK = 32
 _PIECE = 16  # bytes of scales that are read together
-_FEW_ROWS = 64  # no call of up to so many rows takes a workspace
 
 
 def _rows_of(name: str, t: torch.Tensor) -> tuple[int, int]:
@@ -243,7 +242,7 @@ def _linear(x: MXFP8, weight: MXFP8, bias, out, silu: bool, quantize: bool):
         out = _out(out, rows, n, device)
         to, stride, scales, s_stride = out.data_ptr(), out.stride(0), None, 0
     if rows and n:
-        room = _workspace_size(rows, n, k, silu) if rows > _FEW_ROWS else 0
+        room = _workspace_size(rows, n, k, silu)
         # (a tensor of this call's own: calls on several streams and in graphs share nothing)
         workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
         call_on(x.anchor, "mi_linear_mxfp8", x.codes_ptr, x.codes_stride, x.scales_ptr, x.scales_stride,

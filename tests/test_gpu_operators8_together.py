@@ -160,9 +160,10 @@ def _values32(m):
     return m.codes.float() * torch.exp2(m.scales.float() - 127.0).repeat_interleave(32, 1)
 
 
-# rows, n, k: by the kernel's forms. Few rows: 1..64 by counts of 16 and of waves over k; blocks of 128 x 128, whole and
+# rows, n, k: by the kernel's forms. Few rows: 1..64 by counts of 16 and of waves over k, alone and sharing k; blocks of 128 x 128, whole and
 # split over k; blocks of 256 x 256, alone, with rows behind them as few rows, as a block, and with ragged columns and k.
 FORMS = [(1, 33, 32), (1, 4864, 896), (7, 100, 14336), (16, 28672, 512), (17, 20000, 96), (31, 1000, 4128), (48, 257, 8192), (64, 30000, 128),
+         (33, 4099, 12320), (20, 8192, 16416), (64, 3584, 18944), (47, 100, 8192),
          (65, 48, 32), (65, 129, 8224), (200, 1000, 544), (300, 2048, 18944), (1024, 4096, 512),
          (2048, 1056, 8192), (2057, 8192, 1024), (4096, 4112, 288), (4200, 4096, 1056), (2304, 8193, 4096), (8201, 2048, 4064)]
 
@@ -181,6 +182,18 @@ def test_forms_exactly(dev, rows, n, k):
     assert torch.equal(room[1: rows + 1, :n], (want + bias.float()).to(torch.bfloat16))
     assert bool((room[0] == 7).all() and (room[-1] == 7).all() and (room[:, n:] == 7).all())
     assert torch.equal(linear_mxfp8(x, w), want.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("rows,n,k", [(64, 3584, 18944), (33, 4099, 12320), (300, 200, 4128)])
+def test_without_a_workspace(dev, monkeypatch, rows, n, k):
+    """Without room for parts the same sums, by workgroups that share nothing."""
+    from minimal_inference_amd import mxfp8
+
+    x, w = _whole(dev, rows, k, 1), _whole(dev, n, k, 2)
+    assert mxfp8._workspace_size(rows, n, k, False) > 0
+    want = mxfp8.linear_mxfp8(x, w)
+    monkeypatch.setattr(mxfp8, "_workspace_size", lambda *a: 0)
+    assert torch.equal(mxfp8.linear_mxfp8(x, w), want)
 
 
 @pytest.mark.parametrize("rows,n,k", [(1, 64, 64), (20, 4864, 896), (64, 14336, 4096), (65, 96, 64), (300, 1120, 18944), (1030, 4096, 512),
