@@ -109,7 +109,8 @@ class Adapters:
 
 class AdapterPlan:
     """The rows of a batch sorted by adapter.  Runs read the last plan made before them on their stream;
-    a captured graph reads the buffer as it is when it is replayed, for the rows that it was captured with."""
+    a captured graph reads the buffer as it is when it is replayed, for the rows that it was captured with
+    (after a plan of another number of rows its outputs are NaN)."""
 
     __slots__ = ("buffer", "slots", "max_rows", "rows", "device")
 

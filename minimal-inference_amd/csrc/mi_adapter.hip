@@ -40,7 +40,7 @@ struct Tile {
   int slot, first, count, unused;  // slot -1: rows without an adapter
 };
 
-// A plan: the number of tiles in 16 bytes, the tiles, the rows in their order.
+// A plan: the number of tiles and what it is a plan of in 16 bytes, the tiles, the rows in their order.
 int64_t max_tiles(int64_t rows, int64_t slots) { return std::min(rows, slots + 1) + rows / tile_rows(rows); }
 size_t plan_size(int64_t rows, int64_t slots) { return 16 + 16 * size_t(max_tiles(rows, slots)) + 4 * size_t(rows); }
 struct PlanView {
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* slot_of_r
   const int begin = first[tid] - mine, tile = tiles[tid] - need;
   for (int i = 0; i < need; ++i)
     p.tiles[tile + i] = {tid < slots ? tid : -1, begin + i * tile_rows, min(tile_rows, mine - i * tile_rows), 0};
-  if (tid == kPlanThreads - 1) *p.count = tiles[tid];
+  if (tid == kPlanThreads - 1) p.count[0] = tiles[tid], p.count[1] = rows, p.count[2] = slots;
   count[tid] = begin;
   __syncthreads();
   for (int row = tid; row < rows; row += kPlanThreads) p.order[places(at(row), count)] = row;
@@ -112,12 +112,18 @@ struct AdapterParams {
   int64_t o_stride;
   PlanView plan;
   float* parts;  // [part][tile][row of the tile][ranks, padded]
+  int rows, slots;
   int k, n, rank, ranks, padded;  // ranks = pieces * rank, padded to 16
   int n_parts, part_steps, max_tiles, group_ranks;
   int pieces, chunk;  // columns of an expand workgroup
   int end[kMaxPieces];       // columns,
   int end_chunk[kMaxPieces]; // chunks up to and with each piece
 };
+
+// The tiles of a plan, -1 where it is of another batch than the launch (a captured one replayed after another plan).
+__device__ __forceinline__ int plan_tiles(const AdapterParams& p) {
+  return p.plan.count[1] == p.rows && p.plan.count[2] == p.slots ? p.plan.count[0] : -1;
+}
 
 // The waves' sums of a tile's ranks to memory: lane (g, n) holds ranks 4 g .. 4 g + 3 of
 // tile t for row n of block b.
@@ -148,7 +154,7 @@ __device__ __forceinline__ void store_ranks(const AdapterParams& p, const f32x4_
 template <bool X8, int RT>
 __global__ __launch_bounds__(64 * kWaves) void shrink_few_kernel(AdapterParams p) {
   __shared__ __attribute__((aligned(16))) f32x4_t red[kWaves * RT * 64];
-  const int tiles = *p.plan.count;
+  const int tiles = plan_tiles(p);
   const Tile tile = p.plan.tiles[blockIdx.x];
   if (int(blockIdx.x) >= tiles || tile.slot < 0) return;
   const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
@@ -219,7 +225,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void shrink_many_kernel(AdapterPar
   constexpr int WAVE = DEPTH * SLOT + 2 * SBYTES, LOADS = SLOT / 1024;
   static_assert(WAVES * WAVE <= 80 * 1024 && RT * NB * 1024 <= WAVE, "LDS");
   __shared__ __attribute__((aligned(16))) char smem[WAVES * WAVE];
-  const int tiles = *p.plan.count;
+  const int tiles = plan_tiles(p);
   const Tile tile = p.plan.tiles[blockIdx.x];
   if (int(blockIdx.x) >= tiles || tile.slot < 0) return;
   const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
@@ -362,14 +368,20 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
   constexpr int kMaxWeights = 128 * (kPair / 2) + 128;  // a unit's columns of B: eight of them, then 16 bytes apart
   __shared__ __attribute__((aligned(16))) uint16_t vs[ROWS * VSTRIDE];
   __shared__ __attribute__((aligned(16))) uint16_t ws[2][kMaxWeights];
-  const int tiles = *p.plan.count;
-  const Tile tile = p.plan.tiles[blockIdx.x];
-  if (int(blockIdx.x) >= tiles || (tile.slot < 0 && p.out == p.y)) return;
-  const bool adds = tile.slot >= 0;
+  const int tiles = plan_tiles(p);
   int piece = 0;
   while (int(blockIdx.y) >= p.end_chunk[piece]) ++piece;
   const int begin = piece ? p.end[piece - 1] : 0, before = piece ? p.end_chunk[piece - 1] : 0;
   const int c0 = begin + (int(blockIdx.y) - before) * p.chunk, c1 = min(c0 + p.chunk, p.end[piece]);
+  if (tiles < 0) {  // no row's adapter is known: NaN (the tiles are as many as the rows' at least)
+    for (int i = 0; i < ROWS && int(blockIdx.x) * ROWS + i < p.rows; ++i)
+      for (int c = c0 + int(threadIdx.x); c < c1; c += 64 * kWaves)
+        p.out[(int64_t(blockIdx.x) * ROWS + i) * p.o_stride + c] = 0x7fc0;
+    return;
+  }
+  const Tile tile = p.plan.tiles[blockIdx.x];
+  if (int(blockIdx.x) >= tiles || (tile.slot < 0 && p.out == p.y)) return;
+  const bool adds = tile.slot >= 0;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int g = lane >> 4, n = lane & 15;
   const int nb = (tile.count + 15) / 16, groups = (c1 - c0 + 127) / 128;
@@ -637,6 +649,8 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
   p.o_stride = out_stride;
   p.plan = view(const_cast<void*>(plan), rows, slots);
   p.parts = static_cast<float*>(workspace);
+  p.rows = int(rows);
+  p.slots = int(slots);
   p.k = int(k);
   p.n = int(n);
   p.rank = int(rank);

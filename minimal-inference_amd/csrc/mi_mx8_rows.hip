@@ -7,7 +7,7 @@
 //              format's NaN, and zero codes: all of it reads back as NaN.
 //   add_rms  : x' = bf16(x + d), stored when asked; h = x' rsqrt(mean(x'^2) + eps) w, quantised.
 //              The sum and the root are taken in 64 bits and the product x' w (exact in
-//              fp32) times the root is rounded to odd, so that the codes are those of the exact
+//              fp32 where that holds it: weights within 2^+-60) times the root is rounded to odd, so that the codes are those of the exact
 //              norm (in fp32 alone some 4e-7 of them fall on the other side of a border).
 //
 // Bound: HBM.  add_rms reads x and d once, writes x' and 1.03 bytes of h per element.
@@ -116,7 +116,8 @@ __device__ __forceinline__ double wave_sum(double v) {
 __device__ __forceinline__ float product_to_odd(float a, float hi, float lo) {
   const float h = a * hi, rest = fmaf(a, lo, fmaf(a, hi, -h));
   const uint32_t u = __float_as_uint(h);
-  return rest == 0.f ? h : __uint_as_float((u - ((u ^ __float_as_uint(rest)) >> 31)) | 1u);
+  // (an infinity or a NaN leaves a NaN)
+  return !(rest < 0.f || rest > 0.f) ? h : __uint_as_float((u - ((u ^ __float_as_uint(rest)) >> 31)) | 1u);
 }
 
 // One workgroup per row, CH 16-byte chunks per thread; every load of the row is issued

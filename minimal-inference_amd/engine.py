@@ -434,7 +434,7 @@ class Scheduler:
                                   causal=True, max_total_q=total)
         plan = None
         if any(r.adapter >= 0 for r in reqs):
-            slot = torch.tensor([r.adapter for r, x in zip(reqs, lens) for _ in range(x)], dtype=torch.int32)
+            slot = torch.tensor([r.adapter for r in reqs], dtype=torch.int32).repeat_interleave(torch.tensor(lens))
             plan = AdapterPlan(total, self.adapter_slots, dev)
             plan.plan(slot.to(dev, non_blocking=True))
         be = self._backend(self.prefill_wrapper, "prefill", self.p_indptr[: n + 1], self.p_indices,

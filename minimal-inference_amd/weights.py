@@ -125,6 +125,8 @@ def load_adapter(model, slot: int, path: str) -> None:
             or cfg.get("rank_pattern") or cfg.get("alpha_pattern") or cfg.get("modules_to_save") or cfg.get("fan_in_fan_out"):
         raise ValueError(f"{path}: a plain low-rank adapter of one rank without biases expected")
     r = int(cfg["r"])
+    if r < 1:
+        raise ValueError(f"{path}: rank {r}")
     scale = float(cfg["lora_alpha"]) / (r ** 0.5 if cfg.get("use_rslora") else r)
     place = {piece: (name, i) for name, pieces in ADAPTED.items() for i, piece in enumerate(pieces)}
     found: dict[tuple[int, str, int], dict[str, torch.Tensor]] = {}

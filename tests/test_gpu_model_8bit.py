@@ -260,7 +260,7 @@ def test_load_adapter(dev, tmp_path):
     held = [t.clone() for L in model.layers for x in L.adapters.values() for t in (x.a, x.b, x.scale)]
     lone = {key.format(1, "self_attn.v_proj", "A"): torch.zeros(4, 256)}  # (an A without its B)
     wide = {key.format(1, "self_attn.v_proj", "A"): torch.zeros(9, 256), key.format(1, "self_attn.v_proj", "B"): torch.zeros(128, 9)}
-    bad = [(good | {key.format(1, "self_attn.o_proj", "A"): torch.zeros(4, 384)}, {}), (lone, {}), (wide, {"r": 9}), (good, {"r": 5}),
+    bad = [(good | {key.format(1, "self_attn.o_proj", "A"): torch.zeros(4, 384)}, {}), (lone, {}), (wide, {"r": 9}), (good, {"r": 5}), (good, {"r": 0}),
            (good | {key.format(3, "mlp.down_proj", "A"): torch.zeros(4, 672)}, {}), (good | {"x.weight": torch.zeros(1)}, {}),
            (good, {"use_dora": True}), (good, {"bias": "all"}), (good, {"peft_type": "IA3"})]
     for i, (tensors, config) in enumerate(bad):

@@ -144,6 +144,54 @@ def test_replays_and_streams(dev, rows):
     assert all(torch.equal(a, b) for j in range(2) for o in outs[j] for a, b in zip(o, want[j + 2]))
 
 
+@pytest.mark.parametrize("rows,other", [(3, 2), (3, 5), (600, 40), (40, 600)])
+def test_replay_after_another_batch(dev, rows, other):
+    """A replay after a plan of another number of rows gives NaN, everywhere and nowhere else, and after
+    its own the eager bits again."""
+    from minimal_inference_amd.adapters import AdapterPlan, add_adapters
+
+    layer = _Layer(dev)
+    x, y, slot = _inputs(dev, max(rows, other), 3, 1)
+    y = y.repeat(1, 2)[:, : 448 + 128].contiguous()
+    plan = AdapterPlan(max(rows, other), 3, dev)
+    room = torch.full((rows + 2, 448 + 128 + 8), 7.0, dtype=torch.bfloat16, device=dev)
+    out = room[1: rows + 1, : 448 + 128]
+    run = lambda: add_adapters(y[:rows], x[:rows], layer.on_qkv, plan, out=out)  # noqa: E731
+    plan.plan(slot[:rows])
+    want = run().clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for _ in range(3):
+        plan.plan(slot[:other])
+        graph.replay()
+        assert bool(out.isnan().all())
+        with pytest.raises(ValueError, match="the plan is of"):
+            run()
+        plan.plan(slot[:rows])
+        graph.replay()
+        assert torch.equal(out, want)
+    assert bool((room[0] == 7).all() and (room[-1] == 7).all() and (room[:, 448 + 128:] == 7).all())
+
+
+def test_norms_past_fp32(dev):
+    """Norms that fp32 does not hold make their block NaN, and leave the others as they are."""
+    from minimal_inference_amd.mxfp8 import add_rms_norm_mxfp8
+
+    g = torch.Generator(device=dev).manual_seed(3)
+    x = torch.randn(4, 256, device=dev, generator=g).to(torch.bfloat16)
+    w = torch.randn(256, device=dev, generator=g).to(torch.bfloat16)
+    x[:, 40] = torch.tensor([4.0, -4.0, 8.0, -8.0], dtype=torch.bfloat16, device=dev)  # (times w: an infinity of either sign)
+    want = add_rms_norm_mxfp8(x, None, w, 1e-6)
+    w2 = w.clone()
+    w2[40] = 3e38
+    got = add_rms_norm_mxfp8(x, None, w2, 1e-6)
+    assert bool((got.scales[:, 1] == 255).all()) and not bool(got.codes[:, 32:64].view(torch.uint8).any())
+    for a, b in ((got.scales, want.scales), (got.codes.view(torch.uint8), want.codes.view(torch.uint8))):
+        width = a.shape[1] // 8
+        assert torch.equal(a[:, :width], b[:, :width]) and torch.equal(a[:, 2 * width:], b[:, 2 * width:])
+
+
 def _whole(dev, rows, k, seed):
     """Whole numbers of -3..3 as MXFP8 with scales 1, 2 and 4, but the exact values' sums below 2^24."""
     from minimal_inference_amd.mxfp8 import MXFP8
