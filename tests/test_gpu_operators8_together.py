@@ -266,6 +266,30 @@ def test_gated_forms(dev, rows, n, k):
     assert bool((top * (1 - 2.0 ** -20) <= 448 * scale).all() and ((top * (1 + 2.0 ** -20) > 224 * scale) | (m.scales == 0)).all())
 
 
+@pytest.mark.parametrize("exponent", [1, -1, -4, -8, -16, -100])
+@pytest.mark.parametrize("rows", [3, 300])
+def test_gate_alone(dev, rows, exponent):
+    """Every code as a gate of a single product with an up of 1: silu within half a step of bf16 (2^-8 of the
+    value, 2^-134 below its least normal one, which fp32's least, 2^-149, and its products' roundings may add to)."""
+    from minimal_inference_amd.mxfp8 import MXFP8, linear_silu_mxfp8
+
+    every = torch.arange(256, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+    every = every[every.float().isfinite()]
+    n = every.numel()
+    x, w = MXFP8(rows, 32, dev), MXFP8(2 * n, 32, dev)
+    for m in (x, w):
+        m.anchor.zero_()
+        m.scales.fill_(127)
+    x.codes[:, 0] = torch.linspace(0.1, 3.5, rows, device=dev).to(torch.float8_e4m3fn)
+    x.codes[:, 1] = w.codes[n:, 1] = torch.ones((), device=dev).to(torch.float8_e4m3fn)
+    w.codes[:n, 0] = every
+    w.scales[:n] = 127 + exponent
+    gate = x.codes[:, :1].double() * every.double() * 2.0 ** exponent
+    want = gate * torch.sigmoid(gate)
+    got = linear_silu_mxfp8(x, w).double()
+    assert bool(((got - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -20) + 2.0 ** -134 + 2.0 ** -147).all())
+
+
 def test_past_32_bits(dev):
     """Codes of x, of the matrix and an output past 2^32 bytes, rows at the far end."""
     from minimal_inference_amd.mxfp8 import MXFP8, linear_mxfp8
