@@ -73,7 +73,8 @@ __device__ __forceinline__ void end_of_product(const LinearParams& p, const f32x
     return;
   }
   // Two tiles' lanes change places, so that a lane has eight columns and four lanes 64
-  // bytes of a row.
+  // bytes of a row.  All CUs come here at once and out is not read before the launch's end: stores
+  // that L2 need not keep (us, 40,960 x 4,096 x 4,096 537 -> 512, none at all 477; 1,024 x 4,096 x 4,096 24.5 -> 23.5).
   if constexpr (!SPLIT && !OUT8 && NT / HALVES % 2 == 0) {
     if (p.wide) {
 #pragma unroll
@@ -88,8 +89,9 @@ __device__ __forceinline__ void end_of_product(const LinearParams& p, const f32x
           const auto s1 = __builtin_amdgcn_permlane16_swap(u.y, v.y, false, false);
           const int m = row0 + b * 16 + n;
           if (m < rows && col < p.n)
-            *reinterpret_cast<u32x4_t*>(reinterpret_cast<uint16_t*>(p.out) + (m0 + m) * p.o_stride + col) =
-                u32x4_t{s0[0], s1[0], s0[1], s1[1]};
+            __builtin_nontemporal_store(
+                u32x4_t{s0[0], s1[0], s0[1], s1[1]},
+                reinterpret_cast<u32x4_t*>(reinterpret_cast<uint16_t*>(p.out) + (m0 + m) * p.o_stride + col));
         }
       }
       return;
