@@ -37,27 +37,30 @@ constexpr int kMaxParts = 16;
 constexpr int kGroup = 4;  // 16-rank tiles of a workgroup; of 8-bit rows in tiles of 64 half as many
 
 struct Tile {
-  int slot, first, count, unused;  // slot -1: rows without an adapter
+  int slot, count;  // slot -1: rows without an adapter
 };
 
-// A plan: the number of tiles and what it is a plan of in 16 bytes, the tiles, the rows in their order.
+// A plan: the number of tiles and what it is a plan of in 16 bytes, each tile's rows (in a place of their own,
+// so that they are read at once with the tile: a launch of few rows is a chain of such reads), the tiles.
 int64_t max_tiles(int64_t rows, int64_t slots) { return std::min(rows, slots + 1) + rows / tile_rows(rows); }
-size_t plan_size(int64_t rows, int64_t slots) { return 16 + 16 * size_t(max_tiles(rows, slots)) + 4 * size_t(rows); }
+size_t plan_size(int64_t rows, int64_t slots) {
+  return 16 + size_t(max_tiles(rows, slots)) * (sizeof(Tile) + 4 * size_t(tile_rows(rows)));
+}
 struct PlanView {
   int* count;
+  int* rows;
   Tile* tiles;
-  int* order;
 };
 PlanView view(void* plan, int64_t rows, int64_t slots) {
   char* const p = static_cast<char*>(plan);
-  return {reinterpret_cast<int*>(p), reinterpret_cast<Tile*>(p + 16),
-          reinterpret_cast<int*>(p + 16 + 16 * max_tiles(rows, slots))};
+  return {reinterpret_cast<int*>(p), reinterpret_cast<int*>(p + 16),
+          reinterpret_cast<Tile*>(p + 16 + 4 * tile_rows(rows) * max_tiles(rows, slots))};
 }
 
 constexpr int kPlanThreads = 1024;
 
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* slot_of_row, int rows, int slots, int tile_rows, PlanView p) {
-  __shared__ int count[kPlanThreads], first[kPlanThreads], tiles[kPlanThreads];
+  __shared__ int count[kPlanThreads], tiles[kPlanThreads];
   const int tid = threadIdx.x, lane = tid & 63;
   count[tid] = 0;
   __syncthreads();
@@ -79,23 +82,20 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* slot_of_r
   for (int row = tid; row < rows; row += kPlanThreads) places(at(row), count);
   __syncthreads();
   const int mine = count[tid], need = (mine + tile_rows - 1) / tile_rows;
-  first[tid] = mine;
   tiles[tid] = need;
   __syncthreads();
   for (int d = 1; d < kPlanThreads; d *= 2) {  // sums up to and with each slot
-    const int a = tid >= d ? first[tid - d] : 0, b = tid >= d ? tiles[tid - d] : 0;
+    const int a = tid >= d ? tiles[tid - d] : 0;
     __syncthreads();
-    first[tid] += a;
-    tiles[tid] += b;
+    tiles[tid] += a;
     __syncthreads();
   }
-  const int begin = first[tid] - mine, tile = tiles[tid] - need;
-  for (int i = 0; i < need; ++i)
-    p.tiles[tile + i] = {tid < slots ? tid : -1, begin + i * tile_rows, min(tile_rows, mine - i * tile_rows), 0};
+  const int tile = tiles[tid] - need;
+  for (int i = 0; i < need; ++i) p.tiles[tile + i] = {tid < slots ? tid : -1, min(tile_rows, mine - i * tile_rows)};
   if (tid == kPlanThreads - 1) p.count[0] = tiles[tid], p.count[1] = rows, p.count[2] = slots;
-  count[tid] = begin;
+  count[tid] = tile * tile_rows;  // (a slot's tiles lie one behind the other, so its rows do)
   __syncthreads();
-  for (int row = tid; row < rows; row += kPlanThreads) p.order[places(at(row), count)] = row;
+  for (int row = tid; row < rows; row += kPlanThreads) p.rows[places(at(row), count)] = row;
 }
 
 struct AdapterParams {
@@ -154,13 +154,15 @@ __device__ __forceinline__ void store_ranks(const AdapterParams& p, const f32x4_
 template <bool X8, int RT>
 __global__ __launch_bounds__(64 * kWaves) void shrink_few_kernel(AdapterParams p) {
   __shared__ __attribute__((aligned(16))) f32x4_t red[kWaves * RT * 64];
-  const int tiles = plan_tiles(p);
-  const Tile tile = p.plan.tiles[blockIdx.x];
-  if (int(blockIdx.x) >= tiles || tile.slot < 0) return;
   const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, n = lane & 15;
+  const int tiles = plan_tiles(p);
+  const Tile tile = p.plan.tiles[blockIdx.x];
+  const int* const order = p.plan.rows + blockIdx.x * 16;
+  const int own = order[n], any = order[0];
+  if (int(blockIdx.x) >= tiles || tile.slot < 0) return;
   const int rank0 = int(blockIdx.z) * p.group_ranks;
-  const int64_t row = p.plan.order[tile.first + (n < tile.count ? n : 0)];
+  const int64_t row = n < tile.count ? own : any;  // (past the tile's last row any will do)
   const char* const x = p.x + row * p.x_stride + (X8 ? 16 : 32) * g;
   const char* const xs = X8 ? p.xs + row * p.xs_stride + g / 2 : nullptr;
   const uint16_t* a[RT];
@@ -233,13 +235,14 @@ __global__ __launch_bounds__(64 * kManyWaves) void shrink_many_kernel(AdapterPar
   lds_t* const scales = lds + DEPTH * SLOT;
   const int g = lane >> 4, n = lane & 15;
   const int rank0 = int(blockIdx.z) * p.group_ranks, width = X8 ? p.k : 2 * p.k;  // bytes of a row of x
+  const int* const order = p.plan.rows + int64_t(blockIdx.x) * (16 * NB);
   // a load: 8 rows, lane l chunk slot l % 8 of row l / 8
   const int r8 = lane >> 3, chunk = ((lane & 7) ^ r8) * 16;
   const char* x[2 * NB];
 #pragma unroll
   for (int i = 0; i < 2 * NB; ++i) {
     const int at = i * 8 + r8;
-    x[i] = p.x + int64_t(p.plan.order[tile.first + (at < tile.count ? at : 0)]) * p.x_stride + chunk;
+    x[i] = p.x + int64_t(order[at < tile.count ? at : 0]) * p.x_stride + chunk;
   }
   const char* a[2 * RT];
 #pragma unroll
@@ -247,7 +250,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void shrink_many_kernel(AdapterPar
     const int r = rank0 + i * 8 + r8;  // (past the last rank any row will do: its sums are not kept)
     a[i] = reinterpret_cast<const char*>(p.a + (int64_t(tile.slot) * p.ranks + (r < p.ranks ? r : 0)) * p.k) + chunk;
   }
-  const char* const xs = X8 ? p.xs + int64_t(p.plan.order[tile.first + (lane < tile.count ? lane : 0)]) * p.xs_stride : nullptr;
+  const char* const xs = X8 ? p.xs + int64_t(order[lane < tile.count ? lane : 0]) * p.xs_stride : nullptr;
   auto dma = [&](const char* from, lds_t* to) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)const_cast<char*>(from),
@@ -380,10 +383,17 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
     return;
   }
   const Tile tile = p.plan.tiles[blockIdx.x];
-  if (int(blockIdx.x) >= tiles || (tile.slot < 0 && p.out == p.y)) return;
-  const bool adds = tile.slot >= 0;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int g = lane >> 4, n = lane & 15;
+  // wave w takes row block w (of a tile of one block the first wave)
+  const int* const order = p.plan.rows + int64_t(blockIdx.x) * ROWS;
+  int own[4] = {0, 0, 0, 0}, any = order[0];
+  if (w < NB) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) own[i] = order[w * 16 + 4 * g + i];
+  }
+  if (int(blockIdx.x) >= tiles || (tile.slot < 0 && p.out == p.y)) return;
+  const bool adds = tile.slot >= 0;
   const int nb = (tile.count + 15) / 16, groups = (c1 - c0 + 127) / 128;
   const int eighths = p.rank / 8;
   const uint16_t* const weights = p.b + int64_t(max(tile.slot, 0)) * p.n * p.rank;
@@ -407,7 +417,6 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
     }
   };
   fetch(0);
-  // wave w takes row block w
   struct Rows {
     uint4 y[4];
   };
@@ -415,7 +424,7 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int at = w * 16 + 4 * g + i;
-    row[i] = w < nb ? p.plan.order[tile.first + (at < tile.count ? at : 0)] : 0;
+    row[i] = at < tile.count ? own[i] : any;  // (past the tile's last row any will do)
   }
   auto load_rows = [&](Rows& r, int col) {
 #pragma unroll

@@ -114,17 +114,16 @@ def test_plan_lists_every_row_once(dev):
             continue
         height = 16 if rows <= 512 else 64
         most = min(rows, slots + 1) + rows // height
-        order = words[4 + 4 * most:]
-        assert torch.equal(order.sort()[0], torch.arange(rows, dtype=torch.int32))
-        tiles = words[4: 4 + 4 * int(words[0])].view(-1, 4)
-        assert 0 < int(words[0]) <= most
-        seen = 0
-        for s, first, count, _ in tiles.tolist():
-            mine = slot[order[first: first + count].long()]
+        assert 0 < int(words[0]) <= most and words[1:3].tolist() == [rows, slots]
+        lists = words[4: 4 + most * height].view(most, height)
+        seen = []
+        for i, (s, count) in enumerate(words[4 + most * height:][: 2 * int(words[0])].view(-1, 2).tolist()):
+            assert 0 < count <= height
+            seen.append(lists[i, :count])
+            mine = slot[seen[-1].long()]
             own = (mine == s) if s >= 0 else (mine < 0) | (mine >= slots)
-            assert 0 < count <= height and first == seen and bool(own.all())
-            seen += count
-        assert seen == rows
+            assert bool(own.all())
+        assert torch.equal(torch.cat(seen).sort()[0], torch.arange(rows, dtype=torch.int32))
 
 
 def test_a_row_depends_on_no_other(dev):
