@@ -499,7 +499,8 @@ int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void* x_scales,
  * mi_adapter_plan sorts a batch's rows by adapter, once for all its projections:
  * slot_of_row [rows] int32, an id outside 0..slots-1 (as -1) for none; at most 2^22
  * rows, 1,023 adapters.  plan: mi_adapter_plan_size bytes (of rows or more), 16-byte
- * aligned, written here and read by runs with the same rows and slots.
+ * aligned, written here and read by runs with the same rows and slots (others, as a replayed graph
+ * may hold them, leave NaN in out).
  *
  * mi_add_adapters: out = y + scale[s] * B[s] (A[s] x), one rounding to bf16, with row
  * t's adapter s; rows without one are y's.  y, out [rows][n] bf16; x [rows][k] bf16, or,
@@ -508,14 +509,14 @@ int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void* x_scales,
  * their own: a [slots][pieces * rank][k], b [slots][n][rank] bf16 contiguous, scale
  * [slots] fp32.  rank a multiple of 8 up to 128 (smaller ones padded with zeros), k of 32 up
  * to 2^20; rows of x, y and out 16-byte aligned.  out may be y itself; otherwise an out that
- * overlaps another argument is refused.  workspace: mi_add_adapters_workspace_size bytes,
- * need not be initialised, one call at a time.  A row's result depends on no other row.
+ * overlaps another argument is refused.  workspace: mi_add_adapters_workspace_size bytes (none
+ * for some calls), need not be initialised, one call at a time.  A row's result depends on no other row.
  * ------------------------------------------------------------------------ */
 size_t mi_adapter_plan_size(int64_t rows, int64_t slots);
 int mi_adapter_plan(void* plan, size_t plan_bytes, const int32_t* slot_of_row, int64_t rows,
                     int64_t slots, mi_stream_t stream);
 size_t mi_add_adapters_workspace_size(int64_t rows, int64_t slots, int64_t k, int64_t rank,
-                                      int64_t pieces);
+                                      int64_t pieces, int64_t n);
 int mi_add_adapters(const void* y, int64_t y_stride, const void* x, int64_t x_stride,
                     const void* x_scales, int64_t x_scales_stride, const void* a, const void* b,
                     const float* scale, int64_t slots, int64_t k, int64_t rank,

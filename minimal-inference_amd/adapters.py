@@ -5,7 +5,7 @@
 may be several pieces with factors of their own (q, k and v of a fused projection).
 ``AdapterPlan.plan(slot_of_row)`` sorts a batch's rows by adapter on the GPU, once for
 all of its layers and projections; ``add_adapters(y, x, adapters, plan)`` adds to y, in place
-or into ``out``, in two launches.  x is bf16 rows or an ``mxfp8.MXFP8`` matrix.  Sums are
+or into ``out``, in one or two launches.  x is bf16 rows or an ``mxfp8.MXFP8`` matrix.  Sums are
 fp32, rounded once.  There is no backward pass: tensors that ask for gradients or carry
 forward-mode tangents are refused.
 """
@@ -135,8 +135,8 @@ class AdapterPlan:
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_size(rows: int, slots: int, k: int, rank: int, pieces: int) -> int:
-    return int(_lib.load().mi_add_adapters_workspace_size(rows, slots, k, rank, pieces))
+def _workspace_size(rows: int, slots: int, k: int, rank: int, pieces: int, n: int) -> int:
+    return int(_lib.load().mi_add_adapters_workspace_size(rows, slots, k, rank, pieces, n))
 
 
 def add_adapters(y: torch.Tensor, x: torch.Tensor | MXFP8, adapters: Adapters, plan: AdapterPlan,
@@ -163,11 +163,11 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor | MXFP8, adapters: Adapters, p
     elif _rows_of("out", out) != (rows, n) or out.device != device:
         raise ValueError(f"out must be [{rows}, {n}] on {device}; got {tuple(out.shape)} on {out.device}")
     if rows:
-        room = _workspace_size(rows, adapters.slots, adapters.k, adapters.rank, len(adapters.pieces))
+        room = _workspace_size(rows, adapters.slots, adapters.k, adapters.rank, len(adapters.pieces), n)
         # (a tensor of this call's own: calls on several streams and in graphs share nothing)
-        workspace = torch.empty(room, dtype=torch.uint8, device=device)
+        workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
         call_on(y, "mi_add_adapters", y.data_ptr(), y.stride(0), data, stride, scales, s_stride, adapters.a.data_ptr(),
                 adapters.b.data_ptr(), adapters.scale.data_ptr(), adapters.slots, adapters.k, adapters.rank,
                 adapters.columns_ptr, len(adapters.pieces), out.data_ptr(), out.stride(0), plan.buffer.data_ptr(), rows,
-                workspace.data_ptr(), room)
+                workspace.data_ptr() if room else None, room)
     return out

@@ -6,6 +6,7 @@
 //            per batch.  Which row comes where in its adapter's tiles is of no matter: a row's
 //            result depends on its own operands alone.
 //   shrink : v = A x of a tile, k in parts over workgroups; sums in fp32.
+//   (few rows and a short A: both products in one launch)
 //   expand : the parts' sum, times scale, as a pair of bf16 (v and what its rounding left: 16
 //            bits of v), times B in fp32, plus y, one rounding.
 //
@@ -125,6 +126,82 @@ __device__ __forceinline__ int plan_tiles(const AdapterParams& p) {
   return p.plan.count[1] == p.rows && p.plan.count[2] == p.slots ? p.plan.count[0] : -1;
 }
 
+// A workgroup's columns: a chunk of one piece.
+struct Columns {
+  int piece, begin, end;
+};
+__device__ __forceinline__ Columns columns_of(const AdapterParams& p) {
+  int piece = 0;
+  while (int(blockIdx.y) >= p.end_chunk[piece]) ++piece;
+  const int start = piece ? p.end[piece - 1] : 0, before = piece ? p.end_chunk[piece - 1] : 0;
+  const int begin = start + (int(blockIdx.y) - before) * p.chunk;
+  return {piece, begin, min(begin + p.chunk, p.end[piece])};
+}
+// Where no row's adapter is known: NaN (the tiles are as many as the rows' at least).
+__device__ __forceinline__ void write_nan(const AdapterParams& p, int tile_rows, const Columns& c) {
+  for (int i = 0; i < tile_rows && int(blockIdx.x) * tile_rows + i < p.rows; ++i)
+    for (int col = c.begin + int(threadIdx.x); col < c.end; col += int(blockDim.x))
+      p.out[(int64_t(blockIdx.x) * tile_rows + i) * p.o_stride + col] = 0x7fc0;
+}
+// Four sums times scale as pairs of bf16: the values and what their rounding left.
+__device__ __forceinline__ uint4 bf16_pair(f32x4_t sum, float scale) {
+  uint32_t hi[2], lo[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float s = sum[2 * j] * scale, t = sum[2 * j + 1] * scale;
+    hi[j] = mi::cvt_pk_bf16(s, t);
+    const float ds = s - mi::bf16_lo(hi[j]), dt = t - mi::bf16_hi(hi[j]);
+    // (an infinity leaves nothing)
+    lo[j] = mi::cvt_pk_bf16(isfinite(mi::bf16_lo(hi[j])) ? ds : 0.f, isfinite(mi::bf16_hi(hi[j])) ? dt : 0.f);
+  }
+  return make_uint4(hi[0], hi[1], lo[0], lo[1]);
+}
+// y's eight columns with row i of eight products' sums.
+__device__ __forceinline__ uint4 add_rounded(uint4 y, const f32x4_t (&d)[8], int i) {
+  return make_uint4(mi::cvt_pk_bf16(mi::bf16_lo(y.x) + d[0][i], mi::bf16_hi(y.x) + d[1][i]),
+                    mi::cvt_pk_bf16(mi::bf16_lo(y.y) + d[2][i], mi::bf16_hi(y.y) + d[3][i]),
+                    mi::cvt_pk_bf16(mi::bf16_lo(y.z) + d[4][i], mi::bf16_hi(y.z) + d[5][i]),
+                    mi::cvt_pk_bf16(mi::bf16_lo(y.w) + d[6][i], mi::bf16_hi(y.w) + d[7][i]));
+}
+
+// 64 k of a wave's 16 rows of x and of RT tiles of A, straight from memory to registers.  Lane (g, n)
+// holds row n's k from 16 g on: its first eight are one product's operand, the other eight the next
+// one's.  (Which k comes where is of no matter as long as both operands agree.)
+template <bool X8, int RT>
+struct Step {
+  uint4 a[RT][2], x[2];
+  float s;
+  __device__ __forceinline__ void load(const AdapterParams& p, const uint16_t* const (&from)[RT], const char* row, const char* scales,
+                                       int step, int end) {
+    const int k0 = step * kStep, g = (threadIdx.x & 63) >> 4;
+    const bool in = step < end && k0 + 16 * g < p.k;
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      a[t][0] = in ? mi::load16(from[t] + k0) : none;
+      a[t][1] = in ? mi::load16(from[t] + k0 + 8) : none;
+    }
+    x[0] = in ? mi::load16(row + (X8 ? 1 : 2) * k0) : none;
+    if constexpr (X8) s = in ? mi::mx8::scale_f32(uint8_t(scales[k0 / 32])) : 0.f;
+    else x[1] = in ? mi::load16(row + 2 * k0 + 16) : none;
+  }
+  __device__ __forceinline__ void multiply(f32x4_t (&acc)[RT][1]) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      bf16x8_t v;
+      if constexpr (X8) {
+        const u32x2_t lo = mi::mx8::to_bf16(h ? x[0].z : x[0].x, s);
+        const u32x2_t hi = mi::mx8::to_bf16(h ? x[0].w : x[0].y, s);
+        v = mi::as_bf16x8(make_uint4(lo.x, lo.y, hi.x, hi.y));
+      } else {
+        v = mi::as_bf16x8(x[h]);
+      }
+#pragma unroll
+      for (int t = 0; t < RT; ++t) acc[t][0] = mi::mfma_16x16x32_bf16(mi::as_bf16x8(a[t][h]), v, acc[t][0]);
+    }
+  }
+};
+
 // The waves' sums of a tile's ranks to memory: lane (g, n) holds ranks 4 g .. 4 g + 3 of
 // tile t for row n of block b.
 template <int WAVES, int RT, int NB>
@@ -147,10 +224,7 @@ __device__ __forceinline__ void store_ranks(const AdapterParams& p, const f32x4_
   }
 }
 
-// Tiles of 16 rows: a wave takes steps of 64 k in turn, straight from memory to registers, the
-// next step's while this one is multiplied.  In a step lane (g, n) holds row n's k from 16 g on: its
-// first eight are one product's operand, the other eight the next one's.  (Which k comes
-// where is of no matter as long as both operands agree.)
+// Tiles of 16 rows: a wave takes steps in turn, the next one's on their way while this one is multiplied.
 template <bool X8, int RT>
 __global__ __launch_bounds__(64 * kWaves) void shrink_few_kernel(AdapterParams p) {
   __shared__ __attribute__((aligned(16))) f32x4_t red[kWaves * RT * 64];
@@ -172,70 +246,37 @@ __global__ __launch_bounds__(64 * kWaves) void shrink_few_kernel(AdapterParams p
     a[t] = p.a + (int64_t(tile.slot) * p.ranks + (r < p.ranks ? r : 0)) * p.k + 16 * g;
   }
   const int end = min((p.k + kStep - 1) / kStep, int(blockIdx.y + 1) * p.part_steps);
-  struct Set {
-    uint4 a[RT][2], x[2];
-    float s;
-  };
-  auto load = [&](Set& s, int step) {
-    const int k0 = step * kStep;
-    const bool in = step < end && k0 + 16 * g < p.k;
-    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      s.a[t][0] = in ? mi::load16(a[t] + k0) : none;
-      s.a[t][1] = in ? mi::load16(a[t] + k0 + 8) : none;
-    }
-    s.x[0] = in ? mi::load16(x + (X8 ? 1 : 2) * k0) : none;
-    if constexpr (X8) s.s = in ? mi::mx8::scale_f32(uint8_t(xs[k0 / 32])) : 0.f;
-    else s.x[1] = in ? mi::load16(x + 2 * k0 + 16) : none;
-  };
   f32x4_t acc[RT][1];
 #pragma unroll
   for (int t = 0; t < RT; ++t) acc[t][0] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  Set cur, next;
+  Step<X8, RT> cur, next;
   int step = int(blockIdx.y) * p.part_steps + w;
-  load(cur, step);
+  cur.load(p, a, x, xs, step, end);
   for (; step < end; step += kWaves) {
-    load(next, step + kWaves);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      bf16x8_t v;
-      if constexpr (X8) {
-        const u32x2_t lo = mi::mx8::to_bf16(h ? cur.x[0].z : cur.x[0].x, cur.s);
-        const u32x2_t hi = mi::mx8::to_bf16(h ? cur.x[0].w : cur.x[0].y, cur.s);
-        v = mi::as_bf16x8(make_uint4(lo.x, lo.y, hi.x, hi.y));
-      } else {
-        v = mi::as_bf16x8(cur.x[h]);
-      }
-#pragma unroll
-      for (int t = 0; t < RT; ++t) acc[t][0] = mi::mfma_16x16x32_bf16(mi::as_bf16x8(cur.a[t][h]), v, acc[t][0]);
-    }
+    next.load(p, a, x, xs, step + kWaves, end);
+    cur.multiply(acc);
     cur = next;
   }
   store_ranks<kWaves, RT, 1>(p, acc, red, tile.count, rank0);
 }
 
-// Tiles of 64 rows: as the few-row projections, a wave's rows go through a ring of its own in
-// LDS, two steps deep, eight rows of 128 bytes by an instruction (rows read as operands
-// straight from memory are 64 places an instruction, which the address unit takes one by one).
-// A step is 128 bytes of x: 64 k of bf16, 128 of 8 bits, which take two lots of A.
-template <bool X8, int RT>
-__global__ __launch_bounds__(64 * kManyWaves) void shrink_many_kernel(AdapterParams p) {
+// A wave's part of 16 RT ranks from rank0 on times a tile of 16 NB rows: as in the few-row projections, its
+// rows go through a ring of its own in LDS, two steps deep, eight rows of 128 bytes by an
+// instruction (rows read as operands straight from memory are 64 places an instruction, which
+// the address unit takes one by one).  A step is 128 bytes of x: 64 k of bf16, 128 of 8 bits, which
+// take two lots of A.  Steps first .. end - 1, the waves' in turn.
+constexpr int ring_bytes(bool x8, int rt, int nb) { return 2 * (nb + rt * (x8 ? 2 : 1)) * 2048 + (x8 ? 2048 : 0); }
+template <bool X8, int RT, int NB, int WAVES>
+__device__ __forceinline__ void multiply_ring(const AdapterParams& p, const Tile& tile, const int* order, mi::mx8::lds_t* lds, int rank0,
+                                              int first, int end, f32x4_t (&acc)[RT][NB]) {
   using namespace mi::mx8;
-  constexpr int WAVES = kManyWaves, NB = 4, LOTS = X8 ? 2 : 1, DEPTH = 2;
+  constexpr int LOTS = X8 ? 2 : 1, DEPTH = 2;
   constexpr int XBYTES = NB * 2048, SLOT = XBYTES + RT * LOTS * 2048, SBYTES = X8 ? 1024 : 0;
-  constexpr int WAVE = DEPTH * SLOT + 2 * SBYTES, LOADS = SLOT / 1024;
-  static_assert(WAVES * WAVE <= 80 * 1024 && RT * NB * 1024 <= WAVE, "LDS");
-  __shared__ __attribute__((aligned(16))) char smem[WAVES * WAVE];
-  const int tiles = plan_tiles(p);
-  const Tile tile = p.plan.tiles[blockIdx.x];
-  if (int(blockIdx.x) >= tiles || tile.slot < 0) return;
+  constexpr int LOADS = SLOT / 1024;
+  static_assert(DEPTH * SLOT + 2 * SBYTES == ring_bytes(X8, RT, NB), "LDS");
   const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = threadIdx.x & 63;
-  lds_t* const lds = (lds_t*)smem + w * WAVE;
   lds_t* const scales = lds + DEPTH * SLOT;
-  const int g = lane >> 4, n = lane & 15;
-  const int rank0 = int(blockIdx.z) * p.group_ranks, width = X8 ? p.k : 2 * p.k;  // bytes of a row of x
-  const int* const order = p.plan.rows + int64_t(blockIdx.x) * (16 * NB);
+  const int g = lane >> 4, n = lane & 15, width = X8 ? p.k : 2 * p.k;  // bytes of a row of x
   // a load: 8 rows, lane l chunk slot l % 8 of row l / 8
   const int r8 = lane >> 3, chunk = ((lane & 7) ^ r8) * 16;
   const char* x[2 * NB];
@@ -257,7 +298,6 @@ __global__ __launch_bounds__(64 * kManyWaves) void shrink_many_kernel(AdapterPar
                                      (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 #endif
   };
-  const int steps = (width + 127) / 128, first = int(blockIdx.y) * p.part_steps, end = min(steps, first + p.part_steps);
   // (behind the last k anything readable: it meets zeros, below)
   auto load = [&](int step, int slot) {
     lds_t* const to = lds + slot * SLOT;
@@ -278,7 +318,6 @@ __global__ __launch_bounds__(64 * kManyWaves) void shrink_many_kernel(AdapterPar
   const int lo = n * 128 + (g ^ (n & 7)) * 16, hi = n * 128 + ((4 + g) ^ (n & 7)) * 16;
   const int even = n * 128 + ((2 * g) ^ (n & 7)) * 16, odd = n * 128 + ((2 * g + 1) ^ (n & 7)) * 16;
 
-  f32x4_t acc[RT][NB];
 #pragma unroll
   for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -356,9 +395,26 @@ __global__ __launch_bounds__(64 * kManyWaves) void shrink_many_kernel(AdapterPar
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0070);  // (the loads past the end write to LDS)
+}
+
+template <bool X8, int RT>
+__global__ __launch_bounds__(64 * kManyWaves) void shrink_many_kernel(AdapterParams p) {
+  constexpr int WAVES = kManyWaves, NB = 4, WAVE = ring_bytes(X8, RT, NB);
+  static_assert(WAVES * WAVE <= 80 * 1024 && RT * NB * 1024 <= WAVE, "LDS");
+  __shared__ __attribute__((aligned(16))) char smem[WAVES * WAVE];
+  const int tiles = plan_tiles(p);
+  const Tile tile = p.plan.tiles[blockIdx.x];
+  if (int(blockIdx.x) >= tiles || tile.slot < 0) return;
+  const int w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  const int rank0 = int(blockIdx.z) * p.group_ranks, steps = ((X8 ? p.k : 2 * p.k) + 127) / 128;
+  const int first = int(blockIdx.y) * p.part_steps, end = min(steps, first + p.part_steps);
+  f32x4_t acc[RT][NB];
+  multiply_ring<X8, RT, NB, WAVES>(p, tile, p.plan.rows + int64_t(blockIdx.x) * (16 * NB), (mi::mx8::lds_t*)smem + w * WAVE, rank0,
+                                   first, end, acc);
   __syncthreads();
   store_ranks<WAVES, RT, NB>(p, acc, reinterpret_cast<f32x4_t*>(smem), tile.count, rank0);
 }
+
 
 // out = y + B v of a tile of 16 NB rows and a chunk of columns.  J: products of 32 that the
 // pairs of a piece's ranks take.  A unit of work is 16 rows by 128 columns, eight products
@@ -372,16 +428,9 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
   __shared__ __attribute__((aligned(16))) uint16_t vs[ROWS * VSTRIDE];
   __shared__ __attribute__((aligned(16))) uint16_t ws[2][kMaxWeights];
   const int tiles = plan_tiles(p);
-  int piece = 0;
-  while (int(blockIdx.y) >= p.end_chunk[piece]) ++piece;
-  const int begin = piece ? p.end[piece - 1] : 0, before = piece ? p.end_chunk[piece - 1] : 0;
-  const int c0 = begin + (int(blockIdx.y) - before) * p.chunk, c1 = min(c0 + p.chunk, p.end[piece]);
-  if (tiles < 0) {  // no row's adapter is known: NaN (the tiles are as many as the rows' at least)
-    for (int i = 0; i < ROWS && int(blockIdx.x) * ROWS + i < p.rows; ++i)
-      for (int c = c0 + int(threadIdx.x); c < c1; c += 64 * kWaves)
-        p.out[(int64_t(blockIdx.x) * ROWS + i) * p.o_stride + c] = 0x7fc0;
-    return;
-  }
+  const Columns columns = columns_of(p);
+  const int piece = columns.piece, c0 = columns.begin, c1 = columns.end;
+  if (tiles < 0) return write_nan(p, ROWS, columns);
   const Tile tile = p.plan.tiles[blockIdx.x];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int g = lane >> 4, n = lane & 15;
@@ -452,17 +501,9 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
       static_assert(kMaxParts == 16);
       add(0);
       if (p.n_parts > 8) add(8);
-      uint32_t hi[2], lo[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float s = sum[2 * j] * scale, t = sum[2 * j + 1] * scale;
-        hi[j] = mi::cvt_pk_bf16(s, t);
-        const float ds = s - mi::bf16_lo(hi[j]), dt = t - mi::bf16_hi(hi[j]);
-        // (an infinity leaves nothing)
-        lo[j] = mi::cvt_pk_bf16(isfinite(mi::bf16_lo(hi[j])) ? ds : 0.f, isfinite(mi::bf16_hi(hi[j])) ? dt : 0.f);
-      }
-      *reinterpret_cast<uint2*>(vs + row * VSTRIDE + r) = make_uint2(hi[0], hi[1]);
-      *reinterpret_cast<uint2*>(vs + row * VSTRIDE + p.rank + r) = make_uint2(lo[0], lo[1]);
+      const uint4 pair = bf16_pair(sum, scale);
+      *reinterpret_cast<uint2*>(vs + row * VSTRIDE + r) = make_uint2(pair.x, pair.y);
+      *reinterpret_cast<uint2*>(vs + row * VSTRIDE + p.rank + r) = make_uint2(pair.z, pair.w);
     }
   }
   int from[J];  // of a lane's eight ranks of product j, -1: past the last pair
@@ -496,17 +537,93 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint4 o = rows.y[i];
-        if (adds) {
-          o.x = mi::cvt_pk_bf16(mi::bf16_lo(o.x) + d[0][i], mi::bf16_hi(o.x) + d[1][i]);
-          o.y = mi::cvt_pk_bf16(mi::bf16_lo(o.y) + d[2][i], mi::bf16_hi(o.y) + d[3][i]);
-          o.z = mi::cvt_pk_bf16(mi::bf16_lo(o.z) + d[4][i], mi::bf16_hi(o.z) + d[5][i]);
-          o.w = mi::cvt_pk_bf16(mi::bf16_lo(o.w) + d[6][i], mi::bf16_hi(o.w) + d[7][i]);
-        }
+        const uint4 o = adds ? add_rounded(rows.y[i], d, i) : rows.y[i];
         if (col < c1 && w * 16 + 4 * g + i < tile.count) mi::store16(p.out + row[i] * p.o_stride + col, o);
       }
     }
     rows = next_rows;
+  }
+}
+
+// Both products of a tile of 16 rows in one launch: every workgroup multiplies the whole of x by its
+// piece's A, 8 or 16 waves sharing k, and then a chunk of B's columns, units of 128 as in expand_kernel, a
+// wave at a time.  A comes from L2 for all workgroups but an XCD's first; what is won is a launch and
+// the sums' way through memory.
+constexpr int whole_waves(bool x8) { return x8 ? 8 : 16; }
+template <bool X8>
+__global__ __launch_bounds__(64 * whole_waves(X8)) void whole_kernel(AdapterParams p) {
+  constexpr int RT = 1, WAVES = whole_waves(X8), J = RT, VSTRIDE = 32 * J + 8, WAVE = ring_bytes(X8, RT, 1);
+  static_assert(WAVES * WAVE <= 150 * 1024 && RT * 1024 <= WAVE && RT <= WAVES, "LDS");
+  __shared__ __attribute__((aligned(16))) char smem[WAVES * WAVE];
+  __shared__ __attribute__((aligned(16))) uint16_t vs[16 * VSTRIDE];
+  f32x4_t* const red = reinterpret_cast<f32x4_t*>(smem);
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int g = lane >> 4, n = lane & 15;
+  const int tiles = plan_tiles(p);
+  const Tile tile = p.plan.tiles[blockIdx.x];
+  const int* const order = p.plan.rows + blockIdx.x * 16;
+  const int any = order[0];
+  int mine[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mine[i] = order[4 * g + i];
+  const Columns c = columns_of(p);
+  if (tiles < 0) return write_nan(p, 16, c);
+  if (int(blockIdx.x) >= tiles || (tile.slot < 0 && p.out == p.y)) return;
+  const bool adds = tile.slot >= 0;
+  if (adds) {
+    f32x4_t acc[RT][1];
+    multiply_ring<X8, RT, 1, WAVES>(p, tile, order, (mi::mx8::lds_t*)smem + w * WAVE, c.piece * p.rank, 0,
+                                    ((X8 ? p.k : 2 * p.k) + 127) / 128, acc);
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < RT; ++t) red[(w * RT + t) * 64 + lane] = acc[t][0];
+  }
+  __syncthreads();
+  // lane (g, n) of tile t holds ranks 16 t + 4 g .. + 3 of row n
+  if (adds && tid < RT * 64) {
+    const int r = w * 16 + 4 * g;
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int o = 0; o < WAVES; ++o) sum += red[(o * RT + w) * 64 + lane];
+    if (r < p.rank) {
+      const uint4 pair = bf16_pair(sum, p.scale[tile.slot]);
+      *reinterpret_cast<uint2*>(vs + n * VSTRIDE + r) = make_uint2(pair.x, pair.y);
+      *reinterpret_cast<uint2*>(vs + n * VSTRIDE + p.rank + r) = make_uint2(pair.z, pair.w);
+    }
+  }
+  __syncthreads();
+  const int eighths = p.rank / 8;
+  const uint16_t* const weights = p.b + int64_t(max(tile.slot, 0)) * p.n * p.rank;
+  for (int c0 = c.begin + w * 128; c0 < c.end; c0 += WAVES * 128) {
+    const int col = c0 + 8 * n;
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+    uint4 y[4];
+    int64_t row[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      row[i] = 4 * g + i < tile.count ? mine[i] : any;
+      y[i] = col < c.end ? mi::load16_nt(p.y + row[i] * p.y_stride + col) : none;
+    }
+    f32x4_t d[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) d[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if (adds) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const bool in = 4 * j + g < 2 * eighths;  // (or past the last pair)
+        const int from = in ? (4 * j + g) % eighths * 8 : 0;
+        const uint4 q = *reinterpret_cast<const uint4*>(vs + n * VSTRIDE + (4 * j + g) * 8);
+        const bf16x8_t v = mi::as_bf16x8(in ? q : none);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const uint4 m = in && col < c.end ? mi::load16(weights + int64_t(col + t) * p.rank + from) : none;
+          d[t] = mi::mfma_16x16x32_bf16(v, mi::as_bf16x8(m), d[t]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col < c.end && 4 * g + i < tile.count) mi::store16(p.out + row[i] * p.o_stride + col, adds ? add_rounded(y[i], d, i) : y[i]);
   }
 }
 
@@ -561,6 +678,20 @@ Split split_of(int64_t rows, int64_t slots, int64_t k, int64_t padded, bool x8) 
   return s;
 }
 
+// One launch for few rows where its workgroups, which each read their piece's A, are a round at most, and A is
+// short (us in a graph, two launches / one; adapters of rank 16, as many tiles):
+//   1 row, 1 tile      k 896 -> 1,152 7.1 / 5.9    k 4,096 -> 6,144 7.5 / 6.7    k 8,192 -> 10,240 (16 rows) 8.6 / 11.6
+//                      k 14,336 -> 4,096 8.3 / 11.1
+//   32 rows, 8         k 4,096 -> 6,144 9.8 / 9.2  k 4,096 -> 28,672 12.3 / 17.6 (more than a round)
+//   40 rows, 20        k 896 -> 9,728 12.2 / 8.9
+//   48 rows, 24        k 3,584 -> 4,608 10.8 / 9.0 k 18,944 -> 3,584 12.1 / 16.3
+//   64 rows, 32        k 4,096 -> 6,144 14.7 / 11.3
+//   256 rows, 64       k 4,096 -> 6,144 22.0 / 22.5 (more than a round)
+constexpr int kMaxChunk = 1024;
+bool in_one_launch(int64_t rows, int64_t slots, int64_t k, int64_t rank, int64_t pieces, int64_t n) {
+  return tile_rows(rows) == 16 && rank <= 16 && k <= 4096 && max_tiles(rows, slots) * (n / kMaxChunk + pieces) <= mi::num_cus();
+}
+
 }  // namespace
 
 extern "C" size_t mi_adapter_plan_size(int64_t rows, int64_t slots) {
@@ -588,8 +719,9 @@ extern "C" int mi_adapter_plan(void* plan, size_t plan_bytes, const int32_t* slo
   return mi::check_launch(name);
 }
 
-extern "C" size_t mi_add_adapters_workspace_size(int64_t rows, int64_t slots, int64_t k, int64_t rank, int64_t pieces) {
+extern "C" size_t mi_add_adapters_workspace_size(int64_t rows, int64_t slots, int64_t k, int64_t rank, int64_t pieces, int64_t n) {
   if (check_shape("add_adapters_workspace_size", rows, slots, k, rank, pieces) || rows == 0) return 0;
+  if (in_one_launch(rows, slots, k, rank, pieces, n)) return 0;
   const int64_t padded = (pieces * rank + 15) / 16 * 16;
   return std::max(split_of(rows, slots, k, padded, false).bytes, split_of(rows, slots, k, padded, true).bytes);
 }
@@ -615,7 +747,7 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
   const int64_t each = x_scales ? 1 : 2;
   const int64_t scale_bytes = (k / 32 + 15) & ~int64_t(15);
   if (rows == 1) y_stride = out_stride = n, x_stride = (k + 15) & ~int64_t(15), x_scales_stride = scale_bytes;
-  if (!y || !x || !a || !b || !scale || !out || !plan || !workspace)
+  if (!y || !x || !a || !b || !scale || !out || !plan)
     return mi::fail(MI_ERR_INVALID, "%s: null pointer argument", name);
   const uintptr_t aligned = reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(a) |
                             reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(out) |
@@ -629,7 +761,9 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
   const int64_t padded = (pieces * rank + 15) / 16 * 16;
   const Split split = split_of(rows, slots, k, padded, x_scales != nullptr);
   const int64_t tiles = split.tiles;
-  const size_t need = split.bytes;
+  const bool whole = in_one_launch(rows, slots, k, rank, pieces, n);
+  const size_t need = whole ? 0 : split.bytes;
+  if (need && !workspace) return mi::fail(MI_ERR_INVALID, "%s: null pointer argument", name);
   if (workspace_bytes < need)
     return mi::fail(MI_ERR_WORKSPACE, "%s: the workspace takes %zu bytes, %zu given", name, need, workspace_bytes);
   // (rows of out are written while others are still read; a row of y only by who writes it)
@@ -642,7 +776,7 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
                            {b, 0, 1, slots * n * rank * 2},
                            {scale, 0, 1, slots * 4},
                            {plan, 0, 1, int64_t(plan_size(rows, slots))},
-                           {workspace, 0, 1, int64_t(need)}};
+                           {workspace, 0, need ? 1 : 0, int64_t(need)}};
   for (const mi::Rows& r : from)
     if (mi::rows_meet(to, r)) return mi::fail(MI_ERR_INVALID, "%s: out overlaps another argument (it may be y itself)", name);
   p.x = static_cast<const char*>(x);
@@ -670,16 +804,22 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
   p.part_steps = split.part_steps;
   p.n_parts = split.parts;
   p.group_ranks = int(((padded / 16 + split.groups - 1) / split.groups) * 16);
+  const bool x8 = p.xs != nullptr, many = tile_rows(rows) == 64;
   // columns of a workgroup: few where there are few tiles, so that every CU has some
   p.chunk = 128;
-  while (p.chunk < 1024 && tiles * ((n + p.chunk - 1) / p.chunk) > 8 * mi::num_cus()) p.chunk *= 2;
+  const int64_t enough = whole ? mi::num_cus() : 8 * mi::num_cus();
+  while (p.chunk < kMaxChunk && tiles * ((n + p.chunk - 1) / p.chunk) > enough) p.chunk *= 2;
   int chunks = 0;
   for (int i = 0; i < pieces; ++i) p.end_chunk[i] = chunks += (piece_columns[i] + p.chunk - 1) / p.chunk;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid(uint32_t(tiles), uint32_t(p.n_parts), uint32_t(split.groups)), block(64 * kWaves);
   const int rt = p.group_ranks / 16;
-  const bool x8 = p.xs != nullptr, many = tile_rows(rows) == 64;
   using Kernel = void (*)(AdapterParams);
+  if (whole) {
+    hipLaunchKernelGGL(x8 ? whole_kernel<true> : whole_kernel<false>, dim3(uint32_t(tiles), uint32_t(chunks)),
+                       dim3(64 * whole_waves(x8)), 0, s, p);
+    return mi::check_launch(name);
+  }
   const Kernel few[2][kGroup] = {
       {shrink_few_kernel<false, 1>, shrink_few_kernel<false, 2>, shrink_few_kernel<false, 3>, shrink_few_kernel<false, 4>},
       {shrink_few_kernel<true, 1>, shrink_few_kernel<true, 2>, shrink_few_kernel<true, 3>, shrink_few_kernel<true, 4>}};

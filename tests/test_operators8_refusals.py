@@ -104,7 +104,7 @@ def test_plan_sizes():
 
 
 ADAPT = dict(y=FAKE, ys=64, x=FAKE + (1 << 20), xs=96, xsc=None, xss=0, a=FAKE + (1 << 21), b=FAKE + (1 << 22), scale=FAKE + (1 << 23),
-             slots=3, k=96, rank=16, pieces=(48, 16), n_pieces=2, out=FAKE + (1 << 24), os=64, plan=FAKE + (1 << 25), rows=4,
+             slots=3, k=96, rank=24, pieces=(48, 16), n_pieces=2, out=FAKE + (1 << 24), os=64, plan=FAKE + (1 << 25), rows=4,
              work=FAKE + (1 << 26), bytes=1 << 24)
 
 
@@ -115,8 +115,8 @@ ADAPT = dict(y=FAKE, ys=64, x=FAKE + (1 << 20), xs=96, xsc=None, xss=0, a=FAKE +
     {"plan": None}, {"work": None}, {"y": FAKE + 8}, {"x": FAKE + 8}, {"a": FAKE + 8}, {"b": FAKE + 8}, {"scale": FAKE + 2}, {"ys": 68},
     {"os": 68}, {"os": 56}, {"xs": 100}, {"xs": -96}, {"xsc": FAKE + 8, "xss": 16}, {"xsc": FAKE + (1 << 19), "xss": 8},
     {"xsc": FAKE + (1 << 19), "xss": 0}, {"xsc": FAKE + (1 << 19), "xss": 16, "xs": 104},
-    {"out": FAKE + 16}, {"out": FAKE, "os": 72}, {"out": FAKE + (1 << 20)}, {"out": FAKE + (1 << 21) + 3 * 32 * 96 * 2 - 16},
-    {"out": FAKE + (1 << 22) + 3 * 64 * 16 * 2 - 16}, {"out": FAKE + (1 << 25)}, {"out": FAKE + (1 << 26)}, {"scale": FAKE + (1 << 24) + 8}])
+    {"out": FAKE + 16}, {"out": FAKE, "os": 72}, {"out": FAKE + (1 << 20)}, {"out": FAKE + (1 << 21) + 3 * 48 * 96 * 2 - 16},
+    {"out": FAKE + (1 << 22) + 3 * 64 * 24 * 2 - 16}, {"out": FAKE + (1 << 25)}, {"out": FAKE + (1 << 26)}, {"scale": FAKE + (1 << 24) + 8}])
 def test_add_adapters_refuses(change):
     a = ADAPT | change
     held = None if a["pieces"] is None else _pieces(*a["pieces"])
@@ -126,12 +126,13 @@ def test_add_adapters_refuses(change):
 
 def test_add_adapters_workspace():
     mod, lib = _lib()
-    need = lib.mi_add_adapters_workspace_size(4, 3, 96, 16, 2)
-    assert need > 0
+    assert lib.mi_add_adapters_workspace_size(4, 3, 96, 24, 2, 64) > 0  # (two launches)
+    assert lib.mi_add_adapters_workspace_size(4, 3, 96, 16, 2, 64) == 0  # (one)
     held = _pieces(48, 16)
     _refused("mi_add_adapters", ADAPT | {"pieces": ctypes.addressof(held), "bytes": 0}, "add_adapters", mod.MI_ERR_WORKSPACE)
     assert lib.mi_add_adapters(*(ADAPT | {"pieces": ctypes.addressof(held), "rows": 0, "y": None}).values(), None) == mod.MI_OK
-    for bad in ((-1, 3, 96, 16, 2), (4, 0, 96, 16, 2), (4, 3, 80, 16, 2), (4, 3, 96, 12, 2), (4, 3, 96, 16, 9), (0, 3, 96, 16, 2)):
+    for bad in ((-1, 3, 96, 24, 2, 64), (4, 0, 96, 24, 2, 64), (4, 3, 80, 24, 2, 64), (4, 3, 96, 12, 2, 64), (4, 3, 96, 24, 9, 64),
+                (0, 3, 96, 24, 2, 64)):
         assert lib.mi_add_adapters_workspace_size(*bad) == 0
 
 
