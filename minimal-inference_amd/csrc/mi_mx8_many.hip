@@ -145,7 +145,10 @@ __device__ __forceinline__ void mfma_in_place(u32x4_t alo, u32x4_t ahi, uint32_t
 // slots, and what does not fit in them is lost.
 // (us, 8,192 x 8,192 x 10,240 of normal values: two whole slabs staged and read at once 649;
 // these phases with addresses computed in place 649, with constants and pinned sums 503, a
-// barrier in every second phase 482; zeros 417: the clock follows the power that the products take.)
+// barrier in every second phase 485; all of it in L2 462, without the reads from LDS 459, without the loads
+// 421, without both 379, where products alone would take 314.  Zeros 413: the clock follows the power
+// that products and data take.  Workgroups that go from block to block, the next one's first loads under the
+// last one's stores, were no faster: 500 / 498.)
 template <bool GLU, bool OUT8>
 __global__ __launch_bounds__(256) void wide_kernel(LinearParams p) {
   constexpr int HALVES = GLU ? 2 : 1, BM = 256, BN = 256, COLS = BN / HALVES;
@@ -296,8 +299,9 @@ __global__ __launch_bounds__(256) void wide_kernel(LinearParams p) {
 // units of s + 1, into registers of their own; after the barrier of slab s the buffers are
 // filled again that slab s - 1 has read, four slabs ahead.
 //
-// Bound: the way from L2 to LDS, 32 KB for 16 products a wave; at 0.58 us a slab 256 workgroups take 14.5 TB/s of it
-// (2,048 x 8,192 x 10,240 212 us; without the loads 133, without the reads from LDS 208).
+// Bound: the operands' way, 32 KB for 16 products a wave, and what lies beyond L2 of it: 0.61 us a slab, with
+// all of it in L2 0.42 (1,024 x 4,096 x 4,096 24.0 and 18.3 us; 2,048 x 8,192 x 10,240 212, without the
+// loads 133, without the reads from LDS 208).  LDS has no room for more slabs ahead.
 //
 // SPLIT: the workgroup takes p.split_slabs slabs (a multiple of four) and leaves its sums, in
 // fp32, for combine_kernel.
@@ -468,14 +472,15 @@ __global__ __launch_bounds__(256) void combine_kernel(LinearParams p, int parts)
 
 // ---------------------------------------------------------------- which form
 // The time of a launch, counted: its start, and for every round of workgroups their own start and end
-// and a slab's time for every slab; the last round is the faster, the fewer CUs it takes (they
-// share the power).  Workgroups that share k add the combining launch with the parts' way to memory and
-// back.  Counted and measured (us): 8,192 x 8,192 x 10,240 wide 498 / 482, 2,048 x 8,192 x
-// 10,240 wide 184 / 175, block 213 / 212; 1,000 x 4,096 x 6,144 wide 49 / 46, block 45 / 46; 600 x 14,336 x 4,096
-// block 75 / 73, in 3 parts 72 / 71, wide 143 / 131; 512 x 3,584 x 4,608 block 22 / 23; 200 x 4,096 x
-// 6,144 in 2 parts 22 / 21; 77 x 18,944 x 3,584 in 8 parts 24 / 27, whole 94 / 89; 128 x
-// 4,096 x 4,096 in 4 parts 17 / 19.  (Blocks of 128 x 256 were no faster than either in any of
-// these, nor two workgroups of 128 x 128 on a CU.)
+// and a slab's time for every slab; of the largest blocks the last round is the faster, the fewer CUs it
+// takes (they share the power), of the others where another round has left W in the caches.  Workgroups
+// that share k add the combining launch with the parts' way to memory and back.  Counted and measured (us,
+// calls in a graph): 8,192 x 8,192 x 10,240 wide 482 / 491, 2,048 x 8,192 x 10,240 wide 178 / 173, block 209 / 207;
+// 18,240 x 4,096 x 6,144 wide 356 / 349; 1,000 x 4,096 x 6,144 wide 47 / 45, block 43 / 45; 700 rows of it block
+// 41 / 37, wide 46 / 45; 600 x 14,336 x 4,096 block 74 / 74, in 3 parts 71 / 70, wide 137 / 131; 512 x 3,584 x
+// 4,608 block 23 / 23; 200 x 4,096 x 6,144 block 25 / 23, in 2 parts 22 / 21; 77 x 18,944 x 3,584 in 8 parts
+// 24 / 27, whole 96 / 89; 128 x 4,096 x 4,096 in 4 parts 17 / 19.  (Blocks of 128 x 256 were no faster than
+// either in any of these, nor two workgroups of 128 x 128 on a CU.)
 constexpr float kStartUs = 3.5f, kCombineUs = 2.5f, kBytesPerUs = 4.4e6f;
 constexpr int kMaxParts = 32;
 enum class Form { few, block, wide };
@@ -488,12 +493,15 @@ struct Choice {
   int64_t rest;  // rows behind the last whole block, for a launch of their own
 };
 
-float rounds_us(int64_t workgroups, int slabs, float own, float least, float more) {
+// A slab of a round on every CU takes least + more.
+float rounds_us(int64_t workgroups, int slabs, float own, float least, float more, bool first_is_whole) {
   const int cus = mi::num_cus();
   const int64_t whole = workgroups / cus, last = workgroups % cus;
-  return kStartUs + float(whole) * (own + slabs * (least + more)) +
-         (last ? own + slabs * (least + more * float(last) / float(cus)) : 0.f);
+  const float part = first_is_whole && !whole ? 1.f : float(last) / float(cus);
+  return kStartUs + float(whole) * (own + slabs * (least + more)) + (last ? own + slabs * (least + more * part) : 0.f);
 }
+float wide_us(int64_t workgroups, int slabs) { return rounds_us(workgroups, slabs, 6.f, 1.05f, 0.35f, false); }
+float block_us(int64_t workgroups, int slabs) { return rounds_us(workgroups, slabs, 2.f, 0.41f, 0.2f, true); }
 // The few-row kernel's (up to 64 rows): W's bytes from memory, x's into every workgroup.
 float few_us(int64_t rows, int64_t w_rows, int slabs) {
   const float k = float(slabs) * kSlab, workgroups = std::max(1.f, std::min(float(w_rows) / 16, float(w_rows) / 64));
@@ -504,10 +512,10 @@ float few_us(int64_t rows, int64_t w_rows, int slabs) {
 Choice choose(bool glu, int64_t rows, int64_t n, int slabs, size_t room) {
   if (rows <= kFewRows) return {0.f, Form::few, 1, slabs, 0, 0};
   const int64_t w_rows = glu ? 2 * n : n, across = (w_rows + 255) / 256;
-  Choice best = {rounds_us((rows + 255) / 256 * across, slabs, 6.f, 1.1f, 0.35f), Form::wide, 1, slabs, 0, 0};
+  Choice best = {wide_us((rows + 255) / 256 * across, slabs), Form::wide, 1, slabs, 0, 0};
   // (8,201 x 8,192 x 10,240: 33 rows of blocks are a round more than 32 and a launch of nine rows)
   if (const int64_t rest = rows % 256; rest && rest <= kFewRows && rest < rows) {
-    const float us = rounds_us(rows / 256 * across, slabs, 6.f, 1.1f, 0.35f) + few_us(rest, w_rows, slabs);
+    const float us = wide_us(rows / 256 * across, slabs) + few_us(rest, w_rows, slabs);
     if (us < best.us) best.us = us, best.rest = rest;
   }
   const int64_t block = (rows + 127) / 128 * ((w_rows + 127) / 128);
@@ -516,8 +524,7 @@ Choice choose(bool glu, int64_t rows, int64_t n, int slabs, size_t room) {
     if (parts != want || (want > 1 && block * (want - 1) >= 2 * mi::num_cus())) continue;
     const size_t bytes = want > 1 ? size_t(want) * (glu ? 2 : 1) * rows * ((n + 3) / 4) * 16 : 0;
     if (bytes > room) continue;
-    const float us = rounds_us(block * want, each, 1.5f, 0.53f, 0.07f) +
-                     (want > 1 ? kCombineUs + 2 * float(bytes) / kBytesPerUs : 0.f);
+    const float us = block_us(block * want, each) + (want > 1 ? kCombineUs + 2 * float(bytes) / kBytesPerUs : 0.f);
     if (us < best.us) best = {us, Form::block, want, each, bytes, 0};
   }
   return best;
