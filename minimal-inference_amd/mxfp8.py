@@ -177,7 +177,7 @@ def add_rms_norm_mxfp8(x: torch.Tensor, delta: torch.Tensor | None, weight: torc
                        x_out: torch.Tensor | None = None, out: MXFP8 | None = None) -> MXFP8:
     """``dense.add_rms_norm`` with its norm in 8 bits: ``x + delta`` rounded to bf16 (into ``x_out``,
     in place in ``x`` when that is not given; without ``delta`` x itself, which is then not written),
-    and its ``rms_norm(...) * weight`` in fp32, quantised from there as ``quantize_mxfp8`` does.
+    and its ``rms_norm(...) * weight``, quantised as its exact value would be (blocks past fp32's range become NaN).
     Outputs that overlap each other, the weight or another row's input are refused."""
     shape, grad = x.shape, torch.is_grad_enabled()
     if len(shape) != 2:
