@@ -24,8 +24,13 @@ using mi::f32x4_t;
 using mi::mx8::u32x2_t;
 using mi::mx8::u32x4_t;
 
-// Rows of a tile: 16 up to 512 rows, 64 beyond (see mi_add_adapters).
-constexpr int64_t kFewRows = 512;
+// Rows of a tile: 16 up to 320 rows, 64 beyond, which read A a quarter as often (us in a graph, 16 / 64, with 1,
+// 8 and 64 adapters at 512 rows, 4 and 32 at the others, one launch for none):
+//                           256 rows               512 rows                            1,024 rows
+//   k  4,096 ->  6,144, 16  11.4 / 13.1 15.8 / 18.0  16.9 / 15.4 17.3 / 18.2 23.8 / 24.6  24.3 / 23.0 25.2 / 20.5
+//   k  4,096 -> 28,672, 16  19.0 / 18.7 29.7 / 30.1  31.3 / 24.5 30.3 / 24.8 50.8 / 52.0  53.7 / 38.0 56.2 / 44.5
+//   k 14,336 ->  4,096, 64  21.2 / 20.6 35.5 / 34.7  29.6 / 24.5 31.7 / 25.6 57.1 / 50.3  44.7 / 32.5 56.3 / 41.6
+constexpr int64_t kFewRows = 320;
 constexpr int tile_rows(int64_t rows) { return rows <= kFewRows ? 16 : 64; }
 constexpr int kMaxSlots = 1023;  // (and one more count for the rows without)
 constexpr int kMaxRank = 128;
@@ -696,7 +701,7 @@ bool in_one_launch(int64_t rows, int64_t slots, int64_t k, int64_t rank, int64_t
 
 extern "C" size_t mi_adapter_plan_size(int64_t rows, int64_t slots) {
   if (check_plan("adapter_plan_size", rows, slots)) return 0;
-  // (of fewer rows too: those in tiles of 16 may take more)
+  // (of fewer rows too: tiles of 16 may take more)
   return std::max(plan_size(rows, slots), plan_size(std::min(rows, kFewRows), slots));
 }
 

@@ -61,7 +61,7 @@ def _want(values, ad, slot, y):
 @pytest.mark.parametrize("k,pieces,rank", [(32, [16], 8), (96, [48, 16], 16), (896, [896, 128, 128], 16), (1056, [304], 24),
                                            (544, [64, 32, 16], 64), (4864, [896], 32), (256, [160, 160], 128),
                                            (160, [16] * 8, 8)])
-@pytest.mark.parametrize("rows,slots", [(1, 1), (3, 5), (17, 2), (64, 1), (130, 7), (300, 40), (512, 3), (513, 3), (1000, 1),
+@pytest.mark.parametrize("rows,slots", [(1, 1), (3, 5), (17, 2), (64, 1), (130, 7), (300, 40), (320, 3), (321, 3), (512, 3), (513, 3), (1000, 1),
                                         (900, 30)])
 def test_add_adapters(dev, rows, slots, k, pieces, rank, x8):
     """Odd numbers of rows and adapters, rows without one among them; in place and into an out, whose
@@ -112,7 +112,7 @@ def test_plan_lists_every_row_once(dev):
         if rows == 0:
             assert int(words[0]) == 0
             continue
-        height = 16 if rows <= 512 else 64
+        height = 16 if rows <= 320 else 64
         most = min(rows, slots + 1) + rows // height
         assert 0 < int(words[0]) <= most and words[1:3].tolist() == [rows, slots]
         lists = words[4: 4 + most * height].view(most, height)
