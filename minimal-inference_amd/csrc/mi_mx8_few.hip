@@ -1,7 +1,7 @@
 // Projections of few rows with both operands in MXFP8 (decode steps): out = x W^T (+ bias)
 // or silu(x Wg^T) * (x Wu^T), fp32 accumulation and one rounding.
 //
-// Bound: HBM, the one read of W, 1.03 bytes per weight.  A workgroup of 4 or 8 waves owns
+// Bound: HBM, the one read of W, 1.03 bytes per weight.  A workgroup of 1 to 8 waves owns
 // 16 R rows of W over all of k and the waves split k: wave w takes the groups of four slabs
 // w, w + WAVES, ...  Its rows of a slab (of W and of x) go from memory into a ring of its own in
 // LDS, DEPTH slabs ahead, eight rows of 128 bytes by an instruction, and from there, as
@@ -181,10 +181,11 @@ void run(const LinearParams& p, hipStream_t stream) {
 // The form of a launch, from the tiles of W and the 16-row blocks of x (us, weights rotated
 // through 600 MB, calls in a graph; R tiles by 4 or 8 waves, 2 or 4 slabs deep):
 //                            rows  1 4x8  1 4x4  1 2x4  2 2x8  2 2x4  3 2x8  3 2x4  4 2x4  6 2x4
-//   N   896 K   896             8    3.3    3.3    3.7           3.9
-//   N   896 K  4864             8    5.7    6.3    7.1    7.3
-//   N  4096 K  4096             1    6.5    6.4    6.6    6.7
-//   N  3584 K 18944             1   15.5   19.0   21.7   19.5
+//   N   896 K   896             8    3.2    3.2    3.7           3.9
+//   N   896 K  4864             8    5.7    5.4    7.1    7.3
+//   N  4096 K  4096             1    6.5    6.0    6.6    6.7
+//   N  3584 K 18944             1   15.5   14.6   19.1   19.4
+//   N  4096 K 14336            16   14.3   13.9   15.0   18.6
 //   N  4096 K 14336            32          19.6   20.4   22.4   24.0         27.6
 //   N  4096 K 14336            64                 25.3          29.8         35.3   40.6
 //   N  6144 K  4096             1           8.8    8.2    7.6    8.2    8.7    8.6
@@ -200,17 +201,32 @@ void run(const LinearParams& p, hipStream_t stream) {
 //   gated 2 x 29568, K 8192     1                        99.0   84.1                89.4   94.6
 //   gated 2 x 29568, K 8192    64                              141.2               116.8
 // Every workgroup reads x, so as many tiles as make one round of workgroups, four at most;
-// eight waves with a single block of x up to three tiles.  Beyond three rounds a single
+// eight waves with a single block of x and two or three.  Beyond three rounds a single
 // block takes two, whose workgroups run side by side.
+// Four tiles by as many waves as leave room for all workgroups at once: no round starts with empty rings
+// (us, gated, 4 / 2 / 1 waves, * where all fit):
+//   2 x 14336, K 4096  32 rows 30.7 / 27.3* / 28.6*   64 rows 34.5 / 31.0* / 32.9*
+//   2 x 18944, K 3584   1 row  28.8 / 27.2* / 26.0*   64 rows 39.0 / 45.1 / 36.7*
+//   2 x 29568, K 8192  32 rows 99.4 / 100.6 / 100.2*  64 rows 116.5 / 114.1 / 110.2*
+template <int MB, bool GLU, bool OUT8>
+void run_four(const LinearParams& p, hipStream_t stream) {
+  constexpr int COLS = 64 / (GLU ? 2 : 1), kLds = 160 * 1024, kWave = few_lds(4, MB, 2, 1);
+  const int64_t workgroups = (p.n + COLS - 1) / COLS, cus = mi::num_cus();
+  if (workgroups <= cus * (kLds / (4 * kWave))) run<4, MB, 2, GLU, OUT8, 4>(p, stream);
+  else if (workgroups <= cus * (kLds / (2 * kWave))) run<4, MB, 2, GLU, OUT8, 2>(p, stream);
+  else if (workgroups <= cus * (kLds / kWave)) run<4, MB, 2, GLU, OUT8, 1>(p, stream);
+  else run<4, MB, 2, GLU, OUT8, 4>(p, stream);
+}
+
 template <int MB, bool GLU, bool OUT8>
 void pick(const LinearParams& p, hipStream_t stream) {
   if constexpr (OUT8) {
-    run<4, MB, 2, GLU, OUT8, 4>(p, stream);  // (whole blocks of out)
+    run_four<MB, GLU, OUT8>(p, stream);  // (whole blocks of out)
   } else {
     const int tiles = (p.w_rows + 15) / 16, cus = mi::num_cus(), rounds = (tiles + cus - 1) / cus;
     if constexpr (!GLU) {
       if (rounds <= 1) {
-        if constexpr (MB == 1) return run<1, MB, 4, GLU, OUT8, 8>(p, stream);
+        if constexpr (MB == 1) return run<1, MB, 4, GLU, OUT8, 4>(p, stream);
         else return run<1, MB, MB == 2 ? 4 : 2, GLU, OUT8, 4>(p, stream);
       }
       if (rounds == 3) return run<3, MB, 2, GLU, OUT8, MB == 1 ? 8 : 4>(p, stream);
@@ -219,7 +235,7 @@ void pick(const LinearParams& p, hipStream_t stream) {
       }
     }
     if (rounds <= 2 || (MB == 1 && rounds > 3)) run<2, MB, 2, GLU, OUT8, 4>(p, stream);
-    else run<4, MB, 2, GLU, OUT8, 4>(p, stream);
+    else run_four<MB, GLU, OUT8>(p, stream);
   }
 }
 

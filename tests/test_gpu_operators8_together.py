@@ -211,7 +211,7 @@ def _values32(m):
 # rows, n, k: by the kernel's forms. Few rows: 1..64 by counts of 16 and of waves over k, alone and sharing k; blocks of 128 x 128, whole and
 # split over k; blocks of 256 x 256, alone, with rows behind them as few rows, as a block, and with ragged columns and k.
 FORMS = [(1, 33, 32), (1, 4864, 896), (7, 100, 14336), (16, 28672, 512), (17, 20000, 96), (31, 1000, 4128), (48, 257, 8192), (64, 30000, 128),
-         (33, 4099, 12320), (20, 8192, 16416), (64, 3584, 18944), (47, 100, 8192),
+         (40, 40000, 96), (33, 82000, 64), (33, 4099, 12320), (20, 8192, 16416), (64, 3584, 18944), (47, 100, 8192),
          (65, 48, 32), (65, 129, 8224), (200, 1000, 544), (300, 2048, 18944), (1024, 4096, 512),
          (2048, 1056, 8192), (2057, 8192, 1024), (4096, 4112, 288), (4200, 4096, 1056), (2304, 8193, 4096), (8201, 2048, 4064)]
 
@@ -244,7 +244,7 @@ def test_without_a_workspace(dev, monkeypatch, rows, n, k):
     assert torch.equal(mxfp8.linear_mxfp8(x, w), want)
 
 
-@pytest.mark.parametrize("rows,n,k", [(1, 64, 64), (20, 4864, 896), (64, 14336, 4096), (65, 96, 64), (300, 1120, 18944), (1030, 4096, 512),
+@pytest.mark.parametrize("rows,n,k", [(1, 64, 64), (20, 4864, 896), (64, 14336, 4096), (60, 18944, 512), (5, 18944, 416), (33, 41024, 96), (65, 96, 64), (300, 1120, 18944), (1030, 4096, 512),
                                       (2057, 8192, 1024), (4200, 2080, 1056)])
 def test_gated_forms(dev, rows, n, k):
     """SiLU(gate) * up of exact products: bf16 by one rounding of fp32's value (2^-8, and 2^-20 for the exponential
