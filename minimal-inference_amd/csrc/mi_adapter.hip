@@ -13,6 +13,7 @@
 // Bound: for prompts HBM, one read of x, one of y and the write of out; A and B come from the
 // caches.  For decode steps the two launches' start and end, and the read of the adapters.
 #include <algorithm>
+#include <cmath>
 
 #include "mi_mx8.h"
 #include "mi_overlap.h"
@@ -671,9 +672,14 @@ Split split_of(int64_t rows, int64_t slots, int64_t k, int64_t padded, bool x8) 
     best = std::max<int64_t>(1, std::min<int64_t>(most, (2 * cus + s.tiles * s.groups - 1) / (s.tiles * s.groups)));
   } else {
     s.groups = int((rank_tiles + group - 1) / group);
-    int64_t least = INT64_MAX;  // rounds of workgroups, of their steps and a start of twelve
+    // rounds of workgroups (a part of one counts half of a whole more: they start as others end), of their steps
+    // and a start of twelve, and the parts' way (us of both launches in a graph, counted parts and the best measured:
+    // 1,031 x 3,584 -> 4,608, rank 16 in 6 18.3, 1 29.0, 12 20.3; 18,240 x 4,096 -> 6,144 in 3 150, 1 154, 6 162;
+    // 18,240 x 14,336 -> 4,096, 8 bits in 3 154, 1 174; 8,201 x 8,192 -> 10,240, rank 64 in 1 164, 4 190)
+    float least = 1e30f;
     for (int64_t parts = 1; parts <= std::min<int64_t>(kMaxParts, each / unit); ++parts) {
-      const int64_t rounds = (s.tiles * s.groups * parts + 2 * cus - 1) / (2 * cus), cost = rounds * ((each + parts - 1) / parts + 12);
+      const float r = float(s.tiles * s.groups * parts) / float(2 * cus), rounds = r <= 1.f ? 1.f : (std::ceil(r) + r) / 2;
+      const float cost = rounds * (float(each) / float(parts) + 12.f) + 0.8f * float(parts);
       if (cost < least) least = cost, best = parts;
     }
   }
