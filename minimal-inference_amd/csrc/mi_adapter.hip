@@ -672,14 +672,18 @@ Split split_of(int64_t rows, int64_t slots, int64_t k, int64_t padded, bool x8) 
     best = std::max<int64_t>(1, std::min<int64_t>(most, (2 * cus + s.tiles * s.groups - 1) / (s.tiles * s.groups)));
   } else {
     s.groups = int((rank_tiles + group - 1) / group);
-    // rounds of workgroups (a part of one counts half of a whole more: they start as others end), of their steps
-    // and a start of twelve, and the parts' way (us of both launches in a graph, counted parts and the best measured:
-    // 1,031 x 3,584 -> 4,608, rank 16 in 6 18.3, 1 29.0, 12 20.3; 18,240 x 4,096 -> 6,144 in 3 150, 1 154, 6 162;
-    // 18,240 x 14,336 -> 4,096, 8 bits in 3 154, 1 174; 8,201 x 8,192 -> 10,240, rank 64 in 1 164, 4 190)
+    // rounds of workgroups (a part of one counts two thirds and more of a whole), of their steps and a start of
+    // twelve, and the parts' way (us of both launches in a graph, by parts, * taken):
+    //   1,031 x  3,584 ->  4,608, rank 16          1 29.0   2 21.1   5 17.7   6 18.1*  12 20.4
+    //   4,105 x  4,096 ->  6,144, rank 16          1 50.5   2 44.8   4 49.5*  6 50.8    8 58.2
+    //  18,240 x  4,096 ->  6,144, rank 16          1 153*   2 162    3 149    4 154     6 160
+    //  the same, an eighth of the rows without     1 137*            3 144
+    //  18,240 x 14,336 ->  4,096, rank 16, 8 bits  1 171    2 153    3 151*   6 149    12 152
+    //   8,201 x  8,192 -> 10,240, rank 64          1 169*   2 170    3 176    6 189
     float least = 1e30f;
     for (int64_t parts = 1; parts <= std::min<int64_t>(kMaxParts, each / unit); ++parts) {
-      const float r = float(s.tiles * s.groups * parts) / float(2 * cus), rounds = r <= 1.f ? 1.f : (std::ceil(r) + r) / 2;
-      const float cost = rounds * (float(each) / float(parts) + 12.f) + 0.8f * float(parts);
+      const float r = float(s.tiles * s.groups * parts) / float(2 * cus), rounds = r <= 1.f ? 1.f : (2 * std::ceil(r) + r) / 3;
+      const float cost = rounds * (float(each) / float(parts) + 12.f) + (0.6f + 0.012f * float(s.tiles)) * float(parts);
       if (cost < least) least = cost, best = parts;
     }
   }
