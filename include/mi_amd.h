@@ -510,7 +510,8 @@ int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void* x_scales,
  * [slots] fp32.  rank a multiple of 8 up to 128 (smaller ones padded with zeros), k of 32 up
  * to 2^20; rows of x, y and out 16-byte aligned.  out may be y itself; otherwise an out that
  * overlaps another argument is refused.  workspace: mi_add_adapters_workspace_size bytes (none
- * for some calls), need not be initialised, one call at a time.  A row's result depends on no other row.
+ * for some calls), need not be initialised, one call at a time.  A row's result depends on no other
+ * row's values (the order of its sums on the number of rows).
  * ------------------------------------------------------------------------ */
 size_t mi_adapter_plan_size(int64_t rows, int64_t slots);
 int mi_adapter_plan(void* plan, size_t plan_bytes, const int32_t* slot_of_row, int64_t rows,

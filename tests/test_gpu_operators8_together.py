@@ -244,6 +244,39 @@ def test_without_a_workspace(dev, monkeypatch, rows, n, k):
     assert torch.equal(mxfp8.linear_mxfp8(x, w), want)
 
 
+@pytest.mark.parametrize("rows,n,k", [(64, 3584, 18944), (33, 4099, 12320), (77, 512, 8192)])
+def test_captured_with_parts(dev, rows, n, k):
+    """Graphs of products whose workgroups share k, two of them replayed in turn with other inputs between and
+    at once on two streams: each has parts of its own."""
+    from minimal_inference_amd import mxfp8
+
+    assert mxfp8._workspace_size(rows, n, k, False) > 0
+    sets = [(_whole(dev, rows, k, i), _whole(dev, n, k, 10 + i)) for i in range(2)]
+    want = [mxfp8.linear_mxfp8(*s).clone() for s in sets]
+    graphs = []
+    for s in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = mxfp8.linear_mxfp8(*s)
+        graphs.append((graph, out))
+    for turn in range(6):
+        for i in (turn % 2, 1 - turn % 2):
+            graphs[i][1].fill_(7)
+            graphs[i][0].replay()
+            assert torch.equal(mxfp8.linear_mxfp8(*sets[1 - i]), want[1 - i])
+            assert torch.equal(graphs[i][1], want[i])
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    for _, out in graphs:
+        out.fill_(7)
+    torch.cuda.synchronize(dev)
+    for _ in range(8):
+        for (graph, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize(dev)
+    assert all(torch.equal(out, w) for (_, out), w in zip(graphs, want))
+
+
 @pytest.mark.parametrize("rows,n,k", [(1, 64, 64), (20, 4864, 896), (64, 14336, 4096), (60, 18944, 512), (5, 18944, 416), (33, 41024, 96), (65, 96, 64), (300, 1120, 18944), (1030, 4096, 512),
                                       (2057, 8192, 1024), (4200, 2080, 1056)])
 def test_gated_forms(dev, rows, n, k):
