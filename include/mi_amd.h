@@ -509,7 +509,10 @@ int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void* x_scales,
  * their own: a [slots][pieces * rank][k], b [slots][n][rank] bf16 contiguous, scale
  * [slots] fp32.  rank a multiple of 8 up to 128 (smaller ones padded with zeros), k of 32 up
  * to 2^20; rows of x, y and out 16-byte aligned.  out may be y itself; otherwise an out that
- * overlaps another argument is refused.  workspace: mi_add_adapters_workspace_size bytes (none
+ * overlaps another argument is refused.  silu != 0: the two pieces are gate and up, as many
+ * columns each, and out [rows][n / 2] = silu(gate) * up of the sums, held in fp32 up to the one
+ * rounding: bf16, or, out_scales not null, MXFP8 (n / 2 a multiple of 32, strides in bytes); y is
+ * left as it is.  workspace: mi_add_adapters_workspace_size bytes (none
  * for some calls), need not be initialised, one call at a time.  A row's result depends on no other
  * row's values (the order of its sums on the number of rows).
  * ------------------------------------------------------------------------ */
@@ -517,13 +520,13 @@ size_t mi_adapter_plan_size(int64_t rows, int64_t slots);
 int mi_adapter_plan(void* plan, size_t plan_bytes, const int32_t* slot_of_row, int64_t rows,
                     int64_t slots, mi_stream_t stream);
 size_t mi_add_adapters_workspace_size(int64_t rows, int64_t slots, int64_t k, int64_t rank,
-                                      int64_t pieces, int64_t n);
+                                      int64_t pieces, int64_t n, int32_t silu);
 int mi_add_adapters(const void* y, int64_t y_stride, const void* x, int64_t x_stride,
                     const void* x_scales, int64_t x_scales_stride, const void* a, const void* b,
                     const float* scale, int64_t slots, int64_t k, int64_t rank,
                     const int32_t* piece_columns, int64_t pieces, void* out, int64_t out_stride,
-                    const void* plan, int64_t rows, void* workspace, size_t workspace_bytes,
-                    mi_stream_t stream);
+                    void* out_scales, int64_t out_scales_stride, const void* plan, int64_t rows,
+                    int32_t silu, void* workspace, size_t workspace_bytes, mi_stream_t stream);
 
 /* ------------------------------------------------------------------------ *
  * One draw per row from given uniform numbers, with top-k, top-p and min-p.

@@ -116,11 +116,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "mi_adapter_plan_size": (_c_sz, [_c_i64, _c_i64]),
     "mi_adapter_plan": (_c_i32, [_vp, _c_sz, _vp, _c_i64, _c_i64, _vp]),
-    "mi_add_adapters_workspace_size": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64]),
+    "mi_add_adapters_workspace_size": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32]),
     "mi_add_adapters": (
         _c_i32,
         [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp,
-         _c_i64, _vp, _c_sz, _vp],
+         _c_i64, _vp, _c_i64, _c_i32, _vp, _c_sz, _vp],
     ),
     "mi_draw_workspace_size": (_c_sz, [_c_i32, _c_i32]),
     "mi_draw": (

@@ -5,7 +5,8 @@
 may be several pieces with factors of their own (q, k and v of a fused projection).
 ``AdapterPlan.plan(slot_of_row)`` sorts a batch's rows by adapter on the GPU, once for
 all of its layers and projections; ``add_adapters(y, x, adapters, plan)`` adds to y, in place
-or into ``out``, in one or two launches.  x is bf16 rows or an ``mxfp8.MXFP8`` matrix.  Sums are
+or into ``out``, in one or two launches; ``add_adapters_silu``
+ends in SiLU(gate) * up, the down projection's input.  x is bf16 rows or an ``mxfp8.MXFP8`` matrix.  Sums are
 fp32, rounded once.  There is no backward pass: tensors that ask for gradients or carry
 forward-mode tangents are refused.
 """
@@ -19,7 +20,7 @@ import torch
 
 from . import _lib
 from ._util import call_on, refuse_derivatives, require_dtype, require_gpu, require_i32_vector
-from .mxfp8 import MXFP8, _rows_of
+from .mxfp8 import MXFP8, _out, _rows8, _rows_of
 
 MAX_SLOTS = 1023
 MAX_RANK = 128
@@ -135,14 +136,11 @@ class AdapterPlan:
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_size(rows: int, slots: int, k: int, rank: int, pieces: int, n: int) -> int:
-    return int(_lib.load().mi_add_adapters_workspace_size(rows, slots, k, rank, pieces, n))
+def _workspace_size(rows: int, slots: int, k: int, rank: int, pieces: int, n: int, silu: bool) -> int:
+    return int(_lib.load().mi_add_adapters_workspace_size(rows, slots, k, rank, pieces, n, silu))
 
 
-def add_adapters(y: torch.Tensor, x: torch.Tensor | MXFP8, adapters: Adapters, plan: AdapterPlan,
-                 out: torch.Tensor | None = None) -> torch.Tensor:
-    """``y[t] + scale[s] * B[s] @ (A[s] @ x[t])`` with s row t's adapter in the plan; rows without one are
-    y's.  Into ``out``, in place in y when that is not given; an out that overlaps another argument is refused."""
+def _add(y, x, adapters, plan, out, silu: bool, quantize: bool):
     rows, n = _rows_of("y", y)
     device = y.device
     if not isinstance(adapters, Adapters) or not isinstance(plan, AdapterPlan):
@@ -158,16 +156,36 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor | MXFP8, adapters: Adapters, p
         raise ValueError(f"the plan is of {plan.rows} rows and {plan.slots} adapters, the call of {rows} and {adapters.slots}")
     if not device == at == adapters.device == plan.device:
         raise ValueError(f"y on {device}, x on {at}, the adapters on {adapters.device}, the plan on {plan.device}")
-    if out is None:
-        out = y
-    elif _rows_of("out", out) != (rows, n) or out.device != device:
-        raise ValueError(f"out must be [{rows}, {n}] on {device}; got {tuple(out.shape)} on {out.device}")
+    if silu and (len(adapters.pieces) != 2 or adapters.pieces[0] != adapters.pieces[1]):
+        raise ValueError(f"SiLU is of gate and up, two pieces of as many columns; got {adapters.pieces}")
+    out_scales, out_s_stride = None, 0
+    if quantize:
+        out = _rows8(out, rows, n // 2, device)
+        to, out_stride, out_scales, out_s_stride = out.codes_ptr, out.codes_stride, out.scales_ptr, out.scales_stride
+    else:
+        out = y if out is None and not silu else _out(out, rows, n // 2 if silu else n, device)
+        to, out_stride = out.data_ptr(), out.stride(0)
     if rows:
-        room = _workspace_size(rows, adapters.slots, adapters.k, adapters.rank, len(adapters.pieces), n)
+        room = _workspace_size(rows, adapters.slots, adapters.k, adapters.rank, len(adapters.pieces), n, silu)
         # (a tensor of this call's own: calls on several streams and in graphs share nothing)
         workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
         call_on(y, "mi_add_adapters", y.data_ptr(), y.stride(0), data, stride, scales, s_stride, adapters.a.data_ptr(),
                 adapters.b.data_ptr(), adapters.scale.data_ptr(), adapters.slots, adapters.k, adapters.rank,
-                adapters.columns_ptr, len(adapters.pieces), out.data_ptr(), out.stride(0), plan.buffer.data_ptr(), rows,
-                workspace.data_ptr() if room else None, room)
+                adapters.columns_ptr, len(adapters.pieces), to, out_stride, out_scales, out_s_stride, plan.buffer.data_ptr(),
+                rows, silu, workspace.data_ptr() if room else None, room)
     return out
+
+
+def add_adapters(y: torch.Tensor, x: torch.Tensor | MXFP8, adapters: Adapters, plan: AdapterPlan,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """``y[t] + scale[s] * B[s] @ (A[s] @ x[t])`` with s row t's adapter in the plan; rows without one are
+    y's.  Into ``out``, in place in y when that is not given; an out that overlaps another argument is refused."""
+    return _add(y, x, adapters, plan, out, False, False)
+
+
+def add_adapters_silu(y: torch.Tensor, x: torch.Tensor | MXFP8, adapters: Adapters, plan: AdapterPlan,
+                      out: "torch.Tensor | MXFP8 | None" = None, *, quantize: bool = False) -> "torch.Tensor | MXFP8":
+    """``silu(gate) * up`` of what ``add_adapters`` makes of a fused gate and up projection's y [rows, 2 n], held in
+    fp32 up to the one rounding: bf16 [rows, n], or with ``quantize`` MXFP8 (n a multiple of 32).  y is left
+    as it is; the adapters have two pieces of n columns."""
+    return _add(y, x, adapters, plan, out, True, quantize)

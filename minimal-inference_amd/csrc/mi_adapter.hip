@@ -8,7 +8,8 @@
 //   shrink : v = A x of a tile, k in parts over workgroups; sums in fp32.
 //   (few rows and a short A: both products in one launch)
 //   expand : the parts' sum, times scale, as a pair of bf16 (v and what its rounding left: 16
-//            bits of v), times B in fp32, plus y, one rounding.
+//            bits of v), times B in fp32, plus y, one rounding; or SiLU(gate) * up of the sums of a
+//            gate and an up piece.
 //
 // Bound: for prompts HBM, one read of x, one of y and the write of out; A and B come from the
 // caches.  For decode steps the two launches' start and end, and the read of the adapters.
@@ -123,6 +124,9 @@ struct AdapterParams {
   int k, n, rank, ranks, padded;  // ranks = pieces * rank, padded to 16
   int n_parts, part_steps, max_tiles, group_ranks;
   int pieces, chunk;  // columns of an expand workgroup
+  int up;             // the first of the up columns, with SiLU
+  uint8_t* scales;    // of out in 8 bits
+  int64_t s_stride;
   int end[kMaxPieces];       // columns,
   int end_chunk[kMaxPieces]; // chunks up to and with each piece
 };
@@ -143,11 +147,22 @@ __device__ __forceinline__ Columns columns_of(const AdapterParams& p) {
   const int begin = start + (int(blockIdx.y) - before) * p.chunk;
   return {piece, begin, min(begin + p.chunk, p.end[piece])};
 }
+// What becomes of the sums: out's bf16, or, of gate and up columns, SiLU(gate) * up in bf16 or 8 bits.
+enum class End { plain, silu, silu8 };
+
 // Where no row's adapter is known: NaN (the tiles are as many as the rows' at least).
+template <End END>
 __device__ __forceinline__ void write_nan(const AdapterParams& p, int tile_rows, const Columns& c) {
   for (int i = 0; i < tile_rows && int(blockIdx.x) * tile_rows + i < p.rows; ++i)
-    for (int col = c.begin + int(threadIdx.x); col < c.end; col += int(blockDim.x))
-      p.out[(int64_t(blockIdx.x) * tile_rows + i) * p.o_stride + col] = 0x7fc0;
+    for (int col = c.begin + int(threadIdx.x); col < c.end; col += int(blockDim.x)) {
+      const int64_t row = int64_t(blockIdx.x) * tile_rows + i;
+      if constexpr (END == End::silu8) {
+        reinterpret_cast<uint8_t*>(p.out)[row * p.o_stride + col] = 0;
+        if (col % mi::mx8::kBlock == 0) p.scales[row * p.s_stride + col / mi::mx8::kBlock] = 255;
+      } else {
+        p.out[row * p.o_stride + col] = 0x7fc0;
+      }
+    }
 }
 // Four sums times scale as pairs of bf16: the values and what their rounding left.
 __device__ __forceinline__ uint4 bf16_pair(f32x4_t sum, float scale) {
@@ -425,18 +440,20 @@ __global__ __launch_bounds__(64 * kManyWaves) void shrink_many_kernel(AdapterPar
 // out = y + B v of a tile of 16 NB rows and a chunk of columns.  J: products of 32 that the
 // pairs of a piece's ranks take.  A unit of work is 16 rows by 128 columns, eight products
 // side by side: column c of product t is column 8 c + t of the unit, so that lane (g, n) ends with
-// columns 8 n .. 8 n + 7 of rows 4 g .. 4 g + 3, 16 bytes of y and out in the order of the lanes.
-template <int NB, int J>
+// columns 8 n .. 8 n + 7 of rows 4 g .. 4 g + 3, 16 bytes of y and out in the order of the lanes.  With SiLU a
+// unit of gate columns and the same of up columns follow each other, and the gate's values wait in fp32.
+template <int NB, int J, End END>
 __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
   constexpr int ROWS = 16 * NB, kPair = 32 * J;  // a row's ranks in bf16, and what the rounding left of them
   constexpr int VSTRIDE = kPair + 8;              // (the rows of an operand on distinct banks)
   constexpr int kMaxWeights = 128 * (kPair / 2) + 128;  // a unit's columns of B: eight of them, then 16 bytes apart
-  __shared__ __attribute__((aligned(16))) uint16_t vs[ROWS * VSTRIDE];
+  constexpr int HALVES = END == End::plain ? 1 : 2;
+  __shared__ __attribute__((aligned(16))) uint16_t vs[HALVES][ROWS * VSTRIDE];
   __shared__ __attribute__((aligned(16))) uint16_t ws[2][kMaxWeights];
   const int tiles = plan_tiles(p);
   const Columns columns = columns_of(p);
   const int piece = columns.piece, c0 = columns.begin, c1 = columns.end;
-  if (tiles < 0) return write_nan(p, ROWS, columns);
+  if (tiles < 0) return write_nan<END>(p, ROWS, columns);
   const Tile tile = p.plan.tiles[blockIdx.x];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int g = lane >> 4, n = lane & 15;
@@ -447,20 +464,21 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) own[i] = order[w * 16 + 4 * g + i];
   }
-  if (int(blockIdx.x) >= tiles || (tile.slot < 0 && p.out == p.y)) return;
+  if (int(blockIdx.x) >= tiles || (END == End::plain && tile.slot < 0 && p.out == p.y)) return;
   const bool adds = tile.slot >= 0;
-  const int nb = (tile.count + 15) / 16, groups = (c1 - c0 + 127) / 128;
+  const int nb = (tile.count + 15) / 16, units = (c1 - c0 + 127) / 128 * HALVES;
   const int eighths = p.rank / 8;
   const uint16_t* const weights = p.b + int64_t(max(tile.slot, 0)) * p.n * p.rank;
 
   // the weights of a unit's 128 columns, 16 bytes a thread and lot
   constexpr int LOTS = (128 * (kPair / 2) / 8 + 64 * kWaves - 1) / (64 * kWaves);
   uint4 wv[LOTS];
-  auto fetch = [&](int group) {
+  auto fetch = [&](int unit) {
+    const int up = unit % HALVES * p.up;
 #pragma unroll
     for (int i = 0; i < LOTS; ++i) {
-      const int e = i * 64 * kWaves + tid, col = c0 + group * 128 + e / eighths;
-      wv[i] = adds && e < 128 * eighths && col < c1 ? mi::load16(weights + int64_t(col) * p.rank + e % eighths * 8)
+      const int e = i * 64 * kWaves + tid, col = c0 + unit / HALVES * 128 + e / eighths;
+      wv[i] = adds && e < 128 * eighths && col < c1 ? mi::load16(weights + int64_t(up + col) * p.rank + e % eighths * 8)
                                                     : make_uint4(0u, 0u, 0u, 0u);
     }
   };
@@ -481,20 +499,21 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
     const int at = w * 16 + 4 * g + i;
     row[i] = at < tile.count ? own[i] : any;  // (past the tile's last row any will do)
   }
-  auto load_rows = [&](Rows& r, int col) {
+  auto load_rows = [&](Rows& r, int unit) {
+    const int col = c0 + unit / HALVES * 128 + 8 * n, up = unit % HALVES * p.up;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      r.y[i] = w < nb && col < c1 ? mi::load16_nt(p.y + row[i] * p.y_stride + col) : make_uint4(0u, 0u, 0u, 0u);
+      r.y[i] = w < nb && col < c1 ? mi::load16_nt(p.y + row[i] * p.y_stride + up + col) : make_uint4(0u, 0u, 0u, 0u);
   };
   Rows rows, next_rows;
-  load_rows(rows, c0 + 8 * n);
+  load_rows(rows, 0);
   if (adds) {
     const float scale = p.scale[tile.slot];
     const int fours = p.rank / 4;
     const int64_t part = int64_t(p.max_tiles) * ROWS * p.padded;
-    for (int i = tid; i < tile.count * fours; i += 64 * kWaves) {
-      const int row = i / fours, r = i % fours * 4;
-      const float* const from = p.parts + (int64_t(blockIdx.x) * ROWS + row) * p.padded + piece * p.rank + r;
+    for (int i = tid; i < tile.count * fours * HALVES; i += 64 * kWaves) {
+      const int row = i / (fours * HALVES), half = i / fours % HALVES, r = i % fours * 4;
+      const float* const from = p.parts + (int64_t(blockIdx.x) * ROWS + row) * p.padded + (piece + half) * p.rank + r;
       f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
       auto add = [&](int first) {  // eight on their way at once, added in their order
         f32x4_t v[8];
@@ -508,19 +527,20 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
       add(0);
       if (p.n_parts > 8) add(8);
       const uint4 pair = bf16_pair(sum, scale);
-      *reinterpret_cast<uint2*>(vs + row * VSTRIDE + r) = make_uint2(pair.x, pair.y);
-      *reinterpret_cast<uint2*>(vs + row * VSTRIDE + p.rank + r) = make_uint2(pair.z, pair.w);
+      *reinterpret_cast<uint2*>(vs[half] + row * VSTRIDE + r) = make_uint2(pair.x, pair.y);
+      *reinterpret_cast<uint2*>(vs[half] + row * VSTRIDE + p.rank + r) = make_uint2(pair.z, pair.w);
     }
   }
   int from[J];  // of a lane's eight ranks of product j, -1: past the last pair
 #pragma unroll
   for (int j = 0; j < J; ++j) from[j] = 4 * j + g < 2 * eighths ? (4 * j + g) % eighths * 8 : -1;
-  for (int group = 0; group < groups; ++group) {
-    const int col = c0 + group * 128 + 8 * n, buf = group & 1;
+  float gate[END == End::plain ? 1 : 4][8];
+  auto step = [&]<int HALF>(int unit) {
+    const int col = c0 + unit / HALVES * 128 + 8 * n, buf = unit & 1;
     keep(buf);
-    if (group + 1 < groups) {
-      fetch(group + 1);
-      load_rows(next_rows, col + 128);
+    if (unit + 1 < units) {
+      fetch(unit + 1);
+      load_rows(next_rows, unit + 1);
     }
     __syncthreads();
     if (w < nb) {
@@ -531,7 +551,7 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           const uint4 none = make_uint4(0u, 0u, 0u, 0u);
-          const uint4 q = *reinterpret_cast<const uint4*>(vs + (w * 16 + n) * VSTRIDE + (4 * j + g) * 8);
+          const uint4 q = *reinterpret_cast<const uint4*>(vs[HALF] + (w * 16 + n) * VSTRIDE + (4 * j + g) * 8);
           const bf16x8_t v = mi::as_bf16x8(from[j] >= 0 ? q : none);
 #pragma unroll
           for (int t = 0; t < 8; ++t) {
@@ -543,11 +563,42 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint4 o = adds ? add_rounded(rows.y[i], d, i) : rows.y[i];
-        if (col < c1 && w * 16 + 4 * g + i < tile.count) mi::store16(p.out + row[i] * p.o_stride + col, o);
+        const bool in = col < c1 && w * 16 + 4 * g + i < tile.count;
+        if constexpr (END == End::plain) {
+          const uint4 o = adds ? add_rounded(rows.y[i], d, i) : rows.y[i];
+          if (in) mi::store16(p.out + row[i] * p.o_stride + col, o);
+        } else {
+          const uint32_t y[4] = {rows.y[i].x, rows.y[i].y, rows.y[i].z, rows.y[i].w};
+          float v[8];
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            v[t] = (t % 2 ? mi::bf16_hi(y[t / 2]) : mi::bf16_lo(y[t / 2])) + d[t][i];
+            if constexpr (HALF == 0) gate[i][t] = mi::mx8::silu20(v[t]);
+            else v[t] *= gate[i][t];
+          }
+          if constexpr (HALF == 1 && END == End::silu) {
+            if (in)
+              mi::store16(p.out + row[i] * p.o_stride + col, make_uint4(mi::cvt_pk_bf16(v[0], v[1]), mi::cvt_pk_bf16(v[2], v[3]),
+                                                                       mi::cvt_pk_bf16(v[4], v[5]), mi::cvt_pk_bf16(v[6], v[7])));
+          } else if constexpr (HALF == 1) {  // (a block's 32 columns are four lanes')
+            uint32_t top = 0;
+#pragma unroll
+            for (int t = 0; t < 8; ++t) top = max(top, mi::mx8::magnitude(v[t]));
+            const uint32_t byte = mi::mx8::scale_byte(mi::mx8::max4(top));
+            if (in) {
+              *reinterpret_cast<u32x2_t*>(reinterpret_cast<uint8_t*>(p.out) + row[i] * p.o_stride + col) =
+                  u32x2_t{mi::mx8::to_codes(v[0], v[1], v[2], v[3], byte), mi::mx8::to_codes(v[4], v[5], v[6], v[7], byte)};
+              if (n % 4 == 0) p.scales[row[i] * p.s_stride + col / mi::mx8::kBlock] = uint8_t(byte);
+            }
+          }
+        }
       }
     }
     rows = next_rows;
+  };
+  for (int unit = 0; unit < units; unit += HALVES) {
+    step.template operator()<0>(unit);
+    if constexpr (HALVES == 2) step.template operator()<1>(unit + 1);
   }
 }
 
@@ -573,7 +624,7 @@ __global__ __launch_bounds__(64 * whole_waves(X8)) void whole_kernel(AdapterPara
 #pragma unroll
   for (int i = 0; i < 4; ++i) mine[i] = order[4 * g + i];
   const Columns c = columns_of(p);
-  if (tiles < 0) return write_nan(p, 16, c);
+  if (tiles < 0) return write_nan<End::plain>(p, 16, c);
   if (int(blockIdx.x) >= tiles || (tile.slot < 0 && p.out == p.y)) return;
   const bool adds = tile.slot >= 0;
   if (adds) {
@@ -693,6 +744,14 @@ Split split_of(int64_t rows, int64_t slots, int64_t k, int64_t padded, bool x8) 
   return s;
 }
 
+template <End END>
+auto expand_of(bool many, int j) {
+  using Kernel = void (*)(AdapterParams);
+  const Kernel kernels[2][4] = {{expand_kernel<1, 1, END>, expand_kernel<1, 2, END>, expand_kernel<1, 4, END>, expand_kernel<1, 8, END>},
+                                {expand_kernel<4, 1, END>, expand_kernel<4, 2, END>, expand_kernel<4, 4, END>, expand_kernel<4, 8, END>}};
+  return kernels[many][j];
+}
+
 // One launch for few rows where its workgroups, which each read their piece's A, are a round at most, and A is
 // short (us in a graph, two launches / one; adapters of rank 16, as many tiles):
 //   1 row, 1 tile      k 896 -> 1,152 7.1 / 5.9    k 4,096 -> 6,144 7.5 / 6.7    k 8,192 -> 10,240 (16 rows) 8.6 / 11.6
@@ -734,9 +793,10 @@ extern "C" int mi_adapter_plan(void* plan, size_t plan_bytes, const int32_t* slo
   return mi::check_launch(name);
 }
 
-extern "C" size_t mi_add_adapters_workspace_size(int64_t rows, int64_t slots, int64_t k, int64_t rank, int64_t pieces, int64_t n) {
+extern "C" size_t mi_add_adapters_workspace_size(int64_t rows, int64_t slots, int64_t k, int64_t rank, int64_t pieces,
+                                                int64_t n, int32_t silu) {
   if (check_shape("add_adapters_workspace_size", rows, slots, k, rank, pieces) || rows == 0) return 0;
-  if (in_one_launch(rows, slots, k, rank, pieces, n)) return 0;
+  if (!silu && in_one_launch(rows, slots, k, rank, pieces, n)) return 0;
   const int64_t padded = (pieces * rank + 15) / 16 * 16;
   return std::max(split_of(rows, slots, k, padded, false).bytes, split_of(rows, slots, k, padded, true).bytes);
 }
@@ -744,8 +804,8 @@ extern "C" size_t mi_add_adapters_workspace_size(int64_t rows, int64_t slots, in
 extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, int64_t x_stride, const void* x_scales,
                                int64_t x_scales_stride, const void* a, const void* b, const float* scale, int64_t slots,
                                int64_t k, int64_t rank, const int32_t* piece_columns, int64_t pieces, void* out,
-                               int64_t out_stride, const void* plan, int64_t rows, void* workspace,
-                               size_t workspace_bytes, mi_stream_t stream) {
+                               int64_t out_stride, void* out_scales, int64_t out_scales_stride, const void* plan,
+                               int64_t rows, int32_t silu, void* workspace, size_t workspace_bytes, mi_stream_t stream) {
   const char* const name = "add_adapters";
   mi::clear_error();
   if (int rc = check_shape(name, rows, slots, k, rank, pieces)) return rc;
@@ -758,32 +818,42 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
     n += piece_columns[i];
     p.end[i] = int(n);
   }
+  const int64_t out_n = silu ? n / 2 : n;
+  if (silu && (pieces != 2 || piece_columns[0] != piece_columns[1]))
+    return mi::fail(MI_ERR_INVALID, "%s: SiLU is of gate and up, two pieces of as many columns", name);
+  if (out_scales && (!silu || out_n % mi::mx8::kBlock))
+    return mi::fail(MI_ERR_INVALID, "%s: rows in 8 bits are the gated sum's, a multiple of %d columns; got %lld", name,
+                    mi::mx8::kBlock, (long long)out_n);
   if (rows == 0) return MI_OK;
-  const int64_t each = x_scales ? 1 : 2;
+  const int64_t each = x_scales ? 1 : 2, out_each = out_scales ? 1 : 2;
   const int64_t scale_bytes = (k / 32 + 15) & ~int64_t(15);
-  if (rows == 1) y_stride = out_stride = n, x_stride = (k + 15) & ~int64_t(15), x_scales_stride = scale_bytes;
+  if (rows == 1) {  // (nothing lies at a single row's stride)
+    y_stride = n, out_stride = out_n, out_scales_stride = out_n / 32;
+    x_stride = (k + 15) & ~int64_t(15), x_scales_stride = scale_bytes;
+  }
   if (!y || !x || !a || !b || !scale || !out || !plan)
     return mi::fail(MI_ERR_INVALID, "%s: null pointer argument", name);
   const uintptr_t aligned = reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(a) |
                             reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(out) |
                             reinterpret_cast<uintptr_t>(plan) | reinterpret_cast<uintptr_t>(workspace) |
                             reinterpret_cast<uintptr_t>(x_scales);
-  if ((aligned & 15) || ((y_stride | out_stride) & 7) || (x_scales && x_scales_stride % 16) || (x_stride * each) % 16 || (reinterpret_cast<uintptr_t>(scale) & 3))
+  if ((aligned & 15) || (y_stride & 7) || (out_stride * out_each) % 16 || (x_scales && x_scales_stride % 16) || (x_stride * each) % 16 || (reinterpret_cast<uintptr_t>(scale) & 3))
     return mi::fail(MI_ERR_INVALID, "%s: rows, factors, plan and workspace must be 16-byte aligned", name);
-  if (out_stride < n || x_stride < 0 || y_stride < 0 || (x_scales && x_scales_stride < scale_bytes))
+  if (out_stride < out_n || (out_scales && out_scales_stride < out_n / 32) || x_stride < 0 || y_stride < 0 || (x_scales && x_scales_stride < scale_bytes))
     return mi::fail(MI_ERR_INVALID, "%s: row strides %lld, %lld, %lld, %lld for %lld columns", name, (long long)y_stride,
                     (long long)x_stride, (long long)x_scales_stride, (long long)out_stride, (long long)n);
   const int64_t padded = (pieces * rank + 15) / 16 * 16;
   const Split split = split_of(rows, slots, k, padded, x_scales != nullptr);
   const int64_t tiles = split.tiles;
-  const bool whole = in_one_launch(rows, slots, k, rank, pieces, n);
+  const bool whole = !silu && in_one_launch(rows, slots, k, rank, pieces, n);
   const size_t need = whole ? 0 : split.bytes;
   if (need && !workspace) return mi::fail(MI_ERR_INVALID, "%s: null pointer argument", name);
   if (workspace_bytes < need)
     return mi::fail(MI_ERR_WORKSPACE, "%s: the workspace takes %zu bytes, %zu given", name, need, workspace_bytes);
   // (rows of out are written while others are still read; a row of y only by who writes it)
-  const bool in_place = out == y && out_stride == y_stride;
-  const mi::Rows to = {out, out_stride * 2, rows, n * 2};
+  const bool in_place = !silu && out == y && out_stride == y_stride;
+  const mi::Rows to = {out, out_stride * out_each, rows, out_n * out_each},
+                 to_scales = {out_scales, out_scales_stride, out_scales ? rows : 0, out_n / 32};
   const mi::Rows from[] = {{y, y_stride * 2, in_place ? 0 : rows, n * 2},
                            {x, x_stride * each, rows, k * each},
                            {x_scales, x_scales_stride, x_scales ? rows : 0, k / 32},
@@ -792,8 +862,9 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
                            {scale, 0, 1, slots * 4},
                            {plan, 0, 1, int64_t(plan_size(rows, slots))},
                            {workspace, 0, need ? 1 : 0, int64_t(need)}};
-  for (const mi::Rows& r : from)
-    if (mi::rows_meet(to, r)) return mi::fail(MI_ERR_INVALID, "%s: out overlaps another argument (it may be y itself)", name);
+  bool meet = mi::rows_meet(to, to_scales);
+  for (const mi::Rows& r : from) meet = meet || mi::rows_meet(to, r) || mi::rows_meet(to_scales, r);
+  if (meet) return mi::fail(MI_ERR_INVALID, "%s: out overlaps another argument (without SiLU it may be y itself)", name);
   p.x = static_cast<const char*>(x);
   p.x_stride = x_stride * each;
   p.xs = static_cast<const char*>(x_scales);
@@ -805,6 +876,9 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
   p.y_stride = y_stride;
   p.out = static_cast<uint16_t*>(out);
   p.o_stride = out_stride;
+  p.scales = static_cast<uint8_t*>(out_scales);
+  p.s_stride = out_scales_stride;
+  p.up = int(out_n);
   p.plan = view(const_cast<void*>(plan), rows, slots);
   p.parts = static_cast<float*>(workspace);
   p.rows = int(rows);
@@ -823,9 +897,9 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
   // columns of a workgroup: few where there are few tiles, so that every CU has some
   p.chunk = 128;
   const int64_t enough = whole ? mi::num_cus() : 8 * mi::num_cus();
-  while (p.chunk < kMaxChunk && tiles * ((n + p.chunk - 1) / p.chunk) > enough) p.chunk *= 2;
+  while (p.chunk < kMaxChunk && tiles * ((out_n + p.chunk - 1) / p.chunk) > enough) p.chunk *= 2;
   int chunks = 0;
-  for (int i = 0; i < pieces; ++i) p.end_chunk[i] = chunks += (piece_columns[i] + p.chunk - 1) / p.chunk;
+  for (int i = 0; i < (silu ? 1 : pieces); ++i) p.end_chunk[i] = chunks += (piece_columns[i] + p.chunk - 1) / p.chunk;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid(uint32_t(tiles), uint32_t(p.n_parts), uint32_t(split.groups)), block(64 * kWaves);
   const int rt = p.group_ranks / 16;
@@ -843,8 +917,9 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
       {shrink_many_kernel<true, 1>, shrink_many_kernel<true, 2>, nullptr, nullptr}};
   hipLaunchKernelGGL((many ? wide : few)[x8][rt - 1], grid, dim3(64 * (many ? kManyWaves : kWaves)), 0, s, p);
   const int j = rank <= 16 ? 0 : rank <= 32 ? 1 : rank <= 64 ? 2 : 3;
-  const Kernel expand[2][4] = {{expand_kernel<1, 1>, expand_kernel<1, 2>, expand_kernel<1, 4>, expand_kernel<1, 8>},
-                               {expand_kernel<4, 1>, expand_kernel<4, 2>, expand_kernel<4, 4>, expand_kernel<4, 8>}};
-  hipLaunchKernelGGL(expand[many][j], dim3(uint32_t(tiles), uint32_t(chunks)), block, 0, s, p);
+  const Kernel expand = !silu      ? expand_of<End::plain>(many, j)
+                        : p.scales ? expand_of<End::silu8>(many, j)
+                                   : expand_of<End::silu>(many, j);
+  hipLaunchKernelGGL(expand, dim3(uint32_t(tiles), uint32_t(chunks)), block, 0, s, p);
   return mi::check_launch(name);
 }

@@ -73,6 +73,20 @@ __device__ __forceinline__ u32x2_t to_bf16(uint32_t codes, float scale) {
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true))};
 }
 
+// silu(g) within 2^-20, from w = e^(-|g| / 2): g / (1 + w^2), times w^2 where g is negative, a factor at
+// a time, so that nothing underflows before the result does.  The exponent's rounding is made
+// good (it would be |g| 2^-24).  An end of 128 such values a lane is a tenth of a largest block's
+// time: half the instructions of a division rounded to the last bit (us, 2,057 x
+// 4,096 x 2 x 14,336 237 -> 230, 16,384 rows 1,591 -> 1,521).
+__device__ __forceinline__ float silu20(float g) {
+  constexpr float kHalfLog2e = 0.721347511f;
+  const float a = -fminf(fabsf(g), 200.f), h = a * kHalfLog2e;
+  float w = __builtin_amdgcn_exp2f(h);
+  w = fmaf(w, 0.693147181f * fmaf(a, kHalfLog2e, -h), w);
+  const float r = fast_rcp(fmaf(w, w, 1.f)), s = g < 0.f ? w : 1.f;
+  return g * s * r * s;
+}
+
 template <int CTRL>
 __device__ __forceinline__ uint32_t max_dpp(uint32_t v) {
   return max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, 0xf, 0xf, false)));

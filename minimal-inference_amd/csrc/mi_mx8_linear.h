@@ -43,20 +43,6 @@ __device__ __forceinline__ f32x4_t bias4(const LinearParams& p, int col) {
   return v;
 }
 
-// silu(g) within 2^-20, from w = e^(-|g| / 2): g / (1 + w^2), times w^2 where g is negative, a factor at
-// a time, so that nothing underflows before the result does.  The exponent's rounding is made
-// good (it would be |g| 2^-24).  An end of 128 such values a lane is a tenth of a largest block's
-// time: half the instructions of a division rounded to the last bit (us, 2,057 x
-// 4,096 x 2 x 14,336 237 -> 230, 16,384 rows 1,591 -> 1,521).
-__device__ __forceinline__ float silu20(float g) {
-  constexpr float kHalfLog2e = 0.721347511f;
-  const float a = -fminf(fabsf(g), 200.f), h = a * kHalfLog2e;
-  float w = __builtin_amdgcn_exp2f(h);
-  w = fmaf(w, 0.693147181f * fmaf(a, kHalfLog2e, -h), w);
-  const float r = fast_rcp(fmaf(w, w, 1.f)), s = g < 0.f ? w : 1.f;
-  return g * s * r * s;
-}
-
 // A lane's sums (and, gated, those of the up rows): bias or silu(gate) * up in fp32.
 template <bool GLU>
 __device__ __forceinline__ f32x4_t finish(f32x4_t sum, f32x4_t up, f32x4_t bias) {

@@ -47,8 +47,8 @@ import weakref
 import torch
 import torch.nn.functional as F
 
-from .adapters import Adapters, add_adapters
-from .dense import add_rms_norm, linear, linear_silu, silu_mul
+from .adapters import Adapters, add_adapters, add_adapters_silu
+from .dense import add_rms_norm, linear, linear_silu
 from .mxfp4 import BLOCK, MXFP4, linear_mxfp4, linear_silu_mxfp4, quantize_mxfp4
 from .mxfp8 import MXFP8, add_rms_norm_mxfp8, linear_mxfp8, linear_silu_mxfp8, quantize_mxfp8
 from .page import append_paged_kv_cache, rope_append_paged_kv_cache
@@ -341,9 +341,8 @@ class Model:
                 o = quantize_mxfp8(o)
             h = norm(x, adapted(project(o, L.w_o), o, L, "w_o"), L.post_norm, L.w_gate_up)
             if plan is not None and "w_gate_up" in L.adapters:
-                act = silu_mul(adapted(project(h, L.w_gate_up), h, L, "w_gate_up"))
-                if isinstance(L.w_down, MXFP8):
-                    act = quantize_mxfp8(act)
+                act = add_adapters_silu(project(h, L.w_gate_up), h, L.adapters["w_gate_up"], plan,
+                                        quantize=isinstance(L.w_down, MXFP8))
             elif isinstance(L.w_gate_up, MXFP8):
                 act = linear_silu_mxfp8(h, L.w_gate_up, quantize=True)
             else:

@@ -172,3 +172,80 @@ def test_set_and_clear(dev):
     assert bool(((got.double() - want).abs() <= tol).all())
     ad.clear(1)
     assert not bool(add_adapters(y, x, ad, plan, out=torch.empty_like(y))[[1, 4]].any())
+
+
+@pytest.mark.parametrize("x8", [False, True])
+@pytest.mark.parametrize("k,half,rank", [(32, 16, 8), (96, 32, 16), (896, 4864, 16), (1056, 304, 24), (544, 1184, 64), (256, 160, 128)])
+@pytest.mark.parametrize("rows,slots", [(1, 1), (3, 5), (17, 2), (130, 7), (320, 3), (321, 3), (900, 30)])
+def test_add_adapters_silu(dev, rows, slots, k, half, rank, x8):
+    """SiLU(gate) * up of the sums: gate and up within their bars dg and du of the 64-bit sums G and U (without
+    the rounding to bf16), silu's slope is 1.1 at most and its value |G| at most, so the product is within
+    1.1 dg (|U| + du) + |G| du + 2^-20 of itself, and rounded once: bf16 2^-8, or e4m3 2^-4 (2^-10 of the block's
+    unit below its least normal code). y stays, and what lies around out."""
+    from minimal_inference_amd.adapters import AdapterPlan, add_adapters_silu
+
+    x, values, ad, slot, y = _make(dev, rows, k, [half, half], rank, slots, x8=x8)
+    plan = AdapterPlan(rows, slots, dev)
+    plan.plan(slot)
+    ref, tol = _want(values, ad, slot, y)
+    tol = (tol - 2 ** -8 * ref.abs()) / (1 + 2 ** -8) + 2.0 ** -24 * ref.abs()  # (the bar before the rounding; the sum's own)
+    G, U, dg, du = ref[:, :half], ref[:, half:], tol[:, :half], tol[:, half:]
+    want = G * torch.sigmoid(G) * U
+    near = 1.1 * dg * (U.abs() + du) + G.abs() * du + 2.0 ** -20 * want.abs()
+    y0 = y.clone()
+    room = torch.full((rows + 2, half + 8), 7.0, dtype=torch.bfloat16, device=dev)
+    out = add_adapters_silu(y, x, ad, plan, out=room[1: rows + 1, :half])
+    assert bool(((out.double() - want).abs() <= near + 2 ** -8 * (want.abs() + near)).all())
+    assert bool((room[0] == 7).all() and (room[-1] == 7).all() and (room[:, half:] == 7).all())
+    assert torch.equal(add_adapters_silu(y, x, ad, plan), out)
+    if half % 32 == 0:
+        m = add_adapters_silu(y, x, ad, plan, quantize=True)
+        unit = torch.exp2(m.scales.double() - 127.0).repeat_interleave(32, 1)
+        got = om8.values(m.codes, m.scales).to(dev)
+        assert bool(((got - want).abs() <= near + ((want.abs() + near) * 2.0 ** -4).maximum(unit * 2.0 ** -10)).all())
+        top, slack = want.abs().view(rows, half // 32, 32).amax(-1), near.view(rows, half // 32, 32).amax(-1)
+        scale = torch.exp2(m.scales.double() - 127.0)
+        assert bool((top - slack <= 448 * scale).all() and ((top + slack > 224 * scale) | (m.scales == 0)).all())
+    else:
+        with pytest.raises(ValueError):
+            add_adapters_silu(y, x, ad, plan, quantize=True)
+    assert torch.equal(y, y0)
+
+
+def test_add_adapters_silu_refuses(dev):
+    from minimal_inference_amd.adapters import AdapterPlan, add_adapters_silu
+    from minimal_inference_amd.mxfp8 import MXFP8
+
+    x, _, ad, slot, y = _make(dev, 5, 64, [32, 32], 8, 2)
+    plan = AdapterPlan(5, 2, dev)
+    plan.plan(slot)
+    for bad in (y, y[:, :32], torch.empty(5, 64, dtype=torch.bfloat16, device=dev), torch.empty(4, 32, dtype=torch.bfloat16, device=dev)):
+        with pytest.raises(ValueError):
+            add_adapters_silu(y, x, ad, plan, out=bad)
+    for bad in (MXFP8(5, 64, dev), y[:, :32]):
+        with pytest.raises(ValueError):
+            add_adapters_silu(y, x, ad, plan, out=bad, quantize=True)
+    _, _, other, _, _ = _make(dev, 5, 64, [48, 16], 8, 2)
+    with pytest.raises(ValueError, match="gate and up"):
+        add_adapters_silu(y, x, other, plan)
+
+
+def test_add_adapters_silu_replayed_after_another_batch(dev):
+    """NaN in bf16 and in 8 bits after a plan of another number of rows; its own bits again after its own."""
+    from minimal_inference_amd.adapters import AdapterPlan, add_adapters_silu
+
+    x, _, ad, slot, y = _make(dev, 40, 64, [96, 96], 8, 2)
+    plan = AdapterPlan(40, 2, dev)
+    plan.plan(slot)
+    want = [add_adapters_silu(y, x, ad, plan), add_adapters_silu(y, x, ad, plan, quantize=True)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [add_adapters_silu(y, x, ad, plan), add_adapters_silu(y, x, ad, plan, quantize=True)]
+    for _ in range(3):
+        plan.plan(slot[:33])
+        graph.replay()
+        assert bool(got[0].isnan().all() and (got[1].scales == 255).all()) and not bool(got[1].codes.view(torch.uint8).any())
+        plan.plan(slot)
+        graph.replay()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1].scales, want[1].scales)
+        assert torch.equal(got[1].codes.view(torch.uint8), want[1].codes.view(torch.uint8))

@@ -100,12 +100,8 @@ def _restated(model, ids, found=None):
         s = s.masked_fill(torch.ones(t, t, device=s.device).triu(1).bool(), float("-inf"))
         o = bf(torch.matmul(torch.softmax(s, -1), v.transpose(0, 1).contiguous()).transpose(0, 1).reshape(t, nq * d))
         x = bf(x + bf(project(rows8(o, L.w_o), li, "w_o")))
-        gu = project(rows8(rms(x, L.post_norm), L.w_gate_up), li, "w_gate_up")
-        if found:
-            gu = bf(gu)
-        gate, up = gu.chunk(2, -1)
-        act = gate * torch.sigmoid(gate) * up
-        x = bf(x + bf(project(rows8(bf(act) if found else act, L.w_down), li, "w_down")))
+        gate, up = project(rows8(rms(x, L.post_norm), L.w_gate_up), li, "w_gate_up").chunk(2, -1)
+        x = bf(x + bf(project(rows8(gate * torch.sigmoid(gate) * up, L.w_down), li, "w_down")))
     return bf(rms(x[-1:], model.norm)) @ model.lm_head.double().t()
 
 

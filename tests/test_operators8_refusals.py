@@ -104,8 +104,8 @@ def test_plan_sizes():
 
 
 ADAPT = dict(y=FAKE, ys=64, x=FAKE + (1 << 20), xs=96, xsc=None, xss=0, a=FAKE + (1 << 21), b=FAKE + (1 << 22), scale=FAKE + (1 << 23),
-             slots=3, k=96, rank=24, pieces=(48, 16), n_pieces=2, out=FAKE + (1 << 24), os=64, plan=FAKE + (1 << 25), rows=4,
-             work=FAKE + (1 << 26), bytes=1 << 24)
+             slots=3, k=96, rank=24, pieces=(48, 16), n_pieces=2, out=FAKE + (1 << 24), os=64, osc=None, oss=0, plan=FAKE + (1 << 25), rows=4,
+             silu=0, work=FAKE + (1 << 26), bytes=1 << 24)
 
 
 @pytest.mark.parametrize("change", [
@@ -116,7 +116,12 @@ ADAPT = dict(y=FAKE, ys=64, x=FAKE + (1 << 20), xs=96, xsc=None, xss=0, a=FAKE +
     {"os": 68}, {"os": 56}, {"xs": 100}, {"xs": -96}, {"xsc": FAKE + 8, "xss": 16}, {"xsc": FAKE + (1 << 19), "xss": 8},
     {"xsc": FAKE + (1 << 19), "xss": 0}, {"xsc": FAKE + (1 << 19), "xss": 16, "xs": 104},
     {"out": FAKE + 16}, {"out": FAKE, "os": 72}, {"out": FAKE + (1 << 20)}, {"out": FAKE + (1 << 21) + 3 * 48 * 96 * 2 - 16},
-    {"out": FAKE + (1 << 22) + 3 * 64 * 24 * 2 - 16}, {"out": FAKE + (1 << 25)}, {"out": FAKE + (1 << 26)}, {"scale": FAKE + (1 << 24) + 8}])
+    {"out": FAKE + (1 << 22) + 3 * 64 * 24 * 2 - 16}, {"out": FAKE + (1 << 25)}, {"out": FAKE + (1 << 26)}, {"scale": FAKE + (1 << 24) + 8},
+    {"silu": 1}, {"silu": 1, "pieces": (32, 16)}, {"silu": 1, "n_pieces": 1, "pieces": (64,)}, {"osc": FAKE + (1 << 27), "oss": 1},
+    {"silu": 1, "pieces": (16, 16), "osc": FAKE + (1 << 27), "oss": 1}, {"silu": 1, "pieces": (32, 32), "osc": FAKE + (1 << 27)},
+    {"silu": 1, "pieces": (32, 32), "os": 24}, {"silu": 1, "pieces": (32, 32), "os": 40, "osc": FAKE + (1 << 27), "oss": 1},
+    {"silu": 1, "pieces": (32, 32), "out": FAKE}, {"silu": 1, "pieces": (32, 32), "out": FAKE + 64},
+    {"silu": 1, "pieces": (32, 32), "osc": FAKE + (1 << 24) + 31, "oss": 1}, {"silu": 1, "pieces": (32, 32), "osc": FAKE + 9, "oss": 1}])
 def test_add_adapters_refuses(change):
     a = ADAPT | change
     held = None if a["pieces"] is None else _pieces(*a["pieces"])
@@ -126,13 +131,14 @@ def test_add_adapters_refuses(change):
 
 def test_add_adapters_workspace():
     mod, lib = _lib()
-    assert lib.mi_add_adapters_workspace_size(4, 3, 96, 24, 2, 64) > 0  # (two launches)
-    assert lib.mi_add_adapters_workspace_size(4, 3, 96, 16, 2, 64) == 0  # (one)
+    assert lib.mi_add_adapters_workspace_size(4, 3, 96, 24, 2, 64, 0) > 0  # (two launches)
+    assert lib.mi_add_adapters_workspace_size(4, 3, 96, 16, 2, 64, 0) == 0  # (one)
+    assert lib.mi_add_adapters_workspace_size(4, 3, 96, 16, 2, 64, 1) > 0
     held = _pieces(48, 16)
     _refused("mi_add_adapters", ADAPT | {"pieces": ctypes.addressof(held), "bytes": 0}, "add_adapters", mod.MI_ERR_WORKSPACE)
     assert lib.mi_add_adapters(*(ADAPT | {"pieces": ctypes.addressof(held), "rows": 0, "y": None}).values(), None) == mod.MI_OK
-    for bad in ((-1, 3, 96, 24, 2, 64), (4, 0, 96, 24, 2, 64), (4, 3, 80, 24, 2, 64), (4, 3, 96, 12, 2, 64), (4, 3, 96, 24, 9, 64),
-                (0, 3, 96, 24, 2, 64)):
+    for bad in ((-1, 3, 96, 24, 2, 64, 0), (4, 0, 96, 24, 2, 64, 0), (4, 3, 80, 24, 2, 64, 0), (4, 3, 96, 12, 2, 64, 0),
+                (4, 3, 96, 24, 9, 64, 0), (0, 3, 96, 24, 2, 64, 0)):
         assert lib.mi_add_adapters_workspace_size(*bad) == 0
 
 
