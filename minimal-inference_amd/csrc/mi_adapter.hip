@@ -121,6 +121,7 @@ struct AdapterParams {
   PlanView plan;
   float* parts;  // [part][tile][row of the tile][ranks, padded]
   int rows, slots;
+  int eighths, per_eighths;  // rank / 8; 2^16 over it, rounded up
   int k, n, rank, ranks, padded;  // ranks = pieces * rank, padded to 16
   int n_parts, part_steps, max_tiles, group_ranks;
   int pieces, chunk;  // columns of an expand workgroup
@@ -164,6 +165,9 @@ __device__ __forceinline__ void write_nan(const AdapterParams& p, int tile_rows,
       }
     }
 }
+// Piece e of B's rows of a unit, 16 bytes each: its row.  (e is 128 times 16 at most, where this is exact.)
+__device__ __forceinline__ int row_of_piece(const AdapterParams& p, int e) { return e * p.per_eighths >> 16; }
+
 // Four sums times scale as pairs of bf16: the values and what their rounding left.
 __device__ __forceinline__ uint4 bf16_pair(f32x4_t sum, float scale) {
   uint32_t hi[2], lo[2];
@@ -437,13 +441,69 @@ __global__ __launch_bounds__(64 * kManyWaves) void shrink_many_kernel(AdapterPar
 }
 
 
+// What a lane makes of its four rows' y and of its sums for columns col .. col + 7 of them, the first `count` of
+// which are the tile's: out, or, of gate columns, the values that the up columns' turn takes.
+template <End END, int HALF>
+__device__ __forceinline__ void end_of_unit(const AdapterParams& p, bool adds, const uint4 (&y)[4], const f32x4_t (&d)[8],
+                                            float (&gate)[END == End::plain ? 1 : 4][8], const int64_t (&row)[4], int col, int count) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (END == End::plain) {
+      const uint4 o = adds ? add_rounded(y[i], d, i) : y[i];
+      if (i < count) mi::store16(p.out + row[i] * p.o_stride + col, o);
+    } else {
+      const uint32_t pairs[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+      float v[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        v[t] = (t % 2 ? mi::bf16_hi(pairs[t / 2]) : mi::bf16_lo(pairs[t / 2])) + d[t][i];
+        if constexpr (HALF == 0) gate[i][t] = mi::mx8::silu20(v[t]);
+        else v[t] *= gate[i][t];
+      }
+      if constexpr (HALF == 1 && END == End::silu) {
+        if (i < count)
+          mi::store16(p.out + row[i] * p.o_stride + col, make_uint4(mi::cvt_pk_bf16(v[0], v[1]), mi::cvt_pk_bf16(v[2], v[3]),
+                                                                   mi::cvt_pk_bf16(v[4], v[5]), mi::cvt_pk_bf16(v[6], v[7])));
+      } else if constexpr (HALF == 1) {  // (a block's 32 columns are four lanes')
+        uint32_t top = 0;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) top = max(top, mi::mx8::magnitude(v[t]));
+        const uint32_t byte = mi::mx8::scale_byte(mi::mx8::max4(top));
+        if (i < count) {
+          *reinterpret_cast<u32x2_t*>(reinterpret_cast<uint8_t*>(p.out) + row[i] * p.o_stride + col) =
+              u32x2_t{mi::mx8::to_codes(v[0], v[1], v[2], v[3], byte), mi::mx8::to_codes(v[4], v[5], v[6], v[7], byte)};
+          if (col % mi::mx8::kBlock == 0) p.scales[row[i] * p.s_stride + col / mi::mx8::kBlock] = uint8_t(byte);
+        }
+      }
+    }
+  }
+}
+
+// The sum of the parts of four ranks, in their order, eight on their way at once.
+__device__ __forceinline__ f32x4_t sum_of_parts(const AdapterParams& p, const float* from, int64_t part) {
+  f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](int first) {
+    f32x4_t v[8];
+#pragma unroll
+    for (int o = 0; o < 8; ++o)
+      v[o] = first + o < p.n_parts ? *reinterpret_cast<const f32x4_t*>(from + (first + o) * part) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int o = 0; o < 8; ++o) sum += v[o];
+  };
+  static_assert(kMaxParts == 16);
+  add(0);
+  if (p.n_parts > 8) add(8);
+  return sum;
+}
+
 // out = y + B v of a tile of 16 NB rows and a chunk of columns.  J: products of 32 that the
 // pairs of a piece's ranks take.  A unit of work is 16 rows by 128 columns, eight products
 // side by side: column c of product t is column 8 c + t of the unit, so that lane (g, n) ends with
 // columns 8 n .. 8 n + 7 of rows 4 g .. 4 g + 3, 16 bytes of y and out in the order of the lanes.  With SiLU a
 // unit of gate columns and the same of up columns follow each other, and the gate's values wait in fp32.
+// (rank 64 with SiLU: two waves a SIMD)
 template <int NB, int J, End END>
-__global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
+__global__ __launch_bounds__(64 * kWaves, END != End::plain && J == 4 ? 2 : 1) void expand_kernel(AdapterParams p) {
   constexpr int ROWS = 16 * NB, kPair = 32 * J;  // a row's ranks in bf16, and what the rounding left of them
   constexpr int VSTRIDE = kPair + 8;              // (the rows of an operand on distinct banks)
   constexpr int kMaxWeights = 128 * (kPair / 2) + 128;  // a unit's columns of B: eight of them, then 16 bytes apart
@@ -467,7 +527,7 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
   if (int(blockIdx.x) >= tiles || (END == End::plain && tile.slot < 0 && p.out == p.y)) return;
   const bool adds = tile.slot >= 0;
   const int nb = (tile.count + 15) / 16, units = (c1 - c0 + 127) / 128 * HALVES;
-  const int eighths = p.rank / 8;
+  const int eighths = p.eighths;
   const uint16_t* const weights = p.b + int64_t(max(tile.slot, 0)) * p.n * p.rank;
 
   // the weights of a unit's 128 columns, 16 bytes a thread and lot
@@ -477,16 +537,16 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
     const int up = unit % HALVES * p.up;
 #pragma unroll
     for (int i = 0; i < LOTS; ++i) {
-      const int e = i * 64 * kWaves + tid, col = c0 + unit / HALVES * 128 + e / eighths;
-      wv[i] = adds && e < 128 * eighths && col < c1 ? mi::load16(weights + int64_t(up + col) * p.rank + e % eighths * 8)
+      const int e = i * 64 * kWaves + tid, in = row_of_piece(p, e), col = c0 + unit / HALVES * 128 + in;
+      wv[i] = adds && e < 128 * eighths && col < c1 ? mi::load16(weights + int64_t(up + col) * p.rank + (e - in * eighths) * 8)
                                                     : make_uint4(0u, 0u, 0u, 0u);
     }
   };
   auto keep = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < LOTS; ++i) {
-      const int e = i * 64 * kWaves + tid, col = e / eighths;
-      if (e < 128 * eighths) mi::store16(ws[buf] + col * p.rank + col / 8 * 8 + e % eighths * 8, wv[i]);
+      const int e = i * 64 * kWaves + tid, col = row_of_piece(p, e);
+      if (e < 128 * eighths) mi::store16(ws[buf] + col * p.rank + col / 8 * 8 + (e - col * eighths) * 8, wv[i]);
     }
   };
   fetch(0);
@@ -514,18 +574,7 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
     for (int i = tid; i < tile.count * fours * HALVES; i += 64 * kWaves) {
       const int row = i / (fours * HALVES), half = i / fours % HALVES, r = i % fours * 4;
       const float* const from = p.parts + (int64_t(blockIdx.x) * ROWS + row) * p.padded + (piece + half) * p.rank + r;
-      f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-      auto add = [&](int first) {  // eight on their way at once, added in their order
-        f32x4_t v[8];
-#pragma unroll
-        for (int o = 0; o < 8; ++o)
-          v[o] = first + o < p.n_parts ? *reinterpret_cast<const f32x4_t*>(from + (first + o) * part) : f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int o = 0; o < 8; ++o) sum += v[o];
-      };
-      static_assert(kMaxParts == 16);
-      add(0);
-      if (p.n_parts > 8) add(8);
+      const f32x4_t sum = sum_of_parts(p, from, part);
       const uint4 pair = bf16_pair(sum, scale);
       *reinterpret_cast<uint2*>(vs[half] + row * VSTRIDE + r) = make_uint2(pair.x, pair.y);
       *reinterpret_cast<uint2*>(vs[half] + row * VSTRIDE + p.rank + r) = make_uint2(pair.z, pair.w);
@@ -533,7 +582,7 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
   }
   int from[J];  // of a lane's eight ranks of product j, -1: past the last pair
 #pragma unroll
-  for (int j = 0; j < J; ++j) from[j] = 4 * j + g < 2 * eighths ? (4 * j + g) % eighths * 8 : -1;
+  for (int j = 0; j < J; ++j) from[j] = 4 * j + g < 2 * eighths ? (4 * j + g < eighths ? 4 * j + g : 4 * j + g - eighths) * 8 : -1;
   float gate[END == End::plain ? 1 : 4][8];
   auto step = [&]<int HALF>(int unit) {
     const int col = c0 + unit / HALVES * 128 + 8 * n, buf = unit & 1;
@@ -559,40 +608,11 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
             const uint4 m = *reinterpret_cast<const uint4*>(ws[buf] + at);
             d[t] = mi::mfma_16x16x32_bf16(v, mi::as_bf16x8(from[j] >= 0 ? m : none), d[t]);
           }
+          // (with SiLU and all reads ahead a SIMD's registers hold one wave: rank 64 25 us -> 43)
+          if constexpr (END != End::plain && J >= 4) __builtin_amdgcn_sched_barrier(0);
         }
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool in = col < c1 && w * 16 + 4 * g + i < tile.count;
-        if constexpr (END == End::plain) {
-          const uint4 o = adds ? add_rounded(rows.y[i], d, i) : rows.y[i];
-          if (in) mi::store16(p.out + row[i] * p.o_stride + col, o);
-        } else {
-          const uint32_t y[4] = {rows.y[i].x, rows.y[i].y, rows.y[i].z, rows.y[i].w};
-          float v[8];
-#pragma unroll
-          for (int t = 0; t < 8; ++t) {
-            v[t] = (t % 2 ? mi::bf16_hi(y[t / 2]) : mi::bf16_lo(y[t / 2])) + d[t][i];
-            if constexpr (HALF == 0) gate[i][t] = mi::mx8::silu20(v[t]);
-            else v[t] *= gate[i][t];
-          }
-          if constexpr (HALF == 1 && END == End::silu) {
-            if (in)
-              mi::store16(p.out + row[i] * p.o_stride + col, make_uint4(mi::cvt_pk_bf16(v[0], v[1]), mi::cvt_pk_bf16(v[2], v[3]),
-                                                                       mi::cvt_pk_bf16(v[4], v[5]), mi::cvt_pk_bf16(v[6], v[7])));
-          } else if constexpr (HALF == 1) {  // (a block's 32 columns are four lanes')
-            uint32_t top = 0;
-#pragma unroll
-            for (int t = 0; t < 8; ++t) top = max(top, mi::mx8::magnitude(v[t]));
-            const uint32_t byte = mi::mx8::scale_byte(mi::mx8::max4(top));
-            if (in) {
-              *reinterpret_cast<u32x2_t*>(reinterpret_cast<uint8_t*>(p.out) + row[i] * p.o_stride + col) =
-                  u32x2_t{mi::mx8::to_codes(v[0], v[1], v[2], v[3], byte), mi::mx8::to_codes(v[4], v[5], v[6], v[7], byte)};
-              if (n % 4 == 0) p.scales[row[i] * p.s_stride + col / mi::mx8::kBlock] = uint8_t(byte);
-            }
-          }
-        }
-      }
+      end_of_unit<END, HALF>(p, adds, rows.y, d, gate, row, col, col < c1 ? tile.count - w * 16 - 4 * g : 0);
     }
     rows = next_rows;
   };
@@ -602,15 +622,134 @@ __global__ __launch_bounds__(64 * kWaves) void expand_kernel(AdapterParams p) {
   }
 }
 
+// The units of a chunk for a tile of 16 rows, each a wave's own.  B's rows of a unit are one piece of memory, which the
+// wave reads in the order of its lanes and passes to itself through LDS, eight columns and then 16 bytes
+// apart (read as operands straight from memory: a unit of rank 16 1 us more, of rank 64 4).
+template <int J>
+constexpr int kUnitWeights = 128 * 16 * J + 128;
+template <int J, End END, int WAVES>
+struct Units {
+  static constexpr int HALVES = END == End::plain ? 1 : 2, VSTRIDE = 32 * J + 8, LOTS = 4 * J;
+  const AdapterParams& p;
+  const Columns& c;
+  const Tile& tile;
+  const int w, lane, eighths;
+  const uint16_t* weights;
+  int64_t row[4];
+  uint4 b[LOTS], y[4];
+
+  __device__ __forceinline__ Units(const AdapterParams& p, const Columns& c, const Tile& tile, const int (&mine)[4], int any)
+      : p(p), c(c), tile(tile), w(__builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6)), lane(threadIdx.x & 63), eighths(p.eighths) {
+    weights = p.b + int64_t(max(tile.slot, 0)) * p.n * p.rank;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) row[i] = 4 * (lane >> 4) + i < tile.count ? mine[i] : any;  // (past the tile's last row any will do)
+  }
+  // What the wave's unit `i` reads (of gate and up columns in turn).
+  __device__ __forceinline__ void load(int i) {
+    const int c0 = c.begin + (i / HALVES * WAVES + w) * 128, up = i % HALVES * p.up, col = c0 + 8 * (lane & 15);
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int k = 0; k < LOTS; ++k) {
+      const int e = k * 64 + lane, in = row_of_piece(p, e), at = c0 + in;
+      b[k] = tile.slot >= 0 && e < 128 * eighths && at < c.end
+                 ? mi::load16(weights + int64_t(up + at) * p.rank + (e - in * eighths) * 8) : none;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = col < c.end ? mi::load16_nt(p.y + row[k] * p.y_stride + up + col) : none;
+  }
+  // vs: v's pairs, those of the gate and of the up columns; ws: room for a unit's weights, the wave's own.
+  template <int HALF>
+  __device__ __forceinline__ void step(int i, const uint16_t* vs, uint16_t* ws, float (&gate)[END == End::plain ? 1 : 4][8]) {
+    const int g = lane >> 4, n = lane & 15, c0 = c.begin + (i / HALVES * WAVES + w) * 128, col = c0 + 8 * n;
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+    f32x4_t d[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) d[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    const uint4 own[4] = {y[0], y[1], y[2], y[3]};
+    if (tile.slot >= 0) {
+#pragma unroll
+      for (int k = 0; k < LOTS; ++k) {
+        const int e = k * 64 + lane, at = row_of_piece(p, e);
+        if (e < 128 * eighths) mi::store16(ws + at * p.rank + at / 8 * 8 + (e - at * eighths) * 8, b[k]);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    if (c.begin + ((i + 1) / HALVES * WAVES + w) * 128 < c.end) load(i + 1);
+    if (tile.slot >= 0) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const bool in = 4 * j + g < 2 * eighths;  // (or past the last pair)
+        const int from = in ? (4 * j + g < eighths ? 4 * j + g : 4 * j + g - eighths) * 8 : 0;
+        const uint4 q = *reinterpret_cast<const uint4*>(vs + (HALF * 16 + n) * VSTRIDE + (4 * j + g) * 8);
+        const bf16x8_t v = mi::as_bf16x8(in ? q : none);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const uint4 m = *reinterpret_cast<const uint4*>(ws + (8 * n + t) * p.rank + n * 8 + from);
+          d[t] = mi::mfma_16x16x32_bf16(v, mi::as_bf16x8(in ? m : none), d[t]);
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    end_of_unit<END, HALF>(p, tile.slot >= 0, own, d, gate, row, col, col < c.end ? tile.count - 4 * g : 0);
+  }
+  __device__ __forceinline__ void run(const uint16_t* vs, uint16_t* ws) {
+    float gate[END == End::plain ? 1 : 4][8];
+    for (int i = 0; c.begin + (i / HALVES * WAVES + w) * 128 < c.end; i += HALVES) {
+      step<0>(i, vs, ws, gate);
+      if constexpr (HALVES == 2) step<1>(i + 1, vs, ws, gate);
+    }
+  }
+};
+
+// expand_kernel's work for tiles of 16 rows, a unit a wave.
+template <int J, End END>
+__global__ __launch_bounds__(64 * kWaves, END != End::plain ? 2 : 1) void expand_waves_kernel(AdapterParams p) {
+  constexpr int HALVES = END == End::plain ? 1 : 2, VSTRIDE = 32 * J + 8;
+  __shared__ __attribute__((aligned(16))) uint16_t vs[HALVES * 16 * VSTRIDE];
+  __shared__ __attribute__((aligned(16))) uint16_t ws[kWaves][kUnitWeights<J>];
+  const int tid = threadIdx.x, g = (tid & 63) >> 4;
+  const int tiles = plan_tiles(p);
+  const Tile tile = p.plan.tiles[blockIdx.x];
+  const int* const order = p.plan.rows + blockIdx.x * 16;
+  const int any = order[0];
+  int mine[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mine[i] = order[4 * g + i];
+  const Columns c = columns_of(p);
+  if (tiles < 0) return write_nan<END>(p, 16, c);
+  if (int(blockIdx.x) >= tiles || (END == End::plain && tile.slot < 0 && p.out == p.y)) return;
+  Units<J, END, kWaves> units(p, c, tile, mine, any);
+  units.load(0);
+  if (tile.slot >= 0) {
+    const float scale = p.scale[tile.slot];
+    const int fours = p.rank / 4;
+    const int64_t part = int64_t(p.max_tiles) * 16 * p.padded;
+    for (int i = tid; i < tile.count * fours * HALVES; i += 64 * kWaves) {
+      const int row = i / (fours * HALVES), half = i / fours % HALVES, r = i % fours * 4;
+      const f32x4_t sum =
+          sum_of_parts(p, p.parts + (int64_t(blockIdx.x) * 16 + row) * p.padded + (c.piece + half) * p.rank + r, part);
+      const uint4 pair = bf16_pair(sum, scale);
+      *reinterpret_cast<uint2*>(vs + (half * 16 + row) * VSTRIDE + r) = make_uint2(pair.x, pair.y);
+      *reinterpret_cast<uint2*>(vs + (half * 16 + row) * VSTRIDE + p.rank + r) = make_uint2(pair.z, pair.w);
+    }
+  }
+  __syncthreads();
+  units.run(vs, ws[units.w]);
+}
+
 // Both products of a tile of 16 rows in one launch: every workgroup multiplies the whole of x by its
-// piece's A, 8 or 16 waves sharing k, and then a chunk of B's columns, units of 128 as in expand_kernel, a
+// piece's A, 8 or 16 waves sharing k, and then a chunk of B's columns, units of 128, a
 // wave at a time.  A comes from L2 for all workgroups but an XCD's first; what is won is a launch and
 // the sums' way through memory.
 constexpr int whole_waves(bool x8) { return x8 ? 8 : 16; }
 template <bool X8>
 __global__ __launch_bounds__(64 * whole_waves(X8)) void whole_kernel(AdapterParams p) {
   constexpr int RT = 1, WAVES = whole_waves(X8), J = RT, VSTRIDE = 32 * J + 8, WAVE = ring_bytes(X8, RT, 1);
-  static_assert(WAVES * WAVE <= 150 * 1024 && RT * 1024 <= WAVE && RT <= WAVES, "LDS");
+  static_assert(WAVES * WAVE <= 150 * 1024 && RT * 1024 <= WAVE && RT <= WAVES && kUnitWeights<J> * 2 <= WAVE, "LDS");
   __shared__ __attribute__((aligned(16))) char smem[WAVES * WAVE];
   __shared__ __attribute__((aligned(16))) uint16_t vs[16 * VSTRIDE];
   f32x4_t* const red = reinterpret_cast<f32x4_t*>(smem);
@@ -635,6 +774,8 @@ __global__ __launch_bounds__(64 * whole_waves(X8)) void whole_kernel(AdapterPara
 #pragma unroll
     for (int t = 0; t < RT; ++t) red[(w * RT + t) * 64 + lane] = acc[t][0];
   }
+  Units<J, End::plain, WAVES> units(p, c, tile, mine, any);
+  units.load(0);
   __syncthreads();
   // lane (g, n) of tile t holds ranks 16 t + 4 g .. + 3 of row n
   if (adds && tid < RT * 64) {
@@ -649,39 +790,7 @@ __global__ __launch_bounds__(64 * whole_waves(X8)) void whole_kernel(AdapterPara
     }
   }
   __syncthreads();
-  const int eighths = p.rank / 8;
-  const uint16_t* const weights = p.b + int64_t(max(tile.slot, 0)) * p.n * p.rank;
-  for (int c0 = c.begin + w * 128; c0 < c.end; c0 += WAVES * 128) {
-    const int col = c0 + 8 * n;
-    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
-    uint4 y[4];
-    int64_t row[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      row[i] = 4 * g + i < tile.count ? mine[i] : any;
-      y[i] = col < c.end ? mi::load16_nt(p.y + row[i] * p.y_stride + col) : none;
-    }
-    f32x4_t d[8];
-#pragma unroll
-    for (int t = 0; t < 8; ++t) d[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    if (adds) {
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const bool in = 4 * j + g < 2 * eighths;  // (or past the last pair)
-        const int from = in ? (4 * j + g) % eighths * 8 : 0;
-        const uint4 q = *reinterpret_cast<const uint4*>(vs + n * VSTRIDE + (4 * j + g) * 8);
-        const bf16x8_t v = mi::as_bf16x8(in ? q : none);
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          const uint4 m = in && col < c.end ? mi::load16(weights + int64_t(col + t) * p.rank + from) : none;
-          d[t] = mi::mfma_16x16x32_bf16(v, mi::as_bf16x8(m), d[t]);
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (col < c.end && 4 * g + i < tile.count) mi::store16(p.out + row[i] * p.o_stride + col, adds ? add_rounded(y[i], d, i) : y[i]);
-  }
+  units.run(vs, reinterpret_cast<uint16_t*>(smem) + w * kUnitWeights<J>);  // (the ring's and the sums' room)
 }
 
 int check_plan(const char* name, int64_t rows, int64_t slots) {
@@ -745,10 +854,12 @@ Split split_of(int64_t rows, int64_t slots, int64_t k, int64_t padded, bool x8) 
 }
 
 template <End END>
-auto expand_of(bool many, int j) {
+auto expand_of(bool many, bool by_waves, int j) {
   using Kernel = void (*)(AdapterParams);
-  const Kernel kernels[2][4] = {{expand_kernel<1, 1, END>, expand_kernel<1, 2, END>, expand_kernel<1, 4, END>, expand_kernel<1, 8, END>},
-                                {expand_kernel<4, 1, END>, expand_kernel<4, 2, END>, expand_kernel<4, 4, END>, expand_kernel<4, 8, END>}};
+  const Kernel kernels[2][4] = {
+      {expand_kernel<1, 1, END>, expand_kernel<1, 2, END>, expand_kernel<1, 4, END>, expand_kernel<1, 8, END>},
+      {expand_kernel<4, 1, END>, expand_kernel<4, 2, END>, expand_kernel<4, 4, END>, expand_kernel<4, 8, END>}};
+  if (by_waves) return Kernel(j ? expand_waves_kernel<2, END> : expand_waves_kernel<1, END>);
   return kernels[many][j];
 }
 
@@ -886,6 +997,8 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
   p.k = int(k);
   p.n = int(n);
   p.rank = int(rank);
+  p.eighths = int(rank / 8);
+  p.per_eighths = (65536 + p.eighths - 1) / p.eighths;
   p.ranks = int(pieces * rank);
   p.padded = int(padded);
   p.max_tiles = int(tiles);
@@ -895,8 +1008,15 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
   p.group_ranks = int(((padded / 16 + split.groups - 1) / split.groups) * 16);
   const bool x8 = p.xs != nullptr, many = tile_rows(rows) == 64;
   // columns of a workgroup: few where there are few tiles, so that every CU has some
+  // Tiles of 16 rows are a wave's work: a unit a wave where there are units enough for more than two workgroups a CU,
+  // and the rank is small; else a workgroup fetches a unit's B for one of its waves (us of both launches in a
+  // graph, one unit a workgroup / a wave): 32 rows of 8 adapters, 4,096 -> 2 x 14,336 with SiLU, rank 16 17.9 / 13.5,
+  // 32 20.0 / 16.0, 64 24.0 / 26.4; 48 of 24, 3,584 -> 2 x 18,944 35.1 / 16.1; 300 of 8, 14,336 -> 4,096 13.4 / 13.1; 32 of
+  // 8, 14,336 -> 4,096 (352 units) 10.9 / 11.2, rank 64 14.6 / 16.7; one row -> 2 x 14,336 8.8 / 9.7.
+  const int64_t units = tiles * ((out_n + 127) / 128);
+  const bool by_waves = !many && rank <= 32 && units > 2 * mi::num_cus();
   p.chunk = 128;
-  const int64_t enough = whole ? mi::num_cus() : 8 * mi::num_cus();
+  const int64_t enough = whole ? mi::num_cus() : by_waves ? 2 * mi::num_cus() : 8 * mi::num_cus();
   while (p.chunk < kMaxChunk && tiles * ((out_n + p.chunk - 1) / p.chunk) > enough) p.chunk *= 2;
   int chunks = 0;
   for (int i = 0; i < (silu ? 1 : pieces); ++i) p.end_chunk[i] = chunks += (piece_columns[i] + p.chunk - 1) / p.chunk;
@@ -917,9 +1037,9 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
       {shrink_many_kernel<true, 1>, shrink_many_kernel<true, 2>, nullptr, nullptr}};
   hipLaunchKernelGGL((many ? wide : few)[x8][rt - 1], grid, dim3(64 * (many ? kManyWaves : kWaves)), 0, s, p);
   const int j = rank <= 16 ? 0 : rank <= 32 ? 1 : rank <= 64 ? 2 : 3;
-  const Kernel expand = !silu      ? expand_of<End::plain>(many, j)
-                        : p.scales ? expand_of<End::silu8>(many, j)
-                                   : expand_of<End::silu>(many, j);
+  const Kernel expand = !silu      ? expand_of<End::plain>(many, by_waves, j)
+                        : p.scales ? expand_of<End::silu8>(many, by_waves, j)
+                                   : expand_of<End::silu>(many, by_waves, j);
   hipLaunchKernelGGL(expand, dim3(uint32_t(tiles), uint32_t(chunks)), block, 0, s, p);
   return mi::check_launch(name);
 }

@@ -60,6 +60,7 @@ def _want(values, ad, slot, y):
 @pytest.mark.parametrize("x8", [False, True])
 @pytest.mark.parametrize("k,pieces,rank", [(32, [16], 8), (96, [48, 16], 16), (896, [896, 128, 128], 16), (1056, [304], 24),
                                            (544, [64, 32, 16], 64), (4864, [896], 32), (256, [160, 160], 128),
+                                           (1056, [9728], 32), (896, [4864, 4864], 16),
                                            (160, [16] * 8, 8)])
 @pytest.mark.parametrize("rows,slots", [(1, 1), (3, 5), (17, 2), (64, 1), (130, 7), (300, 40), (320, 3), (321, 3), (512, 3), (513, 3), (1000, 1),
                                         (900, 30)])
@@ -175,7 +176,7 @@ def test_set_and_clear(dev):
 
 
 @pytest.mark.parametrize("x8", [False, True])
-@pytest.mark.parametrize("k,half,rank", [(32, 16, 8), (96, 32, 16), (896, 4864, 16), (1056, 304, 24), (544, 1184, 64), (256, 160, 128)])
+@pytest.mark.parametrize("k,half,rank", [(32, 16, 8), (96, 32, 16), (896, 4864, 16), (1056, 304, 24), (544, 1184, 64), (256, 160, 128), (544, 9728, 32)])
 @pytest.mark.parametrize("rows,slots", [(1, 1), (3, 5), (17, 2), (130, 7), (320, 3), (321, 3), (900, 30)])
 def test_add_adapters_silu(dev, rows, slots, k, half, rank, x8):
     """SiLU(gate) * up of the sums: gate and up within their bars dg and du of the 64-bit sums G and U (without
