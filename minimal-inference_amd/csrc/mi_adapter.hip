@@ -864,14 +864,13 @@ auto expand_of(bool many, bool by_waves, int j) {
 }
 
 // One launch for few rows where its workgroups, which each read their piece's A, are a round at most, and A is
-// short (us in a graph, two launches / one; adapters of rank 16, as many tiles):
-//   1 row, 1 tile      k 896 -> 1,152 7.1 / 5.9    k 4,096 -> 6,144 7.5 / 6.7    k 8,192 -> 10,240 (16 rows) 8.6 / 11.6
-//                      k 14,336 -> 4,096 8.3 / 11.1
-//   32 rows, 8         k 4,096 -> 6,144 9.8 / 9.2  k 4,096 -> 28,672 12.3 / 17.6 (more than a round)
-//   40 rows, 20        k 896 -> 9,728 12.2 / 8.9
-//   48 rows, 24        k 3,584 -> 4,608 10.8 / 9.0 k 18,944 -> 3,584 12.1 / 16.3
-//   64 rows, 32        k 4,096 -> 6,144 14.7 / 11.3
-//   256 rows, 64       k 4,096 -> 6,144 22.0 / 22.5 (more than a round)
+// short (us in a graph, two launches / one; adapters of rank 16):
+//   1 row               k 896 -> 1,152 7.1 / 5.9    k 4,096 -> 6,144 7.4 / 6.6    k 8,192 -> 10,240 (16 rows) 8.6 / 10.6
+//                       k 14,336 -> 4,096 8.3 / 11.1
+//   32 rows, 8 adapters k 4,096 -> 6,144 9.9 / 8.9  k 4,096 -> 28,672 11.6 / 15.8 (more than a round)
+//   40 rows, 20         k 896 -> 9,728 10.4 / 8.6
+//   48 rows, 24         k 3,584 -> 4,608 11.0 / 8.6 k 18,944 -> 3,584 12.5 / 17.5
+//   256 rows, 64        k 4,096 -> 6,144 16.8 / 20.1 (more than a round)
 constexpr int kMaxChunk = 1024;
 bool in_one_launch(int64_t rows, int64_t slots, int64_t k, int64_t rank, int64_t pieces, int64_t n) {
   return tile_rows(rows) == 16 && rank <= 16 && k <= 4096 && max_tiles(rows, slots) * (n / kMaxChunk + pieces) <= mi::num_cus();
