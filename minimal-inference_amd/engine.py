@@ -85,10 +85,10 @@ class Request:
     finish_reason: str | None = None
     prefill_done_time: float = 0.0
     last_token_time: float = 0.0
-    # of the model's adapters (Model.enable_adapters), -1 for none
-    adapter: int = -1
     # receives each token id, then None when the request is retired
     sink: Callable[[int | None], None] | None = None
+    # of the model's adapters (Model.enable_adapters), -1 for none
+    adapter: int = -1
 
 
 class _Pinned:

@@ -293,6 +293,8 @@ class Model:
         dense = self.fused_dense
         project = _project if dense else F.linear
         plan = backend.adapter_plan
+        if plan is not None and not dense:
+            raise ValueError("adapters need fused_dense")
 
         def adapted(y, h, L, name):  # y, with what the rows' adapters add to it
             adapters = L.adapters.get(name) if plan is not None else None

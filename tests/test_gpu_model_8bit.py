@@ -218,6 +218,22 @@ def test_model_refuses(dev):
             call()
 
 
+def test_unfused_layers_refuse_adapters(dev):
+    """A model whose fused layers are switched off after adapters were enabled: requests without one run, one
+    with an adapter is refused by the step, not served without it."""
+    from minimal_inference_amd.engine import Request, Scheduler
+
+    model = _model(dev)
+    model.enable_adapters(1, 8)
+    model.fused_dense = False
+    sch = Scheduler(model, max_batch_size=2, max_seq_len=64, use_graphs=False)
+    sch.submit(Request("a", [1, 2, 3], 2, 0.0))
+    sch.run()
+    sch.submit(Request("b", [1, 2, 3], 2, 0.0, adapter=0))
+    with pytest.raises(ValueError, match="fused_dense"):
+        sch.run()
+
+
 def _write(path, tensors, **config):
     from safetensors.torch import save_file
 
