@@ -10,9 +10,10 @@ tensors, ``add_rms_norm_mxfp8`` of the residual stream before a block.
 ``linear_mxfp8(x, weight, bias)`` is ``x @ weight.T + bias`` and
 ``linear_silu_mxfp8(x, gate_up)`` is ``silu(x @ gate.T) * (x @ up.T)`` of a fused gate
 and up weight, both operands MXFP8; the latter leaves MXFP8 rows again with
-``quantize=True``.  Sums are fp32, rounded once (the matrix instruction cuts products
-some 14 bits below the largest of those it adds side by side: 1.5e-5 of the result's
-norm on normal values).  There is no torch fallback and no backward pass: tensors that
+``quantize=True``.  Sums are fp32, rounded once, but the matrix instruction cuts each product to a multiple of
+2^-13 of the largest of its eight neighbours in k: 1.5e-5 of the result's
+norm on normal values, 2.7e-5 where single channels stand out, against 1.7e-3 that the rounding to bf16 makes.
+The same call repeats its bits.  There is no torch fallback and no backward pass: tensors that
 ask for gradients or carry forward-mode tangents are refused.
 """
 
