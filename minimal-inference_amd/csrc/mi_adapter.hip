@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "mi_adapter_ring.h"
 #include "mi_mx8.h"
 #include "mi_overlap.h"
 
@@ -308,13 +309,13 @@ __device__ __forceinline__ void multiply_ring(const AdapterParams& p, const Tile
 #pragma unroll
   for (int i = 0; i < 2 * NB; ++i) {
     const int at = i * 8 + r8;
-    x[i] = p.x + int64_t(order[at < tile.count ? at : 0]) * p.x_stride + chunk;
+    x[i] = p.x + int64_t(order[at < tile.count ? at : 0]) * p.x_stride;
   }
   const char* a[2 * RT];
 #pragma unroll
   for (int i = 0; i < 2 * RT; ++i) {
     const int r = rank0 + i * 8 + r8;  // (past the last rank any row will do: its sums are not kept)
-    a[i] = reinterpret_cast<const char*>(p.a + (int64_t(tile.slot) * p.ranks + (r < p.ranks ? r : 0)) * p.k) + chunk;
+    a[i] = reinterpret_cast<const char*>(p.a + (int64_t(tile.slot) * p.ranks + (r < p.ranks ? r : 0)) * p.k);
   }
   const char* const xs = X8 ? p.xs + int64_t(order[lane < tile.count ? lane : 0]) * p.xs_stride : nullptr;
   auto dma = [&](const char* from, lds_t* to) {
@@ -323,18 +324,18 @@ __device__ __forceinline__ void multiply_ring(const AdapterParams& p, const Tile
                                      (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 #endif
   };
-  // (behind the last k anything readable: it meets zeros, below)
+  // (behind the last k the row's start: it meets zeros, below)
   auto load = [&](int step, int slot) {
     lds_t* const to = lds + slot * SLOT;
     const int off = step < end ? step * 128 : 0;
-    const int xo = off + chunk < width ? off : 0;
+    const int xo = mi::adapter::ring_place(off, chunk, width);
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i) dma(x[i] + xo, to + i * 1024);
 #pragma unroll
     for (int l = 0; l < LOTS; ++l) {
-      const int ao = off * LOTS + l * 128;
+      const int ao = mi::adapter::ring_place(off * LOTS + l * 128, chunk, 2 * p.k);
 #pragma unroll
-      for (int i = 0; i < 2 * RT; ++i) dma(a[i] + (ao + chunk < 2 * p.k ? ao : 0), to + XBYTES + (l * 2 * RT + i) * 1024);
+      for (int i = 0; i < 2 * RT; ++i) dma(a[i] + ao, to + XBYTES + (l * 2 * RT + i) * 1024);
     }
   };
   // (8 bits: the scale bytes of four steps, 16 a row; a wave takes groups of four in turn)
