@@ -482,7 +482,8 @@ int mi_add_rms_norm_mxfp8(const void* x, int64_t x_stride, const void* delta, in
  * out = silu(x Wg^T) * (x Wu^T); no bias then, and with out_scales not null out is MXFP8 too
  * (codes and scale bytes, strides in bytes, n a multiple of 32), quantised from fp32.
  * rows 0..2^22, n 1..2^24 (any), k a multiple of 32 up to 2^20, strides at most 2^22;
- * out_stride in elements.  An out that overlaps x, W, the bias or its scales is refused.
+ * out_stride in elements.  An out that overlaps x, W, the bias or its scales is refused, and a
+ * workspace that overlaps any of them where sums are held there.
  * The result does not depend on timing.  workspace (16-byte aligned; may be null) as in
  * mi_linear_mxfp4. */
 size_t mi_linear_mxfp8_workspace_size(int64_t rows, int64_t n, int64_t k, int32_t silu);
@@ -514,7 +515,7 @@ int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void* x_scales,
  * columns each, and out [rows][n / 2] = silu(gate) * up of the sums, held in fp32 up to the one
  * rounding: bf16, or, out_scales not null, MXFP8 (n / 2 a multiple of 32, strides in bytes); y is
  * left as it is.  workspace: mi_add_adapters_workspace_size bytes (none
- * for some calls), need not be initialised, one call at a time.  A row's result depends on no other
+ * for some calls), need not be initialised, apart from every other argument, one call at a time.  A row's result depends on no other
  * row's values (the order of its sums on the number of rows).
  * ------------------------------------------------------------------------ */
 size_t mi_adapter_plan_size(int64_t rows, int64_t slots);

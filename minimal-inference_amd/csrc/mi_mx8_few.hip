@@ -281,8 +281,8 @@ void run_shared(const LinearParams& p, hipStream_t stream) {
 
 }  // namespace
 
-size_t few_workspace(bool glu, int64_t rows, int64_t n, int slabs) {
-  const int each = split_slabs_of(glu, rows, n, slabs, size_t(1) << 28);
+size_t few_workspace(bool glu, int64_t rows, int64_t n, int slabs, size_t room) {
+  const int each = split_slabs_of(glu, rows, n, slabs, room);
   return each < slabs ? size_t((slabs + each - 1) / each) * rows * ((n + 3) / 4) * 16 : 0;
 }
 

@@ -86,7 +86,7 @@ constexpr int64_t kFewRows = 64;
 constexpr int64_t kMaxRows = 1 << 22, kMaxN = 1 << 24, kMaxStride = 1 << 22;
 
 // (rows at most kFewRows; `room` bytes for parts)
-size_t few_workspace(bool glu, int64_t rows, int64_t n, int slabs);
+size_t few_workspace(bool glu, int64_t rows, int64_t n, int slabs, size_t room);
 void launch_few(const LinearParams& p, bool glu, size_t room, hipStream_t stream);
 // The sum of parts [part][half][row][columns in fours], and the end of the product.
 void launch_combine(const LinearParams& p, bool glu, int parts, hipStream_t stream);

@@ -556,8 +556,9 @@ void launch_combine(const LinearParams& p, bool glu, int parts, hipStream_t stre
   else hipLaunchKernelGGL((combine_kernel<true, false>), grid, block, 0, stream, p, parts);
 }
 
-size_t many_workspace(bool glu, int64_t rows, int64_t n, int slabs) {
-  return choose(glu, rows, n, slabs, size_t(1) << 28).bytes;
+// The bytes of parts that a call with `room` bytes for them writes.
+size_t parts_bytes(bool glu, int64_t rows, int64_t n, int slabs, size_t room) {
+  return rows <= kFewRows ? few_workspace(glu, rows, n, slabs, room) : choose(glu, rows, n, slabs, room).bytes;
 }
 
 void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t stream) {
@@ -581,8 +582,7 @@ void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t strea
 extern "C" size_t mi_linear_mxfp8_workspace_size(int64_t rows, int64_t n, int64_t k, int32_t silu) {
   using namespace mi::mx8;
   if (rows <= 0 || rows > kMaxRows || n <= 0 || n > kMaxN || k <= 0 || k % kBlock || k > kMaxK) return 0;
-  if (rows <= kFewRows) return few_workspace(silu != 0, rows, n, int(slabs(k)));
-  return many_workspace(silu != 0, rows, n, int(slabs(k)));
+  return parts_bytes(silu != 0, rows, n, int(slabs(k)), size_t(1) << 28);
 }
 
 extern "C" int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void* x_scales, int64_t x_scales_stride,
@@ -631,6 +631,14 @@ extern "C" int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void
   for (const mi::Rows& o : to)
     for (const mi::Rows& r : from) meet = meet || mi::rows_meet(o, r);
   if (meet) return mi::fail(MI_ERR_INVALID, "%s: out overlaps x, the weight, the bias or its own scales", name);
+  // (parts are written while others still read x and W, and read while out is written)
+  const size_t room = workspace ? workspace_bytes : 0;
+  if (const size_t bytes = room ? parts_bytes(silu != 0, rows, n, int(slabs(k)), room) : 0) {
+    const mi::Rows parts = {workspace, 0, 1, int64_t(bytes)};
+    for (const mi::Rows& r : to) meet = meet || mi::rows_meet(parts, r);
+    for (const mi::Rows& r : from) meet = meet || mi::rows_meet(parts, r);
+    if (meet) return mi::fail(MI_ERR_INVALID, "%s: the workspace overlaps another argument", name);
+  }
   LinearParams p;
   p.x = static_cast<const char*>(x_codes);
   p.x_stride = x_stride;
@@ -656,7 +664,6 @@ extern "C" int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void
           ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) & 7) == 0;
   p.wide = p.vec && n % 8 == 0 && out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const size_t room = workspace ? workspace_bytes : 0;
   if (rows <= kFewRows) launch_few(p, silu != 0, room, s);
   else launch_many(p, silu != 0, room, s);
   return mi::check_launch(name);
