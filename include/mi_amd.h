@@ -434,7 +434,8 @@ int mi_mxfp4_unpack(const void* codes, const void* scales, void* row_codes, void
  * workspace (16-byte aligned; may be null) holds partial sums of workgroups that
  * share k: mi_linear_mxfp4_workspace_size bytes are what the fastest form takes
  * (often 0); with fewer, one that takes no more is run, with the same results
- * within fp32 rounding.  It need not be initialised; one call at a time. */
+ * within fp32 rounding.  It need not be initialised; apart from every other argument (refused
+ * where sums are held in it); one call at a time. */
 size_t mi_linear_mxfp4_workspace_size(int64_t rows, int64_t n, int64_t k, int32_t silu,
                                       int32_t x_mxfp4);
 int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_scales, const void* codes,

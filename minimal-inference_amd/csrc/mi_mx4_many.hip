@@ -451,20 +451,37 @@ size_t many_workspace(bool mx, bool glu, int64_t rows, int64_t n, int slabs) {
   return few_us(mx, rows, int(row_tiles(glu ? 2 * n : n)), slabs) < c.us ? 0 : c.bytes;
 }
 
+// How a call with `room` bytes for parts goes: rows by blocks, the others by the few-row kernel.
+struct Way {
+  Choice c;
+  int64_t blocks;  // rows
+};
+Way way_of(bool mx, bool glu, int64_t rows, int64_t n, int slabs, size_t room) {
+  const int w_tiles = int(row_tiles(glu ? 2 * n : n));
+  const Choice c = choose(mx, glu, rows, n, slabs, room);
+  if (few_us(mx, rows, w_tiles, slabs) < c.us) return {c, 0};
+  // (4,105 x 4,096 x 6,144: 792 blocks are four rounds; 768 and nine rows of the few-row
+  // kernel three and 7 us)
+  if (const int64_t rest = rest_of(mx, rows)) {
+    const Choice whole = choose(mx, glu, rows - rest, n, slabs, room);
+    if (whole.us + few_us(mx, rest, w_tiles, slabs) < c.us) return {whole, rows - rest};
+  }
+  return {c, rows};
+}
+// The bytes of parts that it writes.
+size_t parts_bytes(bool mx, bool glu, int64_t rows, int64_t n, int64_t k, size_t room) {
+  if (few(mx, rows, glu ? 2 * n : n, k)) return 0;
+  const Way way = way_of(mx, glu, rows, n, int(slabs(k)), room);
+  return way.blocks && way.c.parts > 1 ? way.c.bytes : 0;
+}
+
 void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t stream) {
   const bool mx = p.xs != nullptr;
   LinearParams q = p;
-  Choice c = choose(mx, glu, p.rows, p.n, p.slabs, room);
-  if (few_us(mx, p.rows, p.w_tiles, p.slabs) < c.us) return launch_few(p, glu, stream);
-  // (4,105 x 4,096 x 6,144: 792 blocks are four rounds; 768 and nine rows of the few-row
-  // kernel three and 7 us)
-  if (const int64_t rest = rest_of(mx, p.rows)) {
-    const Choice whole = choose(mx, glu, p.rows - rest, p.n, p.slabs, room);
-    if (whole.us + few_us(mx, rest, p.w_tiles, p.slabs) < c.us) {
-      c = whole;
-      q.rows = p.rows - rest;
-    }
-  }
+  const Way way = way_of(mx, glu, p.rows, p.n, p.slabs, room);
+  if (!way.blocks) return launch_few(p, glu, stream);
+  const Choice& c = way.c;
+  q.rows = way.blocks;
   if (mx) glu ? launch<true, true>(q, c, stream) : launch<true, false>(q, c, stream);
   else glu ? launch<false, true>(q, c, stream) : launch<false, false>(q, c, stream);
   if (q.rows == p.rows) return;
@@ -519,6 +536,14 @@ extern "C" int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_sc
       {bias, 0, bias ? 1 : 0, n * 2}};
   for (const mi::Rows& r : from)
     if (mi::rows_meet(to, r)) return mi::fail(MI_ERR_INVALID, "linear_mxfp4: out overlaps x, the weight or the bias");
+  // (parts are written while others still read x and W, and read while out is written)
+  const size_t room = workspace ? workspace_bytes : 0;
+  if (const size_t bytes = room ? parts_bytes(x_scales != nullptr, silu != 0, rows, n, k, room) : 0) {
+    const mi::Rows parts = {workspace, 0, 1, int64_t(bytes)};
+    bool meet = mi::rows_meet(parts, to);
+    for (const mi::Rows& r : from) meet = meet || mi::rows_meet(parts, r);
+    if (meet) return mi::fail(MI_ERR_INVALID, "linear_mxfp4: the workspace overlaps another argument");
+  }
   LinearParams p;
   p.x = static_cast<const char*>(x);
   p.x_stride = x_stride;
@@ -540,6 +565,6 @@ extern "C" int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_sc
   const hipStream_t s = static_cast<hipStream_t>(stream);
   p.parts = static_cast<mi::f32x4_t*>(workspace);
   if (few(x_scales != nullptr, rows, silu ? 2 * n : n, k)) launch_few(p, silu != 0, s);
-  else launch_many(p, silu != 0, workspace ? workspace_bytes : 0, s);
+  else launch_many(p, silu != 0, room, s);
   return mi::check_launch("linear_mxfp4");
 }

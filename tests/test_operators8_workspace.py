@@ -62,3 +62,24 @@ def test_adapters_refuse_a_workspace_over(at):
     assert lib.mi_add_adapters(*a.values(), None) == mod.MI_ERR_INVALID
     # (y is out itself in place)
     assert mod.last_error().startswith("add_adapters: ") and "overlaps another argument" in mod.last_error()
+
+
+# x at 0 (bf16, or codes), its scales at 2^25, W at 2^26, its scales at 2^30, out at 2^31
+LINEAR4 = dict(x=FAKE, xs=16384, xsc=None, w=FAKE + (1 << 26), wsc=FAKE + (1 << 30), bias=None, out=FAKE + (1 << 31), os=128, rows=200,
+               n=128, k=16384, silu=0, work=FAKE + (1 << 33), bytes=1 << 28)
+
+
+@pytest.mark.parametrize("mx", [0, 1])
+@pytest.mark.parametrize("at", ["x", "xsc", "w", "wsc", "out", "bias"])
+def test_linear_mxfp4_refuses_a_workspace_over(at, mx):
+    if at == "xsc" and not mx:
+        pytest.skip("no such argument")
+    mod, lib = _lib()
+    a = LINEAR4 | ({"xsc": FAKE + (1 << 25)} if mx else {})
+    need = lib.mi_linear_mxfp4_workspace_size(a["rows"], a["n"], a["k"], 0, mx)
+    assert need > 0
+    if at == "bias":
+        a["bias"] = FAKE + (1 << 34)
+    a["work"] = a[at] - need + 16
+    assert lib.mi_linear_mxfp4(*a.values(), None) == mod.MI_ERR_INVALID
+    assert mod.last_error() == "linear_mxfp4: the workspace overlaps another argument"
