@@ -28,6 +28,16 @@ def call_on(t: torch.Tensor, name: str, *args) -> None:
         _lib.check(status, name)
 
 
+def bytes_on(device: int | None, name: str, *args) -> int:
+    """What a size entry answers with ``device`` current (its number of CUs decides how work is shared, here as
+    in the launch, which ``call_on`` makes on the tensors' device); None: the current one."""
+    entry = getattr(_lib.load(), name)
+    if device is None or device == torch._C._cuda_getDevice():
+        return int(entry(*args))
+    with torch.cuda.device(device):
+        return int(entry(*args))
+
+
 def require_gpu(name: str, t: torch.Tensor) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")

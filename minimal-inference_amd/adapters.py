@@ -19,7 +19,7 @@ import functools
 import torch
 
 from . import _lib
-from ._util import call_on, refuse_derivatives, require_dtype, require_gpu, require_i32_vector
+from ._util import bytes_on, call_on, refuse_derivatives, require_dtype, require_gpu, require_i32_vector
 from .mxfp8 import MXFP8, _out, _rows8, _rows_of
 
 MAX_SLOTS = 1023
@@ -136,8 +136,8 @@ class AdapterPlan:
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_size(rows: int, slots: int, k: int, rank: int, pieces: int, n: int, silu: bool) -> int:
-    return int(_lib.load().mi_add_adapters_workspace_size(rows, slots, k, rank, pieces, n, silu))
+def _workspace_size(rows: int, slots: int, k: int, rank: int, pieces: int, n: int, silu: bool, device: int | None = None) -> int:
+    return bytes_on(device, "mi_add_adapters_workspace_size", rows, slots, k, rank, pieces, n, silu)
 
 
 def _add(y, x, adapters, plan, out, silu: bool, quantize: bool):
@@ -166,7 +166,7 @@ def _add(y, x, adapters, plan, out, silu: bool, quantize: bool):
         out = y if out is None and not silu else _out(out, rows, n // 2 if silu else n, device)
         to, out_stride = out.data_ptr(), out.stride(0)
     if rows:
-        room = _workspace_size(rows, adapters.slots, adapters.k, adapters.rank, len(adapters.pieces), n, silu)
+        room = _workspace_size(rows, adapters.slots, adapters.k, adapters.rank, len(adapters.pieces), n, silu, device.index)
         # (a tensor of this call's own: calls on several streams and in graphs share nothing)
         workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
         call_on(y, "mi_add_adapters", y.data_ptr(), y.stride(0), data, stride, scales, s_stride, adapters.a.data_ptr(),

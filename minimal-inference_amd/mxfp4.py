@@ -20,8 +20,7 @@ import functools
 import torch
 from torch.autograd import forward_ad
 
-from . import _lib
-from ._util import call_on, refuse_derivatives, require_dtype, require_gpu
+from ._util import bytes_on, call_on, refuse_derivatives, require_dtype, require_gpu
 
 BLOCK = 32
 _TILE_ROWS, _SLAB, _TILE_BYTES, _QUAD_BYTES = 16, 128, 1024, 256
@@ -155,7 +154,7 @@ def _linear(x, weight: MXFP4, bias, out, silu: bool) -> torch.Tensor:
             refuse_derivatives("bias", bias)
     out = _out(out, rows, n, like)
     if rows and n:
-        room = _workspace_size(rows, n, k, silu, scales is not None) if rows > _FEW_ROWS else 0
+        room = _workspace_size(rows, n, k, silu, scales is not None, like.get_device()) if rows > _FEW_ROWS else 0
         # (a tensor of this call's own: calls on several streams and in graphs share nothing)
         workspace = torch.empty(room, dtype=torch.uint8, device=like.device) if room else None
         call_on(like, "mi_linear_mxfp4", data, stride, scales, weight.codes_ptr, weight.scales_ptr,
@@ -165,8 +164,8 @@ def _linear(x, weight: MXFP4, bias, out, silu: bool) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_size(rows: int, n: int, k: int, silu: bool, x_mxfp4: bool) -> int:
-    return int(_lib.load().mi_linear_mxfp4_workspace_size(rows, n, k, silu, x_mxfp4))
+def _workspace_size(rows: int, n: int, k: int, silu: bool, x_mxfp4: bool, device: int | None = None) -> int:
+    return bytes_on(device, "mi_linear_mxfp4_workspace_size", rows, n, k, silu, x_mxfp4)
 
 
 def linear_mxfp4(x: torch.Tensor | MXFP4, weight: MXFP4, bias: torch.Tensor | None = None,

@@ -24,8 +24,7 @@ import functools
 import torch
 from torch.autograd import forward_ad
 
-from . import _lib
-from ._util import call_on, refuse_derivatives, require_dtype, require_gpu
+from ._util import bytes_on, call_on, refuse_derivatives, require_dtype, require_gpu
 
 BLOCK = 32
 _PIECE = 16  # bytes of scales that are read together
@@ -213,8 +212,8 @@ def add_rms_norm_mxfp8(x: torch.Tensor, delta: torch.Tensor | None, weight: torc
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_size(rows: int, n: int, k: int, silu: bool) -> int:
-    return int(_lib.load().mi_linear_mxfp8_workspace_size(rows, n, k, silu))
+def _workspace_size(rows: int, n: int, k: int, silu: bool, device: int | None = None) -> int:
+    return bytes_on(device, "mi_linear_mxfp8_workspace_size", rows, n, k, silu)
 
 
 def _linear(x: MXFP8, weight: MXFP8, bias, out, silu: bool, quantize: bool):
@@ -243,7 +242,7 @@ def _linear(x: MXFP8, weight: MXFP8, bias, out, silu: bool, quantize: bool):
         out = _out(out, rows, n, device)
         to, stride, scales, s_stride = out.data_ptr(), out.stride(0), None, 0
     if rows and n:
-        room = _workspace_size(rows, n, k, silu)
+        room = _workspace_size(rows, n, k, silu, device.index)
         # (a tensor of this call's own: calls on several streams and in graphs share nothing)
         workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
         call_on(x.anchor, "mi_linear_mxfp8", x.codes_ptr, x.codes_stride, x.scales_ptr, x.scales_stride,
