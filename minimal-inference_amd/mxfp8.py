@@ -262,7 +262,7 @@ def linear_mxfp8(x: MXFP8, weight: MXFP8, bias: torch.Tensor | None = None,
 def linear_silu_mxfp8(x: MXFP8, gate_up: MXFP8, out: "torch.Tensor | MXFP8 | None" = None, *,
                       quantize: bool = False) -> "torch.Tensor | MXFP8":
     """``silu(x @ gate.T) * (x @ up.T)``, gate and up the halves of gate_up's rows, as bf16
-    [rows, n], or with ``quantize`` as MXFP8, rounded from fp32 (n a multiple of 32)."""
+    [rows, n], or with ``quantize`` as MXFP8, rounded from fp32 (n a multiple of 32; silu within 2^-20)."""
     if quantize and isinstance(gate_up, MXFP8) and gate_up.rows // 2 % BLOCK:
         raise ValueError(f"rows in MXFP8 have columns in blocks of {BLOCK}; got {gate_up.rows // 2}")
     return _linear(x, gate_up, None, out, True, quantize)
