@@ -111,10 +111,12 @@ __device__ __forceinline__ double wave_sum(double v) {
 }
 
 // a (hi + lo), rounded to odd: cut, with the last bit set where something was cut off.  Rounded
-// again to the four bits of a code this is the exact product's rounding.  So is a hi rounded to
-// nearest, unless that lies halfway between two codes, with 19 zeros behind its leading bits.
+// again to the four bits of a code this is the exact product's rounding.  So is all of a (hi + lo) rounded to
+// nearest (a hi alone may be an ulp off and pass the middle), unless that lies halfway between two codes, with 19
+// zeros behind its leading bits.
+__device__ __forceinline__ float nearest_product(float a, float hi, float lo) { return fmaf(a, hi, a * lo); }
 __device__ __forceinline__ float product_to_odd(float a, float hi, float lo) {
-  const float h = a * hi, rest = fmaf(a, lo, fmaf(a, hi, -h));
+  const float h = nearest_product(a, hi, lo), rest = fmaf(a, lo, fmaf(a, hi, -h));
   const uint32_t u = __float_as_uint(h);
   // (an infinity or a NaN leaves a NaN)
   return !(rest < 0.f || rest > 0.f) ? h : __uint_as_float((u - ((u ^ __float_as_uint(rest)) >> 31)) | 1u);
@@ -188,7 +190,7 @@ __global__ __launch_bounds__(kMaxThreads) void add_rms_kernel(AddRmsParams p) {
     for (int k = 0; k < 8; ++k) {
       const uint32_t w16 = ww[k / 2];
       v[c][k] *= k % 2 ? mi::bf16_hi(w16) : mi::bf16_lo(w16);
-      h[k] = v[c][k] * hi;
+      h[k] = nearest_product(v[c][k], hi, lo);
       zeros = min(zeros, __float_as_uint(h[k]) & 0x7ffffu);
     }
     if (zeros == 0) {
