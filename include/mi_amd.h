@@ -502,8 +502,8 @@ int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void* x_scales,
  * mi_adapter_plan sorts a batch's rows by adapter, once for all its projections:
  * slot_of_row [rows] int32, an id outside 0..slots-1 (as -1) for none; at most 2^22
  * rows, 1,023 adapters.  plan: mi_adapter_plan_size bytes (of rows or more), 16-byte
- * aligned, written here and read by runs with the same rows and slots (others, as a replayed graph
- * may hold them, leave NaN in out).
+ * aligned, written here (for no rows too) and read by runs with the same rows and slots (others, as a
+ * replayed graph may hold them, leave NaN in out).
  *
  * mi_add_adapters: out = y + scale[s] * B[s] (A[s] x), one rounding to bf16, with row
  * t's adapter s; rows without one are y's.  y, out [rows][n] bf16; x [rows][k] bf16, or,

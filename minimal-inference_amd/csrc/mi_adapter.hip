@@ -890,8 +890,9 @@ extern "C" int mi_adapter_plan(void* plan, size_t plan_bytes, const int32_t* slo
   const char* const name = "adapter_plan";
   mi::clear_error();
   if (int rc = check_plan(name, rows, slots)) return rc;
-  if (rows == 0) return MI_OK;
-  if (!plan || !slot_of_row) return mi::fail(MI_ERR_INVALID, "%s: null pointer argument", name);
+  // (no rows: the plan that was there is none either, for graphs that are replayed with it)
+  if (rows == 0 && !plan) return MI_OK;
+  if (!plan || (rows && !slot_of_row)) return mi::fail(MI_ERR_INVALID, "%s: null pointer argument", name);
   if ((reinterpret_cast<uintptr_t>(plan) & 15) || (reinterpret_cast<uintptr_t>(slot_of_row) & 3))
     return mi::fail(MI_ERR_INVALID, "%s: the plan must be 16-byte aligned, the slots 4-byte", name);
   const size_t need = plan_size(rows, slots);
