@@ -504,7 +504,7 @@ float wide_us(int64_t workgroups, int slabs) { return rounds_us(workgroups, slab
 float block_us(int64_t workgroups, int slabs) { return rounds_us(workgroups, slabs, 2.f, 0.41f, 0.2f, true); }
 // The few-row kernel's (up to 64 rows): W's bytes from memory, x's into every workgroup.
 float few_us(int64_t rows, int64_t w_rows, int slabs) {
-  const float k = float(slabs) * kSlab, workgroups = std::max(1.f, std::min(float(w_rows) / 16, float(w_rows) / 64));
+  const float k = float(slabs) * kSlab, workgroups = std::max(1.f, float(w_rows) / 64);
   return kStartUs + float(w_rows) * k * 33 / 32 / 5.2e6f + float(rows) * k * workgroups / 15e6f;
 }
 
