@@ -30,6 +30,7 @@ import re
 import torch
 
 from .model import ADAPTED
+from .mxfp4 import MXFP4
 
 _LAYER = re.compile(r"^model\.layers\.(\d+)\.(.+)$")
 
@@ -81,7 +82,7 @@ def load_weights(model, model_path: str) -> None:
     for L in model.layers:
         for name in ADAPTED:
             if not isinstance(getattr(L, name), torch.Tensor):
-                bits = 4 if type(getattr(L, name)).__name__ == "MXFP4" else 8
+                bits = 4 if isinstance(getattr(L, name), MXFP4) else 8
                 raise ValueError(f"the model holds {bits}-bit weights: load a checkpoint before quantize_weights()")
     targets = _targets(model)
     seen: set[str] = set()
