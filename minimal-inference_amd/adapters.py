@@ -68,6 +68,10 @@ class Adapters:
         self.columns = (ctypes.c_int32 * len(pieces))(*pieces)
         self.columns_ptr = ctypes.addressof(self.columns)
 
+    @property
+    def nbytes(self) -> int:
+        return self.a.nbytes + self.b.nbytes + self.scale.nbytes
+
     @classmethod
     def empty(cls, slots: int, k: int, pieces, rank: int, device) -> "Adapters":
         """Room for so many adapters that add nothing until they are set."""

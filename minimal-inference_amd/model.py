@@ -209,6 +209,7 @@ class Model:
         self.cos, self.sin = precompute_rope(cfg.head_dim, n, cfg.rope_theta, self.device, dtype)
 
     def weight_bytes(self) -> int:
+        """Of everything that a forward may read, the adapters' room included."""
         t = self.embed.numel() + self.norm.numel()
         if self.lm_head is not self.embed:
             t += self.lm_head.numel()
@@ -217,6 +218,7 @@ class Model:
             for x in (L.in_norm, L.post_norm, L.w_qkv, L.b_qkv, L.w_o, L.w_gate_up, L.w_down):
                 if x is not None:
                     t += x.nbytes
+            t += sum(a.nbytes for a in L.adapters.values())
         return t
 
     def quantize_weights(self, weight_format: str = "mxfp4") -> None:

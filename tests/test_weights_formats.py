@@ -26,3 +26,17 @@ def test_a_checkpoint_over_quantised_weights_is_refused_by_their_format():
         model.layers[1].w_o = w
         with pytest.raises(ValueError, match=f"{bits}-bit weights"):
             load_weights(model, "nowhere")
+
+
+def test_weight_bytes_count_adapters():
+    import torch
+
+    from minimal_inference_amd.adapters import Adapters
+
+    model = _model()
+    before = model.weight_bytes()
+    ad = Adapters.__new__(Adapters)  # (made on a GPU alone)
+    ad.a, ad.b, ad.scale = torch.zeros(3, 8, 64, dtype=torch.bfloat16), torch.zeros(3, 64, 8, dtype=torch.bfloat16), torch.zeros(3)
+    assert ad.nbytes == 2 * 3 * 8 * 128 + 12
+    model.layers[1].adapters = {"w_o": ad, "w_down": ad}
+    assert model.weight_bytes() == before + 2 * ad.nbytes
