@@ -423,11 +423,19 @@ int mi_mxfp4_pack(const void* row_codes, const void* row_scales, void* codes, vo
 int mi_mxfp4_unpack(const void* codes, const void* scales, void* row_codes, void* row_scales,
                     int64_t rows, int64_t cols, mi_stream_t stream);
 
+/* What becomes of a gated product's gate and up sums (`silu` of mi_linear_mxfp4, mi_linear_mxfp8 and
+ * mi_add_adapters; any other number but 0 is MI_SILU). */
+#define MI_SILU 1       /* silu(gate) * up in fp32, rounded once */
+#define MI_SILU_SUMS 2  /* products: the sums themselves, fp32; adapters: y is such sums */
+#define MI_SILU_STEPS 3 /* adapters: rounded to bf16 at every step, as mi_silu_mul is */
+
 /* out = x W^T (+ bias) with W [n][k] in MXFP4, fp32 accumulation, one rounding
  * to bf16.  x_scales null: x is [rows][k] bf16 with row stride x_stride (16-byte
  * aligned rows); else x, x_scales are an MXFP4 matrix [rows][k] and x_stride is
  * not read.  silu != 0: W is [2 n][k], n gate rows and then n up rows, and
- * out = silu(x Wg^T) * (x Wu^T) (MLP, model.py:301-311); no bias then.
+ * out = silu(x Wg^T) * (x Wu^T) (MLP, model.py:301-311); no bias then.  MI_SILU_SUMS: out is
+ * fp32 [rows][2 n], x Wg^T and behind it x Wu^T, the bits that the gated product goes on with (n a multiple of
+ * 4, out 16-byte aligned, out_stride in floats, a multiple of 4).
  * rows 0..2^22, n 1..2^24 (any), k a multiple of 32 up to 2^20, x_stride at most
  * 2^22; bias [n] or null.  An out that overlaps x, W or the bias is refused (rows of
  * one buffer whose columns lie apart do not).  The result does not depend on timing.
@@ -481,7 +489,8 @@ int mi_add_rms_norm_mxfp8(const void* x, int64_t x_stride, const void* delta, in
  * rounding to bf16.  (The matrix instruction cuts each product toward zero to a multiple of 2^-13 of the
  * power of two of the largest among its eight neighbours in k, before fp32: 1.5e-5 of the result's norm on normal values.)  silu != 0: W is [2 n][k], n gate rows and then n up rows, and
  * out = silu(x Wg^T) * (x Wu^T) (silu within 2^-20 of itself); no bias then, and with out_scales not null out is MXFP8 too
- * (codes and scale bytes, strides in bytes, n a multiple of 32), quantised from fp32.
+ * (codes and scale bytes, strides in bytes, n a multiple of 32), quantised from fp32.  MI_SILU_SUMS: fp32
+ * sums as in mi_linear_mxfp4, those of the product that leaves MXFP8.
  * rows 0..2^22, n 1..2^24 (any), k a multiple of 32 up to 2^20, strides at most 2^22;
  * out_stride in elements.  An out that overlaps x, W, the bias or its scales is refused, and a
  * workspace that overlaps any of them where sums are held there.
@@ -515,7 +524,10 @@ int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void* x_scales,
  * overlaps another argument is refused.  silu != 0: the two pieces are gate and up, as many
  * columns each, and out [rows][n / 2] = silu(gate) * up of the sums, held in fp32 up to the one
  * rounding: bf16, or, out_scales not null, MXFP8 (n / 2 a multiple of 32, strides in bytes); y is
- * left as it is.  workspace: mi_add_adapters_workspace_size bytes (none
+ * left as it is.  So that a row without an adapter gets the bits of the projection's own gated form whatever
+ * rows stand beside it: MI_SILU_SUMS, y is fp32, what mi_linear_mxfp4 and mi_linear_mxfp8 leave with that
+ * (y_stride in floats; out in bf16 as the first's gated form makes it, in MXFP8 as the second's); MI_SILU_STEPS, y and
+ * out are bf16 and each step is rounded to it, as mi_linear and mi_silu_mul do.  workspace: mi_add_adapters_workspace_size bytes (none
  * for some calls), need not be initialised, apart from every other argument, one call at a time.  A row's result depends on no other
  * row's values (the order of its sums on the number of rows).
  * ------------------------------------------------------------------------ */

@@ -61,6 +61,23 @@ def refuse_derivatives(name: str, t: torch.Tensor | None) -> None:
         raise ValueError(f"{name} has a forward-mode tangent: there is no derivative")
 
 
+SILU, SILU_SUMS, SILU_STEPS = 1, 2, 3  # MI_SILU, MI_SILU_SUMS, MI_SILU_STEPS
+
+
+def sums_out(out: torch.Tensor | None, rows: int, n: int, device) -> torch.Tensor:
+    """Room for the fp32 sums of a gated product, gate's n and up's n columns."""
+    if n % 4:
+        raise ValueError(f"gate and up of a multiple of 4 columns each; got {n}")
+    if out is None:
+        return torch.empty(rows, 2 * n, dtype=torch.float32, device=device)
+    require_gpu("out", out)
+    require_dtype("out", out, torch.float32)
+    if out.shape != (rows, 2 * n) or out.stride(1) != 1 or out.device != device:
+        raise ValueError(f"out must be [{rows}, {2 * n}] with a contiguous last axis on {device}; got {tuple(out.shape)} on {out.device}")
+    refuse_derivatives("out", out)
+    return out
+
+
 def require_i32_vector(name: str, t: torch.Tensor) -> None:
     require_gpu(name, t)
     require_dtype(name, t, torch.int32)

@@ -19,7 +19,7 @@ import functools
 import torch
 
 from . import _lib
-from ._util import bytes_on, call_on, refuse_derivatives, require_dtype, require_gpu, require_i32_vector
+from ._util import SILU, SILU_STEPS, SILU_SUMS, bytes_on, call_on, refuse_derivatives, require_dtype, require_gpu, require_i32_vector
 from .mxfp8 import MXFP8, _out, _rows8, _rows_of
 
 MAX_SLOTS = 1023
@@ -144,8 +144,17 @@ def _workspace_size(rows: int, slots: int, k: int, rank: int, pieces: int, n: in
     return bytes_on(device, "mi_add_adapters_workspace_size", rows, slots, k, rank, pieces, n, silu)
 
 
-def _add(y, x, adapters, plan, out, silu: bool, quantize: bool):
-    rows, n = _rows_of("y", y)
+def _sums_of(y: torch.Tensor) -> tuple[int, int]:
+    refuse_derivatives("y", y)
+    if y.dim() != 2 or y.stride(1) != 1:
+        raise ValueError(f"y must be [rows, width] with a contiguous last axis; got {tuple(y.shape)}")
+    return y.shape
+
+
+def _add(y, x, adapters, plan, out, silu: int, quantize: bool):
+    if silu == SILU and y.dtype == torch.float32 and y.is_cuda:
+        silu = SILU_SUMS
+    rows, n = _sums_of(y) if silu == SILU_SUMS else _rows_of("y", y)
     device = y.device
     if not isinstance(adapters, Adapters) or not isinstance(plan, AdapterPlan):
         raise TypeError("adapters must be an Adapters and plan an AdapterPlan")
@@ -170,7 +179,7 @@ def _add(y, x, adapters, plan, out, silu: bool, quantize: bool):
         out = y if out is None and not silu else _out(out, rows, n // 2 if silu else n, device)
         to, out_stride = out.data_ptr(), out.stride(0)
     if rows:
-        room = _workspace_size(rows, adapters.slots, adapters.k, adapters.rank, len(adapters.pieces), n, silu, device.index)
+        room = _workspace_size(rows, adapters.slots, adapters.k, adapters.rank, len(adapters.pieces), n, silu != 0, device.index)
         # (a tensor of this call's own: calls on several streams and in graphs share nothing)
         workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
         call_on(y, "mi_add_adapters", y.data_ptr(), y.stride(0), data, stride, scales, s_stride, adapters.a.data_ptr(),
@@ -184,12 +193,20 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor | MXFP8, adapters: Adapters, p
                  out: torch.Tensor | None = None) -> torch.Tensor:
     """``y[t] + scale[s] * B[s] @ (A[s] @ x[t])`` with s row t's adapter in the plan; rows without one are
     y's.  Into ``out``, in place in y when that is not given; an out that overlaps another argument is refused."""
-    return _add(y, x, adapters, plan, out, False, False)
+    return _add(y, x, adapters, plan, out, 0, False)
 
 
 def add_adapters_silu(y: torch.Tensor, x: torch.Tensor | MXFP8, adapters: Adapters, plan: AdapterPlan,
-                      out: "torch.Tensor | MXFP8 | None" = None, *, quantize: bool = False) -> "torch.Tensor | MXFP8":
+                      out: "torch.Tensor | MXFP8 | None" = None, *, quantize: bool = False,
+                      stepwise: bool = False) -> "torch.Tensor | MXFP8":
     """``silu(gate) * up`` of what ``add_adapters`` makes of a fused gate and up projection's y [rows, 2 n], held in
     fp32 up to the one rounding: bf16 [rows, n], or with ``quantize`` MXFP8 (n a multiple of 32).  y is left
-    as it is; the adapters have two pieces of n columns."""
-    return _add(y, x, adapters, plan, out, True, quantize)
+    as it is; the adapters have two pieces of n columns.
+
+    Rows without an adapter get the bits that the projection's own gated form leaves them, whatever rows stand beside
+    them: with y the fp32 sums of ``mxfp8.gate_up_mxfp8`` and ``quantize`` those of ``linear_silu_mxfp8(...,
+    quantize=True)``, with those of ``mxfp4.gate_up_mxfp4`` those of ``linear_silu_mxfp4``, and with ``stepwise``, y the
+    bf16 of ``dense.linear``, those of ``dense.linear_silu`` (sum, silu and product each rounded to bf16)."""
+    if stepwise and quantize:
+        raise ValueError("rows in MXFP8 are rounded once: not stepwise")
+    return _add(y, x, adapters, plan, out, SILU_STEPS if stepwise else SILU, quantize)

@@ -9,7 +9,8 @@
 //   (few rows and a short A: both products in one launch)
 //   expand : the parts' sum, times scale, as a pair of bf16 (v and what its rounding left: 16
 //            bits of v), times B in fp32, plus y, one rounding; or SiLU(gate) * up of the sums of a
-//            gate and an up piece.
+//            gate and an up piece.  Rows without an adapter get the bits that the projection's own
+//            gated form leaves them, whatever rows stand beside them.
 //
 // Bound: for prompts HBM, one read of x, one of y and the write of out; A and B come from the
 // caches.  For decode steps the two launches' start and end, and the read of the adapters.
@@ -149,8 +150,46 @@ __device__ __forceinline__ Columns columns_of(const AdapterParams& p) {
   const int begin = start + (int(blockIdx.y) - before) * p.chunk;
   return {piece, begin, min(begin + p.chunk, p.end[piece])};
 }
-// What becomes of the sums: out's bf16, or, of gate and up columns, SiLU(gate) * up in bf16 or 8 bits.
-enum class End { plain, silu, silu8 };
+// What becomes of the sums: out's bf16, or, of gate and up columns, SiLU(gate) * up in bf16 or 8 bits; `steps`: each
+// step rounded to bf16, as mi_silu_mul is; `sums`: y is fp32, SiLU as linear_mxfp4's gated form takes
+// it (sums) and as linear_mxfp8's (sums8).
+enum class End { plain, silu, silu8, steps, sums, sums8 };
+constexpr bool in_8_bits(End end) { return end == End::silu8 || end == End::sums8; }
+constexpr bool y_is_fp32(End end) { return end == End::sums || end == End::sums8; }
+
+// Eight columns of a row of y.
+template <End END>
+struct Eight {
+  uint4 v[y_is_fp32(END) ? 2 : 1];
+  __device__ __forceinline__ void load(const AdapterParams& p, int64_t row, int col, bool in) {
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (y_is_fp32(END)) {
+      const float* const from = reinterpret_cast<const float*>(p.y) + row * p.y_stride + col;
+      v[0] = in ? mi::load16_nt(from) : none;
+      v[1] = in ? mi::load16_nt(from + 4) : none;
+    } else {
+      v[0] = in ? mi::load16_nt(p.y + row * p.y_stride + col) : none;
+    }
+  }
+  __device__ __forceinline__ float operator[](int t) const {
+    if constexpr (y_is_fp32(END)) {
+      const uint32_t words[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+      return __uint_as_float(words[t]);
+    } else {
+      const uint32_t pairs[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+      return t % 2 ? mi::bf16_hi(pairs[t / 2]) : mi::bf16_lo(pairs[t / 2]);
+    }
+  }
+};
+
+// What a unit's sums start from: y where that is fp32 (which frees its registers while they grow), else zeros.
+template <End END>
+__device__ __forceinline__ void begin_sums(f32x4_t (&d)[8], const Eight<END> (&y)[4]) {
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[t][i] = y_is_fp32(END) ? y[i][t] : 0.f;
+}
 
 // Where no row's adapter is known: NaN (the tiles are as many as the rows' at least).
 template <End END>
@@ -158,7 +197,7 @@ __device__ __forceinline__ void write_nan(const AdapterParams& p, int tile_rows,
   for (int i = 0; i < tile_rows && int(blockIdx.x) * tile_rows + i < p.rows; ++i)
     for (int col = c.begin + int(threadIdx.x); col < c.end; col += int(blockDim.x)) {
       const int64_t row = int64_t(blockIdx.x) * tile_rows + i;
-      if constexpr (END == End::silu8) {
+      if constexpr (in_8_bits(END)) {
         reinterpret_cast<uint8_t*>(p.out)[row * p.o_stride + col] = 0;
         if (col % mi::mx8::kBlock == 0) p.scales[row * p.s_stride + col / mi::mx8::kBlock] = 255;
       } else {
@@ -445,23 +484,26 @@ __global__ __launch_bounds__(64 * kManyWaves) void shrink_many_kernel(AdapterPar
 // What a lane makes of its four rows' y and of its sums for columns col .. col + 7 of them, the first `count` of
 // which are the tile's: out, or, of gate columns, the values that the up columns' turn takes.
 template <End END, int HALF>
-__device__ __forceinline__ void end_of_unit(const AdapterParams& p, bool adds, const uint4 (&y)[4], const f32x4_t (&d)[8],
+__device__ __forceinline__ void end_of_unit(const AdapterParams& p, bool adds, const Eight<END> (&y)[4], const f32x4_t (&d)[8],
                                             float (&gate)[END == End::plain ? 1 : 4][8], const int64_t (&row)[4], int col, int count) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (END == End::plain) {
-      const uint4 o = adds ? add_rounded(y[i], d, i) : y[i];
+      const uint4 o = adds ? add_rounded(y[i].v[0], d, i) : y[i].v[0];
       if (i < count) mi::store16(p.out + row[i] * p.o_stride + col, o);
     } else {
-      const uint32_t pairs[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
       float v[8];
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
-        v[t] = (t % 2 ? mi::bf16_hi(pairs[t / 2]) : mi::bf16_lo(pairs[t / 2])) + d[t][i];
-        if constexpr (HALF == 0) gate[i][t] = mi::mx8::silu20(v[t]);
-        else v[t] *= gate[i][t];
+        if constexpr (y_is_fp32(END)) v[t] = d[t][i];
+        else v[t] = adds ? y[i][t] + d[t][i] : y[i][t];
+        if constexpr (END == End::steps) v[t] = mi::bf16_lo(mi::cvt_pk_bf16(v[t], 0.f));
+        if constexpr (HALF == 1) v[t] *= gate[i][t];
+        else if constexpr (END == End::steps) gate[i][t] = mi::bf16_lo(mi::cvt_pk_bf16(mi::silu(v[t]), 0.f));
+        else if constexpr (END == End::sums) gate[i][t] = mi::silu(v[t]);
+        else gate[i][t] = mi::mx8::silu20(v[t]);
       }
-      if constexpr (HALF == 1 && END == End::silu) {
+      if constexpr (HALF == 1 && !in_8_bits(END)) {
         if (i < count)
           mi::store16(p.out + row[i] * p.o_stride + col, make_uint4(mi::cvt_pk_bf16(v[0], v[1]), mi::cvt_pk_bf16(v[2], v[3]),
                                                                    mi::cvt_pk_bf16(v[4], v[5]), mi::cvt_pk_bf16(v[6], v[7])));
@@ -552,7 +594,7 @@ __global__ __launch_bounds__(64 * kWaves, END != End::plain && J == 4 ? 2 : 1) v
   };
   fetch(0);
   struct Rows {
-    uint4 y[4];
+    Eight<END> y[4];
   };
   int64_t row[4];
 #pragma unroll
@@ -564,7 +606,7 @@ __global__ __launch_bounds__(64 * kWaves, END != End::plain && J == 4 ? 2 : 1) v
     const int col = c0 + unit / HALVES * 128 + 8 * n, up = unit % HALVES * p.up;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      r.y[i] = w < nb && col < c1 ? mi::load16_nt(p.y + row[i] * p.y_stride + up + col) : make_uint4(0u, 0u, 0u, 0u);
+      r.y[i].load(p, row[i], up + col, w < nb && col < c1);
   };
   Rows rows, next_rows;
   load_rows(rows, 0);
@@ -588,15 +630,14 @@ __global__ __launch_bounds__(64 * kWaves, END != End::plain && J == 4 ? 2 : 1) v
   auto step = [&]<int HALF>(int unit) {
     const int col = c0 + unit / HALVES * 128 + 8 * n, buf = unit & 1;
     keep(buf);
+    f32x4_t d[8];
+    begin_sums<END>(d, rows.y);
     if (unit + 1 < units) {
       fetch(unit + 1);
       load_rows(next_rows, unit + 1);
     }
     __syncthreads();
     if (w < nb) {
-      f32x4_t d[8];
-#pragma unroll
-      for (int t = 0; t < 8; ++t) d[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       if (adds) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
@@ -637,7 +678,8 @@ struct Units {
   const int w, lane, eighths;
   const uint16_t* weights;
   int64_t row[4];
-  uint4 b[LOTS], y[4];
+  uint4 b[LOTS];
+  Eight<END> y[4];
 
   __device__ __forceinline__ Units(const AdapterParams& p, const Columns& c, const Tile& tile, const int (&mine)[4], int any)
       : p(p), c(c), tile(tile), w(__builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6)), lane(threadIdx.x & 63), eighths(p.eighths) {
@@ -656,7 +698,7 @@ struct Units {
                  ? mi::load16(weights + int64_t(up + at) * p.rank + (e - in * eighths) * 8) : none;
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) y[k] = col < c.end ? mi::load16_nt(p.y + row[k] * p.y_stride + up + col) : none;
+    for (int k = 0; k < 4; ++k) y[k].load(p, row[k], up + col, col < c.end);
   }
   // vs: v's pairs, those of the gate and of the up columns; ws: room for a unit's weights, the wave's own.
   template <int HALF>
@@ -664,9 +706,8 @@ struct Units {
     const int g = lane >> 4, n = lane & 15, c0 = c.begin + (i / HALVES * WAVES + w) * 128, col = c0 + 8 * n;
     const uint4 none = make_uint4(0u, 0u, 0u, 0u);
     f32x4_t d[8];
-#pragma unroll
-    for (int t = 0; t < 8; ++t) d[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    const uint4 own[4] = {y[0], y[1], y[2], y[3]};
+    begin_sums<END>(d, y);
+    const Eight<END> own[4] = {y[0], y[1], y[2], y[3]};
     if (tile.slot >= 0) {
 #pragma unroll
       for (int k = 0; k < LOTS; ++k) {
@@ -933,11 +974,12 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
   const int64_t out_n = silu ? n / 2 : n;
   if (silu && (pieces != 2 || piece_columns[0] != piece_columns[1]))
     return mi::fail(MI_ERR_INVALID, "%s: SiLU is of gate and up, two pieces of as many columns", name);
-  if (out_scales && (!silu || out_n % mi::mx8::kBlock))
+  const bool sums = silu == MI_SILU_SUMS, steps = silu == MI_SILU_STEPS;
+  if (out_scales && (!silu || steps || out_n % mi::mx8::kBlock))
     return mi::fail(MI_ERR_INVALID, "%s: rows in 8 bits are the gated sum's, a multiple of %d columns; got %lld", name,
                     mi::mx8::kBlock, (long long)out_n);
   if (rows == 0) return MI_OK;
-  const int64_t each = x_scales ? 1 : 2, out_each = out_scales ? 1 : 2;
+  const int64_t each = x_scales ? 1 : 2, out_each = out_scales ? 1 : 2, y_each = sums ? 4 : 2;
   const int64_t scale_bytes = (k / 32 + 15) & ~int64_t(15);
   if (rows == 1) {  // (nothing lies at a single row's stride)
     y_stride = n, out_stride = out_n, out_scales_stride = out_n / 32;
@@ -949,7 +991,7 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
                             reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(out) |
                             reinterpret_cast<uintptr_t>(plan) | reinterpret_cast<uintptr_t>(workspace) |
                             reinterpret_cast<uintptr_t>(x_scales);
-  if ((aligned & 15) || (y_stride & 7) || (out_stride * out_each) % 16 || (x_scales && x_scales_stride % 16) || (x_stride * each) % 16 || (reinterpret_cast<uintptr_t>(scale) & 3))
+  if ((aligned & 15) || (y_stride * y_each) % 16 || (out_stride * out_each) % 16 || (x_scales && x_scales_stride % 16) || (x_stride * each) % 16 || (reinterpret_cast<uintptr_t>(scale) & 3))
     return mi::fail(MI_ERR_INVALID, "%s: rows, factors, plan and workspace must be 16-byte aligned", name);
   if (out_stride < out_n || (out_scales && out_scales_stride < out_n / 32) || x_stride < 0 || y_stride < 0 || (x_scales && x_scales_stride < scale_bytes))
     return mi::fail(MI_ERR_INVALID, "%s: row strides %lld, %lld, %lld, %lld for %lld columns", name, (long long)y_stride,
@@ -966,7 +1008,7 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
   const bool in_place = !silu && out == y && out_stride == y_stride;
   const mi::Rows to = {out, out_stride * out_each, rows, out_n * out_each},
                  to_scales = {out_scales, out_scales_stride, out_scales ? rows : 0, out_n / 32};
-  const mi::Rows from[] = {{y, y_stride * 2, in_place ? 0 : rows, n * 2},
+  const mi::Rows from[] = {{y, y_stride * y_each, in_place ? 0 : rows, n * y_each},
                            {x, x_stride * each, rows, k * each},
                            {x_scales, x_scales_stride, x_scales ? rows : 0, k / 32},
                            {a, 0, 1, slots * pieces * rank * k * 2},
@@ -978,9 +1020,9 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
   for (const mi::Rows& r : from) meet = meet || mi::rows_meet(to, r) || mi::rows_meet(to_scales, r);
   if (meet) return mi::fail(MI_ERR_INVALID, "%s: out overlaps another argument (without SiLU it may be y itself)", name);
   // (sums are written there while others still read x and A, and read before B and y are)
-  const mi::Rows sums = from[7], all_y = {y, y_stride * 2, rows, n * 2};
-  meet = mi::rows_meet(sums, all_y);
-  for (int i = 1; i < 7; ++i) meet = meet || mi::rows_meet(sums, from[i]);
+  const mi::Rows held = from[7], all_y = {y, y_stride * y_each, rows, n * y_each};
+  meet = mi::rows_meet(held, all_y);
+  for (int i = 1; i < 7; ++i) meet = meet || mi::rows_meet(held, from[i]);
   if (meet) return mi::fail(MI_ERR_INVALID, "%s: the workspace overlaps another argument", name);
   p.x = static_cast<const char*>(x);
   p.x_stride = x_stride * each;
@@ -1043,9 +1085,10 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
       {shrink_many_kernel<true, 1>, shrink_many_kernel<true, 2>, nullptr, nullptr}};
   hipLaunchKernelGGL((many ? wide : few)[x8][rt - 1], grid, dim3(64 * (many ? kManyWaves : kWaves)), 0, s, p);
   const int j = rank <= 16 ? 0 : rank <= 32 ? 1 : rank <= 64 ? 2 : 3;
-  const Kernel expand = !silu      ? expand_of<End::plain>(many, by_waves, j)
-                        : p.scales ? expand_of<End::silu8>(many, by_waves, j)
-                                   : expand_of<End::silu>(many, by_waves, j);
+  const Kernel expand = !silu   ? expand_of<End::plain>(many, by_waves, j)
+                        : steps ? expand_of<End::steps>(many, by_waves, j)
+                        : sums  ? (p.scales ? expand_of<End::sums8> : expand_of<End::sums>)(many, by_waves, j)
+                                : (p.scales ? expand_of<End::silu8> : expand_of<End::silu>)(many, by_waves, j);
   hipLaunchKernelGGL(expand, dim3(uint32_t(tiles), uint32_t(chunks)), block, 0, s, p);
   return mi::check_launch(name);
 }

@@ -23,6 +23,8 @@ struct LinearParams {
   int split_slabs;  // slabs that one of them takes
   bool vec;     // out and bias take 8-byte accesses,
   bool wide;    // out 16-byte ones
+  float* sums;  // of the gated product: where gate's and, n columns on, up's sums go as they are; null: silu and out
+  int64_t sums_stride;
 };
 
 // Row h n + first + i of W (i the lane's row of 16): its 16 codes' place from the
@@ -61,6 +63,14 @@ __device__ __forceinline__ u32x2_t round4(f32x4_t sum, f32x4_t up, f32x4_t bias)
 // They are columns col .. col + 3 of out's row m.
 template <bool GLU>
 __device__ __forceinline__ void store4(const LinearParams& p, int64_t m, int col, f32x4_t sum, f32x4_t up, f32x4_t bias) {
+  if constexpr (GLU) {
+    if (p.sums) {
+      float* const to = p.sums + m * p.sums_stride + col;
+      *reinterpret_cast<f32x4_t*>(to) = sum;
+      *reinterpret_cast<f32x4_t*>(to + p.n) = up;
+      return;
+    }
+  }
   uint16_t* const out = p.out + m * p.o_stride + col;
   const u32x2_t v = round4<GLU>(sum, up, bias);
   if (p.vec) {

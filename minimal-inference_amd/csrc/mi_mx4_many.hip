@@ -490,6 +490,7 @@ void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t strea
   rest.x += mx ? q.rows / kTileRows * p.slabs * kTileBytes : q.rows * p.x_stride * 2;
   if (mx) rest.xs += q.rows / kTileRows * p.quads * kQuadBytes;
   rest.out += q.rows * p.o_stride;
+  if (p.sums) rest.sums += q.rows * p.sums_stride;
   launch_few(rest, glu, stream);
 }
 
@@ -513,21 +514,26 @@ extern "C" int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_sc
     return mi::fail(MI_ERR_INVALID, "linear_mxfp4: rows %lld (0..2^22), n %lld (1..2^24), k %lld (multiple of %d, at most %d)",
                     (long long)rows, (long long)n, (long long)k, kBlock, kMaxK);
   if (silu && bias) return mi::fail(MI_ERR_INVALID, "linear_mxfp4: no bias with the gated product");
+  const bool sums = silu == MI_SILU_SUMS;
+  if (sums && n % 4)
+    return mi::fail(MI_ERR_INVALID, "linear_mxfp4: sums are fp32, a multiple of 4 columns each; got %lld", (long long)n);
+  const int64_t out_n = sums ? 2 * n : n;
   if (rows == 0) return MI_OK;
-  if (rows == 1) x_stride = k, out_stride = n;  // (nothing lies at a row stride)
+  if (rows == 1) x_stride = k, out_stride = out_n;  // (nothing lies at a row stride)
   if (!x || !codes || !scales || !out) return mi::fail(MI_ERR_INVALID, "linear_mxfp4: null pointer argument");
   const uintptr_t aligned = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(codes) |
                             reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(x_scales) |
                             reinterpret_cast<uintptr_t>(workspace);
   if ((aligned & 15) || ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) & 1) ||
-      (!x_scales && x_stride % 8))
+      (!x_scales && x_stride % 8) || (sums && ((reinterpret_cast<uintptr_t>(out) & 15) || out_stride % 4)))
     return mi::fail(MI_ERR_INVALID, "linear_mxfp4: x rows, codes, scales and workspace must be 16-byte aligned");
-  if (out_stride < n || (!x_scales && (x_stride < k || x_stride > kMaxStride)))
+  if (out_stride < out_n || (!x_scales && (x_stride < k || x_stride > kMaxStride)))
     return mi::fail(MI_ERR_INVALID, "linear_mxfp4: row strides %lld (at most 2^22) / %lld for k %lld, n %lld",
                     (long long)x_stride, (long long)out_stride, (long long)k, (long long)n);
   // (a workgroup's rows of out are written while others still read all of x, W and bias)
   const int64_t w_rows = silu ? 2 * n : n;
-  const mi::Rows to = {out, out_stride * 2, rows, n * 2};
+  const int64_t each = sums ? 4 : 2;
+  const mi::Rows to = {out, out_stride * each, rows, out_n * each};
   const mi::Rows from[] = {
       x_scales ? mi::Rows{x, 0, 1, row_tiles(rows) * slabs(k) * kTileBytes} : mi::Rows{x, x_stride * 2, rows, k * 2},
       {x_scales, 0, x_scales ? 1 : 0, row_tiles(rows) * quads(k) * kQuadBytes},
@@ -561,7 +567,9 @@ extern "C" int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_sc
   p.w_tiles = int(row_tiles(silu ? 2 * n : n));
   p.vec = n % 4 == 0 && out_stride % 4 == 0 &&
           ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) & 7) == 0;
-  p.wide = p.vec && n % 8 == 0 && out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  p.wide = p.vec && !sums && n % 8 == 0 && out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  p.sums = sums ? static_cast<float*>(out) : nullptr;
+  p.sums_stride = out_stride;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   p.parts = static_cast<mi::f32x4_t*>(workspace);
   if (few(x_scales != nullptr, rows, silu ? 2 * n : n, k)) launch_few(p, silu != 0, s);

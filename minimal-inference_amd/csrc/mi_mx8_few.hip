@@ -163,6 +163,13 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(LinearParams p) {
       if (m < rows && col + 4 * g < p.n)
         p.parts[(int64_t(blockIdx.y) * rows + m) * ((p.n + 3) / 4) + col / 4 + g] = total(q);
     } else if constexpr (OUT8) {
+      if (p.sums) {
+#pragma unroll
+        for (int i = 0; i < STEP; ++i)
+          if (const int at = col + 16 * i + 4 * g; m < rows && at < p.n)
+            store_sums(p, m, at, total(HALVES * (r + i) * MB + b), total((HALVES * (r + i) + 1) * MB + b));
+        continue;
+      }
       store_block(p, m, m < rows && col < p.n, col, g, result(r, b), result(r + 1, b));
     } else {
       const f32x4_t v = result(r, b);
@@ -298,7 +305,7 @@ void launch_few(const LinearParams& p, bool glu, size_t room, hipStream_t stream
     return;
   }
   if (!glu) launch<false, false>(p, stream);
-  else p.scales ? launch<true, true>(p, stream) : launch<true, false>(p, stream);
+  else p.scales || p.sums ? launch<true, true>(p, stream) : launch<true, false>(p, stream);
 }
 
 }  // namespace mi::mx8

@@ -27,7 +27,23 @@ struct LinearParams {
   int split_slabs;  // slabs that one of them takes
   bool vec;   // out and bias take 8-byte accesses,
   bool wide;  // out 16-byte ones
+  float* sums;  // of the gated product: where gate's and, n columns on, up's sums go as they are; null: silu and out
+  int64_t sums_stride;
 };
+
+// Columns col .. col + 3 of a row's gate and up sums in fp32; NT: stores that L2 need not keep.
+template <bool NT = false>
+__device__ __forceinline__ void store_sums(const LinearParams& p, int64_t m, int col, f32x4_t gate, f32x4_t up) {
+  f32x4_t* const to = reinterpret_cast<f32x4_t*>(p.sums + m * p.sums_stride + col);
+  f32x4_t* const to_up = reinterpret_cast<f32x4_t*>(p.sums + m * p.sums_stride + col + p.n);
+  if constexpr (NT) {
+    __builtin_nontemporal_store(gate, to);
+    __builtin_nontemporal_store(up, to_up);
+  } else {
+    *to = gate;
+    *to_up = up;
+  }
+}
 
 // The bias of columns col .. col + 3.
 __device__ __forceinline__ f32x4_t bias4(const LinearParams& p, int col) {

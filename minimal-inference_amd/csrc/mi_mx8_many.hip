@@ -59,6 +59,18 @@ __device__ __forceinline__ void end_of_product(const LinearParams& p, const f32x
   constexpr int HALVES = GLU ? 2 : 1;
   const int g = (threadIdx.x & 63) >> 4, n = threadIdx.x & 15;
   if constexpr (OUT8 && !SPLIT) {
+    // (non-temporal, us: 16,384 x 4,096 x 2 x 14,336 1,807 -> 1,602, with the adapters that read them 2,340 -> 2,247;
+    // 512 rows 92 -> 96, 100 rows the same)
+    if (p.sums) {
+#pragma unroll
+      for (int t = 0; t < NT; t += 2)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) {
+          const int m = row0 + b * 16 + n, col = col0 + (first_tile + t) / 2 * 16 + 4 * g;
+          if (m < rows && col < p.n) store_sums<true>(p, m0 + m, col, acc[t][b], acc[t + 1][b]);
+        }
+      return;
+    }
 #pragma unroll
     for (int t = 0; t < NT; t += 4) {
       const int first = col0 + (first_tile + t) / 2 * 16;
@@ -462,6 +474,7 @@ __global__ __launch_bounds__(256) void combine_kernel(LinearParams p, int parts)
   const int64_t row = at / fours;
   const f32x4_t v = finish<GLU>(sum, up, bias4(p, col));
   if constexpr (OUT8) {
+    if (p.sums) return store_sums(p, row, col, sum, up);
     const uint32_t byte = scale_byte(max8(magnitude4(v)));
     *reinterpret_cast<uint32_t*>(p.out + row * p.o_stride + col) = to_codes(v[0], v[1], v[2], v[3], byte);
     if (col % kBlock == 0) p.scales[row * p.s_stride + col / kBlock] = uint8_t(byte);
@@ -552,7 +565,7 @@ void launch_combine(const LinearParams& p, bool glu, int parts, hipStream_t stre
   const int64_t fours = p.rows * ((p.n + 3) / 4);
   const dim3 grid(uint32_t((fours + 255) / 256)), block(256);
   if (!glu) hipLaunchKernelGGL((combine_kernel<false, false>), grid, block, 0, stream, p, parts);
-  else if (p.scales) hipLaunchKernelGGL((combine_kernel<true, true>), grid, block, 0, stream, p, parts);
+  else if (p.scales || p.sums) hipLaunchKernelGGL((combine_kernel<true, true>), grid, block, 0, stream, p, parts);
   else hipLaunchKernelGGL((combine_kernel<true, false>), grid, block, 0, stream, p, parts);
 }
 
@@ -566,7 +579,7 @@ void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t strea
   LinearParams q = p;
   q.rows = p.rows - c.rest;
   if (!glu) launch<false, false>(q, c, stream);
-  else p.scales ? launch<true, true>(q, c, stream) : launch<true, false>(q, c, stream);
+  else p.scales || p.sums ? launch<true, true>(q, c, stream) : launch<true, false>(q, c, stream);
   if (!c.rest) return;
   LinearParams rest = p;
   rest.rows = c.rest;
@@ -574,6 +587,7 @@ void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t strea
   rest.xs += q.rows * p.xs_stride;
   rest.out += q.rows * p.o_stride * (p.scales ? 1 : 2);
   if (p.scales) rest.scales += q.rows * p.s_stride;
+  if (p.sums) rest.sums += q.rows * p.sums_stride;
   launch_few(rest, glu, 0, stream);
 }
 
@@ -597,13 +611,17 @@ extern "C" int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void
     return mi::fail(MI_ERR_INVALID, "%s: rows %lld (0..2^22), n %lld (1..2^24), k %lld (multiple of %d, at most %d)", name,
                     (long long)rows, (long long)n, (long long)k, kBlock, kMaxK);
   if (silu && bias) return mi::fail(MI_ERR_INVALID, "%s: no bias with the gated product", name);
+  const bool sums = silu == MI_SILU_SUMS;
+  if (sums && (out_scales || n % 4))
+    return mi::fail(MI_ERR_INVALID, "%s: sums are fp32, a multiple of 4 columns each; got %lld", name, (long long)n);
   if (out_scales && (!silu || n % kBlock))
     return mi::fail(MI_ERR_INVALID, "%s: rows in 8 bits are the gated product's, n a multiple of %d; got %lld", name, kBlock,
                     (long long)n);
   if (rows == 0) return MI_OK;
   const int64_t w_rows = silu ? 2 * n : n, blocks = k / kBlock, padded = (blocks + 15) & ~int64_t(15);
   // (nothing lies at a single row's stride)
-  if (rows == 1) x_stride = (k + 15) & ~int64_t(15), x_scales_stride = padded, out_stride = n, out_scales_stride = n / kBlock;
+  const int64_t out_n = sums ? 2 * n : n;
+  if (rows == 1) x_stride = (k + 15) & ~int64_t(15), x_scales_stride = padded, out_stride = out_n, out_scales_stride = n / kBlock;
   if (w_rows == 1) w_stride = (k + 15) & ~int64_t(15), w_scales_stride = padded;
   if (!x_codes || !x_scales || !w_codes || !w_scales || !out)
     return mi::fail(MI_ERR_INVALID, "%s: null pointer argument", name);
@@ -612,17 +630,18 @@ extern "C" int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void
                             reinterpret_cast<uintptr_t>(workspace);
   if ((aligned & 15) || ((x_stride | x_scales_stride | w_stride | w_scales_stride) & 15) ||
       ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) & 1) ||
-      (out_scales && ((reinterpret_cast<uintptr_t>(out) & 15) || out_stride % 16)))
+      (out_scales && ((reinterpret_cast<uintptr_t>(out) & 15) || out_stride % 16)) ||
+      (sums && ((reinterpret_cast<uintptr_t>(out) & 15) || out_stride % 4)))
     return mi::fail(MI_ERR_INVALID, "%s: rows of codes and scales, and the workspace, must be 16-byte aligned", name);
   if (x_stride < k || w_stride < k || x_stride > kMaxStride || w_stride > kMaxStride || x_scales_stride < padded ||
-      w_scales_stride < padded || x_scales_stride > kMaxStride || w_scales_stride > kMaxStride || out_stride < n ||
+      w_scales_stride < padded || x_scales_stride > kMaxStride || w_scales_stride > kMaxStride || out_stride < out_n ||
       (out_scales && out_scales_stride < n / kBlock))
     return mi::fail(MI_ERR_INVALID, "%s: row strides %lld, %lld, %lld, %lld (at most 2^22), %lld, %lld for k %lld, n %lld", name,
                     (long long)x_stride, (long long)x_scales_stride, (long long)w_stride, (long long)w_scales_stride,
                     (long long)out_stride, (long long)out_scales_stride, (long long)k, (long long)n);
   // (a workgroup's rows of out are written while others still read all of x, W and bias)
-  const int64_t each = out_scales ? 1 : 2;
-  const mi::Rows to[] = {{out, out_stride * each, rows, n * each},
+  const int64_t each = out_scales ? 1 : sums ? 4 : 2;
+  const mi::Rows to[] = {{out, out_stride * each, rows, out_n * each},
                          {out_scales, out_scales_stride, out_scales ? rows : 0, n / kBlock}};
   const mi::Rows from[] = {{x_codes, x_stride, rows, k}, {x_scales, x_scales_stride, rows, blocks},
                            {w_codes, w_stride, w_rows, k}, {w_scales, w_scales_stride, w_rows, blocks},
@@ -663,6 +682,8 @@ extern "C" int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void
   p.vec = n % 4 == 0 && out_stride % 4 == 0 &&
           ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) & 7) == 0;
   p.wide = p.vec && n % 8 == 0 && out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  p.sums = sums ? static_cast<float*>(out) : nullptr;
+  p.sums_stride = out_stride;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (rows <= kFewRows) launch_few(p, silu != 0, room, s);
   else launch_many(p, silu != 0, room, s);

@@ -49,8 +49,8 @@ import torch.nn.functional as F
 
 from .adapters import Adapters, add_adapters, add_adapters_silu
 from .dense import add_rms_norm, linear, linear_silu
-from .mxfp4 import BLOCK, MXFP4, linear_mxfp4, linear_silu_mxfp4, quantize_mxfp4
-from .mxfp8 import MXFP8, add_rms_norm_mxfp8, linear_mxfp8, linear_silu_mxfp8, quantize_mxfp8
+from .mxfp4 import BLOCK, MXFP4, gate_up_mxfp4, linear_mxfp4, linear_silu_mxfp4, quantize_mxfp4
+from .mxfp8 import MXFP8, add_rms_norm_mxfp8, gate_up_mxfp8, linear_mxfp8, linear_silu_mxfp8, quantize_mxfp8
 from .page import append_paged_kv_cache, rope_append_paged_kv_cache
 
 
@@ -345,8 +345,10 @@ class Model:
                 o = quantize_mxfp8(o)
             h = norm(x, adapted(project(o, L.w_o), o, L, "w_o"), L.post_norm, L.w_gate_up)
             if plan is not None and "w_gate_up" in L.adapters:
-                act = add_adapters_silu(project(h, L.w_gate_up), h, L.adapters["w_gate_up"], plan,
-                                        quantize=isinstance(L.w_down, MXFP8))
+                # (rows without an adapter get the bits of the forms below, whatever rows stand beside them)
+                sums = gate_up_mxfp8 if isinstance(L.w_gate_up, MXFP8) else gate_up_mxfp4 if isinstance(L.w_gate_up, MXFP4) else linear
+                act = add_adapters_silu(sums(h, L.w_gate_up), h, L.adapters["w_gate_up"], plan,
+                                        quantize=isinstance(L.w_gate_up, MXFP8), stepwise=sums is linear)
             elif isinstance(L.w_gate_up, MXFP8):
                 act = linear_silu_mxfp8(h, L.w_gate_up, quantize=True)
             else:

@@ -20,7 +20,7 @@ import functools
 import torch
 from torch.autograd import forward_ad
 
-from ._util import bytes_on, call_on, refuse_derivatives, require_dtype, require_gpu
+from ._util import SILU, SILU_SUMS, bytes_on, call_on, refuse_derivatives, require_dtype, require_gpu, sums_out
 
 BLOCK = 32
 _TILE_ROWS, _SLAB, _TILE_BYTES, _QUAD_BYTES = 16, 128, 1024, 256
@@ -127,7 +127,7 @@ def quantize_mxfp4(x: torch.Tensor, out: MXFP4 | None = None) -> MXFP4:
     return out
 
 
-def _linear(x, weight: MXFP4, bias, out, silu: bool) -> torch.Tensor:
+def _linear(x, weight: MXFP4, bias, out, silu: int) -> torch.Tensor:
     if not isinstance(weight, MXFP4):
         raise TypeError("the weight must be an MXFP4 matrix")
     n = weight.rows
@@ -152,14 +152,14 @@ def _linear(x, weight: MXFP4, bias, out, silu: bool) -> torch.Tensor:
             raise ValueError(f"bias must be a contiguous [{n}] tensor on {like.device}")
         if bias.requires_grad or forward_ad._current_level >= 0:
             refuse_derivatives("bias", bias)
-    out = _out(out, rows, n, like)
+    out = sums_out(out, rows, n, like.device) if silu == SILU_SUMS else _out(out, rows, n, like)
     if rows and n:
-        room = _workspace_size(rows, n, k, silu, scales is not None, like.get_device()) if rows > _FEW_ROWS else 0
+        room = _workspace_size(rows, n, k, silu != 0, scales is not None, like.get_device()) if rows > _FEW_ROWS else 0
         # (a tensor of this call's own: calls on several streams and in graphs share nothing)
         workspace = torch.empty(room, dtype=torch.uint8, device=like.device) if room else None
         call_on(like, "mi_linear_mxfp4", data, stride, scales, weight.codes_ptr, weight.scales_ptr,
                 bias.data_ptr() if bias is not None else None, out.data_ptr(), out.stride(0), rows, n, k,
-                1 if silu else 0, workspace.data_ptr() if room else None, room)
+                silu, workspace.data_ptr() if room else None, room)
     return out
 
 
@@ -172,9 +172,15 @@ def linear_mxfp4(x: torch.Tensor | MXFP4, weight: MXFP4, bias: torch.Tensor | No
                  out: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T + bias`` as bf16 [rows, n]; x is bf16 [rows, k] or MXFP4.  An out
     that overlaps x, the weight or the bias is refused (columns of one buffer need not)."""
-    return _linear(x, weight, bias, out, False)
+    return _linear(x, weight, bias, out, 0)
 
 
 def linear_silu_mxfp4(x: torch.Tensor | MXFP4, gate_up: MXFP4, out: torch.Tensor | None = None) -> torch.Tensor:
     """``silu(x @ gate.T) * (x @ up.T)``, gate and up the halves of gate_up's rows."""
-    return _linear(x, gate_up, None, out, True)
+    return _linear(x, gate_up, None, out, SILU)
+
+
+def gate_up_mxfp4(x: torch.Tensor | MXFP4, gate_up: MXFP4, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The sums ``x @ gate_up.T`` in fp32 [rows, 2 n], bit for bit those that ``linear_silu_mxfp4`` goes on with: what
+    ``adapters.add_adapters_silu`` adds to (n a multiple of 4)."""
+    return _linear(x, gate_up, None, out, SILU_SUMS)

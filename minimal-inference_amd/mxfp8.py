@@ -10,7 +10,7 @@ tensors, ``add_rms_norm_mxfp8`` of the residual stream before a block.
 ``linear_mxfp8(x, weight, bias)`` is ``x @ weight.T + bias`` and
 ``linear_silu_mxfp8(x, gate_up)`` is ``silu(x @ gate.T) * (x @ up.T)`` of a fused gate
 and up weight, both operands MXFP8; the latter leaves MXFP8 rows again with
-``quantize=True``.  Sums are fp32, rounded once, but the matrix instruction cuts each product to a multiple of
+``quantize=True``, and ``gate_up_mxfp8(x, gate_up)`` leaves its sums as they are.  Sums are fp32, rounded once, but the matrix instruction cuts each product to a multiple of
 2^-13 of the largest of its eight neighbours in k: 1.5e-5 of the result's
 norm on normal values, 2.7e-5 where single channels stand out, against 1.7e-3 that the rounding to bf16 makes.
 The same call repeats its bits.  There is no torch fallback and no backward pass: tensors that
@@ -24,7 +24,7 @@ import functools
 import torch
 from torch.autograd import forward_ad
 
-from ._util import bytes_on, call_on, refuse_derivatives, require_dtype, require_gpu
+from ._util import SILU, SILU_SUMS, bytes_on, call_on, refuse_derivatives, require_dtype, require_gpu, sums_out
 
 BLOCK = 32
 _PIECE = 16  # bytes of scales that are read together
@@ -216,7 +216,7 @@ def _workspace_size(rows: int, n: int, k: int, silu: bool, device: int | None = 
     return bytes_on(device, "mi_linear_mxfp8_workspace_size", rows, n, k, silu)
 
 
-def _linear(x: MXFP8, weight: MXFP8, bias, out, silu: bool, quantize: bool):
+def _linear(x: MXFP8, weight: MXFP8, bias, out, silu: int, quantize: bool):
     if not isinstance(x, MXFP8) or not isinstance(weight, MXFP8):
         raise TypeError("x and the weight must be MXFP8 matrices (quantize_mxfp8 makes one of bf16 rows)")
     rows, k, n, device = x.rows, x.cols, weight.rows, x.device
@@ -239,15 +239,15 @@ def _linear(x: MXFP8, weight: MXFP8, bias, out, silu: bool, quantize: bool):
         out = _rows8(out, rows, n, device)
         to, stride, scales, s_stride = out.codes_ptr, out.codes_stride, out.scales_ptr, out.scales_stride
     else:
-        out = _out(out, rows, n, device)
+        out = sums_out(out, rows, n, device) if silu == SILU_SUMS else _out(out, rows, n, device)
         to, stride, scales, s_stride = out.data_ptr(), out.stride(0), None, 0
     if rows and n:
-        room = _workspace_size(rows, n, k, silu, device.index)
+        room = _workspace_size(rows, n, k, silu != 0, device.index)
         # (a tensor of this call's own: calls on several streams and in graphs share nothing)
         workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
         call_on(x.anchor, "mi_linear_mxfp8", x.codes_ptr, x.codes_stride, x.scales_ptr, x.scales_stride,
                 weight.codes_ptr, weight.codes_stride, weight.scales_ptr, weight.scales_stride,
-                bias.data_ptr() if bias is not None else None, to, stride, scales, s_stride, rows, n, k, 1 if silu else 0,
+                bias.data_ptr() if bias is not None else None, to, stride, scales, s_stride, rows, n, k, silu,
                 workspace.data_ptr() if room else None, room)
     return out
 
@@ -256,7 +256,7 @@ def linear_mxfp8(x: MXFP8, weight: MXFP8, bias: torch.Tensor | None = None,
                  out: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T + bias`` as bf16 [rows, n].  An out that overlaps x, the weight or
     the bias is refused."""
-    return _linear(x, weight, bias, out, False, False)
+    return _linear(x, weight, bias, out, 0, False)
 
 
 def linear_silu_mxfp8(x: MXFP8, gate_up: MXFP8, out: "torch.Tensor | MXFP8 | None" = None, *,
@@ -265,4 +265,10 @@ def linear_silu_mxfp8(x: MXFP8, gate_up: MXFP8, out: "torch.Tensor | MXFP8 | Non
     [rows, n], or with ``quantize`` as MXFP8, rounded from fp32 (n a multiple of 32; silu within 2^-20)."""
     if quantize and isinstance(gate_up, MXFP8) and gate_up.rows // 2 % BLOCK:
         raise ValueError(f"rows in MXFP8 have columns in blocks of {BLOCK}; got {gate_up.rows // 2}")
-    return _linear(x, gate_up, None, out, True, quantize)
+    return _linear(x, gate_up, None, out, SILU, quantize)
+
+
+def gate_up_mxfp8(x: MXFP8, gate_up: MXFP8, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The sums ``x @ gate_up.T`` in fp32 [rows, 2 n], bit for bit those of which ``linear_silu_mxfp8`` makes MXFP8
+    rows: what ``adapters.add_adapters_silu`` adds to (n a multiple of 4)."""
+    return _linear(x, gate_up, None, out, SILU_SUMS, False)
