@@ -875,7 +875,8 @@ Split split_of(int64_t rows, int64_t slots, int64_t k, int64_t padded, bool x8) 
   } else {
     s.groups = int((rank_tiles + group - 1) / group);
     // rounds of workgroups (a part of one counts two thirds and more of a whole), of their steps and a start of
-    // twelve, and the parts' way (us of both launches in a graph, by parts, * taken):
+    // twelve, and the parts' way (us of both launches in a graph, by parts, * taken: the least or within 3 % of
+    // it but at 4,105 rows, where two parts would be a tenth faster, which a count that fits the others does not give):
     //   1,031 x  3,584 ->  4,608, rank 16          1 29.0   2 21.1   5 17.7   6 18.1*  12 20.4
     //   4,105 x  4,096 ->  6,144, rank 16          1 50.5   2 44.8   4 49.5*  6 50.8    8 58.2
     //  18,240 x  4,096 ->  6,144, rank 16          1 153*   2 162    3 149    4 154     6 160
