@@ -1021,9 +1021,11 @@ extern "C" int mi_add_adapters(const void* y, int64_t y_stride, const void* x, i
   for (const mi::Rows& r : from) meet = meet || mi::rows_meet(to, r) || mi::rows_meet(to_scales, r);
   if (meet) return mi::fail(MI_ERR_INVALID, "%s: out overlaps another argument (without SiLU it may be y itself)", name);
   // (sums are written there while others still read x and A, and read before B and y are)
-  const mi::Rows held = from[7], all_y = {y, y_stride * y_each, rows, n * y_each};
-  meet = mi::rows_meet(held, all_y);
-  for (int i = 1; i < 7; ++i) meet = meet || mi::rows_meet(held, from[i]);
+  if (need) {
+    const mi::Rows held = from[7], all_y = {y, y_stride * y_each, rows, n * y_each};
+    meet = mi::rows_meet(held, all_y);
+    for (int i = 1; i < 7; ++i) meet = meet || mi::rows_meet(held, from[i]);
+  }
   if (meet) return mi::fail(MI_ERR_INVALID, "%s: the workspace overlaps another argument", name);
   p.x = static_cast<const char*>(x);
   p.x_stride = x_stride * each;

@@ -98,6 +98,5 @@ inline bool few(bool mx, int64_t rows, int64_t w_rows, int64_t k) {
   return mx ? rows <= 64 : rows <= 16 || (rows <= 32 && (w_rows > 4096 || k < 8192));
 }
 void launch_few(const LinearParams& p, bool glu, hipStream_t stream);
-void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t stream);
 
 }  // namespace mi::mx4

@@ -468,17 +468,10 @@ Way way_of(bool mx, bool glu, int64_t rows, int64_t n, int slabs, size_t room) {
   }
   return {c, rows};
 }
-// The bytes of parts that it writes.
-size_t parts_bytes(bool mx, bool glu, int64_t rows, int64_t n, int64_t k, size_t room) {
-  if (few(mx, rows, glu ? 2 * n : n, k)) return 0;
-  const Way way = way_of(mx, glu, rows, n, int(slabs(k)), room);
-  return way.blocks && way.c.parts > 1 ? way.c.bytes : 0;
-}
 
-void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t stream) {
+void launch_way(const LinearParams& p, bool glu, const Way& way, hipStream_t stream) {
   const bool mx = p.xs != nullptr;
   LinearParams q = p;
-  const Way way = way_of(mx, glu, p.rows, p.n, p.slabs, room);
   if (!way.blocks) return launch_few(p, glu, stream);
   const Choice& c = way.c;
   q.rows = way.blocks;
@@ -543,9 +536,11 @@ extern "C" int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_sc
   for (const mi::Rows& r : from)
     if (mi::rows_meet(to, r)) return mi::fail(MI_ERR_INVALID, "linear_mxfp4: out overlaps x, the weight or the bias");
   // (parts are written while others still read x and W, and read while out is written)
-  const size_t room = workspace ? workspace_bytes : 0;
-  if (const size_t bytes = room ? parts_bytes(x_scales != nullptr, silu != 0, rows, n, k, room) : 0) {
-    const mi::Rows parts = {workspace, 0, 1, int64_t(bytes)};
+  Way way = {};
+  if (!few(x_scales != nullptr, rows, w_rows, k))
+    way = way_of(x_scales != nullptr, silu != 0, rows, n, int(slabs(k)), workspace ? workspace_bytes : 0);
+  if (way.blocks && way.c.parts > 1) {
+    const mi::Rows parts = {workspace, 0, 1, int64_t(way.c.bytes)};
     bool meet = mi::rows_meet(parts, to);
     for (const mi::Rows& r : from) meet = meet || mi::rows_meet(parts, r);
     if (meet) return mi::fail(MI_ERR_INVALID, "linear_mxfp4: the workspace overlaps another argument");
@@ -572,7 +567,6 @@ extern "C" int mi_linear_mxfp4(const void* x, int64_t x_stride, const void* x_sc
   p.sums_stride = out_stride;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   p.parts = static_cast<mi::f32x4_t*>(workspace);
-  if (few(x_scales != nullptr, rows, silu ? 2 * n : n, k)) launch_few(p, silu != 0, s);
-  else launch_many(p, silu != 0, room, s);
+  launch_way(p, silu != 0, way, s);
   return mi::check_launch("linear_mxfp4");
 }

@@ -106,6 +106,5 @@ size_t few_workspace(bool glu, int64_t rows, int64_t n, int slabs, size_t room);
 void launch_few(const LinearParams& p, bool glu, size_t room, hipStream_t stream);
 // The sum of parts [part][half][row][columns in fours], and the end of the product.
 void launch_combine(const LinearParams& p, bool glu, int parts, hipStream_t stream);
-void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t stream);
 
 }  // namespace mi::mx8

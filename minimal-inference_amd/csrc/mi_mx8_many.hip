@@ -569,13 +569,7 @@ void launch_combine(const LinearParams& p, bool glu, int parts, hipStream_t stre
   else hipLaunchKernelGGL((combine_kernel<true, false>), grid, block, 0, stream, p, parts);
 }
 
-// The bytes of parts that a call with `room` bytes for them writes.
-size_t parts_bytes(bool glu, int64_t rows, int64_t n, int slabs, size_t room) {
-  return rows <= kFewRows ? few_workspace(glu, rows, n, slabs, room) : choose(glu, rows, n, slabs, room).bytes;
-}
-
-void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t stream) {
-  const Choice c = choose(glu, p.rows, p.n, p.slabs, room);
+void launch_many(const LinearParams& p, bool glu, const Choice& c, hipStream_t stream) {
   LinearParams q = p;
   q.rows = p.rows - c.rest;
   if (!glu) launch<false, false>(q, c, stream);
@@ -596,7 +590,9 @@ void launch_many(const LinearParams& p, bool glu, size_t room, hipStream_t strea
 extern "C" size_t mi_linear_mxfp8_workspace_size(int64_t rows, int64_t n, int64_t k, int32_t silu) {
   using namespace mi::mx8;
   if (rows <= 0 || rows > kMaxRows || n <= 0 || n > kMaxN || k <= 0 || k % kBlock || k > kMaxK) return 0;
-  return parts_bytes(silu != 0, rows, n, int(slabs(k)), size_t(1) << 28);
+  const size_t room = size_t(1) << 28;
+  if (rows <= kFewRows) return few_workspace(silu != 0, rows, n, int(slabs(k)), room);
+  return choose(silu != 0, rows, n, int(slabs(k)), room).bytes;
 }
 
 extern "C" int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void* x_scales, int64_t x_scales_stride,
@@ -652,7 +648,8 @@ extern "C" int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void
   if (meet) return mi::fail(MI_ERR_INVALID, "%s: out overlaps x, the weight, the bias or its own scales", name);
   // (parts are written while others still read x and W, and read while out is written)
   const size_t room = workspace ? workspace_bytes : 0;
-  if (const size_t bytes = room ? parts_bytes(silu != 0, rows, n, int(slabs(k)), room) : 0) {
+  const Choice choice = choose(silu != 0, rows, n, int(slabs(k)), room);
+  if (const size_t bytes = choice.form == Form::few ? few_workspace(silu != 0, rows, n, int(slabs(k)), room) : choice.bytes) {
     const mi::Rows parts = {workspace, 0, 1, int64_t(bytes)};
     for (const mi::Rows& r : to) meet = meet || mi::rows_meet(parts, r);
     for (const mi::Rows& r : from) meet = meet || mi::rows_meet(parts, r);
@@ -685,7 +682,7 @@ extern "C" int mi_linear_mxfp8(const void* x_codes, int64_t x_stride, const void
   p.sums = sums ? static_cast<float*>(out) : nullptr;
   p.sums_stride = out_stride;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (rows <= kFewRows) launch_few(p, silu != 0, room, s);
-  else launch_many(p, silu != 0, room, s);
+  if (choice.form == Form::few) launch_few(p, silu != 0, room, s);
+  else launch_many(p, silu != 0, choice, s);
   return mi::check_launch(name);
 }
