@@ -11,6 +11,7 @@ Public surface (mirrors what the reference's model.py / scheduler.py call):
   mxfp4.MXFP4 / quantize_mxfp4 / linear_mxfp4       -- 4-bit weights (no counterpart)
   mxfp8.MXFP8 / quantize_mxfp8 / linear_mxfp8       -- 8-bit weights and rows (no counterpart)
   mxfp8.add_rms_norm_mxfp8                          -- residual and norm to 8-bit rows
+  mxfp8.gate_up_mxfp8 / mxfp4.gate_up_mxfp4         -- fp32 sums for adapters beside them
   adapters.Adapters / AdapterPlan / add_adapters[_silu]  -- low-rank adapters by request (no counterpart)
   dense.post_norm_add_rms_norm                      -- norms around a block (no counterpart)
   kv_cache.PagedKVCache / build_csr_metadata        -- scheduler.py:168-302

@@ -78,8 +78,8 @@ __device__ __forceinline__ u32x2_t to_bf16(uint32_t codes, float scale) {
 // out is made good (they would be |g| 2^-24 and |g| 2^-26).  Then w is within 1.5 2^-23 (the exponential 2^-23, the
 // correction 2^-24), w^2 twice that, its part in 1 + w^2 of the other sign, the reciprocal and the sum under it
 // 1.5 2^-23, three products 1.5 2^-23: 6 2^-23 in all.  An end of 128 such values a lane is a tenth of a largest block's
-// time: half the instructions of a division rounded to the last bit (us, 2,057 x
-// 4,096 x 2 x 14,336 237 -> 230, 16,384 rows 1,591 -> 1,521).
+// time: half the instructions of a division rounded to the last bit took 237 us of 2,057 x 4,096 x 2 x 14,336
+// to 230, 1,591 of 16,384 rows to 1,521; with other stores since and the constant's rest 214.
 __device__ __forceinline__ float silu20(float g) {
   constexpr float kHalfLog2e = 0.721347511f, kHalfLog2eRest = 9.62981496e-9f;
   const float a = -fminf(fabsf(g), 200.f), h = a * kHalfLog2e;
